@@ -542,6 +542,48 @@ int mhc_glu_fwd(const void* x, const void* gate_w, const void* up_w, void* out, 
  * slower than library products of these sizes, 0 where it is or takes them not. */
 int mhc_linear_pays(const int* n, int count, int64_t M, int K, int glu);
 
+/* ------------------------------------------- attention over packed sequences
+ * B sequences one after another in 16-bit tensors (bf16 or fp16) of one dtype:
+ * q [Tq, heads, head_dim], k and v [Tk, kv_heads, head_dim], head_dim 64, 96 or
+ * 128, heads a multiple of kv_heads.  A head's elements are contiguous; the
+ * strides of a row and of a head are given in elements (multiples of 8), data
+ * pointers are 16-byte aligned.  cu_q, cu_k [B + 1] (device, int32): sequence i
+ * has the query rows cu_q[i] .. cu_q[i + 1] and the key rows cu_k[i] ..
+ * cu_k[i + 1]; the first entry of both is taken as 0.  key_lengths [B] (device,
+ * int32, or NULL): only the first key_lengths[i] of those key rows are in use (a
+ * cache slot).  The last query of a sequence sits at its last key, and each query
+ * sees the keys up to its own position.  Rows that see no key, and the rows
+ * behind the last sequence, come out 0.  The bounds are clamped to the tensors;
+ * bounds that decrease give unspecified rows.
+ * Tq and Tk are at most 2^30.
+ */
+
+/* Bytes of workspace mhc_packed_attn_fwd needs (0: none), or -1 for a shape it
+ * does not take. */
+int64_t mhc_packed_attn_workspace_bytes(int B, int64_t Tq, int64_t Tk, int heads, int kv_heads,
+                                        int head_dim);
+
+/* out [Tq, heads, head_dim] (contiguous) = softmax(scale q k^T) v, scale > 0.
+ * lse (NULL, or [heads, Tq] fp32): the base-2 logarithms of the softmax's sums,
+ * for mhc_packed_attn_bwd. */
+int mhc_packed_attn_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+                        int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
+                        int64_t v_stride_h, const int* cu_q, const int* cu_k, const int* key_lengths,
+                        void* out, float* lse, void* workspace, int64_t workspace_bytes, int B,
+                        int64_t Tq, int64_t Tk, int heads, int kv_heads, int head_dim, int dtype,
+                        float scale, hipStream_t stream);
+
+/* Gradients g_q [Tq, heads, head_dim], g_k and g_v [Tk, kv_heads, head_dim]
+ * (contiguous; every row is written) for g_out, contiguous as out.  out and lse
+ * are the forward's; delta [heads, Tq] fp32 is scratch.  No atomics: the same bits on every
+ * run. */
+int mhc_packed_attn_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+                        int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
+                        int64_t v_stride_h, const int* cu_q, const int* cu_k, const int* key_lengths,
+                        const void* out, const float* lse, const void* g_out, float* delta, void* g_q,
+                        void* g_k, void* g_v, int B, int64_t Tq, int64_t Tk, int heads, int kv_heads,
+                        int head_dim, int dtype, float scale, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

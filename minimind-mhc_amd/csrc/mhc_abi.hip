@@ -733,6 +733,89 @@ int mhc_attn_decode_fwd(const void* q, const void* k, const void* v, const void*
   return hip_status(mhc::launch_attn_decode(a, stream), fn);
 }
 
+// ------------------------------------------- attention over packed sequences
+
+static int check_packed(const mhc::PackedAttnArgs& a, int64_t Tq, int64_t Tk, int dtype, const char* fn) {
+  if (a.B < 0 || Tq < 0 || Tk < 0 || Tq > 1 << 30 || Tk > 1 << 30)
+    return fail(hipErrorInvalidValue, "%s: bad shape (B=%d Tq=%lld Tk=%lld)", fn, a.B, (long long)Tq, (long long)Tk);
+  if (int rc = check_attn(Tq, a.heads, a.kv_heads, a.head_dim, dtype, fn)) return rc;
+  if (!(a.scale > 0.f) || a.scale > 3e38f) return fail(hipErrorInvalidValue, "%s: scale must be positive (got %g)", fn, (double)a.scale);
+  // the most workgroups of any of the launches: a tile number for every row and sequence
+  if ((Tq + a.B + 1) * a.heads > kMaxBlocks || (Tk / 64 + a.B + 1) * a.kv_heads > kMaxBlocks)
+    return fail(hipErrorInvalidValue, "%s: too large", fn);
+  for (int64_t st : {a.qs_t, a.qs_h, a.ks_t, a.ks_h, a.vs_t, a.vs_h})
+    if (st % 8 != 0 || st < 0) return fail(hipErrorInvalidValue, "%s: strides must be multiples of 8 elements", fn);
+  return 0;
+}
+
+static mhc::PackedAttnArgs packed_args(const void* q, int64_t qs_t, int64_t qs_h, const void* k, int64_t ks_t,
+                                       int64_t ks_h, const void* v, int64_t vs_t, int64_t vs_h, const int* cu_q,
+                                       const int* cu_k, const int* k_len, int B, int64_t Tq, int64_t Tk, int heads,
+                                       int kv_heads, int head_dim, int dtype, float scale) {
+  mhc::PackedAttnArgs a{};
+  a.q = q; a.k = k; a.v = v;
+  a.qs_t = qs_t; a.qs_h = qs_h; a.ks_t = ks_t; a.ks_h = ks_h; a.vs_t = vs_t; a.vs_h = vs_h;
+  a.cu_q = cu_q; a.cu_k = cu_k; a.k_len = k_len;
+  a.B = B; a.Tq = (int)Tq; a.Tk = (int)Tk; a.heads = heads; a.kv_heads = kv_heads; a.head_dim = head_dim;
+  a.f16 = dtype == mhc::kF16; a.scale = scale;
+  return a;
+}
+
+int64_t mhc_packed_attn_workspace_bytes(int B, int64_t Tq, int64_t Tk, int heads, int kv_heads, int head_dim) {
+  mhc::PackedAttnArgs a = packed_args(nullptr, 0, 0, nullptr, 0, 0, nullptr, 0, 0, nullptr, nullptr, nullptr, B, Tq,
+                                      Tk, heads, kv_heads, head_dim, mhc::kBF16, 1.f);
+  if (check_packed(a, Tq, Tk, mhc::kBF16, "mhc_packed_attn_workspace_bytes")) return -1;
+  if (Tq == 0) return 0;
+  mhc::packed_attn_plan(a);
+  return mhc::packed_attn_workspace(a);
+}
+
+int mhc_packed_attn_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+                        int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
+                        int64_t v_stride_h, const int* cu_q, const int* cu_k, const int* key_lengths,
+                        void* out, float* lse, void* workspace, int64_t workspace_bytes, int B,
+                        int64_t Tq, int64_t Tk, int heads, int kv_heads, int head_dim, int dtype,
+                        float scale, hipStream_t stream) {
+  const char* fn = "mhc_packed_attn_fwd";
+  mhc::PackedAttnArgs a = packed_args(q, q_stride_t, q_stride_h, k, k_stride_t, k_stride_h, v, v_stride_t, v_stride_h,
+                                      cu_q, cu_k, key_lengths, B, Tq, Tk, heads, kv_heads, head_dim, dtype, scale);
+  if (int rc = check_packed(a, Tq, Tk, dtype, fn)) return rc;
+  if (Tq == 0) return 0;
+  for (const void* p : {q, (const void*)out, Tk ? k : q, Tk ? v : q})
+    if (!p || !aligned16(p)) return fail(hipErrorInvalidValue, "%s: null or unaligned pointer", fn);
+  if (!cu_q || !cu_k) return fail(hipErrorInvalidValue, "%s: the sequences' bounds are required", fn);
+  mhc::packed_attn_plan(a);
+  const int64_t need = mhc::packed_attn_workspace(a);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(hipErrorInvalidValue, "%s: workspace of %lld bytes needed (got %lld)", fn, (long long)need, (long long)workspace_bytes);
+  a.out = out; a.lse = lse; a.work = static_cast<float*>(workspace);
+  return hip_status(mhc::launch_packed_attn(a, stream), fn);
+}
+
+int mhc_packed_attn_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+                        int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
+                        int64_t v_stride_h, const int* cu_q, const int* cu_k, const int* key_lengths,
+                        const void* out, const float* lse, const void* g_out, float* delta, void* g_q,
+                        void* g_k, void* g_v, int B, int64_t Tq, int64_t Tk, int heads, int kv_heads,
+                        int head_dim, int dtype, float scale, hipStream_t stream) {
+  const char* fn = "mhc_packed_attn_bwd";
+  mhc::PackedAttnArgs a = packed_args(q, q_stride_t, q_stride_h, k, k_stride_t, k_stride_h, v, v_stride_t, v_stride_h,
+                                      cu_q, cu_k, key_lengths, B, Tq, Tk, heads, kv_heads, head_dim, dtype, scale);
+  if (int rc = check_packed(a, Tq, Tk, dtype, fn)) return rc;
+  if (Tq == 0 && Tk == 0) return 0;
+  if (Tq > 0)
+    for (const void* p : {q, out, g_out, (const void*)g_q})
+      if (!p || !aligned16(p)) return fail(hipErrorInvalidValue, "%s: null or unaligned pointer", fn);
+  if (Tk > 0)
+    for (const void* p : {k, v, (const void*)g_k, (const void*)g_v})
+      if (!p || !aligned16(p)) return fail(hipErrorInvalidValue, "%s: null or unaligned pointer", fn);
+  if (!cu_q || !cu_k) return fail(hipErrorInvalidValue, "%s: the sequences' bounds are required", fn);
+  if (Tq > 0 && (!lse || !delta)) return fail(hipErrorInvalidValue, "%s: lse and delta are required", fn);
+  a.out = const_cast<void*>(out); a.lse = const_cast<float*>(lse); a.g_out = g_out; a.delta = delta;
+  a.g_q = g_q; a.g_k = g_k; a.g_v = g_v;
+  return hip_status(mhc::launch_packed_attn_bwd(a, stream), fn);
+}
+
 // ------------------------------------------- routed-expert layer (inference)
 
 int64_t mhc_moe_workspace_bytes(int64_t M, int hidden, int inter, int experts, int topk) {

@@ -290,6 +290,40 @@ struct AttnPrefillArgs {
 };
 hipError_t launch_attn_prefill(const AttnPrefillArgs& a, hipStream_t s);
 
+// Causal attention over packed sequences (16-bit tensors, head_dim 64, 96 or 128).  q
+// [Tq, heads, head_dim], k, v [Tk, kv_heads, head_dim] with the given element strides of a
+// row and of a head; cu_q, cu_k [B + 1] the sequences' first rows (and the last one's end),
+// k_len [B] the keys in use of each (null: all); out, g_out, g_q, g_k, g_v contiguous; lse
+// [heads, Tq], log2 of the sums of exponentials (forward: null where no gradient follows).
+struct PackedAttnArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  const int* cu_q;
+  const int* cu_k;
+  const int* k_len;
+  void* out;
+  float* lse;
+  float* work;
+  int64_t qs_t, qs_h, ks_t, ks_h, vs_t, vs_h;
+  int B, Tq, Tk, heads, kv_heads, head_dim;
+  bool f16;
+  float scale;
+  // packed_attn_plan: whether rows are few, heads a workgroup takes, tile numbers, ranges of the keys
+  bool few;
+  int row_heads, qtiles, splits;
+  // backward
+  const void* g_out;
+  float* delta;  // [heads, Tq]
+  void* g_q;
+  void* g_k;
+  void* g_v;
+};
+void packed_attn_plan(PackedAttnArgs& a);
+int64_t packed_attn_workspace(const PackedAttnArgs& a);
+hipError_t launch_packed_attn(const PackedAttnArgs& a, hipStream_t s);
+hipError_t launch_packed_attn_bwd(const PackedAttnArgs& a, hipStream_t s);
+
 // Routed-expert SwiGLU layer (inference, 16-bit tensors).  x, out [M, hidden];
 // probs [M, experts] (the router's softmax); gate_w / up_w [inter, hidden] and
 // down_w [hidden, inter] per expert.  hidden and inter are multiples of 32.

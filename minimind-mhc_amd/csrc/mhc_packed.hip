@@ -1,0 +1,496 @@
+// Causal attention over packed sequences: forward.  q [Tq, heads, HD], k and v
+// [Tk, kv_heads, HD] hold the sequences one after another (k and v perhaps in cache slots
+// that are only partly used); the last query of a sequence sits at its last key.  16-bit
+// tensors (bf16 or fp16), fp32 scores, sums and outputs, one rounding of the probabilities
+// (they are a product's operand) and one of the output.
+//   S_ij = scale q_i . k_j (j <= i + keys - queries),  O_i = sum_j softmax(S_i)_j v_j
+#include "mhc_packed.hpp"
+
+namespace mhc {
+namespace {
+
+// ------------------------------------------------------------- tiles of many queries
+// One 4-wave workgroup per (tile of 128 query rows of one kv head, range of the keys): HP
+// query heads times 128 / HP positions, 32 rows a wave.
+template <bool F16, int HD, int HP>
+__global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedAttnArgs a) {
+  constexpr int NC = HD / 32, ND = HD / 16, KT = 64;
+  constexpr int PW = 128 / HP;
+  constexpr int KST = HD + 8, VST = HD + 16;
+  constexpr int PPT = KT * (HD / 8) / 256;  // 16-byte pieces a thread moves per tile
+  __shared__ __align__(16) uint16_t ks[2][KT * KST];
+  __shared__ __align__(16) uint16_t vs[2][KT * VST];
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int r = lane & 15, g = lane >> 4;
+  const int groups = a.heads / HP;
+  const int grp = blockIdx.x % groups;
+  const int rest = blockIdx.x / groups;
+  const int split = rest % a.splits;
+  const PackedTile t = packed_tile(a.cu_q, a.B, a.Tq, PW, a.qtiles - 1 - rest / a.splits);
+  if (t.first >= t.end) return;
+  const PackedKeys kk = packed_keys(a.cu_k, a.k_len, a.B, a.Tk, t.seq);
+  const int h = grp * HP + (HP == 2 ? wave >> 1 : 0);
+  const int kvh = grp * HP / (a.heads / a.kv_heads);
+  const int pb = t.first + (HP == 2 ? (wave & 1) * 32 : wave * 32);  // the wave's first row
+  const int shift = kk.len - t.end;       // row x sees the keys up to x + shift
+  const int last = min(t.first + PW, t.end) - 1 + shift;  // last key any row of the tile sees
+  // this workgroup's range of the tile's keys, in whole key tiles
+  const int nt_all = last < 0 ? 0 : last / KT + 1;
+  const int per = (nt_all + a.splits - 1) / a.splits;
+  const int t0 = split * per, t1 = min(t0 + per, nt_all);
+
+  const int64_t ks_t = a.ks_t, vs_t = a.vs_t;
+  const uint16_t* kg = static_cast<const uint16_t*>(a.k) + kk.start * ks_t + kvh * a.ks_h;
+  const uint16_t* vg = static_cast<const uint16_t*>(a.v) + kk.start * vs_t + kvh * a.vs_h;
+  U32x4 kr[PPT], vr[PPT];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int p = 0; p < PPT; ++p) {
+      const int piece = p * 256 + tid;
+      const int row = min(s0 + piece / (HD / 8), kk.len - 1);
+      const int col = (piece % (HD / 8)) * 8;
+      kr[p] = ld16(kg + row * ks_t + col);
+      vr[p] = ld16(vg + row * vs_t + col);
+    }
+  };
+  auto stash = [&](int buf, int s0) {
+#pragma unroll
+    for (int p = 0; p < PPT; ++p) {
+      const int piece = p * 256 + tid;
+      const int row = piece / (HD / 8);
+      const int col = (piece % (HD / 8)) * 8;
+      *reinterpret_cast<U32x4*>(&ks[buf][row * KST + col]) = kr[p];
+      *reinterpret_cast<U32x4*>(&vs[buf][row * VST + col]) = vr[p];
+    }
+    // rows that are not there: probability 0 times what the clamped load found would be
+    // NaN for an infinity
+    if (s0 + KT > kk.len)
+#pragma unroll
+      for (int p = 0; p < PPT; ++p) {
+        const int piece = p * 256 + tid;
+        const int row = piece / (HD / 8);
+        if (s0 + row >= kk.len) *reinterpret_cast<U32x4*>(&vs[buf][row * VST + (piece % (HD / 8)) * 8]) = U32x4{};
+      }
+  };
+  if (t0 < t1) load(t0 * KT);
+  U32x4 qb[2][NC];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int64_t row = min(pb + u * 16 + r, t.end - 1);
+    const uint16_t* q = static_cast<const uint16_t*>(a.q) + row * a.qs_t + h * a.qs_h + 8 * g;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) qb[u][c] = ld16(q + 32 * c);
+  }
+  const float scale = a.scale * kPackedLog2e;
+  constexpr float kHead = packed_head<F16>;
+  float m[2] = {kNoScore, kNoScore}, l[2] = {0.f, 0.f};
+  f32x4_t o[2][ND];
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[u][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  for (int kt = t0; kt < t1; ++kt) {
+    const int buf = (kt - t0) & 1;
+    const int s0 = kt * KT;
+    stash(buf, s0);
+    __syncthreads();
+    if (kt + 1 < t1) load(s0 + KT);
+    if (pb >= t.end || s0 > pb + 31 + shift) continue;  // no rows, or wholly above their diagonal
+    f32x4_t s[2][4];
+#pragma unroll
+    for (int st = 0; st < 4; ++st) {
+      s[0][st] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      s[1][st] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const U32x4 ka = *reinterpret_cast<const U32x4*>(&ks[buf][(st * 16 + r) * KST + 32 * c + 8 * g]);
+        s[0][st] = mfma16<F16>(ka, qb[0][c], s[0][st]);
+        s[1][st] = mfma16<F16>(ka, qb[1][c], s[1][st]);
+      }
+    }
+    if (s0 + KT - 1 > pb + shift) {  // uniform: only the tiles on the diagonal are compared
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (s0 + st * 16 + 4 * g + i > pb + u * 16 + r + shift) s[u][st][i] = -__builtin_inff();
+    }
+    U32x4 pf[2][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      float mx = -__builtin_inff();
+#pragma unroll
+      for (int st = 0; st < 4; ++st)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[u][st][i]);
+      mx *= scale;
+      if (__any(!(mx <= m[u] + kPackedLazyMax + kHead))) {
+        mx = fmaxf(mx, xor_lane16(mx));
+        mx = fmaxf(mx, xor_lane32(mx));
+        mx = fmaxf(mx - kHead, m[u]);
+        const float f = exp2_f(m[u] - mx);
+        m[u] = mx;
+        l[u] *= f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[u][d][i] *= f;
+      }
+      float sum = 0.f;
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[i] = exp2_f(fmaf(s[u][st][i], scale, -m[u]));
+          sum += p[i];
+        }
+        pf[u][st >> 1].v[2 * (st & 1)] = pack2<F16>(p[0], p[1]);
+        pf[u][st >> 1].v[2 * (st & 1) + 1] = pack2<F16>(p[2], p[3]);
+      }
+      l[u] += sum;
+    }
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        U32x4 va;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const u32x2_v w = lds_tr4(&vs[buf][(hh * 32 + q * 16 + 4 * g + (r >> 2)) * VST + 16 * d + 4 * (r & 3)]);
+          va.v[2 * q] = w.x;
+          va.v[2 * q + 1] = w.y;
+        }
+        o[0][d] = mfma16<F16>(va, pf[0][hh], o[0][d]);
+        o[1][d] = mfma16<F16>(va, pf[1][hh], o[1][d]);
+      }
+  }
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    float ls = l[u];
+    ls += xor_lane16(ls);
+    ls += xor_lane32(ls);
+    const int row = pb + u * 16 + r;
+    if (row >= t.end) continue;
+    const int64_t at = (int64_t)row * a.heads + h;
+    if (a.splits > 1) {
+      const int64_t part = (int64_t)split * a.Tq * a.heads + at;
+      float* w = a.work + part * HD + 4 * g;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4_t*>(w + 16 * d) = o[u][d];
+      if (g == 0) {
+        float* ml = a.work + (int64_t)a.splits * a.Tq * a.heads * HD + 2 * part;
+        ml[0] = m[u];
+        ml[1] = ls;
+      }
+      continue;
+    }
+    const float inv = ls > 0.f || ls != ls ? 1.f / ls : 0.f;  // a row without keys: zeros
+    uint16_t* out = static_cast<uint16_t*>(a.out) + at * HD + 4 * g;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      uint2 w;
+      w.x = pack2<F16>(o[u][d][0] * inv, o[u][d][1] * inv);
+      w.y = pack2<F16>(o[u][d][2] * inv, o[u][d][3] * inv);
+      *reinterpret_cast<uint2*>(out + 16 * d) = w;
+    }
+    if (a.lse && g == 0) a.lse[(int64_t)h * a.Tq + row] = packed_lse(m[u], ls);
+  }
+}
+
+// --------------------------------------------------------------- few queries, many keys
+// A workgroup takes up to 16 rows (tokens times query heads of one kv head) and a range of
+// the keys; its four waves take the range's 64-key tiles in turn, each with sums and LDS of
+// its own, and join at the end.
+template <bool F16, int HD>
+__global__ __launch_bounds__(256) void packed_few_kernel(PackedAttnArgs a) {
+  constexpr int NC = HD / 32, ND = HD / 16, KT = 32;
+  constexpr int KST = HD + 8, VST = HD + 16;
+  constexpr int PPT = KT * (HD / 8) / 64;
+  constexpr int WAVE_LDS = KT * (KST + VST);  // elements
+  static_assert(WAVE_LDS * 2 >= (16 * HD + 32) * 4, "the waves' sums take the tiles' place");
+  __shared__ __align__(16) uint16_t lds[4][WAVE_LDS];
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int r = lane & 15, g = lane >> 4;
+  const int rep = a.heads / a.kv_heads;
+  const int HB = a.row_heads, nb = (rep + HB - 1) / HB;  // heads of a workgroup, workgroups of a kv head
+  const int RT = 16 / HB;
+  const int groups = a.kv_heads * nb;
+  const int grp = blockIdx.x % groups;
+  const int rest = blockIdx.x / groups;
+  const int split = rest % a.splits;
+  const PackedTile t = packed_tile(a.cu_q, a.B, a.Tq, RT, rest / a.splits);
+  if (t.first >= t.end) return;
+  const PackedKeys kk = packed_keys(a.cu_k, a.k_len, a.B, a.Tk, t.seq);
+  const int kvh = grp / nb;
+  const int hr = grp % nb * HB + r % HB;  // the lane's head in its group
+  const int row = t.first + r / HB;
+  const bool live = r < RT * HB && hr < rep && row < t.end;
+  const int h = kvh * rep + (live ? hr : 0);
+  const int shift = kk.len - t.end;
+  const int last = min(t.first + RT, t.end) - 1 + shift;
+  const int nt_all = last < 0 ? 0 : last / KT + 1;
+  const int per = (nt_all + a.splits - 1) / a.splits;
+  const int t0 = split * per, t1 = min(t0 + per, nt_all);
+
+  const int64_t ks_t = a.ks_t, vs_t = a.vs_t;
+  const uint16_t* kg = static_cast<const uint16_t*>(a.k) + kk.start * ks_t + kvh * a.ks_h;
+  const uint16_t* vg = static_cast<const uint16_t*>(a.v) + kk.start * vs_t + kvh * a.vs_h;
+  uint16_t* ks = lds[wave];
+  uint16_t* vs = ks + KT * KST;
+  U32x4 kr[PPT], vr[PPT];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int p = 0; p < PPT; ++p) {
+      const int piece = p * 64 + lane;
+      const int at = min(s0 + piece / (HD / 8), kk.len - 1);
+      const int col = (piece % (HD / 8)) * 8;
+      kr[p] = ld16_nt(kg + at * ks_t + col);
+      vr[p] = ld16_nt(vg + at * vs_t + col);
+    }
+  };
+  if (t0 + wave < t1) load((t0 + wave) * KT);
+  U32x4 qb[NC];
+  {
+    const uint16_t* q = static_cast<const uint16_t*>(a.q) + (int64_t)(live ? row : t.first) * a.qs_t + h * a.qs_h + 8 * g;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) qb[c] = ld16(q + 32 * c);
+  }
+  const float scale = a.scale * kPackedLog2e;
+  constexpr float kHead = packed_head<F16>;
+  const int limit = live ? row + shift : -1;  // last key the lane's row sees
+  float m = kNoScore, l = 0.f;
+  f32x4_t o[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) o[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int kt = t0 + wave; kt < t1; kt += 4) {
+    const int s0 = kt * KT;
+#pragma unroll
+    for (int p = 0; p < PPT; ++p) {
+      const int piece = p * 64 + lane;
+      const int at = piece / (HD / 8);
+      const int col = (piece % (HD / 8)) * 8;
+      *reinterpret_cast<U32x4*>(&ks[at * KST + col]) = kr[p];
+      *reinterpret_cast<U32x4*>(&vs[at * VST + col]) = vr[p];
+    }
+    if (s0 + KT > kk.len)  // rows that are not there: 0 x infinity would be NaN
+#pragma unroll
+      for (int p = 0; p < PPT; ++p) {
+        const int piece = p * 64 + lane;
+        const int at = piece / (HD / 8);
+        if (s0 + at >= kk.len) *reinterpret_cast<U32x4*>(&vs[at * VST + (piece % (HD / 8)) * 8]) = U32x4{};
+      }
+    if (kt + 4 < t1) load(s0 + 4 * KT);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    f32x4_t s[2];
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      s[st] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        s[st] = mfma16<F16>(*reinterpret_cast<const U32x4*>(&ks[(st * 16 + r) * KST + 32 * c + 8 * g]), qb[c], s[st]);
+    }
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (s0 + st * 16 + 4 * g + i > limit) s[st][i] = -__builtin_inff();
+    float mx = -__builtin_inff();
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[st][i]);
+    mx *= scale;
+    if (__any(!(mx <= m + kPackedLazyMax + kHead))) {
+      mx = fmaxf(mx, xor_lane16(mx));
+      mx = fmaxf(mx, xor_lane32(mx));
+      mx = fmaxf(mx - kHead, m);
+      const float f = exp2_f(m - mx);
+      m = mx;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[d][i] *= f;
+    }
+    U32x4 pf;
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      float p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[i] = exp2_f(fmaf(s[st][i], scale, -m));
+        l += p[i];
+      }
+      pf.v[2 * st] = pack2<F16>(p[0], p[1]);
+      pf.v[2 * st + 1] = pack2<F16>(p[2], p[3]);
+    }
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      U32x4 va;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const u32x2_v w = lds_tr4(&vs[(q * 16 + 4 * g + (r >> 2)) * VST + 16 * d + 4 * (r & 3)]);
+        va.v[2 * q] = w.x;
+        va.v[2 * q + 1] = w.y;
+      }
+      o[d] = mfma16<F16>(va, pf, o[d]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  l += xor_lane16(l);
+  l += xor_lane32(l);
+  // the waves' sums meet in LDS: [16 rows][HD] and then each row's maximum and sum
+  __syncthreads();
+  float* mine = reinterpret_cast<float*>(lds[wave]);
+#pragma unroll
+  for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4_t*>(mine + r * HD + 16 * d + 4 * g) = o[d];
+  if (g == 0) {
+    mine[16 * HD + r] = m;
+    mine[16 * HD + 16 + r] = l;
+  }
+  __syncthreads();
+  // thread (row of 16, 1/16 of the columns)
+  const int tr = tid >> 4, tc = tid & 15;
+  const int ohr = grp % nb * HB + tr % HB, orow = t.first + tr / HB;
+  if (tr >= RT * HB || ohr >= rep || orow >= t.end) return;
+  float mx = kNoScore, ls = 0.f, f[4];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) mx = fmaxf(mx, reinterpret_cast<const float*>(lds[w])[16 * HD + tr]);
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float* p = reinterpret_cast<const float*>(lds[w]);
+    f[w] = exp2_f(p[16 * HD + tr] - mx);
+    ls += f[w] * p[16 * HD + 16 + tr];
+  }
+  const int oh = kvh * rep + ohr;
+  const int64_t at = (int64_t)orow * a.heads + oh;
+  const int64_t part = (int64_t)split * a.Tq * a.heads + at;
+  const float inv = a.splits > 1 ? 1.f : ls > 0.f || ls != ls ? 1.f / ls : 0.f;
+#pragma unroll
+  for (int c = 2 * tc; c < HD; c += 32) {
+    float x = 0.f, y = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float* p = reinterpret_cast<const float*>(lds[w]) + tr * HD + c;
+      x += f[w] * p[0];
+      y += f[w] * p[1];
+    }
+    if (a.splits > 1)
+      *reinterpret_cast<float2*>(a.work + part * HD + c) = make_float2(x, y);
+    else
+      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at * HD + c) = pack2<F16>(x * inv, y * inv);
+  }
+  if (tc != 0) return;
+  if (a.splits > 1) {
+    float* ml = a.work + (int64_t)a.splits * a.Tq * a.heads * HD + 2 * part;
+    ml[0] = mx;
+    ml[1] = ls;
+  } else if (a.lse) {
+    a.lse[(int64_t)oh * a.Tq + orow] = packed_lse(mx, ls);
+  }
+}
+
+// Joins the key ranges of one row and head: a wave a row, HD / 4 lanes four columns each,
+// the other lane groups every second (fourth) range.
+template <bool F16, int HD>
+__global__ __launch_bounds__(256) void packed_merge_kernel(PackedAttnArgs a) {
+  constexpr int LPR = HD <= 64 ? 16 : 32;
+  constexpr int PAR = 64 / LPR;
+  const int64_t rows = (int64_t)a.Tq * a.heads;
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= rows) return;
+  const int lane = threadIdx.x & 63, col = lane % LPR, sub = lane / LPR;
+  const bool live = col < HD / 4;
+  const float* part = a.work + at * HD + (live ? 4 * col : 0);
+  const float* ml = a.work + (int64_t)a.splits * rows * HD + 2 * at;
+  float mx = kNoScore;
+  for (int s = lane; s < a.splits; s += 64) mx = fmaxf(mx, ml[2 * s * rows]);
+  mx = wave_max(mx);
+  float l = 0.f;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  for (int s = sub; s < a.splits; s += PAR) {
+    const float ls = ml[2 * s * rows + 1];
+    if (ls == 0.f) continue;  // a range without keys
+    const float f = exp2_f(ml[2 * s * rows] - mx);
+    l += f * ls;
+    const f32x4_t v = *reinterpret_cast<const f32x4_t*>(part + s * rows * HD);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += f * v[e];
+  }
+  if constexpr (PAR == 4) {
+    l += xor_lane16(l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += xor_lane16(o[e]);
+  }
+  l += xor_lane32(l);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] += xor_lane32(o[e]);
+  if (sub != 0 || !live) return;
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  uint2 w;
+  w.x = pack2<F16>(o[0] * inv, o[1] * inv);
+  w.y = pack2<F16>(o[2] * inv, o[3] * inv);
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at * HD + 4 * col) = w;
+  if (a.lse && col == 0) a.lse[at % a.heads * a.Tq + at / a.heads] = packed_lse(mx, l);
+}
+
+template <bool F16, int HD>
+hipError_t packed_fwd_hd(const PackedAttnArgs& a, hipStream_t s) {
+  if (a.few) {
+    const int nb = (a.heads / a.kv_heads + a.row_heads - 1) / a.row_heads;
+    packed_few_kernel<F16, HD><<<dim3((unsigned)((int64_t)a.qtiles * a.splits * a.kv_heads * nb)), 256, 0, s>>>(a);
+  } else if (a.row_heads == 2) {
+    packed_fwd_kernel<F16, HD, 2><<<dim3((unsigned)((int64_t)a.qtiles * a.splits * (a.heads / 2))), 256, 0, s>>>(a);
+  } else {
+    packed_fwd_kernel<F16, HD, 1><<<dim3((unsigned)((int64_t)a.qtiles * a.splits * a.heads)), 256, 0, s>>>(a);
+  }
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  if (a.splits > 1)
+    packed_merge_kernel<F16, HD><<<dim3((unsigned)(((int64_t)a.Tq * a.heads + 3) / 4)), 256, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+// Which kernel, how many heads a workgroup takes and into how many ranges the keys go.
+// Only the totals are known here; the sequences' own lengths are read on the device.
+void packed_attn_plan(PackedAttnArgs& a) {
+  const int rep = a.heads / a.kv_heads;
+  const int B = a.B > 0 ? a.B : 1;
+  a.few = (int64_t)a.Tq * rep <= 16 * (int64_t)B;
+  int64_t units;
+  int tile;
+  if (a.few) {
+    const int nb = (rep + 15) / 16;
+    a.row_heads = (rep + nb - 1) / nb;
+    a.qtiles = (int)packed_tiles(a.Tq, a.B, 16 / a.row_heads);
+    const int64_t full = (a.Tq + 16 / a.row_heads - 1) / (16 / a.row_heads);  // tiles with rows, about
+    units = (full < B ? full : B) * a.kv_heads * nb;
+    tile = 128;
+  } else {
+    a.row_heads = rep % 2 == 0 ? 2 : 1;
+    a.qtiles = (int)packed_tiles(a.Tq, a.B, 128 / a.row_heads);
+    units = ((int64_t)a.Tq * a.row_heads / 128 + 1) * (a.heads / a.row_heads);
+    tile = 256;
+  }
+  const int64_t keys = a.Tk / B;  // of a sequence, on average
+  int64_t want = units > 0 ? (int64_t)device_cus() * (a.few ? 4 : 2) / units : 1;
+  if (want > keys / tile) want = keys / tile;
+  if (want > 128) want = 128;
+  a.splits = want < 1 ? 1 : (int)want;
+}
+int64_t packed_attn_workspace(const PackedAttnArgs& a) {
+  return a.splits > 1 ? (int64_t)a.splits * a.Tq * a.heads * (a.head_dim + 2) * 4 : 0;
+}
+
+hipError_t launch_packed_attn(const PackedAttnArgs& a, hipStream_t s) { MHC_PACKED_HD(packed_fwd_hd, a, s) }
+
+}  // namespace mhc

@@ -7,6 +7,7 @@ current stream.  Inputs are made contiguous, as the reference's Functions do
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import threading
@@ -661,6 +662,22 @@ def on_current_device(t: torch.Tensor) -> bool:
     return t.get_device() == _current_device()
 
 
+_HERE = contextlib.nullcontext()
+
+
+def launch_device(t: torch.Tensor):
+    """A context in which the library's launches go to the GPU that t lies on."""
+    return _HERE if on_current_device(t) else torch.cuda.device(t.device)
+
+
+def wants_graph(*ts: torch.Tensor) -> bool:
+    """Whether a call on these tensors has to go through its autograd Function: one of them
+    wants a gradient, or a forward-mode level is on (which the Function refuses)."""
+    if not torch.is_grad_enabled():
+        return CAN_TELL and forward_ad._current_level >= 0
+    return not CAN_TELL or forward_ad._current_level >= 0 or any(t.requires_grad for t in ts)
+
+
 def _function_modes() -> bool:
     """Whether one of the torch-function modes on the stack could see or replace the torch
     ops.  The one that torch.set_default_device and `with torch.device(...)` leave there
@@ -714,7 +731,7 @@ def _linear_pays(M: int, K: int, ns: tuple, glu: bool = False) -> bool:
     return bool(H.load().mhc_linear_pays((ctypes.c_int * len(ns))(*ns), len(ns), M, K, int(glu)))
 
 
-_HALF = (torch.bfloat16, torch.float16)
+_HALF = HALF = (torch.bfloat16, torch.float16)
 
 
 def _linear_weights(x: torch.Tensor, mods, glu: bool = False, closely: bool = True):
