@@ -584,6 +584,55 @@ int mhc_packed_attn_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, c
                         void* g_k, void* g_v, int B, int64_t Tq, int64_t Tk, int heads, int kv_heads,
                         int head_dim, int dtype, float scale, hipStream_t stream);
 
+/* ------------------------------------------------------------------- losses
+ * Logits and scores are fp32, bf16 or fp16; sums and log-probabilities fp32 or
+ * wider.  Row strides are in elements; rows may begin at any element.
+ */
+
+/* logprobs [T] fp32: log softmax(logits row)[label], 0 where labels[t] (int64)
+ * is `ignore`, NaN for another label outside [0, V).  lse (NULL, or [T, 2]
+ * fp32): a row's maximum and the base-2 logarithm of its sum of exponentials
+ * below that, for the backward entry points. */
+int mhc_logprobs_fwd(const void* logits, int64_t stride, int dtype, const int64_t* labels, int64_t ignore,
+                     float* logprobs, float* lse, int64_t T, int V, hipStream_t stream);
+
+/* g_logits [T, V] (contiguous) = g [T] times d logprobs / d logits. */
+int mhc_logprobs_bwd(const void* logits, int64_t stride, int dtype, const int64_t* labels, int64_t ignore,
+                     const float* lse, const float* g, void* g_logits, int64_t T, int V,
+                     hipStream_t stream);
+
+/* Preference loss of P pairs of packed sequences (chosen 0 .. P - 1, rejected
+ * P .. 2 P - 1; cu [2 P + 1] int32, sequence i the rows cu[i] .. cu[i + 1], the
+ * first entry taken as 0): with S the sums of a sequence's logprobs (average:
+ * their means over the counted labels), rewards beta (S - reference) and z
+ * the chosen reward less the rejected one, loss (one element) = the mean of
+ * -((1 - smoothing) log sigmoid(z) + smoothing log sigmoid(-z)).  g_seq [2 P]:
+ * the loss's derivative by each logprob of a sequence.  scratch: 8 P bytes, 8-byte
+ * aligned. */
+int mhc_preference_fwd(const float* logprobs, const int64_t* labels, int64_t ignore, const int* cu,
+                       const float* reference, float* loss, float* chosen, float* rejected,
+                       float* g_seq, void* scratch, int64_t T, int P, double beta,
+                       double smoothing, int average, hipStream_t stream);
+
+/* g_logits [T, V] for g_loss (one element); rows of no sequence get zeros. */
+int mhc_preference_bwd(const void* logits, int64_t stride, int dtype, const int64_t* labels,
+                       int64_t ignore, const float* lse, const int* cu, const float* g_seq,
+                       const float* g_loss, void* g_logits, int64_t T, int V, int P,
+                       hipStream_t stream);
+
+/* Balance loss of a router over T tokens, E <= 4096 experts: scores [T, E],
+ * index [T, K] (int64, contiguous) the experts of each token (others than 0 .. E -
+ * 1 are not counted).  loss (one element) = coef E sum_e (count_e / T) mean_e.  cu (NULL, or
+ * [B + 1]): the mean of the losses of B sequences, over those with rows.  counts [B, E]
+ * int64 (B = 1 without cu); filled: one int, the sequences with rows. */
+int64_t mhc_balance_workspace_bytes(int64_t T, int E, int B);
+int mhc_balance_fwd(const void* scores, int64_t stride, int dtype, const int64_t* index, const int* cu,
+                    float* loss, int64_t* counts, int* filled, void* workspace, int64_t workspace_bytes,
+                    int64_t T, int E, int K, int B, double coef, hipStream_t stream);
+/* g_scores [T, E] (contiguous, in dtype) for g_loss (one element). */
+int mhc_balance_bwd(const int* cu, const int64_t* counts, const int* filled, const float* g_loss,
+                    void* g_scores, int dtype, int64_t T, int E, int B, double coef, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

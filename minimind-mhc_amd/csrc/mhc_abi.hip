@@ -816,6 +816,122 @@ int mhc_packed_attn_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, c
   return hip_status(mhc::launch_packed_attn_bwd(a, stream), fn);
 }
 
+// ------------------------------------------------------------------- losses
+
+static int check_logits(const void* logits, int64_t stride, int dtype, const int64_t* labels, int64_t T, int V,
+                        const char* fn) {
+  if (T < 0 || T > 1 << 30 || V < 1 || stride < 0)
+    return fail(hipErrorInvalidValue, "%s: bad shape (T=%lld V=%d stride=%lld)", fn, (long long)T, V, (long long)stride);
+  if (!dtype_ok(dtype)) return fail(hipErrorInvalidValue, "%s: bad dtype %d", fn, dtype);
+  if (T > 0 && (!logits || !labels || reinterpret_cast<uintptr_t>(logits) % mhc::dtype_bytes(dtype)))
+    return fail(hipErrorInvalidValue, "%s: null or unaligned pointer", fn);
+  return 0;
+}
+
+int mhc_logprobs_fwd(const void* logits, int64_t stride, int dtype, const int64_t* labels, int64_t ignore,
+                     float* logprobs, float* lse, int64_t T, int V, hipStream_t stream) {
+  const char* fn = "mhc_logprobs_fwd";
+  if (int rc = check_logits(logits, stride, dtype, labels, T, V, fn)) return rc;
+  if (T == 0) return 0;
+  if (!logprobs) return fail(hipErrorInvalidValue, "%s: null pointer", fn);
+  mhc::LogitArgs a{};
+  a.logits = logits; a.stride = stride; a.dtype = dtype; a.labels = labels; a.ignore = ignore;
+  a.logprobs = logprobs; a.lse = lse; a.T = T; a.V = V;
+  return hip_status(mhc::launch_logprobs(a, stream), fn);
+}
+
+int mhc_logprobs_bwd(const void* logits, int64_t stride, int dtype, const int64_t* labels, int64_t ignore,
+                     const float* lse, const float* g, void* g_logits, int64_t T, int V, hipStream_t stream) {
+  const char* fn = "mhc_logprobs_bwd";
+  if (int rc = check_logits(logits, stride, dtype, labels, T, V, fn)) return rc;
+  if (T == 0) return 0;
+  if (!lse || !g || !g_logits) return fail(hipErrorInvalidValue, "%s: null pointer", fn);
+  mhc::LogitArgs a{};
+  a.logits = logits; a.stride = stride; a.dtype = dtype; a.labels = labels; a.ignore = ignore;
+  a.lse = const_cast<float*>(lse); a.g_row = g; a.g_logits = g_logits; a.T = T; a.V = V;
+  return hip_status(mhc::launch_logprobs_bwd(a, stream), fn);
+}
+
+int mhc_preference_fwd(const float* logprobs, const int64_t* labels, int64_t ignore, const int* cu,
+                       const float* reference, float* loss, float* chosen, float* rejected,
+                       float* g_seq, void* scratch, int64_t T, int P, double beta,
+                       double smoothing, int average, hipStream_t stream) {
+  const char* fn = "mhc_preference_fwd";
+  if (T < 0 || T > 1 << 30 || P < 1 || P > 1 << 29)
+    return fail(hipErrorInvalidValue, "%s: bad shape (T=%lld pairs=%d)", fn, (long long)T, P);
+  if ((T > 0 && (!logprobs || !labels)) || !cu || !reference || !loss || !chosen || !rejected || !g_seq || !scratch ||
+      reinterpret_cast<uintptr_t>(scratch) % 8)
+    return fail(hipErrorInvalidValue, "%s: null or unaligned pointer", fn);
+  mhc::PreferenceArgs a{};
+  a.logprobs = logprobs; a.labels = labels; a.ignore = ignore; a.cu = cu; a.reference = reference;
+  a.loss = loss; a.chosen = chosen; a.rejected = rejected; a.g_seq = g_seq;
+  a.pair_loss = static_cast<double*>(scratch);
+  a.T = (int)T; a.P = P; a.beta = beta; a.smoothing = smoothing; a.average = average != 0;
+  return hip_status(mhc::launch_preference(a, stream), fn);
+}
+
+int mhc_preference_bwd(const void* logits, int64_t stride, int dtype, const int64_t* labels,
+                       int64_t ignore, const float* lse, const int* cu, const float* g_seq,
+                       const float* g_loss, void* g_logits, int64_t T, int V, int P, hipStream_t stream) {
+  const char* fn = "mhc_preference_bwd";
+  if (int rc = check_logits(logits, stride, dtype, labels, T, V, fn)) return rc;
+  if (P < 1 || P > 1 << 29) return fail(hipErrorInvalidValue, "%s: bad shape (pairs=%d)", fn, P);
+  if (T == 0) return 0;
+  if (!lse || !cu || !g_seq || !g_loss || !g_logits) return fail(hipErrorInvalidValue, "%s: null pointer", fn);
+  mhc::LogitArgs a{};
+  a.logits = logits; a.stride = stride; a.dtype = dtype; a.labels = labels; a.ignore = ignore;
+  a.lse = const_cast<float*>(lse); a.cu = cu; a.B = 2 * P; a.g_seq = g_seq; a.g_loss = g_loss;
+  a.g_logits = g_logits; a.T = T; a.V = V;
+  return hip_status(mhc::launch_logprobs_bwd(a, stream), fn);
+}
+
+static int check_balance(int64_t T, int E, int B, const char* fn) {
+  if (T < 0 || T > 1 << 30 || E < 1 || E > mhc::kBalanceMaxExperts || B < 0 || (int64_t)B * E > kMaxBlocks ||
+      T * E / 256 >= kMaxBlocks)
+    return fail(hipErrorInvalidValue, "%s: bad shape (T=%lld E=%d B=%d)", fn, (long long)T, E, B);
+  return 0;
+}
+
+int64_t mhc_balance_workspace_bytes(int64_t T, int E, int B) {
+  if (check_balance(T, E, B, "mhc_balance_workspace_bytes")) return -1;
+  return (int64_t)B * mhc::balance_parts(T, B) * E * 8;
+}
+
+int mhc_balance_fwd(const void* scores, int64_t stride, int dtype, const int64_t* index, const int* cu,
+                    float* loss, int64_t* counts, int* filled, void* workspace, int64_t workspace_bytes,
+                    int64_t T, int E, int K, int B, double coef, hipStream_t stream) {
+  const char* fn = "mhc_balance_fwd";
+  if (int rc = check_balance(T, E, B, fn)) return rc;
+  if (!dtype_ok(dtype)) return fail(hipErrorInvalidValue, "%s: bad dtype %d", fn, dtype);
+  if (K < 1 || stride < 0 || (!cu && B != 1)) return fail(hipErrorInvalidValue, "%s: bad shape (K=%d stride=%lld B=%d)", fn, K, (long long)stride, B);
+  if ((T > 0 && (!scores || !index)) || !loss || !filled || (B > 0 && !counts))
+    return fail(hipErrorInvalidValue, "%s: null pointer", fn);
+  const int64_t need = mhc_balance_workspace_bytes(T, E, B);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(hipErrorInvalidValue, "%s: workspace of %lld bytes needed (got %lld)", fn, (long long)need, (long long)workspace_bytes);
+  mhc::BalanceArgs a{};
+  a.scores = scores; a.stride = stride; a.dtype = dtype; a.index = index; a.cu = cu;
+  a.loss = loss; a.counts = counts; a.filled = filled;
+  a.T = (int)T; a.E = E; a.K = K; a.B = B; a.coef = coef; a.parts = mhc::balance_parts(T, B);
+  a.part_sum = static_cast<float*>(workspace);
+  a.part_count = reinterpret_cast<int*>(a.part_sum + (int64_t)B * a.parts * E);
+  return hip_status(mhc::launch_balance(a, stream), fn);
+}
+
+int mhc_balance_bwd(const int* cu, const int64_t* counts, const int* filled, const float* g_loss,
+                    void* g_scores, int dtype, int64_t T, int E, int B, double coef, hipStream_t stream) {
+  const char* fn = "mhc_balance_bwd";
+  if (int rc = check_balance(T, E, B, fn)) return rc;
+  if (!dtype_ok(dtype)) return fail(hipErrorInvalidValue, "%s: bad dtype %d", fn, dtype);
+  if (!cu && B != 1) return fail(hipErrorInvalidValue, "%s: bad shape (B=%d)", fn, B);
+  if (T == 0) return 0;
+  if (!counts || !filled || !g_loss || !g_scores) return fail(hipErrorInvalidValue, "%s: null pointer", fn);
+  mhc::BalanceArgs a{};
+  a.cu = cu; a.counts = const_cast<int64_t*>(counts); a.filled = const_cast<int*>(filled); a.g_loss = g_loss;
+  a.g_scores = g_scores; a.dtype = dtype; a.T = (int)T; a.E = E; a.B = B; a.coef = coef;
+  return hip_status(mhc::launch_balance_bwd(a, stream), fn);
+}
+
 // ------------------------------------------- routed-expert layer (inference)
 
 int64_t mhc_moe_workspace_bytes(int64_t M, int hidden, int inter, int experts, int topk) {

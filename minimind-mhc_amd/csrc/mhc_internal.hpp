@@ -324,6 +324,63 @@ int64_t packed_attn_workspace(const PackedAttnArgs& a);
 hipError_t launch_packed_attn(const PackedAttnArgs& a, hipStream_t s);
 hipError_t launch_packed_attn_bwd(const PackedAttnArgs& a, hipStream_t s);
 
+// Log-probabilities of labels under rows of logits [T, V] (rows `stride` elements apart).
+struct LogitArgs {
+  const void* logits;
+  const int64_t* labels;  // [T]
+  float* logprobs;        // [T], 0 where the label is `ignore`
+  float* lse;             // [T, 2]: a row's maximum and log2 of its sum of exponentials (or null)
+  // backward: the rows' factors, or (cu set) those of the sequences a row is of
+  void* g_logits;         // [T, V]
+  const float* g_row;     // [T]
+  const int* cu;          // [B + 1]
+  const float* g_seq;     // [B]
+  const float* g_loss;    // one element, times g_seq
+  int64_t stride, T, ignore;
+  int V, B, dtype;
+};
+hipError_t launch_logprobs(const LogitArgs& a, hipStream_t s);
+hipError_t launch_logprobs_bwd(const LogitArgs& a, hipStream_t s);
+
+// Preference loss of P pairs: sequences 0 .. P - 1 are chosen, P .. 2 P - 1 rejected.
+struct PreferenceArgs {
+  const float* logprobs;   // [T]
+  const int64_t* labels;   // [T]
+  const int* cu;           // [2 P + 1]
+  const float* reference;  // [2 P]
+  double* pair_loss;       // [P] scratch
+  float* loss;             // one element
+  float* chosen;           // [P] rewards
+  float* rejected;
+  float* g_seq;            // [2 P] d loss / d lp of a sequence's rows
+  int64_t ignore;
+  int T, P;
+  bool average;
+  double beta, smoothing;
+};
+hipError_t launch_preference(const PreferenceArgs& a, hipStream_t s);
+
+// Balance loss of a router: scores [T, E] (rows `stride` elements apart), index [T, K].
+constexpr int kBalanceMaxExperts = 4096;
+struct BalanceArgs {
+  const void* scores;
+  const int64_t* index;
+  const int* cu;        // [B + 1], or null: one sequence of all rows
+  float* loss;          // one element
+  int* filled;          // one element: sequences with rows
+  int64_t* counts;      // [B, E]
+  float* part_sum;      // [B, parts, E] scratch
+  int* part_count;
+  void* g_scores;       // backward: [T, E]
+  const float* g_loss;  // one element
+  int64_t stride;
+  int T, E, K, B, parts, dtype;
+  double coef;
+};
+int balance_parts(int64_t T, int B);
+hipError_t launch_balance(const BalanceArgs& a, hipStream_t s);
+hipError_t launch_balance_bwd(const BalanceArgs& a, hipStream_t s);
+
 // Routed-expert SwiGLU layer (inference, 16-bit tensors).  x, out [M, hidden];
 // probs [M, experts] (the router's softmax); gate_w / up_w [inter, hidden] and
 // down_w [hidden, inter] per expert.  hidden and inter are multiples of 32.

@@ -27,6 +27,7 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _I64 = ctypes.c_int64
 _F = ctypes.c_float
+_D = ctypes.c_double
 
 # name -> (restype, argtypes); mirrors include/mhc_amd.h
 _SIGNATURES = {
@@ -119,6 +120,17 @@ _SIGNATURES = {
                                  _P, _P, _P, _P, _P, _P, _P,      # cu_q, cu_k, key_lengths, out, lse, g_out, delta
                                  _P, _P, _P,                      # g_q, g_k, g_v
                                  _I, _I64, _I64, _I, _I, _I, _I, _F, _P]),
+    "mhc_logprobs_fwd": (_I, [_P, _I64, _I, _P, _I64, _P, _P, _I64, _I, _P]),
+    "mhc_logprobs_bwd": (_I, [_P, _I64, _I, _P, _I64, _P, _P, _P, _I64, _I, _P]),
+    "mhc_preference_fwd": (_I, [_P, _P, _I64, _P, _P,             # logprobs, labels, ignore, cu, reference
+                                _P, _P, _P, _P, _P,               # loss, chosen, rejected, g_seq, scratch
+                                _I64, _I, _D, _D, _I, _P]),
+    "mhc_preference_bwd": (_I, [_P, _I64, _I, _P, _I64, _P, _P, _P, _P, _P, _I64, _I, _I, _P]),
+    "mhc_balance_workspace_bytes": (_I64, [_I64, _I, _I]),
+    "mhc_balance_fwd": (_I, [_P, _I64, _I, _P, _P,                # scores, stride, dtype, index, cu
+                             _P, _P, _P, _P, _I64,                # loss, counts, filled, workspace, bytes
+                             _I64, _I, _I, _I, _D, _P]),
+    "mhc_balance_bwd": (_I, [_P, _P, _P, _P, _P, _I, _I64, _I, _I, _D, _P]),
 }
 
 ABI_VERSION = 8

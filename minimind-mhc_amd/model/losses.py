@@ -1,0 +1,239 @@
+"""Losses of language models on HIP kernels: log-probabilities of labels, the preference
+loss of pairs of answers, and the balance loss of a router.
+
+The reference forms them with chains of torch ops (trainer/train_dpo.py,
+model/model_minimind.py:290-297 and :421-425).
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _hip as H
+from . import _ops
+from .packed import _bounds
+
+IGNORE_INDEX = -100
+
+
+def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
+    """t [..., V] as rows one stride apart, its last dimension in order."""
+    if t.dim() < 1 or t.shape[-1] < 1:
+        raise ValueError(f"mhc_amd: {name} must be [..., n] with n >= 1, got {tuple(t.shape)}")
+    H.dtype_tag(t)
+    try:
+        t = t.view(-1, t.shape[-1]) if t.dim() != 2 else t
+    except RuntimeError:  # rows that no one stride joins
+        t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _labels(labels: torch.Tensor, logits: torch.Tensor) -> torch.Tensor:
+    if labels.dtype != torch.int64:
+        raise TypeError(f"mhc_amd: labels must be int64, got {labels.dtype}")
+    if labels.shape != logits.shape[:-1]:
+        raise ValueError(f"mhc_amd: labels {tuple(labels.shape)} do not belong to logits "
+                         f"{tuple(logits.shape)}")
+    return labels.reshape(-1).contiguous()
+
+
+def _scalar(g: torch.Tensor) -> torch.Tensor:
+    return g.to(torch.float32).contiguous()
+
+
+def _stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _logprobs(x, labels, ignore, want_lse):
+    T, V = x.shape
+    lp = torch.empty(T, dtype=torch.float32, device=x.device)
+    lse = torch.empty((T, 2), dtype=torch.float32, device=x.device) if want_lse else None
+    with _ops.launch_device(x):
+        H.check(H.load().mhc_logprobs_fwd(x.data_ptr(), _stride(x), H.dtype_tag(x), labels.data_ptr(),
+                                          ignore, lp.data_ptr(), H.ptr(lse), T, V, H.stream(x.device)),
+                "mhc_logprobs_fwd")
+    return lp, lse
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, labels, ignore):
+        lp, lse = _logprobs(x, labels, ignore, True)
+        ctx.save_for_backward(x, labels, lse)
+        ctx.ignore = ignore
+        return lp
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, labels, lse = ctx.saved_tensors
+        T, V = x.shape
+        g = g.to(torch.float32).contiguous()
+        out = torch.empty((T, V), dtype=x.dtype, device=x.device)
+        with _ops.launch_device(x):
+            H.check(H.load().mhc_logprobs_bwd(
+                x.data_ptr(), _stride(x), H.dtype_tag(x), labels.data_ptr(), ctx.ignore, lse.data_ptr(),
+                g.data_ptr(), out.data_ptr(), T, V, H.stream(x.device)), "mhc_logprobs_bwd")
+        return out, None, None
+
+
+def token_logprobs(logits: torch.Tensor, labels: torch.Tensor,
+                   ignore_index: int = IGNORE_INDEX) -> torch.Tensor:
+    """log softmax(logits)[label] of each row, fp32, in labels' shape.
+
+    logits [..., V] fp32, bf16 or fp16 (rows any stride apart); labels [...] int64.  A row
+    whose label is ignore_index gets 0 (and no gradient, and is not read); a label outside
+    [0, V) otherwise gives NaN.  Differentiable once in logits; the gradient has logits' type.
+    """
+    H.require_device(logits, labels)
+    x, y = _rows(logits, "logits"), _labels(labels, logits)
+    if _ops.wants_graph(logits):
+        lp = _TokenLogprobs.apply(x, y, int(ignore_index))
+    else:
+        lp = _logprobs(x, y, int(ignore_index), False)[0]
+    return lp.view(labels.shape)
+
+
+class _PreferenceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, labels, cu, reference, beta, smoothing, average, ignore, graph):
+        lp, lse = _logprobs(x, labels, ignore, graph)
+        T, P = x.shape[0], reference.numel() // 2
+        new = torch.empty
+        loss = new((), dtype=torch.float32, device=x.device)
+        rewards = new((2, P), dtype=torch.float32, device=x.device)
+        g_seq = new(2 * P, dtype=torch.float32, device=x.device)
+        scratch = new(P, dtype=torch.float64, device=x.device)
+        with _ops.launch_device(x):
+            H.check(H.load().mhc_preference_fwd(
+                lp.data_ptr(), labels.data_ptr(), ignore, cu.data_ptr(), reference.data_ptr(),
+                loss.data_ptr(), rewards[0].data_ptr(), rewards[1].data_ptr(), g_seq.data_ptr(),
+                scratch.data_ptr(), T, P, beta, smoothing, int(average), H.stream(x.device)),
+                "mhc_preference_fwd")
+        chosen, rejected = rewards.unbind(0)
+        if graph:
+            ctx.save_for_backward(x, labels, cu, lse, g_seq)
+            ctx.ignore = ignore
+            ctx.mark_non_differentiable(chosen, rejected)
+            ctx.set_materialize_grads(False)
+        return loss, chosen, rejected
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, *_):
+        if g is None:
+            return (None,) * 9
+        x, labels, cu, lse, g_seq = ctx.saved_tensors
+        T, V = x.shape
+        g = _scalar(g)
+        out = torch.empty((T, V), dtype=x.dtype, device=x.device)
+        with _ops.launch_device(x):
+            H.check(H.load().mhc_preference_bwd(
+                x.data_ptr(), _stride(x), H.dtype_tag(x), labels.data_ptr(), ctx.ignore, lse.data_ptr(),
+                cu.data_ptr(), g_seq.data_ptr(), g.data_ptr(), out.data_ptr(), T, V, g_seq.numel() // 2,
+                H.stream(x.device)), "mhc_preference_bwd")
+        return (out,) + (None,) * 8
+
+
+def preference_loss(logits: torch.Tensor, labels: torch.Tensor, cu_seqlens: torch.Tensor,
+                    reference: torch.Tensor, beta: float = 0.1, label_smoothing: float = 0.0,
+                    average: bool = False, ignore_index: int = IGNORE_INDEX):
+    """(loss, chosen rewards [n], rejected rewards [n]) of n pairs of packed answers, fp32.
+
+    logits [rows, V] fp32, bf16 or fp16; labels [rows] int64, ignore_index where a row does
+    not count (a prompt).  cu_seqlens [2 n + 1] int32: the first n sequences are the chosen
+    answers, the last n the rejected ones, in the same order; sequence i has the rows
+    cu_seqlens[i] to cu_seqlens[i + 1], beginning with row 0, and rows behind the last count
+    for nothing.  reference [2 n]: the reference model's sums (average: means) of the
+    sequences' token_logprobs.
+
+    With S a sequence's sum (mean over its counted rows) of token_logprobs, its reward is
+    beta (S - reference); with z the chosen reward less the rejected one, the loss is the
+    mean over the pairs of -((1 - e) log sigmoid(z) + e log sigmoid(-z)), e = label_smoothing.
+    The sums are taken in 64 bits.  The loss is differentiable once, in logits; the rewards
+    carry no gradient.
+    """
+    dev = H.require_device(logits, labels, reference)
+    if logits.dim() != 2:
+        raise ValueError(f"mhc_amd: logits must be [rows, V], got {tuple(logits.shape)}")
+    x, y = _rows(logits, "logits"), _labels(labels, logits)
+    if reference.dim() != 1 or reference.numel() < 2 or reference.numel() % 2:
+        raise ValueError(f"mhc_amd: reference must hold two values a pair, got {tuple(reference.shape)}")
+    if not 0.0 <= label_smoothing < 1.0:
+        raise ValueError(f"mhc_amd: label_smoothing must be in [0, 1), got {label_smoothing}")
+    cu = _bounds("cu_seqlens", cu_seqlens, reference.numel() + 1, dev)
+    ref = reference.detach().to(torch.float32).contiguous()
+    args = (x, y, cu, ref, float(beta), float(label_smoothing), bool(average), int(ignore_index))
+    if _ops.wants_graph(logits):
+        return _PreferenceLoss.apply(*args, True)
+    return _PreferenceLoss.forward(None, *args, False)
+
+
+class _BalanceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, scores, index, cu, coef):
+        T, E = scores.shape
+        B = 1 if cu is None else cu.numel() - 1
+        dev, new, lib = scores.device, torch.empty, H.load()
+        loss = new((), dtype=torch.float32, device=dev)
+        counts = new((B, E), dtype=torch.int64, device=dev)
+        filled = new((), dtype=torch.int32, device=dev)
+        with _ops.launch_device(scores):
+            nbytes = lib.mhc_balance_workspace_bytes(T, E, B)
+            ws = new(max(nbytes, 0), dtype=torch.uint8, device=dev)
+            H.check(lib.mhc_balance_fwd(
+                scores.data_ptr(), _stride(scores), H.dtype_tag(scores), index.data_ptr(), H.ptr(cu),
+                loss.data_ptr(), counts.data_ptr(), filled.data_ptr(), ws.data_ptr(), max(nbytes, 0),
+                T, E, index.shape[1], B, coef, H.stream(dev)), "mhc_balance_fwd")
+        if ctx is not None:
+            ctx.save_for_backward(cu, counts, filled)
+            ctx.shape, ctx.dtype, ctx.coef = (T, E), scores.dtype, coef
+            ctx.mark_non_differentiable(counts)
+            ctx.set_materialize_grads(False)
+        return loss, counts
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, *_):
+        if g is None:
+            return (None,) * 4
+        cu, counts, filled = ctx.saved_tensors
+        (T, E), g = ctx.shape, _scalar(g)
+        out = torch.empty((T, E), dtype=ctx.dtype, device=counts.device)
+        with _ops.launch_device(counts):
+            H.check(H.load().mhc_balance_bwd(
+                H.ptr(cu), counts.data_ptr(), filled.data_ptr(), g.data_ptr(), out.data_ptr(),
+                H.dtype_tag(out), T, E, counts.shape[0], ctx.coef, H.stream(counts.device)),
+                "mhc_balance_bwd")
+        return out, None, None, None
+
+
+def balance_loss(scores: torch.Tensor, index: torch.Tensor, coef: float,
+                 cu_seqlens: Optional[torch.Tensor] = None):
+    """(loss, counts) of a router: coef E sum_e f_e P_e over E experts, f_e the times expert e
+    was taken divided by the number of tokens, P_e its mean score.
+
+    scores [..., E] fp32, bf16 or fp16, the router's probabilities; index [..., k] int64, the
+    experts each token went to.  counts [E] int64: how often each was taken.  loss: fp32,
+    differentiable once, in scores (counts are constants).
+    cu_seqlens [n + 1] int32: the mean over the sequences (rows cu_seqlens[i] to
+    cu_seqlens[i + 1], beginning with row 0) of each one's own loss instead, and counts
+    [n, E].  Sequences without rows do not enter the mean; rows behind the last are
+    in none.  Without any row the loss is 0.
+    """
+    dev = H.require_device(scores, index)
+    x = _rows(scores, "scores")
+    if index.dtype != torch.int64:
+        raise TypeError(f"mhc_amd: index must be int64, got {index.dtype}")
+    if index.dim() != scores.dim() or index.shape[:-1] != scores.shape[:-1] or index.shape[-1] < 1:
+        raise ValueError(f"mhc_amd: index {tuple(index.shape)} does not belong to scores {tuple(scores.shape)}")
+    idx = index.reshape(-1, index.shape[-1]).contiguous()
+    cu = None if cu_seqlens is None else _bounds("cu_seqlens", cu_seqlens, None, dev)
+    if _ops.wants_graph(scores):
+        loss, counts = _BalanceLoss.apply(x, idx, cu, float(coef))
+    else:
+        loss, counts = _BalanceLoss.forward(None, x, idx, cu, float(coef))
+    return loss, counts if cu is not None else counts[0]
