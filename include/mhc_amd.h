@@ -564,23 +564,24 @@ int64_t mhc_packed_attn_workspace_bytes(int B, int64_t Tq, int64_t Tk, int heads
                                         int head_dim);
 
 /* out [Tq, heads, head_dim] (contiguous) = softmax(scale q k^T) v, scale > 0.
- * lse (NULL, or [heads, Tq] fp32): the base-2 logarithms of the softmax's sums,
- * for mhc_packed_attn_bwd. */
+ * For mhc_packed_attn_bwd (both or neither): lse [heads, Tq] fp32, the base-2
+ * logarithms of the softmax's sums, and rest, shaped and typed as out, what
+ * rounding took from out. */
 int mhc_packed_attn_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
                         int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
                         int64_t v_stride_h, const int* cu_q, const int* cu_k, const int* key_lengths,
-                        void* out, float* lse, void* workspace, int64_t workspace_bytes, int B,
+                        void* out, void* rest, float* lse, void* workspace, int64_t workspace_bytes, int B,
                         int64_t Tq, int64_t Tk, int heads, int kv_heads, int head_dim, int dtype,
                         float scale, hipStream_t stream);
 
 /* Gradients g_q [Tq, heads, head_dim], g_k and g_v [Tk, kv_heads, head_dim]
- * (contiguous; every row is written) for g_out, contiguous as out.  out and lse
+ * (contiguous; every row is written) for g_out, contiguous as out.  out, rest and lse
  * are the forward's; delta [heads, Tq] fp32 is scratch.  No atomics: the same bits on every
  * run. */
 int mhc_packed_attn_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
                         int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
                         int64_t v_stride_h, const int* cu_q, const int* cu_k, const int* key_lengths,
-                        const void* out, const float* lse, const void* g_out, float* delta, void* g_q,
+                        const void* out, const void* rest, const float* lse, const void* g_out, float* delta, void* g_q,
                         void* g_k, void* g_v, int B, int64_t Tq, int64_t Tk, int heads, int kv_heads,
                         int head_dim, int dtype, float scale, hipStream_t stream);
 

@@ -773,7 +773,7 @@ int64_t mhc_packed_attn_workspace_bytes(int B, int64_t Tq, int64_t Tk, int heads
 int mhc_packed_attn_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
                         int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
                         int64_t v_stride_h, const int* cu_q, const int* cu_k, const int* key_lengths,
-                        void* out, float* lse, void* workspace, int64_t workspace_bytes, int B,
+                        void* out, void* rest, float* lse, void* workspace, int64_t workspace_bytes, int B,
                         int64_t Tq, int64_t Tk, int heads, int kv_heads, int head_dim, int dtype,
                         float scale, hipStream_t stream) {
   const char* fn = "mhc_packed_attn_fwd";
@@ -784,18 +784,19 @@ int mhc_packed_attn_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, c
   for (const void* p : {q, (const void*)out, Tk ? k : q, Tk ? v : q})
     if (!p || !aligned16(p)) return fail(hipErrorInvalidValue, "%s: null or unaligned pointer", fn);
   if (!cu_q || !cu_k) return fail(hipErrorInvalidValue, "%s: the sequences' bounds are required", fn);
+  if (!rest != !lse || !aligned16(rest)) return fail(hipErrorInvalidValue, "%s: rest and lse are both given, 16-byte aligned, or neither", fn);
   mhc::packed_attn_plan(a);
   const int64_t need = mhc::packed_attn_workspace(a);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(hipErrorInvalidValue, "%s: workspace of %lld bytes needed (got %lld)", fn, (long long)need, (long long)workspace_bytes);
-  a.out = out; a.lse = lse; a.work = static_cast<float*>(workspace);
+  a.out = out; a.rest = rest; a.lse = lse; a.work = static_cast<float*>(workspace);
   return hip_status(mhc::launch_packed_attn(a, stream), fn);
 }
 
 int mhc_packed_attn_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
                         int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
                         int64_t v_stride_h, const int* cu_q, const int* cu_k, const int* key_lengths,
-                        const void* out, const float* lse, const void* g_out, float* delta, void* g_q,
+                        const void* out, const void* rest, const float* lse, const void* g_out, float* delta, void* g_q,
                         void* g_k, void* g_v, int B, int64_t Tq, int64_t Tk, int heads, int kv_heads,
                         int head_dim, int dtype, float scale, hipStream_t stream) {
   const char* fn = "mhc_packed_attn_bwd";
@@ -804,14 +805,14 @@ int mhc_packed_attn_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, c
   if (int rc = check_packed(a, Tq, Tk, dtype, fn)) return rc;
   if (Tq == 0 && Tk == 0) return 0;
   if (Tq > 0)
-    for (const void* p : {q, out, g_out, (const void*)g_q})
+    for (const void* p : {q, out, rest, g_out, (const void*)g_q})
       if (!p || !aligned16(p)) return fail(hipErrorInvalidValue, "%s: null or unaligned pointer", fn);
   if (Tk > 0)
     for (const void* p : {k, v, (const void*)g_k, (const void*)g_v})
       if (!p || !aligned16(p)) return fail(hipErrorInvalidValue, "%s: null or unaligned pointer", fn);
   if (!cu_q || !cu_k) return fail(hipErrorInvalidValue, "%s: the sequences' bounds are required", fn);
   if (Tq > 0 && (!lse || !delta)) return fail(hipErrorInvalidValue, "%s: lse and delta are required", fn);
-  a.out = const_cast<void*>(out); a.lse = const_cast<float*>(lse); a.g_out = g_out; a.delta = delta;
+  a.out = const_cast<void*>(out); a.rest = const_cast<void*>(rest); a.lse = const_cast<float*>(lse); a.g_out = g_out; a.delta = delta;
   a.g_q = g_q; a.g_k = g_k; a.g_v = g_v;
   return hip_status(mhc::launch_packed_attn_bwd(a, stream), fn);
 }

@@ -294,7 +294,8 @@ hipError_t launch_attn_prefill(const AttnPrefillArgs& a, hipStream_t s);
 // [Tq, heads, head_dim], k, v [Tk, kv_heads, head_dim] with the given element strides of a
 // row and of a head; cu_q, cu_k [B + 1] the sequences' first rows (and the last one's end),
 // k_len [B] the keys in use of each (null: all); out, g_out, g_q, g_k, g_v contiguous; lse
-// [heads, Tq], log2 of the sums of exponentials (forward: null where no gradient follows).
+// [heads, Tq], log2 of the sums of exponentials, and rest, shaped as out, what rounding took
+// from out (forward: null where no gradient follows).
 struct PackedAttnArgs {
   const void* q;
   const void* k;
@@ -303,6 +304,7 @@ struct PackedAttnArgs {
   const int* cu_k;
   const int* k_len;
   void* out;
+  void* rest;
   float* lse;
   float* work;
   int64_t qs_t, qs_h, ks_t, ks_h, vs_t, vs_h;

@@ -193,10 +193,11 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedAttnArgs a) {
     uint16_t* out = static_cast<uint16_t*>(a.out) + at * HD + 4 * g;
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
-      uint2 w;
-      w.x = pack2<F16>(o[u][d][0] * inv, o[u][d][1] * inv);
-      w.y = pack2<F16>(o[u][d][2] * inv, o[u][d][3] * inv);
+      uint2 w, x;
+      w.x = round2<F16>(o[u][d][0] * inv, o[u][d][1] * inv, a.rest ? &x.x : nullptr);
+      w.y = round2<F16>(o[u][d][2] * inv, o[u][d][3] * inv, a.rest ? &x.y : nullptr);
       *reinterpret_cast<uint2*>(out + 16 * d) = w;
+      if (a.rest) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.rest) + at * HD + 4 * g + 16 * d) = x;
     }
     if (a.lse && g == 0) a.lse[(int64_t)h * a.Tq + row] = packed_lse(m[u], ls);
   }
@@ -383,10 +384,14 @@ __global__ __launch_bounds__(256) void packed_few_kernel(PackedAttnArgs a) {
       x += f[w] * p[0];
       y += f[w] * p[1];
     }
-    if (a.splits > 1)
+    if (a.splits > 1) {
       *reinterpret_cast<float2*>(a.work + part * HD + c) = make_float2(x, y);
-    else
-      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at * HD + c) = pack2<F16>(x * inv, y * inv);
+      continue;
+    }
+    uint32_t rest;
+    *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at * HD + c) =
+        round2<F16>(x * inv, y * inv, a.rest ? &rest : nullptr);
+    if (a.rest) *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.rest) + at * HD + c) = rest;
   }
   if (tc != 0) return;
   if (a.splits > 1) {
@@ -435,10 +440,11 @@ __global__ __launch_bounds__(256) void packed_merge_kernel(PackedAttnArgs a) {
   for (int e = 0; e < 4; ++e) o[e] += xor_lane32(o[e]);
   if (sub != 0 || !live) return;
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-  uint2 w;
-  w.x = pack2<F16>(o[0] * inv, o[1] * inv);
-  w.y = pack2<F16>(o[2] * inv, o[3] * inv);
+  uint2 w, x;
+  w.x = round2<F16>(o[0] * inv, o[1] * inv, a.rest ? &x.x : nullptr);
+  w.y = round2<F16>(o[2] * inv, o[3] * inv, a.rest ? &x.y : nullptr);
   *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at * HD + 4 * col) = w;
+  if (a.rest) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.rest) + at * HD + 4 * col) = x;
   if (a.lse && col == 0) a.lse[at % a.heads * a.Tq + at / a.heads] = packed_lse(mx, l);
 }
 

@@ -35,6 +35,16 @@ __device__ __forceinline__ int seq_start(const int* cu, int i, int T) {
 __device__ __forceinline__ float packed_lse(float m, float l) {
   return l == 0.f ? __builtin_inff() : m + __builtin_amdgcn_logf(l);
 }
+// Two outputs, rounded once, and (rest set, where a backward pass follows) what the rounding
+// took from them: D = G . O is formed from both.  With the rounded output alone the error of
+// D, the same for all keys of a row, was most of the error of dQ and dK (2.2e-3 of their
+// size at short lengths, one rounding being 1.7e-3).
+template <bool F16>
+__device__ __forceinline__ uint32_t round2(float a, float b, uint32_t* rest) {
+  const uint32_t w = pack2<F16>(a, b);
+  if (rest) *rest = pack2<F16>(a - elem_lo<F16>(w), b - elem_hi<F16>(w));
+  return w;
+}
 __device__ __forceinline__ float wave_max(float v) {
   v = fmaxf(v, dpp_f<kDppXor1>(v));
   v = fmaxf(v, dpp_f<kDppXor2>(v));

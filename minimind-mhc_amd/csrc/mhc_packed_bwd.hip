@@ -61,16 +61,17 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
     const int64_t off = (at * a.heads + h) * HD + 8 * g;
     const uint16_t* go = static_cast<const uint16_t*>(a.g_out) + off;
     const uint16_t* oo = static_cast<const uint16_t*>(a.out) + off;
+    const uint16_t* ro = static_cast<const uint16_t*>(a.rest) + off;
     float d = 0.f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       qb[u][c] = ld16(q + 32 * c);
       gb[u][c] = ld16(go + 32 * c);
-      const U32x4 o = ld16(oo + 32 * c);
+      const U32x4 o = ld16(oo + 32 * c), rest = ld16(ro + 32 * c);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        d += elem_lo<F16>(gb[u][c].v[j]) * elem_lo<F16>(o.v[j]);
-        d += elem_hi<F16>(gb[u][c].v[j]) * elem_hi<F16>(o.v[j]);
+        d += elem_lo<F16>(gb[u][c].v[j]) * (elem_lo<F16>(o.v[j]) + elem_lo<F16>(rest.v[j]));
+        d += elem_hi<F16>(gb[u][c].v[j]) * (elem_hi<F16>(o.v[j]) + elem_hi<F16>(rest.v[j]));
       }
     }
     d += xor_lane16(d);

@@ -55,35 +55,36 @@ def _dims(q, k, v):
     return Tq, heads, hd, Tk, kv
 
 
-def _forward(q, k, v, cu_q, cu_k, used, scale, want_lse):
+def _forward(q, k, v, cu_q, cu_k, used, scale, graph):
     (q, *qs), (k, *ks), (v, *vs) = _strided(q), _strided(k), _strided(v)
     Tq, heads, hd = q.shape
     Tk, kv, B = k.shape[0], k.shape[1], cu_q.numel() - 1
     dev, lib = q.device, H.load()
     out = torch.empty((Tq, heads, hd), dtype=q.dtype, device=dev)
-    lse = torch.empty((heads, Tq), dtype=torch.float32, device=dev) if want_lse else None
+    rest = torch.empty_like(out) if graph else None
+    lse = torch.empty((heads, Tq), dtype=torch.float32, device=dev) if graph else None
     with _ops.launch_device(q):
         nbytes = lib.mhc_packed_attn_workspace_bytes(B, Tq, Tk, heads, kv, hd)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
         H.check(lib.mhc_packed_attn_fwd(
             q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs, cu_q.data_ptr(), cu_k.data_ptr(),
-            H.ptr(used), out.data_ptr(), H.ptr(lse), H.ptr(ws), max(nbytes, 0), B, Tq, Tk, heads, kv,
-            hd, H.dtype_tag(q), scale, H.stream(dev)), "mhc_packed_attn_fwd")
-    return out, lse
+            H.ptr(used), out.data_ptr(), H.ptr(rest), H.ptr(lse), H.ptr(ws), max(nbytes, 0), B, Tq, Tk,
+            heads, kv, hd, H.dtype_tag(q), scale, H.stream(dev)), "mhc_packed_attn_fwd")
+    return out, rest, lse
 
 
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, used, scale):
-        out, lse = _forward(q, k, v, cu_q, cu_k, used, scale, True)
-        ctx.save_for_backward(q, k, v, cu_q, cu_k, used, out, lse)
+        out, rest, lse = _forward(q, k, v, cu_q, cu_k, used, scale, True)
+        ctx.save_for_backward(q, k, v, cu_q, cu_k, used, out, rest, lse)
         ctx.scale = scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        q, k, v, cu_q, cu_k, used, out, lse = ctx.saved_tensors
+        q, k, v, cu_q, cu_k, used, out, rest, lse = ctx.saved_tensors
         (q, *qs), (k, *ks), (v, *vs) = _strided(q), _strided(k), _strided(v)
         g = g.to(out.dtype).contiguous()
         if g.data_ptr() % 16:  # a caller's view; the kernels load 16 bytes
@@ -97,7 +98,7 @@ class _PackedAttention(torch.autograd.Function):
         with _ops.launch_device(q):
             H.check(H.load().mhc_packed_attn_bwd(
                 q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs, cu_q.data_ptr(),
-                cu_k.data_ptr(), H.ptr(used), out.data_ptr(), lse.data_ptr(), g.data_ptr(),
+                cu_k.data_ptr(), H.ptr(used), out.data_ptr(), rest.data_ptr(), lse.data_ptr(), g.data_ptr(),
                 delta.data_ptr(), g_q.data_ptr(), g_k.data_ptr(), g_v.data_ptr(), cu_q.numel() - 1,
                 Tq, Tk, heads, kv, hd, H.dtype_tag(q), ctx.scale, H.stream(dev)), "mhc_packed_attn_bwd")
         return g_q, g_k, g_v, None, None, None, None

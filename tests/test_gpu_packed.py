@@ -77,8 +77,8 @@ def _make(dev, dtype, rows, krows, heads, kv, hd, seed=0):
 
 # Roundings, in half steps of the type on the absolute sums.  Output: the probabilities' one
 # (fp32 scores of up to 60 units with 2^-24 relative errors add 2^-17 and less: under half a
-# fp16 step).  Gradients of q and k: dS's one, and D's, which is formed with the rounded
-# output (half a step of |G . O|).  Gradient of v: the probabilities' one.
+# fp16 step).  Gradients of q and k: dS's one, and what the output's two roundings and the
+# probabilities' one leave in D (half a step of |G . O|).  Gradient of v: the probabilities' one.
 OUT, GRAD = 1.5, 2.5
 
 TRAIN = [
