@@ -4,6 +4,7 @@
 // tensors (bf16 or fp16), fp32 scores, sums and outputs, one rounding of the probabilities
 // (they are a product's operand) and one of the output.
 //   S_ij = scale q_i . k_j (j <= i + keys - queries),  O_i = sum_j softmax(S_i)_j v_j
+#include <stdlib.h>
 #include "mhc_packed.hpp"
 
 namespace mhc {
@@ -27,9 +28,10 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedAttnArgs a) {
   const int grp = blockIdx.x % groups;
   const int rest = blockIdx.x / groups;
   const int split = rest % a.splits;
-  const PackedTile t = packed_tile(a.cu_q, a.B, a.Tq, PW, a.qtiles - 1 - rest / a.splits);
+  PackedTile t;
+  PackedKeys kk;
+  packed_find(a.cu_q, a.B, a.Tq, PW, a.qtiles - 1 - rest / a.splits, a.cu_k, a.Tk, nullptr, a.k_len, t, kk);
   if (t.first >= t.end) return;
-  const PackedKeys kk = packed_keys(a.cu_k, a.k_len, a.B, a.Tk, t.seq);
   const int h = grp * HP + (HP == 2 ? wave >> 1 : 0);
   const int kvh = grp * HP / (a.heads / a.kv_heads);
   const int pb = t.first + (HP == 2 ? (wave & 1) * 32 : wave * 32);  // the wave's first row
@@ -222,12 +224,18 @@ __global__ __launch_bounds__(256) void packed_few_kernel(PackedAttnArgs a) {
   const int HB = a.row_heads, nb = (rep + HB - 1) / HB;  // heads of a workgroup, workgroups of a kv head
   const int RT = 16 / HB;
   const int groups = a.kv_heads * nb;
-  const int grp = blockIdx.x % groups;
-  const int rest = blockIdx.x / groups;
+  // the heads of one range go to one XCD, whose L2 then sees whole lines of a key's row:
+  // workgroups are dealt to the 8 XCDs in turn
+  const int block = blockIdx.x / (8 * groups), in = blockIdx.x % (8 * groups);
+  const int grp = in / 8;
+  const int rest = block * 8 + in % 8;
   const int split = rest % a.splits;
-  const PackedTile t = packed_tile(a.cu_q, a.B, a.Tq, RT, rest / a.splits);
+  const int tile = rest / a.splits;
+  if (tile >= a.qtiles) return;
+  PackedTile t;
+  PackedKeys kk;
+  packed_find(a.cu_q, a.B, a.Tq, RT, tile, a.cu_k, a.Tk, nullptr, a.k_len, t, kk);
   if (t.first >= t.end) return;
-  const PackedKeys kk = packed_keys(a.cu_k, a.k_len, a.B, a.Tk, t.seq);
   const int kvh = grp / nb;
   const int hr = grp % nb * HB + r % HB;  // the lane's head in its group
   const int row = t.first + r / HB;
@@ -403,56 +411,64 @@ __global__ __launch_bounds__(256) void packed_few_kernel(PackedAttnArgs a) {
   }
 }
 
-// Joins the key ranges of one row and head: a wave a row, HD / 4 lanes four columns each,
-// the other lane groups every second (fourth) range.
+// Joins the key ranges of one row and head: HD / 4 lanes take four columns each, the other
+// lanes of the workgroup every 8th (16th) range, and the sums meet in LDS.
 template <bool F16, int HD>
 __global__ __launch_bounds__(256) void packed_merge_kernel(PackedAttnArgs a) {
   constexpr int LPR = HD <= 64 ? 16 : 32;
-  constexpr int PAR = 64 / LPR;
+  constexpr int PAR = 256 / LPR;
+  __shared__ __align__(16) float acc[PAR][HD + 4];
   const int64_t rows = (int64_t)a.Tq * a.heads;
-  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (at >= rows) return;
-  const int lane = threadIdx.x & 63, col = lane % LPR, sub = lane / LPR;
+  const int64_t at = blockIdx.x;
+  const int col = threadIdx.x % LPR, sub = threadIdx.x / LPR;
   const bool live = col < HD / 4;
   const float* part = a.work + at * HD + (live ? 4 * col : 0);
-  const float* ml = a.work + (int64_t)a.splits * rows * HD + 2 * at;
-  float mx = kNoScore;
-  for (int s = lane; s < a.splits; s += 64) mx = fmaxf(mx, ml[2 * s * rows]);
-  mx = wave_max(mx);
-  float l = 0.f;
+  const float2* ml = reinterpret_cast<const float2*>(a.work + (int64_t)a.splits * rows * HD) + at;
+  float mx = kNoScore, l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
   for (int s = sub; s < a.splits; s += PAR) {
-    const float ls = ml[2 * s * rows + 1];
-    if (ls == 0.f) continue;  // a range without keys
-    const float f = exp2_f(ml[2 * s * rows] - mx);
-    l += f * ls;
+    const float2 w = ml[s * rows];
     const f32x4_t v = *reinterpret_cast<const f32x4_t*>(part + s * rows * HD);
+    const float mn = fmaxf(mx, w.x);
+    const float f = exp2_f(mx - mn), e = exp2_f(w.x - mn);
+    mx = mn;
+    l = l * f + w.y * e;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] += f * v[e];
+    for (int j = 0; j < 4; ++j) o[j] = o[j] * f + v[j] * e;
   }
-  if constexpr (PAR == 4) {
-    l += xor_lane16(l);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] += xor_lane16(o[e]);
+  if (live) *reinterpret_cast<f32x4_t*>(&acc[sub][4 * col]) = o;
+  if (col == 0) {
+    acc[sub][HD] = mx;
+    acc[sub][HD + 1] = l;
   }
-  l += xor_lane32(l);
+  __syncthreads();
+  if (threadIdx.x >= HD / 2) return;
+  float m = kNoScore, ls = 0.f, x = 0.f, y = 0.f;
+  const int c = 2 * threadIdx.x;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) o[e] += xor_lane32(o[e]);
-  if (sub != 0 || !live) return;
-  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-  uint2 w, x;
-  w.x = round2<F16>(o[0] * inv, o[1] * inv, a.rest ? &x.x : nullptr);
-  w.y = round2<F16>(o[2] * inv, o[3] * inv, a.rest ? &x.y : nullptr);
-  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at * HD + 4 * col) = w;
-  if (a.rest) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.rest) + at * HD + 4 * col) = x;
-  if (a.lse && col == 0) a.lse[at % a.heads * a.Tq + at / a.heads] = packed_lse(mx, l);
+  for (int s = 0; s < PAR; ++s) m = fmaxf(m, acc[s][HD]);
+#pragma unroll
+  for (int s = 0; s < PAR; ++s) {
+    const float f = exp2_f(acc[s][HD] - m);
+    ls += f * acc[s][HD + 1];
+    x += f * acc[s][c];
+    y += f * acc[s][c + 1];
+  }
+  const float inv = ls > 0.f || ls != ls ? 1.f / ls : 0.f;
+  uint32_t rest;
+  *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at * HD + c) =
+      round2<F16>(x * inv, y * inv, a.rest ? &rest : nullptr);
+  if (a.rest) *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.rest) + at * HD + c) = rest;
+  if (a.lse && c == 0) a.lse[at % a.heads * a.Tq + at / a.heads] = packed_lse(m, ls);
 }
 
 template <bool F16, int HD>
 hipError_t packed_fwd_hd(const PackedAttnArgs& a, hipStream_t s) {
   if (a.few) {
     const int nb = (a.heads / a.kv_heads + a.row_heads - 1) / a.row_heads;
-    packed_few_kernel<F16, HD><<<dim3((unsigned)((int64_t)a.qtiles * a.splits * a.kv_heads * nb)), 256, 0, s>>>(a);
+    const int64_t ranges = ((int64_t)a.qtiles * a.splits + 7) / 8 * 8;
+    packed_few_kernel<F16, HD><<<dim3((unsigned)(ranges * a.kv_heads * nb)), 256, 0, s>>>(a);
   } else if (a.row_heads == 2) {
     packed_fwd_kernel<F16, HD, 2><<<dim3((unsigned)((int64_t)a.qtiles * a.splits * (a.heads / 2))), 256, 0, s>>>(a);
   } else {
@@ -460,7 +476,7 @@ hipError_t packed_fwd_hd(const PackedAttnArgs& a, hipStream_t s) {
   }
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   if (a.splits > 1)
-    packed_merge_kernel<F16, HD><<<dim3((unsigned)(((int64_t)a.Tq * a.heads + 3) / 4)), 256, 0, s>>>(a);
+    packed_merge_kernel<F16, HD><<<dim3((unsigned)((int64_t)a.Tq * a.heads)), 256, 0, s>>>(a);
   return hipGetLastError();
 }
 
@@ -479,7 +495,7 @@ void packed_attn_plan(PackedAttnArgs& a) {
     a.row_heads = (rep + nb - 1) / nb;
     a.qtiles = (int)packed_tiles(a.Tq, a.B, 16 / a.row_heads);
     const int64_t full = (a.Tq + 16 / a.row_heads - 1) / (16 / a.row_heads);  // tiles with rows, about
-    units = (full < B ? full : B) * a.kv_heads * nb;
+    units = (full > B ? full : B < a.Tq ? B : a.Tq) * a.kv_heads * nb;
     tile = 128;
   } else {
     a.row_heads = rep % 2 == 0 ? 2 : 1;
@@ -491,6 +507,7 @@ void packed_attn_plan(PackedAttnArgs& a) {
   int64_t want = units > 0 ? (int64_t)device_cus() * (a.few ? 4 : 2) / units : 1;
   if (want > keys / tile) want = keys / tile;
   if (want > 128) want = 128;
+  if (getenv("SPL")) want = atoi(getenv("SPL"));
   a.splits = want < 1 ? 1 : (int)want;
 }
 int64_t packed_attn_workspace(const PackedAttnArgs& a) {

@@ -58,11 +58,20 @@ __device__ __forceinline__ float wave_max(float v) {
 // start(i) / M + i on: enough for its rows wherever it starts, and found without a sum
 // over the sequences before it.  The rows behind the last sequence are one more "sequence"
 // (number B).  Every lane of the wave takes part: 64 bounds are looked at a step.
+// packed_find also gives the sequence's rows in the other tensor (cu_o, To rows); used_t and
+// used_o (or null) say how many of the rows are in use.
 struct PackedTile {
   int seq, first, end;  // sequence, first row of the tile, end of the sequence's rows
   int start;            // first row of the sequence
+  int used;             // its rows in use
 };
-__device__ __forceinline__ PackedTile packed_tile(const int* cu, int B, int T, int M, int tile) {
+// The other tensor's rows of a sequence: first row, how many (of them in use), none for the
+// rows behind the last sequence.
+struct PackedKeys {
+  int start, len;
+};
+__device__ __forceinline__ void packed_find(const int* cu, int B, int T, int M, int tile, const int* cu_o, int To,
+                                            const int* used_t, const int* used_o, PackedTile& t, PackedKeys& o) {
   const int lane = __lane_id();
   int lo = 0, hi = B + 1;
   while (hi - lo > 1) {
@@ -74,29 +83,21 @@ __device__ __forceinline__ PackedTile packed_tile(const int* cu, int B, int T, i
     hi = min(hi, lo + step);
   }
   lo = __builtin_amdgcn_readfirstlane(lo);
-  PackedTile t;
+  // all loads of the sequence's bounds before the first use of one
+  const bool in = lo < B;
+  const int next = in ? lo + 1 : lo, at = in ? lo : 0;
+  const int s0 = cu[lo], s1 = cu[next], o0 = cu_o[lo], o1 = cu_o[next];
+  const int ut = used_t && in ? used_t[at] : 0x7fffffff, uo = used_o && in ? used_o[at] : 0x7fffffff;
   t.seq = lo;
-  t.start = __builtin_amdgcn_readfirstlane(seq_start(cu, lo, T));
-  const int end = lo >= B ? T : seq_start(cu, lo + 1, T);
-  t.end = __builtin_amdgcn_readfirstlane(max(end, t.start));
+  t.start = lo == 0 ? 0 : min(max(s0, 0), T);
+  t.end = max(in ? min(max(s1, 0), T) : T, t.start);
   t.first = t.start + (tile - (t.start / M + lo)) * M;
-  return t;
+  o.start = lo == 0 ? 0 : min(max(o0, 0), To);
+  o.len = in ? min(max(uo, 0), max(min(max(o1, 0), To) - o.start, 0)) : 0;
+  t.used = in ? min(max(ut, 0), t.end - t.start) : 0;
 }
 // Tile numbers of T rows in B sequences.
 inline int64_t packed_tiles(int64_t T, int64_t B, int M) { return T / M + B + 1; }
-
-// The key rows of sequence i: first row and their number (0 for the rows behind the last).
-struct PackedKeys {
-  int start, len, slot;  // slot: rows up to the next sequence's first
-};
-__device__ __forceinline__ PackedKeys packed_keys(const int* cu, const int* used, int B, int T, int i) {
-  PackedKeys k;
-  k.start = __builtin_amdgcn_readfirstlane(seq_start(cu, min(i, B), T));
-  const int end = i >= B ? T : seq_start(cu, i + 1, T);
-  k.slot = __builtin_amdgcn_readfirstlane(max(end - k.start, 0));
-  k.len = i >= B ? 0 : used ? __builtin_amdgcn_readfirstlane(min(max(used[i], 0), k.slot)) : k.slot;
-  return k;
-}
 
 // The transposing LDS load: the 16 lanes of a group point at 4 rows x 16 columns, four
 // columns a lane (lane r at row r / 4, column 4 (r % 4)), and lane r gets column r.

@@ -26,9 +26,10 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
   const int r = lane & 15, g = lane >> 4;
   const int groups = a.heads / HP;
   const int grp = blockIdx.x % groups;
-  const PackedTile t = packed_tile(a.cu_q, a.B, a.Tq, PW, a.qtiles - 1 - blockIdx.x / groups);
+  PackedTile t;
+  PackedKeys kk;
+  packed_find(a.cu_q, a.B, a.Tq, PW, a.qtiles - 1 - blockIdx.x / groups, a.cu_k, a.Tk, nullptr, a.k_len, t, kk);
   if (t.first >= t.end) return;
-  const PackedKeys kk = packed_keys(a.cu_k, a.k_len, a.B, a.Tk, t.seq);
   const int h = grp * HP + (HP == 2 ? wave >> 1 : 0);
   const int kvh = grp * HP / (a.heads / a.kv_heads);
   const int pb = t.first + (HP == 2 ? (wave & 1) * 32 : wave * 32);
@@ -197,10 +198,11 @@ __global__ __launch_bounds__(256, HD <= 96 ? 2 : 1) void packed_dkv_kernel(Packe
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 15, g = lane >> 4;
   const int kvh = blockIdx.x % a.kv_heads;
-  const PackedTile t = packed_tile(a.cu_k, a.B, a.Tk, KW, blockIdx.x / a.kv_heads);
+  PackedTile t;
+  PackedKeys qq;  // the sequence's query rows
+  packed_find(a.cu_k, a.B, a.Tk, KW, blockIdx.x / a.kv_heads, a.cu_q, a.Tq, a.k_len, nullptr, t, qq);
   if (t.first >= t.end) return;
-  const PackedKeys kk = packed_keys(a.cu_k, a.k_len, a.B, a.Tk, t.seq);
-  const PackedKeys qq = packed_keys(a.cu_q, nullptr, a.B, a.Tq, t.seq);  // its query rows
+  const PackedKeys kk{t.start, t.used};
   const int rep = a.heads / a.kv_heads;
   const int k0 = t.first - t.start;       // first key of the tile, in the sequence
   const int kb0 = k0 + wave * 32;         // of the wave
