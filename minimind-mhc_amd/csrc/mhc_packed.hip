@@ -46,34 +46,27 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedAttnArgs a) {
   const uint16_t* kg = static_cast<const uint16_t*>(a.k) + kk.start * ks_t + kvh * a.ks_h;
   const uint16_t* vg = static_cast<const uint16_t*>(a.v) + kk.start * vs_t + kvh * a.vs_h;
   U32x4 kr[PPT], vr[PPT];
+  uint32_t koff[PPT], voff[PPT];
+#pragma unroll
+  for (int p = 0; p < PPT; ++p) {
+    const int piece = p * 256 + tid, row = piece / (HD / 8), col = piece % (HD / 8) * 8;
+    koff[p] = (uint32_t)(row * ks_t + col) * 2;
+    voff[p] = (uint32_t)(row * vs_t + col) * 2;
+  }
   auto load = [&](int s0) {
+    const auto kd = tile_rsrc(kg, ks_t, s0, kk.len, KT, HD), vd = tile_rsrc(vg, vs_t, s0, kk.len, KT, HD);
 #pragma unroll
-    for (int p = 0; p < PPT; ++p) {
-      const int piece = p * 256 + tid;
-      const int row = min(s0 + piece / (HD / 8), kk.len - 1);
-      const int col = (piece % (HD / 8)) * 8;
-      kr[p] = ld16(kg + row * ks_t + col);
-      vr[p] = ld16(vg + row * vs_t + col);
-    }
+    for (int p = 0; p < PPT; ++p) kr[p] = buf_load16(kd, koff[p]);
+#pragma unroll
+    for (int p = 0; p < PPT; ++p) vr[p] = buf_load16(vd, voff[p]);
   };
-  auto stash = [&](int buf, int s0) {
+  auto stash = [&](int buf) {
 #pragma unroll
     for (int p = 0; p < PPT; ++p) {
-      const int piece = p * 256 + tid;
-      const int row = piece / (HD / 8);
-      const int col = (piece % (HD / 8)) * 8;
+      const int piece = p * 256 + tid, row = piece / (HD / 8), col = piece % (HD / 8) * 8;
       *reinterpret_cast<U32x4*>(&ks[buf][row * KST + col]) = kr[p];
       *reinterpret_cast<U32x4*>(&vs[buf][row * VST + col]) = vr[p];
     }
-    // rows that are not there: probability 0 times what the clamped load found would be
-    // NaN for an infinity
-    if (s0 + KT > kk.len)
-#pragma unroll
-      for (int p = 0; p < PPT; ++p) {
-        const int piece = p * 256 + tid;
-        const int row = piece / (HD / 8);
-        if (s0 + row >= kk.len) *reinterpret_cast<U32x4*>(&vs[buf][row * VST + (piece % (HD / 8)) * 8]) = U32x4{};
-      }
   };
   if (t0 < t1) load(t0 * KT);
   U32x4 qb[2][NC];
@@ -86,7 +79,9 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedAttnArgs a) {
   }
   const float scale = a.scale * kPackedLog2e;
   constexpr float kHead = packed_head<F16>;
-  float m[2] = {kNoScore, kNoScore}, l[2] = {0.f, 0.f};
+  float m[2] = {kNoScore, kNoScore};
+  f32x4_t l[2] = {f32x4_t{0.f, 0.f, 0.f, 0.f}, f32x4_t{0.f, 0.f, 0.f, 0.f}};
+  const U32x4 ones = packed_ones<F16>();
   f32x4_t o[2][ND];
 #pragma unroll
   for (int u = 0; u < 2; ++u)
@@ -96,7 +91,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedAttnArgs a) {
   for (int kt = t0; kt < t1; ++kt) {
     const int buf = (kt - t0) & 1;
     const int s0 = kt * KT;
-    stash(buf, s0);
+    stash(buf);
     __syncthreads();
     if (kt + 1 < t1) load(s0 + KT);
     if (pb >= t.end || s0 > pb + 31 + shift) continue;  // no rows, or wholly above their diagonal
@@ -136,25 +131,26 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedAttnArgs a) {
         mx = fmaxf(mx - kHead, m[u]);
         const float f = exp2_f(m[u] - mx);
         m[u] = mx;
-        l[u] *= f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l[u][i] *= f;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[u][d][i] *= f;
       }
-      float sum = 0.f;
 #pragma unroll
       for (int st = 0; st < 4; ++st) {
         float p[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[i] = exp2_f(fmaf(s[u][st][i], scale, -m[u]));
-          sum += p[i];
-        }
+        for (int i = 0; i < 4; ++i) p[i] = exp2_f(fmaf(s[u][st][i], scale, -m[u]));
         pf[u][st >> 1].v[2 * (st & 1)] = pack2<F16>(p[0], p[1]);
         pf[u][st >> 1].v[2 * (st & 1) + 1] = pack2<F16>(p[2], p[3]);
       }
-      l[u] += sum;
+    }
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      l[0] = mfma16<F16>(ones, pf[0][hh], l[0]);
+      l[1] = mfma16<F16>(ones, pf[1][hh], l[1]);
     }
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -173,9 +169,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedAttnArgs a) {
   }
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    float ls = l[u];
-    ls += xor_lane16(ls);
-    ls += xor_lane32(ls);
+    const float ls = l[u][0];
     const int row = pb + u * 16 + r;
     if (row >= t.end) continue;
     const int64_t at = (int64_t)row * a.heads + h;

@@ -99,6 +99,24 @@ __device__ __forceinline__ void packed_find(const int* cu, int B, int T, int M, 
 // Tile numbers of T rows in B sequences.
 inline int64_t packed_tiles(int64_t T, int64_t B, int M) { return T / M + B + 1; }
 
+// An operand of ones: its product with the probabilities sums them on the matrix cores, over
+// all lanes at once, and sums what the outputs are formed of, the rounded ones.
+template <bool F16>
+__device__ __forceinline__ U32x4 packed_ones() {
+  const uint32_t w = F16 ? 0x3c003c00u : 0x3f803f80u;
+  return U32x4{{w, w, w, w}};
+}
+
+// A tile of up to `rows` rows (stride `st` elements) from row r0 on, of a tensor's head whose
+// first row is at p and which has n rows: 16 bytes at the byte offset `off` (of row and
+// column) in it.  The descriptor's size cuts off the rows behind the last, which read as
+// zeros: no comparison per lane, and no garbage beside probabilities of 0.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const uint16_t* p, int64_t st, int64_t r0, int n, int rows,
+                                                            int hd) {
+  const int left = (int)min((int64_t)rows, n - r0);
+  return make_rsrc(p + r0 * st, left > 0 ? (uint32_t)(((left - 1) * st + hd) * 2) : 0u);
+}
+
 // The transposing LDS load: the 16 lanes of a group point at 4 rows x 16 columns, four
 // columns a lane (lane r at row r / 4, column 4 (r % 4)), and lane r gets column r.
 __device__ __forceinline__ u32x2_v lds_tr4(const uint16_t* p) {
