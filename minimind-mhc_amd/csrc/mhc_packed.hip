@@ -11,17 +11,25 @@ namespace mhc {
 namespace {
 
 // ------------------------------------------------------------- tiles of many queries
-// One 4-wave workgroup per (tile of 128 query rows of one kv head, range of the keys): HP
-// query heads times 128 / HP positions, 32 rows a wave.
-template <bool F16, int HD, int HP>
-__global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedAttnArgs a) {
+// A workgroup per (tile of 128 query rows of one kv head, range of the keys): HP query heads
+// times 128 / HP positions, 32 rows a wave; with KS = 2 four more waves take every second key
+// tile of the same rows and the halves join at the end.
+//   * S^T = K Q^T and O^T = V^T P^T on v_mfma 16x16x32: a lane holds scores and outputs of
+//     one query row, and S^T's registers, rounded, are P^T's operand as they stand.  V^T comes
+//     from the row-major tile by the transposing LDS load.
+//   * K and V tiles of 64 keys come through a ring of LDS stages by direct-to-LDS loads,
+//     one tile (head_dim 128) or two ahead.
+template <bool F16, int HD, int HP, int KS>
+__global__ __launch_bounds__(256 * KS, 2) void packed_fwd_kernel(PackedAttnArgs a) {
   constexpr int NC = HD / 32, ND = HD / 16, KT = 64;
   constexpr int PW = 128 / HP;
-  constexpr int KST = HD + 8, VST = HD + 16;
-  constexpr int PPT = KT * (HD / 8) / 256;  // 16-byte pieces a thread moves per tile
-  __shared__ __align__(16) uint16_t ks[2][KT * KST];
-  __shared__ __align__(16) uint16_t vs[2][KT * VST];
-  const int tid = threadIdx.x;
+  constexpr int S = HD == 128 ? 2 : 3;     // stages
+  constexpr int TILE = KT * HD;            // elements
+  constexpr int UW = TILE * 2 / 1024 / 4;  // 1 KiB units of a tile a wave loads
+  __shared__ __align__(16) uint16_t lds[KS][S][2][TILE];
+  static_assert(KS == 1 || sizeof(lds) >= 4 * 64 * (2 * ND * 16 + 16), "the second half's sums take the tiles' place");
+  const int tid = threadIdx.x & 255;
+  const int half = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 15, g = lane >> 4;
   const int groups = a.heads / HP;
@@ -30,7 +38,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedAttnArgs a) {
   const int split = rest % a.splits;
   PackedTile t;
   PackedKeys kk;
-  packed_find(a.cu_q, a.B, a.Tq, PW, a.qtiles - 1 - rest / a.splits, a.cu_k, a.Tk, nullptr, a.k_len, t, kk);
+  packed_rank<false>(a.cu_q, a.B, a.Tq, PW, a.qtiles, rest / a.splits, a.cu_k, a.Tk, nullptr, a.k_len, t, kk);
   if (t.first >= t.end) return;
   const int h = grp * HP + (HP == 2 ? wave >> 1 : 0);
   const int kvh = grp * HP / (a.heads / a.kv_heads);
@@ -45,30 +53,18 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedAttnArgs a) {
   const int64_t ks_t = a.ks_t, vs_t = a.vs_t;
   const uint16_t* kg = static_cast<const uint16_t*>(a.k) + kk.start * ks_t + kvh * a.ks_h;
   const uint16_t* vg = static_cast<const uint16_t*>(a.v) + kk.start * vs_t + kvh * a.vs_h;
-  U32x4 kr[PPT], vr[PPT];
-  uint32_t koff[PPT], voff[PPT];
-#pragma unroll
-  for (int p = 0; p < PPT; ++p) {
-    const int piece = p * 256 + tid, row = piece / (HD / 8), col = piece % (HD / 8) * 8;
-    koff[p] = (uint32_t)(row * ks_t + col) * 2;
-    voff[p] = (uint32_t)(row * vs_t + col) * 2;
-  }
-  auto load = [&](int s0) {
-    const auto kd = tile_rsrc(kg, ks_t, s0, kk.len, KT, HD), vd = tile_rsrc(vg, vs_t, s0, kk.len, KT, HD);
-#pragma unroll
-    for (int p = 0; p < PPT; ++p) kr[p] = buf_load16(kd, koff[p]);
-#pragma unroll
-    for (int p = 0; p < PPT; ++p) vr[p] = buf_load16(vd, voff[p]);
+  TileLoader<HD, UW> kl, vl;
+  kl.init(wave * UW, ks_t);
+  vl.init(wave * UW, vs_t);
+  // the i-th key tile of this half; past the range the last one again, so that every step
+  // has as many loads in flight
+  auto issue = [&](int i, uint16_t* __restrict__ kd, uint16_t* __restrict__ vd) {
+    const int kt = min(t0 + i * KS + half, t1 - 1);
+    const int left = kk.len - kt * KT;
+    kl.issue(kd, kg + (int64_t)kt * KT * ks_t, wave * UW, ks_t, KT, left);
+    vl.issue(vd, vg + (int64_t)kt * KT * vs_t, wave * UW, vs_t, KT, left);
   };
-  auto stash = [&](int buf) {
-#pragma unroll
-    for (int p = 0; p < PPT; ++p) {
-      const int piece = p * 256 + tid, row = piece / (HD / 8), col = piece % (HD / 8) * 8;
-      *reinterpret_cast<U32x4*>(&ks[buf][row * KST + col]) = kr[p];
-      *reinterpret_cast<U32x4*>(&vs[buf][row * VST + col]) = vr[p];
-    }
-  };
-  if (t0 < t1) load(t0 * KT);
+  const int steps = t0 < t1 ? (t1 - t0 + KS - 1) / KS : 0;
   U32x4 qb[2][NC];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -76,6 +72,10 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedAttnArgs a) {
     const uint16_t* q = static_cast<const uint16_t*>(a.q) + row * a.qs_t + h * a.qs_h + 8 * g;
 #pragma unroll
     for (int c = 0; c < NC; ++c) qb[u][c] = ld16(q + 32 * c);
+  }
+  if (steps > 0) {
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) issue(i, lds[half][i][0], lds[half][i][1]);
   }
   const float scale = a.scale * kPackedLog2e;
   constexpr float kHead = packed_head<F16>;
@@ -87,26 +87,57 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedAttnArgs a) {
   for (int u = 0; u < 2; ++u)
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[u][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  // this lane's places in a tile: K rows 16 st + r, columns 32 c + 8 g; V rows 4 g + r / 4 of
+  // 16, columns 16 d + 4 (r % 4)
+  TileReads<HD> at;
+  at.init(r, g);
 
-  for (int kt = t0; kt < t1; ++kt) {
-    const int buf = (kt - t0) & 1;
-    const int s0 = kt * KT;
-    stash(buf);
-    __syncthreads();
-    if (kt + 1 < t1) load(s0 + KT);
-    if (pb >= t.end || s0 > pb + 31 + shift) continue;  // no rows, or wholly above their diagonal
+  // Step i: the tile in ks and vs, while one lands in kd and vd.  As restrict parameters the
+  // compiler sees that they differ; else it waits for every load in flight at each step.
+  auto step = [&](int i, const uint16_t* __restrict__ ks, uint16_t* __restrict__ vs, uint16_t* __restrict__ kd,
+                  uint16_t* __restrict__ vd) {
+    const int kt = t0 + i * KS + half, s0 = kt * KT;
+    issue(i + S - 1, kd, vd);
+    // V rows that are not there: probability 0 times an infinite copy of the last would be
+    // NaN.  Only a sequence's last tile has any (uniform over the workgroup's half; both
+    // halves take part in the barrier).
+    if (t0 * KT + (i + 1) * KS * KT > kk.len) {
+      if (kt < t1) {
+        for (int x = tid; x < KT * (HD / 8); x += 256)
+          if (s0 + x / (HD / 8) >= kk.len) *reinterpret_cast<U32x4*>(&vs[x * 8]) = U32x4{};
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      tile_barrier();
+    }
+    if (kt >= t1 || pb >= t.end || s0 > pb + 31 + shift) return;  // no rows, or wholly above their diagonal
+    // Operands are read from LDS a step ahead of their products; the barriers keep the
+    // compiler from sinking each read to its use, where every pair of products would wait.
     f32x4_t s[2][4];
+    U32x4 ka[4][NC];
+#pragma unroll
+    for (int st = 0; st < 4; ++st)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) ka[st][c] = at.row16(ks, st, c);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int st = 0; st < 4; ++st) {
       s[0][st] = f32x4_t{0.f, 0.f, 0.f, 0.f};
       s[1][st] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const U32x4 ka = *reinterpret_cast<const U32x4*>(&ks[buf][(st * 16 + r) * KST + 32 * c + 8 * g]);
-        s[0][st] = mfma16<F16>(ka, qb[0][c], s[0][st]);
-        s[1][st] = mfma16<F16>(ka, qb[1][c], s[1][st]);
-      }
     }
+#pragma unroll
+    for (int sp = 0; sp < 4; sp += 2)
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int st = sp; st < sp + 2; ++st) {
+          s[0][st] = mfma16<F16>(ka[st][c], qb[0][c], s[0][st]);
+          s[1][st] = mfma16<F16>(ka[st][c], qb[1][c], s[1][st]);
+        }
+    U32x4 va[2][ND];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) va[0][d] = at.columns32(vs, 0, d);
+    __builtin_amdgcn_sched_barrier(0);
     if (s0 + KT - 1 > pb + shift) {  // uniform: only the tiles on the diagonal are compared
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -147,25 +178,56 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackedAttnArgs a) {
         pf[u][st >> 1].v[2 * (st & 1) + 1] = pack2<F16>(p[2], p[3]);
       }
     }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) va[1][d] = at.columns32(vs, 1, d);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
       l[0] = mfma16<F16>(ones, pf[0][hh], l[0]);
       l[1] = mfma16<F16>(ones, pf[1][hh], l[1]);
-    }
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        U32x4 va;
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const u32x2_v w = lds_tr4(&vs[buf][(hh * 32 + q * 16 + 4 * g + (r >> 2)) * VST + 16 * d + 4 * (r & 3)]);
-          va.v[2 * q] = w.x;
-          va.v[2 * q + 1] = w.y;
-        }
-        o[0][d] = mfma16<F16>(va, pf[0][hh], o[0][d]);
-        o[1][d] = mfma16<F16>(va, pf[1][hh], o[1][d]);
+      for (int d = 0; d < ND; ++d) {
+        o[0][d] = mfma16<F16>(va[hh][d], pf[0][hh], o[0][d]);
+        o[1][d] = mfma16<F16>(va[hh][d], pf[1][hh], o[1][d]);
       }
+    }
+  };
+  int stage = 0;
+  for (int i = 0; i < steps; ++i) {
+    tile_wait<(S - 2) * 2 * UW>();
+    tile_barrier();  // this step's tile has landed, and every wave is done with the one before
+    const int next = stage == 0 ? S - 1 : stage - 1;
+    step(i, lds[half][stage][0], lds[half][stage][1], lds[half][next][0], lds[half][next][1]);
+    stage = stage == S - 1 ? 0 : stage + 1;
+  }
+  if (steps > 0) tile_wait<0>();  // the loads past the range: nothing may land after this
+  if constexpr (KS == 2) {  // the halves meet in LDS
+    __syncthreads();
+    float* x = reinterpret_cast<float*>(lds) + wave * 64 * (2 * ND * 4 + 4) + lane * 4;
+    if (half == 1) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4_t*>(x + (u * ND + d) * 256) = o[u][d];
+      *reinterpret_cast<f32x4_t*>(x + 2 * ND * 256) = f32x4_t{m[0], m[1], l[0][0], l[1][0]};
+    }
+    __syncthreads();
+    if (half == 1) return;
+    const f32x4_t ml = *reinterpret_cast<const f32x4_t*>(x + 2 * ND * 256);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const float mx = fmaxf(m[u], ml[u]);
+      const float f = exp2_f(m[u] - mx), e = exp2_f(ml[u] - mx);
+      m[u] = mx;
+      l[u][0] = l[u][0] * f + ml[2 + u] * e;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const f32x4_t y = *reinterpret_cast<const f32x4_t*>(x + (u * ND + d) * 256);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[u][d][i] = o[u][d][i] * f + y[i] * e;
+      }
+    }
   }
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -463,10 +525,16 @@ hipError_t packed_fwd_hd(const PackedAttnArgs& a, hipStream_t s) {
     const int nb = (a.heads / a.kv_heads + a.row_heads - 1) / a.row_heads;
     const int64_t ranges = ((int64_t)a.qtiles * a.splits + 7) / 8 * 8;
     packed_few_kernel<F16, HD><<<dim3((unsigned)(ranges * a.kv_heads * nb)), 256, 0, s>>>(a);
-  } else if (a.row_heads == 2) {
-    packed_fwd_kernel<F16, HD, 2><<<dim3((unsigned)((int64_t)a.qtiles * a.splits * (a.heads / 2))), 256, 0, s>>>(a);
   } else {
-    packed_fwd_kernel<F16, HD, 1><<<dim3((unsigned)((int64_t)a.qtiles * a.splits * a.heads)), 256, 0, s>>>(a);
+    const dim3 grid((unsigned)((int64_t)a.qtiles * a.splits * (a.heads / a.row_heads)));
+    const int ks = getenv("KS") ? atoi(getenv("KS")) : 2;
+    if (a.row_heads == 2) {
+      if (ks == 2) packed_fwd_kernel<F16, HD, 2, 2><<<grid, 512, 0, s>>>(a);
+      else packed_fwd_kernel<F16, HD, 2, 1><<<grid, 256, 0, s>>>(a);
+    } else {
+      if (ks == 2) packed_fwd_kernel<F16, HD, 1, 2><<<grid, 512, 0, s>>>(a);
+      else packed_fwd_kernel<F16, HD, 1, 1><<<grid, 256, 0, s>>>(a);
+    }
   }
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   if (a.splits > 1)

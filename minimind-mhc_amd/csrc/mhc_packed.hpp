@@ -70,6 +70,22 @@ struct PackedTile {
 struct PackedKeys {
   int start, len;
 };
+__device__ __forceinline__ void packed_bounds(const int* cu, int B, int T, int M, int seq, int tile, const int* cu_o,
+                                              int To, const int* used_t, const int* used_o, PackedTile& t,
+                                              PackedKeys& o) {
+  // all loads of the sequence's bounds before the first use of one
+  const bool in = seq < B;
+  const int next = in ? seq + 1 : seq, at = in ? seq : 0;
+  const int s0 = cu[seq], s1 = cu[next], o0 = cu_o[seq], o1 = cu_o[next];
+  const int ut = used_t && in ? used_t[at] : 0x7fffffff, uo = used_o && in ? used_o[at] : 0x7fffffff;
+  t.seq = seq;
+  t.start = seq == 0 ? 0 : min(max(s0, 0), T);
+  t.end = max(in ? min(max(s1, 0), T) : T, t.start);
+  t.first = t.start + min(tile, (T - t.start) / M + 1) * M;
+  o.start = seq == 0 ? 0 : min(max(o0, 0), To);
+  o.len = in ? min(max(uo, 0), max(min(max(o1, 0), To) - o.start, 0)) : 0;
+  t.used = in ? min(max(ut, 0), t.end - t.start) : 0;
+}
 __device__ __forceinline__ void packed_find(const int* cu, int B, int T, int M, int tile, const int* cu_o, int To,
                                             const int* used_t, const int* used_o, PackedTile& t, PackedKeys& o) {
   const int lane = __lane_id();
@@ -83,18 +99,81 @@ __device__ __forceinline__ void packed_find(const int* cu, int B, int T, int M, 
     hi = min(hi, lo + step);
   }
   lo = __builtin_amdgcn_readfirstlane(lo);
-  // all loads of the sequence's bounds before the first use of one
-  const bool in = lo < B;
-  const int next = in ? lo + 1 : lo, at = in ? lo : 0;
-  const int s0 = cu[lo], s1 = cu[next], o0 = cu_o[lo], o1 = cu_o[next];
-  const int ut = used_t && in ? used_t[at] : 0x7fffffff, uo = used_o && in ? used_o[at] : 0x7fffffff;
-  t.seq = lo;
-  t.start = lo == 0 ? 0 : min(max(s0, 0), T);
-  t.end = max(in ? min(max(s1, 0), T) : T, t.start);
-  t.first = t.start + (tile - (t.start / M + lo)) * M;
-  o.start = lo == 0 ? 0 : min(max(o0, 0), To);
-  o.len = in ? min(max(uo, 0), max(min(max(o1, 0), To) - o.start, 0)) : 0;
-  t.used = in ? min(max(ut, 0), t.end - t.start) : 0;
+  packed_bounds(cu, B, T, M, lo, tile - (seq_start(cu, lo, T) / M + lo), cu_o, To, used_t, used_o, t, o);
+}
+
+// The same by rank: the tiles of all sequences, those with the most work first (the last
+// of a sequence's query tiles; backward: the first of its key tiles), so that the longest chains
+// start at once and the short ones fill the ends.  A tile's level is its number in the
+// sequence (`past`: and the tiles of keys before it); the rank's level is found by counting the
+// tiles from each level up, four sequences a lane.  For up to 256 sequences; more of them
+// even out by themselves.
+constexpr int kRankSeqs = 256;
+template <bool FIRST>
+__device__ __forceinline__ void packed_rank(const int* cu, int B, int T, int M, int tiles, int rank, const int* cu_o,
+                                            int To, const int* used_t, const int* used_o, PackedTile& t,
+                                            PackedKeys& o) {
+  if (B > kRankSeqs || T > 1 << 28) {
+    packed_find(cu, B, T, M, FIRST ? rank : tiles - 1 - rank, cu_o, To, used_t, used_o, t, o);
+    return;
+  }
+  constexpr int C = kRankSeqs / 64;
+  const int lane = __lane_id();
+  float n[C], past[C];  // small whole numbers, exact in fp32
+  float most = 0.f;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int i = c * 64 + lane;
+    n[c] = past[c] = 0.f;
+    if (c * 64 < B && i < B) {
+      const int len = max(seq_start(cu, i + 1, T) - seq_start(cu, i, T), 0);
+      n[c] = (float)((len + M - 1) / M);
+      if (!FIRST) {
+        int keys = max(seq_start(cu_o, i + 1, To) - seq_start(cu_o, i, To), 0);
+        if (used_o) keys = min(max(used_o[i], 0), keys);
+        past[c] = (float)(max(keys - len, 0) / M);
+      }
+      most = fmaxf(most, n[c] + past[c]);
+    }
+  }
+  auto count = [&](float level) {  // tiles of that level and above
+    float x = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (c * 64 < B) x += fmaxf(n[c] + past[c] - fmaxf(level, past[c]), 0.f);
+    return __builtin_amdgcn_readfirstlane((int)wave_sum(x));
+  };
+  const int total = count(0.f);
+  int seq = B, tile = rank - total;
+  if (rank < total) {
+    int lo = 0, hi = __builtin_amdgcn_readfirstlane((int)wave_max(most)), above = 0;  // count(lo) > rank >= count(hi)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2, x = count((float)mid);
+      if (x > rank) {
+        lo = mid;
+      } else {
+        hi = mid;
+        above = x;
+      }
+    }
+    int k = rank - above;  // which of the level's tiles
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const bool has = past[c] <= (float)lo && (float)lo < past[c] + n[c];
+      const uint64_t mask = __ballot(has);
+      const int here = __popcll(mask);
+      if (k >= 0 && k < here) {
+        const uint64_t me = __ballot(has && __popcll(mask & ((1ull << lane) - 1)) == k);
+        const int l = __ffsll((unsigned long long)me) - 1;
+        seq = c * 64 + l;
+        const int first = (int)__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, past[c]), l));
+        const int num = (int)__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, n[c]), l));
+        tile = FIRST ? num - 1 - (lo - first) : lo - first;
+      }
+      k -= here;
+    }
+  }
+  packed_bounds(cu, B, T, M, seq, tile, cu_o, To, used_t, used_o, t, o);
 }
 // Tile numbers of T rows in B sequences.
 inline int64_t packed_tiles(int64_t T, int64_t B, int M) { return T / M + B + 1; }
@@ -107,14 +186,58 @@ __device__ __forceinline__ U32x4 packed_ones() {
   return U32x4{{w, w, w, w}};
 }
 
-// A tile of up to `rows` rows (stride `st` elements) from row r0 on, of a tensor's head whose
-// first row is at p and which has n rows: 16 bytes at the byte offset `off` (of row and
-// column) in it.  The descriptor's size cuts off the rows behind the last, which read as
-// zeros: no comparison per lane, and no garbage beside probabilities of 0.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const uint16_t* p, int64_t st, int64_t r0, int n, int rows,
-                                                            int hd) {
-  const int left = (int)min((int64_t)rows, n - r0);
-  return make_rsrc(p + r0 * st, left > 0 ? (uint32_t)(((left - 1) * st + hd) * 2) : 0u);
+// A tile of ROWS rows of one head in LDS, filled by direct-to-LDS loads: a wave's load
+// writes 64 lanes x 16 bytes in a row, so rows lie without padding and their 16-byte slots are
+// permuted instead (on the global side), so that 16 rows of one column, and 16 rows of 32
+// bytes, spread over all 64 banks: an exclusive or with bits of the row where 8 or 16 slots
+// make the row, a rotation by row / 4 where 12 do.
+template <int HD>
+__device__ __forceinline__ int tile_slot(int row, int slot) {
+  if constexpr (HD == 64) return slot ^ ((row >> 1) & 7);
+  else if constexpr (HD == 128) return slot ^ (row & 15);
+  else return (slot + (row >> 2)) % 12;
+}
+template <int HD>
+__device__ __forceinline__ int tile_column(int row, int place) {  // the slot that lies there
+  if constexpr (HD == 96) return (place + 24 - (row >> 2)) % 12;
+  else return tile_slot<HD>(row, place);
+}
+// `N` of the tile's 1 KiB units, from unit u0 on, by this wave.
+template <int HD, int N>
+struct TileLoader {
+  uint32_t off[N];  // this lane's byte offset in the tile's rows
+  __device__ __forceinline__ void init(int u0, int64_t st) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = (u0 + i) * 64 + __lane_id(), row = at / (HD / 8);
+      off[i] = (uint32_t)(row * st + tile_column<HD>(row, at % (HD / 8)) * 8) * 2;
+    }
+  }
+  // p: the tile's first row; left >= 1: rows that exist from there on (rows behind them
+  // become copies of the last, uniform branch).
+  __device__ __forceinline__ void issue(uint16_t* lds, const uint16_t* p, int u0, int64_t st, int rows, int left) const {
+    const char* base = reinterpret_cast<const char*>(p);
+    char* to = reinterpret_cast<char*>(lds) + u0 * 1024;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      uint32_t o = off[i];
+      if (left < rows) {
+        const int at = (u0 + i) * 64 + __lane_id(), row = at / (HD / 8);
+        o = (uint32_t)(min(row, left - 1) * st + tile_column<HD>(row, at % (HD / 8)) * 8) * 2;
+      }
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base + o),
+                                       (__attribute__((address_space(3))) void*)(to + i * 1024), 16, 0, 0);
+    }
+  }
+};
+// At most N direct-to-LDS loads of this wave in flight, and no LDS read; then every wave's.
+template <int N>
+__device__ __forceinline__ void tile_wait() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(N) : "memory");
+}
+__device__ __forceinline__ void tile_barrier() {
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
 // The transposing LDS load: the 16 lanes of a group point at 4 rows x 16 columns, four
@@ -132,5 +255,42 @@ __device__ __forceinline__ u32x2_v lds_tr4(const uint16_t* p) {
     case 128: return a.f16 ? fn<true, 128>(a, s) : fn<false, 128>(a, s); \
     default: return hipErrorInvalidValue;                                \
   }
+
+// A lane's reads of a tile: 16 bytes of row 16 st + r at columns 32 c + 8 g (an operand
+// whose rows are the tile's), and columns 16 d + r of the rows 32 h + 16 (j / 4) + 4 g + j % 4
+// (an operand whose rows are the tile's columns; the rows are in the order in which a product
+// leaves its results to a lane).
+template <int HD>
+struct TileReads {
+  static constexpr int NK = HD == 96 ? 3 : HD / 32, NV = HD == 96 ? 6 : HD / 16;
+  int k[NK], v[NV];  // elements
+  __device__ __forceinline__ void init(int r, int g) {
+    if constexpr (HD == 96) {  // rotated by row / 4: constants of the column and of the row add up modulo 12
+#pragma unroll
+      for (int i = 0; i < NK; ++i) k[i] = r * HD + (4 * i + g + (r >> 2)) % 12 * 8;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) v[i] = (4 * g + (r >> 2)) * HD + (2 * i + ((r & 3) >> 1) + g) % 12 * 8 + 4 * (r & 1);
+    } else {  // bits of the lane's part of the row only
+#pragma unroll
+      for (int i = 0; i < NK; ++i) k[i] = r * HD + tile_slot<HD>(r, 4 * i + g) * 8;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        v[i] = (4 * g + (r >> 2)) * HD + tile_slot<HD>(4 * g + (r >> 2), 2 * i + ((r & 3) >> 1)) * 8 + 4 * (r & 1);
+    }
+  }
+  __device__ __forceinline__ U32x4 row16(const uint16_t* t, int st, int c) const {
+    return *reinterpret_cast<const U32x4*>(t + k[HD == 96 ? (c + st) % 3 : c] + st * 16 * HD);
+  }
+  __device__ __forceinline__ U32x4 columns32(const uint16_t* t, int h, int d) const {
+    U32x4 o;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const u32x2_v w = lds_tr4(t + v[HD == 96 ? (d + 2 * q + 4 * h) % 6 : d] + (h * 32 + q * 16) * HD);
+      o.v[2 * q] = w.x;
+      o.v[2 * q + 1] = w.y;
+    }
+    return o;
+  }
+};
 
 }  // namespace mhc

@@ -28,7 +28,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
   const int grp = blockIdx.x % groups;
   PackedTile t;
   PackedKeys kk;
-  packed_find(a.cu_q, a.B, a.Tq, PW, a.qtiles - 1 - blockIdx.x / groups, a.cu_k, a.Tk, nullptr, a.k_len, t, kk);
+  packed_rank<false>(a.cu_q, a.B, a.Tq, PW, a.qtiles, blockIdx.x / groups, a.cu_k, a.Tk, nullptr, a.k_len, t, kk);
   if (t.first >= t.end) return;
   const int h = grp * HP + (HP == 2 ? wave >> 1 : 0);
   const int kvh = grp * HP / (a.heads / a.kv_heads);
@@ -200,7 +200,7 @@ __global__ __launch_bounds__(256, HD <= 96 ? 2 : 1) void packed_dkv_kernel(Packe
   const int kvh = blockIdx.x % a.kv_heads;
   PackedTile t;
   PackedKeys qq;  // the sequence's query rows
-  packed_find(a.cu_k, a.B, a.Tk, KW, blockIdx.x / a.kv_heads, a.cu_q, a.Tq, a.k_len, nullptr, t, qq);
+  packed_rank<true>(a.cu_k, a.B, a.Tk, KW, 0, blockIdx.x / a.kv_heads, a.cu_q, a.Tq, a.k_len, nullptr, t, qq);
   if (t.first >= t.end) return;
   const PackedKeys kk{t.start, t.used};
   const int rep = a.heads / a.kv_heads;
