@@ -527,7 +527,7 @@ hipError_t packed_fwd_hd(const PackedAttnArgs& a, hipStream_t s) {
     packed_few_kernel<F16, HD><<<dim3((unsigned)(ranges * a.kv_heads * nb)), 256, 0, s>>>(a);
   } else {
     const dim3 grid((unsigned)((int64_t)a.qtiles * a.splits * (a.heads / a.row_heads)));
-    const int ks = getenv("KS") ? atoi(getenv("KS")) : 2;
+    const int ks = getenv("KS") ? atoi(getenv("KS")) : grid.x <= (unsigned)device_cus() * 5 / 4 ? 2 : 1;
     if (a.row_heads == 2) {
       if (ks == 2) packed_fwd_kernel<F16, HD, 2, 2><<<grid, 512, 0, s>>>(a);
       else packed_fwd_kernel<F16, HD, 2, 1><<<grid, 256, 0, s>>>(a);

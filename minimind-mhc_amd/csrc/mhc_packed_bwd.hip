@@ -17,10 +17,10 @@ template <bool F16, int HD, int HP>
 __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
   constexpr int NC = HD / 32, ND = HD / 16, KT = 64;
   constexpr int PW = 128 / HP;
-  constexpr int KST = HD + 16, VST = HD + 8;
-  constexpr int PPT = KT * (HD / 8) / 256;
-  __shared__ __align__(16) uint16_t ks[2][KT * KST];
-  __shared__ __align__(16) uint16_t vs[2][KT * VST];
+  constexpr int S = HD == 128 ? 2 : 3;     // stages
+  constexpr int TILE = KT * HD;            // elements
+  constexpr int UW = TILE * 2 / 1024 / 4;  // 1 KiB units of a tile a wave loads
+  __shared__ __align__(16) uint16_t lds[S][2][TILE];
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 15, g = lane >> 4;
@@ -40,18 +40,14 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
   const int64_t ks_t = a.ks_t, vs_t = a.vs_t;
   const uint16_t* kg = static_cast<const uint16_t*>(a.k) + kk.start * ks_t + kvh * a.ks_h;
   const uint16_t* vg = static_cast<const uint16_t*>(a.v) + kk.start * vs_t + kvh * a.vs_h;
-  U32x4 kr[PPT], vr[PPT];
-  auto load = [&](int s0) {
-#pragma unroll
-    for (int p = 0; p < PPT; ++p) {
-      const int piece = p * 256 + tid;
-      const int row = min(s0 + piece / (HD / 8), kk.len - 1);
-      const int col = (piece % (HD / 8)) * 8;
-      kr[p] = ld16(kg + row * ks_t + col);
-      vr[p] = ld16(vg + row * vs_t + col);
-    }
+  TileLoader<HD, UW> kl, vl;
+  kl.init(wave * UW, ks_t);
+  vl.init(wave * UW, vs_t);
+  auto issue = [&](int i, uint16_t* __restrict__ kd, uint16_t* __restrict__ vd) {
+    const int kt = min(i, nt - 1), left = kk.len - kt * KT;
+    kl.issue(kd, kg + (int64_t)kt * KT * ks_t, wave * UW, ks_t, KT, left);
+    vl.issue(vd, vg + (int64_t)kt * KT * vs_t, wave * UW, vs_t, KT, left);
   };
-  if (nt > 0) load(0);
   U32x4 qb[2][NC], gb[2][NC];
   float lse[2], delta[2];
 #pragma unroll
@@ -81,60 +77,73 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
     lse[u] = a.lse[(int64_t)h * a.Tq + at];
     if (g == 0 && row < t.end) a.delta[(int64_t)h * a.Tq + row] = d;
   }
+  if (nt > 0) {
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) issue(i, lds[i][0], lds[i][1]);
+  }
   const float scale = a.scale * kPackedLog2e;
   f32x4_t dq[2][ND];
 #pragma unroll
   for (int u = 0; u < 2; ++u)
 #pragma unroll
     for (int d = 0; d < ND; ++d) dq[u][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  TileReads<HD> at;
+  at.init(r, g);
 
-  for (int kt = 0; kt < nt; ++kt) {
-    const int buf = kt & 1;
-    const int s0 = kt * KT;
-#pragma unroll
-    for (int p = 0; p < PPT; ++p) {
-      const int piece = p * 256 + tid;
-      const int row = piece / (HD / 8);
-      const int col = (piece % (HD / 8)) * 8;
-      *reinterpret_cast<U32x4*>(&ks[buf][row * KST + col]) = kr[p];
-      *reinterpret_cast<U32x4*>(&vs[buf][row * VST + col]) = vr[p];
-    }
-    __syncthreads();
-    if (kt + 1 < nt) load(s0 + KT);
-    if (pb >= t.end || s0 > pb + 31 + shift) continue;
+  // step i: the tile in ks and vs, while one lands in kd and vd (which differ: restrict)
+  auto step = [&](int i, const uint16_t* __restrict__ ks, const uint16_t* __restrict__ vs, uint16_t* __restrict__ kd,
+                  uint16_t* __restrict__ vd) {
+    const int s0 = i * KT;
+    issue(i + S - 1, kd, vd);
+    if (pb >= t.end || s0 > pb + 31 + shift) return;
     const bool diagonal = s0 + KT - 1 > pb + shift;
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
       f32x4_t s[2][2], dp[2][2];
+      constexpr int QS = HD == 128 ? 1 : 2;  // 16-key parts read ahead together (registers)
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
+      for (int q0 = 0; q0 < 2; q0 += QS) {
+        U32x4 ka[QS][NC], va[QS][NC];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          s[u][q] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-          dp[u][q] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        }
+        for (int q = 0; q < QS; ++q)
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const int row = hh * 32 + q * 16 + r;
-          const U32x4 ka = *reinterpret_cast<const U32x4*>(&ks[buf][row * KST + 32 * c + 8 * g]);
-          const U32x4 va = *reinterpret_cast<const U32x4*>(&vs[buf][row * VST + 32 * c + 8 * g]);
+          for (int c = 0; c < NC; ++c) {
+            ka[q][c] = at.row16(ks, hh * 2 + q0 + q, c);
+            va[q][c] = at.row16(vs, hh * 2 + q0 + q, c);
+          }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = q0; q < q0 + QS; ++q)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            s[u][q] = mfma16<F16>(ka, qb[u][c], s[u][q]);
-            dp[u][q] = mfma16<F16>(va, gb[u][c], dp[u][q]);
+            s[u][q] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            dp[u][q] = f32x4_t{0.f, 0.f, 0.f, 0.f};
           }
-        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int q = 0; q < QS; ++q)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              s[u][q0 + q] = mfma16<F16>(ka[q][c], qb[u][c], s[u][q0 + q]);
+              dp[u][q0 + q] = mfma16<F16>(va[q][c], gb[u][c], dp[u][q0 + q]);
+            }
       }
+      U32x4 kc[ND];
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int d = 0; d < ND; ++d) kc[d] = at.columns32(ks, hh, d);
+      __builtin_amdgcn_sched_barrier(0);
       if (diagonal) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int q = 0; q < 2; ++q)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (s0 + hh * 32 + q * 16 + 4 * g + i > pb + u * 16 + r + shift) {
-                s[u][q][i] = -__builtin_inff();
-                dp[u][q][i] = 0.f;
+            for (int j = 0; j < 4; ++j)
+              if (s0 + hh * 32 + q * 16 + 4 * g + j > pb + u * 16 + r + shift) {
+                s[u][q][j] = -__builtin_inff();
+                dp[u][q][j] = 0.f;
               }
       }
       U32x4 pf[2];
@@ -144,25 +153,27 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
         for (int q = 0; q < 2; ++q) {
           float ds[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            ds[i] = exp2_f(fmaf(s[u][q][i], scale, -lse[u])) * (dp[u][q][i] - delta[u]);
+          for (int j = 0; j < 4; ++j)
+            ds[j] = exp2_f(fmaf(s[u][q][j], scale, -lse[u])) * (dp[u][q][j] - delta[u]);
           pf[u].v[2 * q] = pack2<F16>(ds[0], ds[1]);
           pf[u].v[2 * q + 1] = pack2<F16>(ds[2], ds[3]);
         }
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        U32x4 ka;
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const u32x2_v w = lds_tr4(&ks[buf][(hh * 32 + q * 16 + 4 * g + (r >> 2)) * KST + 16 * d + 4 * (r & 3)]);
-          ka.v[2 * q] = w.x;
-          ka.v[2 * q + 1] = w.y;
-        }
-        dq[0][d] = mfma16<F16>(ka, pf[0], dq[0][d]);
-        dq[1][d] = mfma16<F16>(ka, pf[1], dq[1][d]);
+        dq[0][d] = mfma16<F16>(kc[d], pf[0], dq[0][d]);
+        dq[1][d] = mfma16<F16>(kc[d], pf[1], dq[1][d]);
       }
     }
+  };
+  int stage = 0;
+  for (int i = 0; i < nt; ++i) {
+    tile_wait<(S - 2) * 2 * UW>();
+    tile_barrier();
+    const int next = stage == 0 ? S - 1 : stage - 1;
+    step(i, lds[stage][0], lds[stage][1], lds[next][0], lds[next][1]);
+    stage = stage == S - 1 ? 0 : stage + 1;
   }
+  if (nt > 0) tile_wait<0>();  // the loads past the range: nothing may land after the end
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int row = pb + u * 16 + r;
@@ -188,12 +199,11 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
 template <bool F16, int HD>
 __global__ __launch_bounds__(256, HD <= 96 ? 2 : 1) void packed_dkv_kernel(PackedAttnArgs a) {
   constexpr int NC = HD / 32, ND = HD / 16, QT = 32, KW = 128;
-  constexpr int ST = HD + 16;
+  constexpr int S = 4;                     // stages
+  constexpr int TILE = QT * HD;            // elements
+  constexpr int UW = TILE * 2 / 1024 / 2;  // 1 KiB units a wave loads: waves 0 and 1 q, 2 and 3 g
   constexpr float kUp = F16 ? 14.f : 0.f, kDown = F16 ? 0x1p-14f : 1.f;
-  constexpr int PPT = QT * (HD / 8) / 128;  // half the threads move q, half g
-  __shared__ __align__(16) uint16_t qs[2][QT * ST];
-  __shared__ __align__(16) uint16_t gs[2][QT * ST];
-  __shared__ __align__(16) float ls[2][QT], ds_[2][QT];
+  __shared__ __align__(16) uint16_t lds[S][2 * TILE + 128];  // q, g, and the rows' 32 log sums and 32 D (fp32)
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 15, g = lane >> 4;
@@ -212,29 +222,36 @@ __global__ __launch_bounds__(256, HD <= 96 ? 2 : 1) void packed_dkv_kernel(Packe
   const int per_head = (n_rows + QT - 1) / QT;
   const int nt = per_head * rep;
 
-  const bool loads_g = tid >= 128;
-  const uint16_t* src = static_cast<const uint16_t*>(loads_g ? a.g_out : a.q);
+  const bool loads_g = wave >= 2;
+  const int u0 = (wave & 1) * UW;
   const int64_t row_st = loads_g ? (int64_t)a.heads * HD : a.qs_t, head_st = loads_g ? HD : a.qs_h;
-  src += qq.start * row_st + (int64_t)kvh * rep * head_st;
-  U32x4 st[PPT];
-  float st_l = 0.f;
-  auto load = [&](int it) {
-    const int hh = it / per_head, q0 = q_first + (it - hh * per_head) * QT;
-    const uint16_t* p0 = src + hh * head_st;
-#pragma unroll
-    for (int p = 0; p < PPT; ++p) {
-      const int piece = p * 128 + (tid & 127);
-      st[p] = ld16(p0 + min(q0 + piece / (HD / 8), qq.len - 1) * row_st + (piece % (HD / 8)) * 8);
-    }
-    if (tid < 2 * QT) {
-      const int row = q0 + (tid & (QT - 1));
-      const float* lp = (tid < QT ? a.lse : a.delta) + (int64_t)(kvh * rep + hh) * a.Tq + qq.start;
-      // a row that is not there: its probabilities are 0
-      st_l = row < qq.len ? lp[row] : tid < QT ? __builtin_inff() : 0.f;
-      st_l = tid < QT ? st_l - kUp : st_l * kDown;
-    }
+  const uint16_t* src = static_cast<const uint16_t*>(loads_g ? a.g_out : a.q) + qq.start * row_st +
+                        (int64_t)kvh * rep * head_st;
+  TileLoader<HD, UW> tl;
+  tl.init(u0, row_st);
+  const int to = loads_g ? TILE : 0;
+  int ih = 0, iq = 0;  // head and row tile of the next tile to load
+  auto issue = [&](uint16_t* __restrict__ d) {
+    const int q0 = q_first + iq * QT;
+    const uint16_t* p0 = src + ih * head_st + q0 * row_st;
+    tl.issue(d + to, p0, u0, row_st, QT, qq.len - q0);
+    // every wave loads the rows' sums, so that each has as many loads in flight; the same
+    // values to the same place
+    const int row = min(q0 + (lane & 31), qq.len - 1);
+    const float* p = (lane < 32 ? a.lse : a.delta) + (int64_t)(kvh * rep + ih) * a.Tq + qq.start + row;
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
+                                     (__attribute__((address_space(3))) void*)(d + 2 * TILE), 4, 0, 0);
+    if (iq + 1 < per_head) {
+      ++iq;
+    } else if (ih + 1 < rep) {
+      iq = 0;
+      ++ih;
+    }  // past the last: that one again
   };
-  if (nt > 0) load(0);
+  if (nt > 0) {
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) issue(lds[i]);
+  }
   U32x4 kb[2][NC], vb[2][NC];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -256,90 +273,105 @@ __global__ __launch_bounds__(256, HD <= 96 ? 2 : 1) void packed_dkv_kernel(Packe
       dk[u][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
       dv[u][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
-  for (int it = 0; it < nt; ++it) {
-    const int buf = it & 1;
+  TileReads<HD> at;
+  at.init(r, g);
+  auto step = [&](int q0, const uint16_t* __restrict__ qs, uint16_t* __restrict__ d) {
+    issue(d);
+    const uint16_t* gs = qs + TILE;
+    if (kb0 >= kk.len || q0 + QT - 1 + shift < kb0) return;  // no keys, or none that these rows see
+    // the diagonal, and the sequence's last rows, behind which lie copies of the last
+    const bool edge = q0 + shift < kb0 + 31 || q0 + QT > qq.len;
+    U32x4 qa[2][NC], ga[2][NC];
 #pragma unroll
-    for (int p = 0; p < PPT; ++p) {
-      const int piece = p * 128 + (tid & 127);
-      uint16_t* to = loads_g ? gs[buf] : qs[buf];
-      *reinterpret_cast<U32x4*>(&to[piece / (HD / 8) * ST + (piece % (HD / 8)) * 8]) = st[p];
-    }
-    if (tid < 2 * QT) (tid < QT ? ls[buf] : ds_[buf])[tid & (QT - 1)] = st_l;
-    __syncthreads();
-    if (it + 1 < nt) load(it + 1);
-    const int q0 = q_first + it % per_head * QT;
-    if (kb0 >= kk.len || q0 + QT - 1 + shift < kb0) continue;  // no keys, or none that these rows see
-    const bool diagonal = q0 + shift < kb0 + 31;
-    f32x4_t s[2][2], dp[2][2];  // [16 query rows][16 keys]
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        qa[q][c] = at.row16(qs, q, c);
+        ga[q][c] = at.row16(gs, q, c);
+      }
+    f32x4_t l4[2], d4[2];
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
+      l4[q] = *reinterpret_cast<const f32x4_t*>(&gs[TILE + 2 * (q * 16 + 4 * g)]);
+      d4[q] = *reinterpret_cast<const f32x4_t*>(&gs[TILE + 2 * (32 + q * 16 + 4 * g)]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    f32x4_t s[2][2], dp[2][2];  // [16 query rows][16 keys]
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         s[q][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         dp[q][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
       }
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const U32x4 qa = *reinterpret_cast<const U32x4*>(&qs[buf][(q * 16 + r) * ST + 32 * c + 8 * g]);
-        const U32x4 ga = *reinterpret_cast<const U32x4*>(&gs[buf][(q * 16 + r) * ST + 32 * c + 8 * g]);
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          s[q][u] = mfma16<F16>(qa, kb[u][c], s[q][u]);
-          dp[q][u] = mfma16<F16>(ga, vb[u][c], dp[q][u]);
+          s[q][u] = mfma16<F16>(qa[q][c], kb[u][c], s[q][u]);
+          dp[q][u] = mfma16<F16>(ga[q][c], vb[u][c], dp[q][u]);
         }
-      }
-    }
-    if (diagonal) {
+    U32x4 gc[ND];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) gc[d] = at.columns32(gs, 0, d);
+    __builtin_amdgcn_sched_barrier(0);
+    if (edge) {
 #pragma unroll
       for (int q = 0; q < 2; ++q)
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (kb0 + u * 16 + r > q0 + q * 16 + 4 * g + i + shift) {
+          for (int i = 0; i < 4; ++i) {
+            const int row = q0 + q * 16 + 4 * g + i;
+            if (kb0 + u * 16 + r > row + shift || row >= qq.len) {
               s[q][u][i] = -__builtin_inff();
               dp[q][u][i] = 0.f;
             }
+          }
     }
     U32x4 pf[2], df[2];
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const f32x4_t l4 = *reinterpret_cast<const f32x4_t*>(&ls[buf][q * 16 + 4 * g]);
-      const f32x4_t d4 = *reinterpret_cast<const f32x4_t*>(&ds_[buf][q * 16 + 4 * g]);
+    for (int q = 0; q < 2; ++q)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         float p[4], ds[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          p[i] = exp2_f(fmaf(s[q][u][i], scale, -l4[i]));
-          ds[i] = p[i] * fmaf(dp[q][u][i], kDown, -d4[i]);
+          p[i] = exp2_f(fmaf(s[q][u][i], scale, kUp - l4[q][i]));
+          ds[i] = p[i] * (F16 ? fmaf(dp[q][u][i], kDown, -d4[q][i] * kDown) : dp[q][u][i] - d4[q][i]);
         }
         pf[u].v[2 * q] = pack2<F16>(p[0], p[1]);
         pf[u].v[2 * q + 1] = pack2<F16>(p[2], p[3]);
         df[u].v[2 * q] = pack2<F16>(ds[0], ds[1]);
         df[u].v[2 * q + 1] = pack2<F16>(ds[2], ds[3]);
       }
-    }
+    U32x4 qc[ND];
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int d = 0; d < ND; ++d) {
-      U32x4 ga, qa;
+    for (int d = 0; d < ND; ++d) qc[d] = at.columns32(qs, 0, d);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int at = (q * 16 + 4 * g + (r >> 2)) * ST + 16 * d + 4 * (r & 3);
-        const u32x2_v w = lds_tr4(&gs[buf][at]);
-        const u32x2_v x = lds_tr4(&qs[buf][at]);
-        ga.v[2 * q] = w.x;
-        ga.v[2 * q + 1] = w.y;
-        qa.v[2 * q] = x.x;
-        qa.v[2 * q + 1] = x.y;
-      }
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        dv[u][d] = mfma16<F16>(ga, pf[u], dv[u][d]);
-        dk[u][d] = mfma16<F16>(qa, df[u], dk[u][d]);
-      }
-    }
+      for (int u = 0; u < 2; ++u) dv[u][d] = mfma16<F16>(gc[d], pf[u], dv[u][d]);
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) dk[u][d] = mfma16<F16>(qc[d], df[u], dk[u][d]);
+  };
+  int stage = 0;
+  for (int it = 0, q = 0; it < nt; ++it) {
+    tile_wait<(S - 2) * (UW + 1)>();
+    tile_barrier();
+    const int next = stage == 0 ? S - 1 : stage - 1;
+    step(q_first + q * QT, lds[stage], lds[next]);
+    stage = stage == S - 1 ? 0 : stage + 1;
+    q = q + 1 == per_head ? 0 : q + 1;
   }
+  if (nt > 0) tile_wait<0>();
   // every row of the slot is written: those behind its length with zeros
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
