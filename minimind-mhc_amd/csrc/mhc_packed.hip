@@ -4,7 +4,6 @@
 // tensors (bf16 or fp16), fp32 scores, sums and outputs, one rounding of the probabilities
 // (they are a product's operand) and one of the output.
 //   S_ij = scale q_i . k_j (j <= i + keys - queries),  O_i = sum_j softmax(S_i)_j v_j
-#include <stdlib.h>
 #include "mhc_packed.hpp"
 
 namespace mhc {
@@ -56,8 +55,8 @@ __global__ __launch_bounds__(256 * KS, 2) void packed_fwd_kernel(PackedAttnArgs 
   TileLoader<HD, UW> kl, vl;
   kl.init(wave * UW, ks_t);
   vl.init(wave * UW, vs_t);
-  // the i-th key tile of this half; past the range the last one again, so that every step
-  // has as many loads in flight
+  // the i-th key tile of this half (a half without one loads the last again: the barriers and
+  // waits are the same for all)
   auto issue = [&](int i, uint16_t* __restrict__ kd, uint16_t* __restrict__ vd) {
     const int kt = min(t0 + i * KS + half, t1 - 1);
     const int left = kk.len - kt * KT;
@@ -73,10 +72,9 @@ __global__ __launch_bounds__(256 * KS, 2) void packed_fwd_kernel(PackedAttnArgs 
 #pragma unroll
     for (int c = 0; c < NC; ++c) qb[u][c] = ld16(q + 32 * c);
   }
-  if (steps > 0) {
 #pragma unroll
-    for (int i = 0; i < S - 1; ++i) issue(i, lds[half][i][0], lds[half][i][1]);
-  }
+  for (int i = 0; i < S - 1; ++i)
+    if (i < steps) issue(i, lds[half][i][0], lds[half][i][1]);
   const float scale = a.scale * kPackedLog2e;
   constexpr float kHead = packed_head<F16>;
   float m[2] = {kNoScore, kNoScore};
@@ -97,7 +95,7 @@ __global__ __launch_bounds__(256 * KS, 2) void packed_fwd_kernel(PackedAttnArgs 
   auto step = [&](int i, const uint16_t* __restrict__ ks, uint16_t* __restrict__ vs, uint16_t* __restrict__ kd,
                   uint16_t* __restrict__ vd) {
     const int kt = t0 + i * KS + half, s0 = kt * KT;
-    issue(i + S - 1, kd, vd);
+    if (i + S - 1 < steps) issue(i + S - 1, kd, vd);
     // V rows that are not there: probability 0 times an infinite copy of the last would be
     // NaN.  Only a sequence's last tile has any (uniform over the workgroup's half; both
     // halves take part in the barrier).
@@ -147,14 +145,13 @@ __global__ __launch_bounds__(256 * KS, 2) void packed_fwd_kernel(PackedAttnArgs 
           for (int i = 0; i < 4; ++i)
             if (s0 + st * 16 + 4 * g + i > pb + u * 16 + r + shift) s[u][st][i] = -__builtin_inff();
     }
-    U32x4 pf[2][2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       float mx = -__builtin_inff();
 #pragma unroll
       for (int st = 0; st < 4; ++st)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[u][st][i]);
+        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[u][st][j]);
       mx *= scale;
       if (__any(!(mx <= m[u] + kPackedLazyMax + kHead))) {
         mx = fmaxf(mx, xor_lane16(mx));
@@ -163,45 +160,59 @@ __global__ __launch_bounds__(256 * KS, 2) void packed_fwd_kernel(PackedAttnArgs 
         const float f = exp2_f(m[u] - mx);
         m[u] = mx;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) l[u][i] *= f;
+        for (int j = 0; j < 4; ++j) l[u][j] *= f;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[u][d][i] *= f;
-      }
-#pragma unroll
-      for (int st = 0; st < 4; ++st) {
-        float p[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = exp2_f(fmaf(s[u][st][i], scale, -m[u]));
-        pf[u][st >> 1].v[2 * (st & 1)] = pack2<F16>(p[0], p[1]);
-        pf[u][st >> 1].v[2 * (st & 1) + 1] = pack2<F16>(p[2], p[3]);
+          for (int j = 0; j < 4; ++j) o[u][d][j] *= f;
       }
     }
+    U32x4 pf[2][2];
+    auto softmax = [&](int hh) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          float p[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) p[j] = exp2_f(fmaf(s[u][2 * hh + q][j], scale, -m[u]));
+          pf[u][hh].v[2 * q] = pack2<F16>(p[0], p[1]);
+          pf[u][hh].v[2 * q + 1] = pack2<F16>(p[2], p[3]);
+        }
+    };
+    auto outputs = [&](int hh) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) l[u] = mfma16<F16>(ones, pf[u][hh], l[u]);
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) o[u][d] = mfma16<F16>(va[hh][d], pf[u][hh], o[u][d]);
+    };
+    softmax(0);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int d = 0; d < ND; ++d) va[1][d] = at.columns32(vs, 1, d);
     __builtin_amdgcn_sched_barrier(0);
+    // the first half's products with the second half's softmax between them
+    outputs(0);
+    softmax(1);
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      l[0] = mfma16<F16>(ones, pf[0][hh], l[0]);
-      l[1] = mfma16<F16>(ones, pf[1][hh], l[1]);
-#pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        o[0][d] = mfma16<F16>(va[hh][d], pf[0][hh], o[0][d]);
-        o[1][d] = mfma16<F16>(va[hh][d], pf[1][hh], o[1][d]);
-      }
+    for (int x = 0; x < 2 * ND + 2; ++x) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x402, ND == 4 ? 4 : 3, 0);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    outputs(1);
   };
   int stage = 0;
   for (int i = 0; i < steps; ++i) {
-    tile_wait<(S - 2) * 2 * UW>();
+    if (S > 2 && i + S - 1 <= steps) tile_wait<(S - 2) * 2 * UW>();
+    else tile_wait<0>();
     tile_barrier();  // this step's tile has landed, and every wave is done with the one before
     const int next = stage == 0 ? S - 1 : stage - 1;
     step(i, lds[half][stage][0], lds[half][stage][1], lds[half][next][0], lds[half][next][1]);
     stage = stage == S - 1 ? 0 : stage + 1;
   }
-  if (steps > 0) tile_wait<0>();  // the loads past the range: nothing may land after this
   if constexpr (KS == 2) {  // the halves meet in LDS
     __syncthreads();
     float* x = reinterpret_cast<float*>(lds) + wave * 64 * (2 * ND * 4 + 4) + lane * 4;
@@ -527,12 +538,12 @@ hipError_t packed_fwd_hd(const PackedAttnArgs& a, hipStream_t s) {
     packed_few_kernel<F16, HD><<<dim3((unsigned)(ranges * a.kv_heads * nb)), 256, 0, s>>>(a);
   } else {
     const dim3 grid((unsigned)((int64_t)a.qtiles * a.splits * (a.heads / a.row_heads)));
-    const int ks = getenv("KS") ? atoi(getenv("KS")) : grid.x <= (unsigned)device_cus() * 5 / 4 ? 2 : 1;
+    const bool halves = packed_halves(grid.x);
     if (a.row_heads == 2) {
-      if (ks == 2) packed_fwd_kernel<F16, HD, 2, 2><<<grid, 512, 0, s>>>(a);
+      if (halves) packed_fwd_kernel<F16, HD, 2, 2><<<grid, 512, 0, s>>>(a);
       else packed_fwd_kernel<F16, HD, 2, 1><<<grid, 256, 0, s>>>(a);
     } else {
-      if (ks == 2) packed_fwd_kernel<F16, HD, 1, 2><<<grid, 512, 0, s>>>(a);
+      if (halves) packed_fwd_kernel<F16, HD, 1, 2><<<grid, 512, 0, s>>>(a);
       else packed_fwd_kernel<F16, HD, 1, 1><<<grid, 256, 0, s>>>(a);
     }
   }
@@ -563,13 +574,12 @@ void packed_attn_plan(PackedAttnArgs& a) {
     a.row_heads = rep % 2 == 0 ? 2 : 1;
     a.qtiles = (int)packed_tiles(a.Tq, a.B, 128 / a.row_heads);
     units = ((int64_t)a.Tq * a.row_heads / 128 + 1) * (a.heads / a.row_heads);
-    tile = 256;
+    tile = 512;
   }
   const int64_t keys = a.Tk / B;  // of a sequence, on average
   int64_t want = units > 0 ? (int64_t)device_cus() * (a.few ? 4 : 2) / units : 1;
   if (want > keys / tile) want = keys / tile;
   if (want > 128) want = 128;
-  if (getenv("SPL")) want = atoi(getenv("SPL"));
   a.splits = want < 1 ? 1 : (int)want;
 }
 int64_t packed_attn_workspace(const PackedAttnArgs& a) {

@@ -119,20 +119,24 @@ __device__ __forceinline__ void packed_rank(const int* cu, int B, int T, int M, 
   }
   constexpr int C = kRankSeqs / 64;
   const int lane = __lane_id();
+  int start[C], len[C], other[C], olen[C], used[C];
   float n[C], past[C];  // small whole numbers, exact in fp32
   float most = 0.f;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int i = c * 64 + lane;
+    start[c] = len[c] = other[c] = olen[c] = used[c] = 0;
     n[c] = past[c] = 0.f;
     if (c * 64 < B && i < B) {
-      const int len = max(seq_start(cu, i + 1, T) - seq_start(cu, i, T), 0);
-      n[c] = (float)((len + M - 1) / M);
-      if (!FIRST) {
-        int keys = max(seq_start(cu_o, i + 1, To) - seq_start(cu_o, i, To), 0);
-        if (used_o) keys = min(max(used_o[i], 0), keys);
-        past[c] = (float)(max(keys - len, 0) / M);
-      }
+      const int s0 = cu[i], s1 = cu[i + 1], o0 = cu_o[i], o1 = cu_o[i + 1];  // all before the first use
+      const int ut = used_t ? used_t[i] : 0x7fffffff, uo = used_o ? used_o[i] : 0x7fffffff;
+      start[c] = i == 0 ? 0 : min(max(s0, 0), T);
+      len[c] = max(min(max(s1, 0), T) - start[c], 0);
+      used[c] = min(max(ut, 0), len[c]);
+      other[c] = i == 0 ? 0 : min(max(o0, 0), To);
+      olen[c] = min(max(uo, 0), max(min(max(o1, 0), To) - other[c], 0));
+      n[c] = (float)((len[c] + M - 1) / M);
+      if (!FIRST) past[c] = (float)(max(olen[c] - len[c], 0) / M);
       most = fmaxf(most, n[c] + past[c]);
     }
   }
@@ -144,37 +148,48 @@ __device__ __forceinline__ void packed_rank(const int* cu, int B, int T, int M, 
     return __builtin_amdgcn_readfirstlane((int)wave_sum(x));
   };
   const int total = count(0.f);
-  int seq = B, tile = rank - total;
-  if (rank < total) {
-    int lo = 0, hi = __builtin_amdgcn_readfirstlane((int)wave_max(most)), above = 0;  // count(lo) > rank >= count(hi)
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2, x = count((float)mid);
-      if (x > rank) {
-        lo = mid;
-      } else {
-        hi = mid;
-        above = x;
-      }
-    }
-    int k = rank - above;  // which of the level's tiles
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const bool has = past[c] <= (float)lo && (float)lo < past[c] + n[c];
-      const uint64_t mask = __ballot(has);
-      const int here = __popcll(mask);
-      if (k >= 0 && k < here) {
-        const uint64_t me = __ballot(has && __popcll(mask & ((1ull << lane) - 1)) == k);
-        const int l = __ffsll((unsigned long long)me) - 1;
-        seq = c * 64 + l;
-        const int first = (int)__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, past[c]), l));
-        const int num = (int)__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, n[c]), l));
-        tile = FIRST ? num - 1 - (lo - first) : lo - first;
-      }
-      k -= here;
+  if (rank >= total) {  // rows behind the last sequence
+    packed_bounds(cu, B, T, M, B, rank - total, cu_o, To, used_t, used_o, t, o);
+    return;
+  }
+  int lo = 0, hi = __builtin_amdgcn_readfirstlane((int)wave_max(most)), above = 0;  // count(lo) > rank >= count(hi)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2, x = count((float)mid);
+    if (x > rank) {
+      lo = mid;
+    } else {
+      hi = mid;
+      above = x;
     }
   }
-  packed_bounds(cu, B, T, M, seq, tile, cu_o, To, used_t, used_o, t, o);
+  int k = rank - above;  // which of the level's tiles
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const bool has = past[c] <= (float)lo && (float)lo < past[c] + n[c];
+    const uint64_t mask = __ballot(has);
+    const int here = __popcll(mask);
+    if (k >= 0 && k < here) {
+      const uint64_t me = __ballot(has && __popcll(mask & ((1ull << lane) - 1)) == k);
+      const int l = __ffsll((unsigned long long)me) - 1;
+      const int level = lo - (int)__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, past[c]), l));
+      const int num = (int)__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, n[c]), l));
+      t.seq = c * 64 + l;
+      t.start = __builtin_amdgcn_readlane(start[c], l);
+      t.end = t.start + __builtin_amdgcn_readlane(len[c], l);
+      t.used = __builtin_amdgcn_readlane(used[c], l);
+      t.first = t.start + (FIRST ? num - 1 - level : level) * M;
+      o.start = __builtin_amdgcn_readlane(other[c], l);
+      o.len = __builtin_amdgcn_readlane(olen[c], l);
+    }
+    k -= here;
+  }
 }
+// Whether a workgroup is two halves of four waves that share its tiles: where the launch has
+// about one workgroup a CU, so the longest chain of tiles sets its time.  Forward: one sequence
+// of 4096 tokens, 8 / 4 heads of 96 (264 workgroups), 71 us and 91 without; 12 sequences of 8192
+// tokens together (564), 52 and 47.  dK and dV of those (308): 102 and 139; of 3 sequences of
+// 16001 tokens, 8 heads of 64 (1032): 372 and 350.
+inline bool packed_halves(unsigned workgroups) { return workgroups <= (unsigned)device_cus() * 5 / 4; }
 // Tile numbers of T rows in B sequences.
 inline int64_t packed_tiles(int64_t T, int64_t B, int M) { return T / M + B + 1; }
 
@@ -199,7 +214,7 @@ __device__ __forceinline__ int tile_slot(int row, int slot) {
 }
 template <int HD>
 __device__ __forceinline__ int tile_column(int row, int place) {  // the slot that lies there
-  if constexpr (HD == 96) return (place + 24 - (row >> 2)) % 12;
+  if constexpr (HD == 96) return (place + 36 - (row >> 2)) % 12;  // 36: no negative remainder up to row 147
   else return tile_slot<HD>(row, place);
 }
 // `N` of the tile's 1 KiB units, from unit u0 on, by this wave.

@@ -44,9 +44,9 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
   kl.init(wave * UW, ks_t);
   vl.init(wave * UW, vs_t);
   auto issue = [&](int i, uint16_t* __restrict__ kd, uint16_t* __restrict__ vd) {
-    const int kt = min(i, nt - 1), left = kk.len - kt * KT;
-    kl.issue(kd, kg + (int64_t)kt * KT * ks_t, wave * UW, ks_t, KT, left);
-    vl.issue(vd, vg + (int64_t)kt * KT * vs_t, wave * UW, vs_t, KT, left);
+    const int left = kk.len - i * KT;
+    kl.issue(kd, kg + (int64_t)i * KT * ks_t, wave * UW, ks_t, KT, left);
+    vl.issue(vd, vg + (int64_t)i * KT * vs_t, wave * UW, vs_t, KT, left);
   };
   U32x4 qb[2][NC], gb[2][NC];
   float lse[2], delta[2];
@@ -77,10 +77,9 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
     lse[u] = a.lse[(int64_t)h * a.Tq + at];
     if (g == 0 && row < t.end) a.delta[(int64_t)h * a.Tq + row] = d;
   }
-  if (nt > 0) {
 #pragma unroll
-    for (int i = 0; i < S - 1; ++i) issue(i, lds[i][0], lds[i][1]);
-  }
+  for (int i = 0; i < S - 1; ++i)
+    if (i < nt) issue(i, lds[i][0], lds[i][1]);
   const float scale = a.scale * kPackedLog2e;
   f32x4_t dq[2][ND];
 #pragma unroll
@@ -94,12 +93,12 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
   auto step = [&](int i, const uint16_t* __restrict__ ks, const uint16_t* __restrict__ vs, uint16_t* __restrict__ kd,
                   uint16_t* __restrict__ vd) {
     const int s0 = i * KT;
-    issue(i + S - 1, kd, vd);
+    if (i + S - 1 < nt) issue(i + S - 1, kd, vd);
     if (pb >= t.end || s0 > pb + 31 + shift) return;
     const bool diagonal = s0 + KT - 1 > pb + shift;
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      f32x4_t s[2][2], dp[2][2];
+    f32x4_t s[2][2][2], dp[2][2][2];  // [half of the tile][16 query rows][16 keys]
+    U32x4 kc[2][ND], pf[2][2];
+    auto scores = [&](int hh) {
       constexpr int QS = HD == 128 ? 1 : 2;  // 16-key parts read ahead together (registers)
 #pragma unroll
       for (int q0 = 0; q0 < 2; q0 += QS) {
@@ -116,8 +115,8 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
         for (int q = q0; q < q0 + QS; ++q)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            s[u][q] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-            dp[u][q] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            s[hh][u][q] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            dp[hh][u][q] = f32x4_t{0.f, 0.f, 0.f, 0.f};
           }
 #pragma unroll
         for (int c = 0; c < NC; ++c)
@@ -125,28 +124,30 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
           for (int q = 0; q < QS; ++q)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-              s[u][q0 + q] = mfma16<F16>(ka[q][c], qb[u][c], s[u][q0 + q]);
-              dp[u][q0 + q] = mfma16<F16>(va[q][c], gb[u][c], dp[u][q0 + q]);
+              s[hh][u][q0 + q] = mfma16<F16>(ka[q][c], qb[u][c], s[hh][u][q0 + q]);
+              dp[hh][u][q0 + q] = mfma16<F16>(va[q][c], gb[u][c], dp[hh][u][q0 + q]);
             }
       }
-      U32x4 kc[ND];
+    };
+    auto mask = [&](int hh) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (s0 + hh * 32 + q * 16 + 4 * g + j > pb + u * 16 + r + shift) {
+              s[hh][u][q][j] = -__builtin_inff();
+              dp[hh][u][q][j] = 0.f;
+            }
+    };
+    auto columns = [&](int hh) {
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int d = 0; d < ND; ++d) kc[d] = at.columns32(ks, hh, d);
+      for (int d = 0; d < ND; ++d) kc[hh][d] = at.columns32(ks, hh, d);
       __builtin_amdgcn_sched_barrier(0);
-      if (diagonal) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int q = 0; q < 2; ++q)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (s0 + hh * 32 + q * 16 + 4 * g + j > pb + u * 16 + r + shift) {
-                s[u][q][j] = -__builtin_inff();
-                dp[u][q][j] = 0.f;
-              }
-      }
-      U32x4 pf[2];
+    };
+    auto softmax = [&](int hh) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -154,26 +155,57 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
           float ds[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            ds[j] = exp2_f(fmaf(s[u][q][j], scale, -lse[u])) * (dp[u][q][j] - delta[u]);
-          pf[u].v[2 * q] = pack2<F16>(ds[0], ds[1]);
-          pf[u].v[2 * q + 1] = pack2<F16>(ds[2], ds[3]);
+            ds[j] = exp2_f(fmaf(s[hh][u][q][j], scale, -lse[u])) * (dp[hh][u][q][j] - delta[u]);
+          pf[hh][u].v[2 * q] = pack2<F16>(ds[0], ds[1]);
+          pf[hh][u].v[2 * q + 1] = pack2<F16>(ds[2], ds[3]);
         }
+    };
+    auto outputs = [&](int hh) {
 #pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        dq[0][d] = mfma16<F16>(kc[d], pf[0], dq[0][d]);
-        dq[1][d] = mfma16<F16>(kc[d], pf[1], dq[1][d]);
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) dq[u][d] = mfma16<F16>(kc[hh][d], pf[hh][u], dq[u][d]);
+    };
+    scores(0);
+    if constexpr (HD == 128) {  // no registers for two halves side by side
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        if (hh) scores(1);
+        columns(hh);
+        if (diagonal) mask(hh);
+        softmax(hh);
+        outputs(hh);
       }
+    } else {
+      scores(1);
+      columns(0);
+      if (diagonal) {
+        mask(0);
+        mask(1);
+      }
+      softmax(0);
+      columns(1);
+      // the first half's products with the second half's probabilities between them
+      outputs(0);
+      softmax(1);
+#pragma unroll
+      for (int x = 0; x < 2 * ND; ++x) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x402, ND == 4 ? 8 : 6, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      outputs(1);
     }
   };
   int stage = 0;
   for (int i = 0; i < nt; ++i) {
-    tile_wait<(S - 2) * 2 * UW>();
+    if (S > 2 && i + S - 1 <= nt) tile_wait<(S - 2) * 2 * UW>();
+    else tile_wait<0>();
     tile_barrier();
     const int next = stage == 0 ? S - 1 : stage - 1;
     step(i, lds[stage][0], lds[stage][1], lds[next][0], lds[next][1]);
     stage = stage == S - 1 ? 0 : stage + 1;
   }
-  if (nt > 0) tile_wait<0>();  // the loads past the range: nothing may land after the end
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int row = pb + u * 16 + r;
@@ -196,15 +228,19 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
 // An fp16 P is 2^14 times as large, which is taken out of dS as it is formed and of dV at the
 // end: a row of many keys has probabilities below fp16's smallest normal number.  dS has
 // no bound and stays as it is: its terms under 2^-14 round at 2^-25, as any fp16 gradient does.
-template <bool F16, int HD>
-__global__ __launch_bounds__(256, HD <= 96 ? 2 : 1) void packed_dkv_kernel(PackedAttnArgs a) {
+// KS = 2: four more waves take every second tile of rows, and the halves add up at the end.
+template <bool F16, int HD, int KS>
+__global__ __launch_bounds__(256 * KS, HD <= 96 ? 2 : 1) void packed_dkv_kernel(PackedAttnArgs a) {
   constexpr int NC = HD / 32, ND = HD / 16, QT = 32, KW = 128;
   constexpr int S = 4;                     // stages
   constexpr int TILE = QT * HD;            // elements
   constexpr int UW = TILE * 2 / 1024 / 2;  // 1 KiB units a wave loads: waves 0 and 1 q, 2 and 3 g
   constexpr float kUp = F16 ? 14.f : 0.f, kDown = F16 ? 0x1p-14f : 1.f;
-  __shared__ __align__(16) uint16_t lds[S][2 * TILE + 128];  // q, g, and the rows' 32 log sums and 32 D (fp32)
-  const int tid = threadIdx.x;
+  __shared__ __align__(16) uint16_t lds_[KS][S][2 * TILE + 128];  // q, g, and the rows' 32 log sums and 32 D (fp32)
+  static_assert(KS == 1 || sizeof(lds_) >= 4 * 64 * 4 * ND * 16, "the second half's sums take the tiles' place");
+  const int tid = threadIdx.x & 255;
+  const int half = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  auto& lds = lds_[half];
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 15, g = lane >> 4;
   const int kvh = blockIdx.x % a.kv_heads;
@@ -220,7 +256,8 @@ __global__ __launch_bounds__(256, HD <= 96 ? 2 : 1) void packed_dkv_kernel(Packe
   const int q_first = max(k0 - shift, 0);
   const int n_rows = t.seq < a.B && k0 < kk.len ? max(qq.len - q_first, 0) : 0;
   const int per_head = (n_rows + QT - 1) / QT;
-  const int nt = per_head * rep;
+  const int nt = per_head * rep;          // tiles of rows, of all heads
+  const int mine = (nt - half + KS - 1) / KS, steps = (nt + KS - 1) / KS;
 
   const bool loads_g = wave >= 2;
   const int u0 = (wave & 1) * UW;
@@ -231,6 +268,16 @@ __global__ __launch_bounds__(256, HD <= 96 ? 2 : 1) void packed_dkv_kernel(Packe
   tl.init(u0, row_st);
   const int to = loads_g ? TILE : 0;
   int ih = 0, iq = 0;  // head and row tile of the next tile to load
+  auto forth = [&](int n, int& hh, int& q) {  // n <= KS tiles on
+    q += n;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      const bool over = q >= per_head;
+      q -= over ? per_head : 0;
+      hh += over;
+    }
+  };
+  if (nt > 0) forth(half, ih, iq);
   auto issue = [&](uint16_t* __restrict__ d) {
     const int q0 = q_first + iq * QT;
     const uint16_t* p0 = src + ih * head_st + q0 * row_st;
@@ -241,17 +288,11 @@ __global__ __launch_bounds__(256, HD <= 96 ? 2 : 1) void packed_dkv_kernel(Packe
     const float* p = (lane < 32 ? a.lse : a.delta) + (int64_t)(kvh * rep + ih) * a.Tq + qq.start + row;
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
                                      (__attribute__((address_space(3))) void*)(d + 2 * TILE), 4, 0, 0);
-    if (iq + 1 < per_head) {
-      ++iq;
-    } else if (ih + 1 < rep) {
-      iq = 0;
-      ++ih;
-    }  // past the last: that one again
+    forth(KS, ih, iq);
   };
-  if (nt > 0) {
 #pragma unroll
-    for (int i = 0; i < S - 1; ++i) issue(lds[i]);
-  }
+  for (int i = 0; i < S - 1; ++i)
+    if (i < mine) issue(lds[i]);
   U32x4 kb[2][NC], vb[2][NC];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -275,46 +316,50 @@ __global__ __launch_bounds__(256, HD <= 96 ? 2 : 1) void packed_dkv_kernel(Packe
     }
   TileReads<HD> at;
   at.init(r, g);
-  auto step = [&](int q0, const uint16_t* __restrict__ qs, uint16_t* __restrict__ d) {
-    issue(d);
+  auto step = [&](int q0, bool more, const uint16_t* __restrict__ qs, uint16_t* __restrict__ d) {
+    if (more) issue(d);
     const uint16_t* gs = qs + TILE;
     if (kb0 >= kk.len || q0 + QT - 1 + shift < kb0) return;  // no keys, or none that these rows see
     // the diagonal, and the sequence's last rows, behind which lie copies of the last
     const bool edge = q0 + shift < kb0 + 31 || q0 + QT > qq.len;
-    U32x4 qa[2][NC], ga[2][NC];
+    f32x4_t s[2][2], dp[2][2];  // [16 query rows][16 keys]
+    constexpr int QS = HD == 96 ? 1 : 2;  // 16-row parts read ahead together (registers)
 #pragma unroll
-    for (int q = 0; q < 2; ++q)
+    for (int q0_ = 0; q0_ < 2; q0_ += QS) {
+      U32x4 qa[QS][NC], ga[QS][NC];
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        qa[q][c] = at.row16(qs, q, c);
-        ga[q][c] = at.row16(gs, q, c);
-      }
+      for (int q = 0; q < QS; ++q)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          qa[q][c] = at.row16(qs, q0_ + q, c);
+          ga[q][c] = at.row16(gs, q0_ + q, c);
+        }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int q = q0_; q < q0_ + QS; ++q)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          s[q][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+          dp[q][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        }
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int q = 0; q < QS; ++q)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            s[q0_ + q][u] = mfma16<F16>(qa[q][c], kb[u][c], s[q0_ + q][u]);
+            dp[q0_ + q][u] = mfma16<F16>(ga[q][c], vb[u][c], dp[q0_ + q][u]);
+          }
+    }
+    U32x4 gc[ND];
     f32x4_t l4[2], d4[2];
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       l4[q] = *reinterpret_cast<const f32x4_t*>(&gs[TILE + 2 * (q * 16 + 4 * g)]);
       d4[q] = *reinterpret_cast<const f32x4_t*>(&gs[TILE + 2 * (32 + q * 16 + 4 * g)]);
     }
-    __builtin_amdgcn_sched_barrier(0);
-    f32x4_t s[2][2], dp[2][2];  // [16 query rows][16 keys]
-#pragma unroll
-    for (int q = 0; q < 2; ++q)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        s[q][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        dp[q][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-      }
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int q = 0; q < 2; ++q)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          s[q][u] = mfma16<F16>(qa[q][c], kb[u][c], s[q][u]);
-          dp[q][u] = mfma16<F16>(ga[q][c], vb[u][c], dp[q][u]);
-        }
-    U32x4 gc[ND];
-    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int d = 0; d < ND; ++d) gc[d] = at.columns32(gs, 0, d);
     __builtin_amdgcn_sched_barrier(0);
@@ -337,41 +382,96 @@ __global__ __launch_bounds__(256, HD <= 96 ? 2 : 1) void packed_dkv_kernel(Packe
     for (int q = 0; q < 2; ++q)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        float p[4], ds[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[i] = exp2_f(fmaf(s[q][u][i], scale, kUp - l4[q][i]));
-          ds[i] = p[i] * (F16 ? fmaf(dp[q][u][i], kDown, -d4[q][i] * kDown) : dp[q][u][i] - d4[q][i]);
-        }
-        pf[u].v[2 * q] = pack2<F16>(p[0], p[1]);
-        pf[u].v[2 * q + 1] = pack2<F16>(p[2], p[3]);
-        df[u].v[2 * q] = pack2<F16>(ds[0], ds[1]);
-        df[u].v[2 * q + 1] = pack2<F16>(ds[2], ds[3]);
+        for (int i = 0; i < 4; ++i) s[q][u][i] = exp2_f(fmaf(s[q][u][i], scale, kUp - l4[q][i]));
+        pf[u].v[2 * q] = pack2<F16>(s[q][u][0], s[q][u][1]);
+        pf[u].v[2 * q + 1] = pack2<F16>(s[q][u][2], s[q][u][3]);
       }
+    auto terms = [&] {  // dS
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float ds[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            ds[i] = s[q][u][i] * (F16 ? fmaf(dp[q][u][i], kDown, -d4[q][i] * kDown) : dp[q][u][i] - d4[q][i]);
+          df[u].v[2 * q] = pack2<F16>(ds[0], ds[1]);
+          df[u].v[2 * q + 1] = pack2<F16>(ds[2], ds[3]);
+        }
+    };
     U32x4 qc[ND];
-    __builtin_amdgcn_sched_barrier(0);
+    auto columns = [&] {
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int d = 0; d < ND; ++d) qc[d] = at.columns32(qs, 0, d);
-    __builtin_amdgcn_sched_barrier(0);
+      for (int d = 0; d < ND; ++d) qc[d] = at.columns32(qs, 0, d);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto values = [&] {
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
+      for (int d = 0; d < ND; ++d)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) dv[u][d] = mfma16<F16>(gc[d], pf[u], dv[u][d]);
+        for (int u = 0; u < 2; ++u) dv[u][d] = mfma16<F16>(gc[d], pf[u], dv[u][d]);
+    };
+    if constexpr (HD == 96) {  // with dV's products beside dS the registers spill
+      terms();
+      columns();
+      values();
+    } else {  // dV's products with dS between them
+      columns();
+      values();
+      terms();
+#pragma unroll
+      for (int x = 0; x < 2 * ND; ++x) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x402, ND == 4 ? 5 : 4, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int u = 0; u < 2; ++u) dk[u][d] = mfma16<F16>(qc[d], df[u], dk[u][d]);
   };
-  int stage = 0;
-  for (int it = 0, q = 0; it < nt; ++it) {
-    tile_wait<(S - 2) * (UW + 1)>();
+  int stage = 0, ch = 0, cq = 0;  // head and row tile of this step
+  if (nt > 0) forth(half, ch, cq);
+  for (int it = 0; it < steps; ++it) {
+    if (it + S - 1 <= mine) tile_wait<(S - 2) * (UW + 1)>();
+    else if (it + S - 2 <= mine) tile_wait<(S - 3) * (UW + 1)>();
+    else tile_wait<0>();
     tile_barrier();
     const int next = stage == 0 ? S - 1 : stage - 1;
-    step(q_first + q * QT, lds[stage], lds[next]);
+    if (it < mine) step(q_first + cq * QT, it + S - 1 < mine, lds[stage], lds[next]);
     stage = stage == S - 1 ? 0 : stage + 1;
-    q = q + 1 == per_head ? 0 : q + 1;
+    forth(KS, ch, cq);
   }
-  if (nt > 0) tile_wait<0>();
+  if constexpr (KS == 2) {
+    __syncthreads();
+    float* x = reinterpret_cast<float*>(lds_) + wave * 64 * (4 * ND * 4) + lane * 4;
+    if (half == 1) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          *reinterpret_cast<f32x4_t*>(x + (u * ND + d) * 256) = dk[u][d];
+          *reinterpret_cast<f32x4_t*>(x + (2 * ND + u * ND + d) * 256) = dv[u][d];
+        }
+    }
+    __syncthreads();
+    if (half == 1) return;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const f32x4_t y = *reinterpret_cast<const f32x4_t*>(x + (u * ND + d) * 256);
+        const f32x4_t z = *reinterpret_cast<const f32x4_t*>(x + (2 * ND + u * ND + d) * 256);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          dk[u][d][i] += y[i];
+          dv[u][d][i] += z[i];
+        }
+      }
+  }
   // every row of the slot is written: those behind its length with zeros
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -408,7 +508,11 @@ hipError_t packed_bwd_hd(PackedAttnArgs a, hipStream_t s) {
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
   if (a.Tk == 0) return hipSuccess;
-  packed_dkv_kernel<F16, HD><<<dim3((unsigned)(packed_tiles(a.Tk, a.B, 128) * a.kv_heads)), 256, 0, s>>>(a);
+  const dim3 kgrid((unsigned)(packed_tiles(a.Tk, a.B, 128) * a.kv_heads));
+  if (HD <= 96 && packed_halves(kgrid.x))  // at 128 eight waves do not fit the registers
+    packed_dkv_kernel<F16, HD <= 96 ? HD : 64, 2><<<kgrid, 512, 0, s>>>(a);
+  else
+    packed_dkv_kernel<F16, HD, 1><<<kgrid, 256, 0, s>>>(a);
   return hipGetLastError();
 }
 
