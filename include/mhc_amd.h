@@ -546,8 +546,8 @@ int mhc_linear_pays(const int* n, int count, int64_t M, int K, int glu);
  * B sequences one after another in 16-bit tensors (bf16 or fp16) of one dtype:
  * q [Tq, heads, head_dim], k and v [Tk, kv_heads, head_dim], head_dim 64, 96 or
  * 128, heads a multiple of kv_heads.  A head's elements are contiguous; the
- * strides of a row and of a head are given in elements (multiples of 8), data
- * pointers are 16-byte aligned.  cu_q, cu_k [B + 1] (device, int32): sequence i
+ * strides of a row (under 2^23) and of a head are given in elements (multiples
+ * of 8), data pointers are 16-byte aligned.  cu_q, cu_k [B + 1] (device, int32): sequence i
  * has the query rows cu_q[i] .. cu_q[i + 1] and the key rows cu_k[i] ..
  * cu_k[i + 1]; the first entry of both is taken as 0.  key_lengths [B] (device,
  * int32, or NULL): only the first key_lengths[i] of those key rows are in use (a

@@ -745,6 +745,9 @@ static int check_packed(const mhc::PackedAttnArgs& a, int64_t Tq, int64_t Tk, in
     return fail(hipErrorInvalidValue, "%s: too large", fn);
   for (int64_t st : {a.qs_t, a.qs_h, a.ks_t, a.ks_h, a.vs_t, a.vs_h})
     if (st % 8 != 0 || st < 0) return fail(hipErrorInvalidValue, "%s: strides must be multiples of 8 elements", fn);
+  // a tile's rows are 32-bit byte offsets apart
+  for (int64_t st : {a.qs_t, a.ks_t, a.vs_t})
+    if (st >= 1 << 23) return fail(hipErrorInvalidValue, "%s: rows must be under 2^23 elements apart", fn);
   return 0;
 }
 

@@ -697,6 +697,15 @@ def plain_call() -> bool:
                 or torch.jit.is_tracing())
 
 
+def eager_call() -> bool:
+    """Whether nothing but autograd and autocast looks at the torch ops here: no tracing,
+    compiling, transform or mode that could not follow a call into the library."""
+    return not (torch.compiler.is_compiling() or not CAN_TELL or forward_ad._current_level >= 0
+                or _len_torch_dispatch_stack() > 0
+                or (_len_torch_function_stack() > 0 and _function_modes())
+                or peek_interpreter_stack() is not None or torch.jit.is_tracing())
+
+
 def plain_module(m: torch.nn.Module, kind: type) -> bool:
     """Whether m is exactly a `kind` whose call is its class's forward: no hooks
     on it or on all modules, no forward of its own."""

@@ -21,6 +21,8 @@ Differences from the reference, all outside the mHC path:
     RMSNorm to MHCHead (out_norm).  Without autograd each runs inside the
     neighbouring HIP launch; with autograd they run as separate ops in the
     reference's order (model/model_minimind.py:326-336, :365-370);
+  * `packed` (a PackedBatch) says that the rows of a batch of one are several sequences one
+    after another; a PackedCache then takes the place of the caches that grow by copies;
   * one StreamChain per forward is passed to every mHC call, so each launch
     that writes the residual stream hands its rows' sums of squares to the
     next pre launch (used at n >= 8 or hidden > 1024).
@@ -34,11 +36,12 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from . import _ops
+from . import _ops, losses
 from ._ops import StreamChain
 from .mhc_common import MHCHead, StreamExpand
 from .mhc_fused import MHCConnection_Fused
 from .mhc_fused_no_hres import MHCConnection_FusedNoHres
+from .packed import PackedBatch, PackedCache, PackedCall
 
 
 class MiniMindConfig:
@@ -76,6 +79,8 @@ class MiniMindConfig:
         self.moe_intermediate_size = kwargs.get("moe_intermediate_size", self.intermediate_size)
         self.norm_topk_prob = kwargs.get("norm_topk_prob", True)
         self.router_aux_loss_coef = kwargs.get("router_aux_loss_coef", 5e-4)
+        # the balance loss of each sequence, averaged, instead of one over all tokens
+        self.router_aux_loss_per_sequence = kwargs.get("router_aux_loss_per_sequence", False)
         self.use_mhc = use_mhc
         self.mhc_residual_expansion = mhc_residual_expansion
         assert use_mhc in (0, 1, 2), f"use_mhc must be in {{0,1,2}}, got {use_mhc}"
@@ -148,11 +153,11 @@ class Attention(nn.Module):
         self.dropout = config.dropout
 
     def forward(self, x, position_embeddings, past_key_value=None, use_cache=False,
-                attention_mask=None):
+                attention_mask=None, packed=None, layer_id=0):
         bsz, seq_len, _ = x.shape
         xq, xk, xv = (_ops.linears(x, self.q_proj, self.k_proj, self.v_proj)
                       or (self.q_proj(x), self.k_proj(x), self.v_proj(x)))
-        route = None if attention_mask is not None else _ops.attn_route(
+        route = None if attention_mask is not None or packed is not None else _ops.attn_route(
             self, xq, xk, xv, position_embeddings, past_key_value)
         if route == "decode":
             out, past_kv = _ops.attn_decode(self, xq, xk, xv, position_embeddings,
@@ -168,6 +173,9 @@ class Attention(nn.Module):
         xq, xk = self.q_norm(xq), self.k_norm(xk)
         cos, sin = position_embeddings
         xq, xk = apply_rotary_pos_emb(xq, xk, cos, sin)
+        if packed is not None:
+            out = packed.attention(xq, xk, xv, layer_id, self.dropout if self.training else 0.0)
+            return _ops.linear(out, self.o_proj), None
         if past_key_value is not None:
             xk = torch.cat([past_key_value[0], xk], dim=1)
             xv = torch.cat([past_key_value[1], xv], dim=1)
@@ -230,8 +238,9 @@ class MOEFeedForward(nn.Module):
         self.experts = nn.ModuleList([FeedForward(config, config.moe_intermediate_size)
                                       for _ in range(config.num_experts)])
         self.aux_loss = None
+        self.expert_counts = None  # of the last training call: tokens each expert got (by sequence)
 
-    def forward(self, x):
+    def forward(self, x, cu_seqlens=None):
         b, l, d = x.shape
         xf = x.view(-1, d)
         scores = F.softmax(self.gate(xf), dim=-1)
@@ -252,12 +261,32 @@ class MOEFeedForward(nn.Module):
             if tok.numel():
                 y.index_add_(0, tok, (expert(xf[tok]) * w[mask].view(-1, 1)).to(y.dtype))
         if self.training and self.config.router_aux_loss_coef > 0:
-            load = F.one_hot(idx, self.config.num_experts).float().mean(0)
-            self.aux_loss = (load * scores.mean(0)).sum() * self.config.num_experts * \
-                self.config.router_aux_loss_coef
+            self.aux_loss, self.expert_counts = self._balance(scores, idx, b, l, cu_seqlens)
         else:
             self.aux_loss = scores.new_zeros(1).squeeze()
         return y.view(b, l, d)
+
+
+    def _balance(self, scores, idx, b, l, cu_seqlens):
+        """(balance loss, the experts' counts): on the kernels for fp32 scores on the GPU, as
+        the trainers' autocast gives, and for the loss of each sequence (cu_seqlens, or the
+        batch's rows); else one loss over all tokens on torch ops."""
+        cfg = self.config
+        each = getattr(cfg, "router_aux_loss_per_sequence", False)
+        if each and cu_seqlens is None:
+            cu_seqlens = torch.arange(b + 1, dtype=torch.int32, device=scores.device) * l
+        if scores.is_cuda and (each or scores.dtype == torch.float32) and _ops.eager_call():
+            return losses.balance_loss(scores, idx, cfg.router_aux_loss_coef, cu_seqlens if each else None)
+        hot = F.one_hot(idx, cfg.num_experts)
+        if not each:
+            load = hot.float().mean(0)
+            return (load * scores.mean(0)).sum() * cfg.num_experts * cfg.router_aux_loss_coef, None
+        ends = cu_seqlens.tolist()
+        parts = [(hot[i:j].float().sum((0, 1)) / (j - i) * scores[i:j].float().mean(0)).sum()
+                 for i, j in zip(ends, ends[1:]) if j > i]
+        counts = torch.stack([hot[i:j].sum((0, 1)) for i, j in zip(ends, ends[1:])])
+        loss = torch.stack(parts).mean() if parts else scores.float().sum() * 0.0
+        return loss * cfg.num_experts * cfg.router_aux_loss_coef, counts
 
 
 class MiniMindBlock(nn.Module):
@@ -268,7 +297,7 @@ class MiniMindBlock(nn.Module):
         super().__init__()
         self.self_attn = Attention(config)
         self.mlp = FeedForward(config) if not config.use_moe else MOEFeedForward(config)
-        self.use_mhc = config.use_mhc
+        self.use_mhc, self.layer_id = config.use_mhc, layer_id
         eps, D = config.rms_norm_eps, config.hidden_size
         self.attn_in_norm = nn.RMSNorm(D, eps=eps)
         self.ffn_in_norm = nn.RMSNorm(D, eps=eps)
@@ -279,7 +308,13 @@ class MiniMindBlock(nn.Module):
             self.mlp_mhc = cls(n, D, eps=eps)
 
     def forward(self, hidden_states, position_embeddings, past_key_value=None, use_cache=False,
-                attention_mask=None, chain=None):
+                attention_mask=None, chain=None, packed=None):
+        more, mlp = {}, self.mlp
+        if packed is not None:
+            more = {"packed": packed, "layer_id": self.layer_id}
+            if isinstance(mlp, MOEFeedForward):
+                def mlp(z):
+                    return self.mlp(z, packed.batch.cu_seqlens)
         if self.use_mhc:
             holder = [None]
 
@@ -287,19 +322,19 @@ class MiniMindBlock(nn.Module):
             # its pre launch when no autograd is needed).
             def attn_fn(zn):
                 out, kv = self.self_attn(zn, position_embeddings, past_key_value, use_cache,
-                                         attention_mask)
+                                         attention_mask, **more)
                 holder[0] = kv
                 return out
 
             hidden_states = self.attn_mhc(hidden_states, attn_fn, in_norm=self.attn_in_norm,
                                           chain=chain)
-            hidden_states = self.mlp_mhc(hidden_states, self.mlp, in_norm=self.ffn_in_norm,
+            hidden_states = self.mlp_mhc(hidden_states, mlp, in_norm=self.ffn_in_norm,
                                          chain=chain)
             return hidden_states, holder[0]
         attn_out, kv = self.self_attn(self.attn_in_norm(hidden_states), position_embeddings,
-                                      past_key_value, use_cache, attention_mask)
+                                      past_key_value, use_cache, attention_mask, **more)
         hidden_states = hidden_states + attn_out
-        hidden_states = hidden_states + self.mlp(self.ffn_in_norm(hidden_states))
+        hidden_states = hidden_states + mlp(self.ffn_in_norm(hidden_states))
         return hidden_states, kv
 
 
@@ -329,8 +364,11 @@ class MiniMindModel(nn.Module):
         self.register_buffer("freqs_sin", sin, persistent=False)
 
     def forward(self, input_ids, attention_mask=None, past_key_values=None, use_cache=False,
-                **kwargs):
+                packed=None, **kwargs):
         bsz, seq_len = input_ids.shape
+        call, cache = None, None
+        if packed is not None:
+            call, cache, past_key_values = self._packed_call(input_ids, attention_mask, past_key_values, packed)
         past_key_values = past_key_values or [None] * len(self.layers)
         start = past_key_values[0][0].shape[1] if past_key_values[0] is not None else 0
         h = self.dropout(self.embed_tokens(input_ids))
@@ -342,12 +380,20 @@ class MiniMindModel(nn.Module):
             h = self.embed_up_norm[1].forward_normed(h, self.embed_up_norm[0], chain=chain)
         else:
             h = self.embed_up_norm(h)
-        pos = (self.freqs_cos[start:start + seq_len], self.freqs_sin[start:start + seq_len])
+        if call is None:
+            pos = (self.freqs_cos[start:start + seq_len], self.freqs_sin[start:start + seq_len])
+        else:  # each row's position in its own sequence (rows of none: any)
+            at = call.positions.clamp(0, self.freqs_cos.shape[0] - 1)
+            pos = (self.freqs_cos[at], self.freqs_sin[at])
+        more = {} if call is None else {"packed": call}
         presents = []
         for layer, pkv in zip(self.layers, past_key_values):
             h, present = layer(h, pos, past_key_value=pkv, use_cache=use_cache,
-                               attention_mask=attention_mask, chain=chain)
+                               attention_mask=attention_mask, chain=chain, **more)
             presents.append(present)
+        if call is not None:
+            call.done()
+            presents = cache
         if self.config.use_mhc:  # MHCHead + final RMSNorm, one launch without autograd
             h = self.norm[0](h, out_norm=self.norm[1], chain=chain)
         else:
@@ -355,6 +401,18 @@ class MiniMindModel(nn.Module):
         aux = sum([l.mlp.aux_loss for l in self.layers if isinstance(l.mlp, MOEFeedForward)],
                   h.new_zeros(1).squeeze())
         return h, presents, aux
+
+
+    def _packed_call(self, input_ids, attention_mask, cache, packed):
+        """(the PackedCall, its cache or None, past_key_values for the layers)."""
+        if not isinstance(packed, PackedBatch) or tuple(input_ids.shape) != (1, packed.rows):
+            raise ValueError(f"packed must be a PackedBatch of input_ids' rows, [1, rows], not of "
+                             f"{tuple(input_ids.shape)}")
+        if attention_mask is not None:
+            raise ValueError("packed sequences take no attention_mask: nothing of them is padding")
+        if cache is not None and not isinstance(cache, PackedCache):
+            raise ValueError("packed sequences need a PackedCache as past_key_values")
+        return PackedCall(packed, cache), cache, None
 
 
 class MiniMindForCausalLM(nn.Module):
@@ -374,11 +432,51 @@ class MiniMindForCausalLM(nn.Module):
         sl = slice(-logits_to_keep, None) if isinstance(logits_to_keep, int) else logits_to_keep
         logits = _ops.linear(h[:, sl, :], self.lm_head)
         loss = None
-        if labels is not None:
+        packed = kwargs.get("packed")
+        if labels is not None and packed is not None:
+            loss = self._packed_loss(logits, labels, packed)
+        elif labels is not None:
             x, y = logits[..., :-1, :].contiguous(), labels[..., 1:].contiguous()
             loss = F.cross_entropy(x.view(-1, x.size(-1)), y.view(-1), ignore_index=-100)
         return SimpleNamespace(loss=loss, aux_loss=aux, logits=logits, past_key_values=pkv,
                                hidden_states=h)
+
+
+    @staticmethod
+    def _token_logprobs(logits, labels):
+        if logits.is_cuda and _ops.eager_call():
+            return losses.token_logprobs(logits, labels)
+        return -F.cross_entropy(logits.float(), labels, ignore_index=-100, reduction="none")
+
+    def _packed_loss(self, logits, labels, packed):
+        """The mean cross entropy of the next tokens, within each sequence."""
+        if logits.shape[1] != packed.rows:
+            raise ValueError("labels of packed sequences need the logits of every row (logits_to_keep=0)")
+        y = packed.next_labels(labels)
+        return -self._token_logprobs(logits[0], y[0]).sum() / (y != -100).sum()
+
+    def sequence_logprobs(self, input_ids, labels, packed, average=False):
+        """The sum (average: mean) of the log-probabilities of each packed sequence's counted
+        labels, fp32 [n]: what preference_loss takes from its reference model.  Sums in 64 bits."""
+        y = packed.next_labels(labels)[0]
+        lp = self._token_logprobs(self(input_ids, packed=packed).logits[0], y)
+        at = packed.cu_seqlens.long()
+        def sums(t):  # noqa: E306
+            return F.pad(t.double().cumsum(0), (1, 0))[at].diff()
+        total = sums(lp)
+        return (total / sums(y != -100).clamp_min(1) if average else total).float()
+
+    def preference_loss(self, input_ids, labels, packed, reference, beta=0.1, label_smoothing=0.0,
+                        average=False):
+        """The preference loss of packed pairs of answers (losses.preference_loss: the first
+        half of the sequences chosen, the second rejected; labels -100 where a token does not
+        count) plus the routers' balance loss, with the rewards."""
+        out = self(input_ids, packed=packed)
+        loss, chosen, rejected = losses.preference_loss(
+            out.logits[0], packed.next_labels(labels)[0], packed.cu_seqlens, reference, beta,
+            label_smoothing, average)
+        return SimpleNamespace(loss=loss + out.aux_loss, aux_loss=out.aux_loss, chosen_rewards=chosen,
+                               rejected_rewards=rejected, logits=out.logits)
 
 
 def init_normal_(model: nn.Module, std: float = 0.02) -> nn.Module:

@@ -32,7 +32,7 @@ def _bounds(name: str, t, n: Optional[int], dev: torch.device) -> torch.Tensor:
 def _strided(t: torch.Tensor):
     """(t, its row and head strides); a copy in order where the kernels cannot take t's."""
     row, head = (t.stride(i) if t.shape[i] > 1 else 0 for i in (0, 1))
-    if t.stride(2) != 1 or row % 8 or head % 8 or t.data_ptr() % 16:
+    if t.stride(2) != 1 or row % 8 or head % 8 or row >= 1 << 23 or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
         row, head = t.shape[1] * t.shape[2], t.shape[2]
     return t, row, head
@@ -148,3 +148,140 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     if _ops.wants_graph(q, k, v):
         return _PackedAttention.apply(q, k, v, cu_q, cu_k, used, scale)
     return _forward(q, k, v, cu_q, cu_k, used, scale, False)[0]
+
+
+class PackedBatch:
+    """The sequences of one packed call: their bounds, and each row's place in its own.
+
+    cu_seqlens [n + 1] int32: sequence i has the rows cu_seqlens[i] to cu_seqlens[i + 1] of
+    `rows`, beginning with row 0; rows behind the last belong to none (their outputs mean
+    nothing).  Everything stays on cu_seqlens' device, without a synchronisation."""
+
+    def __init__(self, cu_seqlens: torch.Tensor, rows: int):
+        self.cu_seqlens = _bounds("cu_seqlens", cu_seqlens, None, cu_seqlens.device)
+        self.rows = int(rows)
+        self.longest: Optional[int] = None  # of the sequences, where the host knows
+        r = torch.arange(self.rows, dtype=torch.int32, device=cu_seqlens.device)
+        self.sequence = torch.searchsorted(self.cu_seqlens[1:], r, right=True)  # n behind the last
+        self.positions = (r - self.cu_seqlens[self.sequence]).long()
+
+    @classmethod
+    def from_lengths(cls, lengths, rows: Optional[int] = None, device="cuda") -> "PackedBatch":
+        """Of these lengths; rows: their sum, or more."""
+        ends = [0]
+        for n in lengths:
+            if n < 0:
+                raise ValueError(f"mhc_amd: a sequence of {n} tokens")
+            ends.append(ends[-1] + int(n))
+        rows = ends[-1] if rows is None else rows
+        if rows < ends[-1]:
+            raise ValueError(f"mhc_amd: {ends[-1]} tokens do not fit {rows} rows")
+        b = cls(torch.tensor(ends, dtype=torch.int32, device=device), rows)
+        b.longest = max(lengths, default=0)
+        return b
+
+    def __len__(self) -> int:
+        return self.cu_seqlens.numel() - 1
+
+    def next_labels(self, labels: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
+        """labels [1, rows] moved up by one row within each sequence: what each row is to
+        predict, ignore_index in a sequence's last row and behind the last."""
+        if tuple(labels.shape) != (1, self.rows):
+            raise ValueError(f"mhc_amd: labels {tuple(labels.shape)} are not [1, {self.rows}]")
+        n = len(self)
+        after = torch.cat([self.sequence[1:], self.sequence.new_full((1,), n)]) if self.rows else self.sequence
+        moved = torch.cat([labels[:, 1:], labels[:, :1]], 1)
+        return moved.masked_fill((after != self.sequence) | (self.sequence == n), ignore_index)
+
+
+class PackedCache:
+    """Keys and values of n sequences that grow in place, each in a slot of `capacity` rows
+    with a length of its own: pass it as past_key_values with a PackedBatch of n sequences.
+
+    A call appends its sequences' tokens and moves `lengths` on (on the device, so a captured
+    decode step can be replayed).  Tokens that a slot has no room for are not stored, and
+    their sequence's outputs mean nothing from then on; a batch made from_lengths is refused
+    before that.  Rows of no sequence change nothing."""
+
+    def __init__(self, config, sequences: int, capacity: int, dtype=torch.bfloat16, device="cuda"):
+        if sequences < 1 or capacity < 1:
+            raise ValueError(f"mhc_amd: a cache of {sequences} slots of {capacity} rows")
+        shape = (sequences * capacity + 1, config.num_key_value_heads, config.head_dim)  # the last: what is dropped
+        self.layers = [tuple(torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
+                       for _ in range(config.num_hidden_layers)]
+        self.slots = torch.arange(sequences + 1, dtype=torch.int32, device=device) * capacity
+        self.lengths = torch.zeros(sequences, dtype=torch.int32, device=device)
+        self.sequences, self.capacity = sequences, capacity
+        self._most = 0  # a bound on the lengths, as far as the host has seen
+
+    def clear(self) -> None:
+        """Empties every slot."""
+        self.lengths.zero_()
+        self._most = 0
+
+
+class PackedCall:
+    """One model call on a PackedBatch: positions, and with a cache where rows go."""
+
+    def __init__(self, batch: PackedBatch, cache: Optional[PackedCache] = None):
+        self.batch, self.cache = batch, cache
+        self.positions, self.lengths, self.rows = batch.positions, None, None
+        if cache is None:
+            return
+        n, cap = cache.sequences, cache.capacity
+        if len(batch) != n:
+            raise ValueError(f"mhc_amd: a batch of {len(batch)} sequences on a cache of {n}")
+        if batch.longest is not None:
+            if cache._most + batch.longest > cap:
+                raise ValueError(f"mhc_amd: {cache._most} + {batch.longest} tokens may not fit slots of {cap} rows")
+            cache._most += batch.longest
+        seq = batch.sequence.clamp_max(n - 1)
+        self.positions = cache.lengths[seq] + batch.positions
+        room = (batch.sequence < n) & (self.positions < cap)
+        self.rows = torch.where(room, seq * cap + self.positions, n * cap)
+        self.lengths = (cache.lengths + batch.cu_seqlens.diff()).clamp_max_(cap)
+
+    def done(self) -> None:
+        if self.cache is not None:
+            self.cache.lengths.copy_(self.lengths)
+
+    def attention(self, q, k, v, layer: int, dropout: float = 0.0) -> torch.Tensor:
+        """q [1, rows, heads, head_dim], k, v [1, rows, kv heads, head_dim] of the new tokens:
+        [1, rows, heads * head_dim], over their sequences' keys so far."""
+        q, k, v, cu = q[0], k[0], v[0], self.batch.cu_seqlens
+        cu_k, used = cu, None
+        if self.cache is not None:
+            if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+                raise RuntimeError("mhc_amd: a cache is for inference; call under torch.no_grad()")
+            ck, cv = self.cache.layers[layer]
+            ck.index_copy_(0, self.rows, k.to(ck.dtype))
+            cv.index_copy_(0, self.rows, v.to(cv.dtype))
+            q, k, v, cu_k, used = q.to(ck.dtype), ck, cv, self.cache.slots, self.lengths
+        half = q.dtype in _ops.HALF or torch.is_autocast_enabled("cuda")
+        if q.is_cuda and half and q.shape[2] in HEAD_DIMS and dropout == 0.0 and _ops.eager_call():
+            out = packed_attention(q, k, v, cu, cu_seqlens_k=cu_k, key_lengths=used)
+        else:
+            out = _plain_attention(q, k, v, cu, cu_k, used, dropout)
+        return out.reshape(1, out.shape[0], -1)
+
+
+def _plain_attention(q, k, v, cu_q, cu_k, used, dropout):
+    """packed_attention on torch ops, for what the kernels do not take (fp32, the CPU, other
+    head_dims, dropout): one attention under a mask over all rows."""
+    def places(cu, rows):
+        r = torch.arange(rows, dtype=torch.int32, device=q.device)
+        seq = torch.searchsorted(cu[1:], r, right=True)
+        return seq, r - cu[seq]
+    (qs, qp), (ks, kp) = places(cu_q, q.shape[0]), places(cu_k, k.shape[0])
+    n = cu_q.numel() - 1
+    new, have = cu_q.diff(), cu_k.diff() if used is None else used
+    shift = torch.cat([have - new, new.new_zeros(1)])  # the last query sits at the last key
+    inside = kp < torch.cat([have, new.new_zeros(1)])[ks]
+    seen = (qs[:, None] == ks) & inside & (kp <= (qp + shift[qs])[:, None]) & (qs < n)[:, None]
+    rep = q.shape[1] // k.shape[1]
+    k, v = (torch.where((inside & (ks < n))[:, None, None], t, 0).repeat_interleave(rep, 1).transpose(0, 1)
+            for t in (k, v))
+    some = seen.any(1)
+    out = torch.nn.functional.scaled_dot_product_attention(
+        q.transpose(0, 1)[None], k[None], v[None], attn_mask=seen | ~some[:, None], dropout_p=dropout)
+    return torch.where(some[:, None, None], out[0].transpose(0, 1), 0)
