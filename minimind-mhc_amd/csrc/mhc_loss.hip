@@ -139,7 +139,8 @@ template <int DT>
 __global__ __launch_bounds__(256) void logprob_bwd_kernel(LogitArgs a) {
   constexpr int PER = kPer16<DT>;
   constexpr int EB = DT == kF32 ? 4 : 2;
-  const int64_t row = blockIdx.x;
+  // from the last row back: the forward pass's last rows are still in the memory-side cache
+  const int64_t row = a.T - 1 - blockIdx.x;
   const int64_t label = a.labels[row];
   const int tid = threadIdx.x;
   const bool counts = label != a.ignore;
@@ -271,35 +272,62 @@ __global__ __launch_bounds__(256) void balance_kernel(BalanceArgs a) {
   for (int e = tid; e < a.E; e += 256) a.part_count[at + e] = counts[e];
 }
 
-// One workgroup: the sequences in turn, then the mean over those with rows.
-__global__ __launch_bounds__(256) void balance_join_kernel(BalanceArgs a) {
-  __shared__ double red[4];
-  const int tid = threadIdx.x;
+// One workgroup joins the ranges: LP lanes a (sequence, expert) pair, each every LP-th range
+// in order, in 64 bits; then the mean over the sequences with rows.  One launch after the sums
+// takes as long as a launch does; with the sequences in turn and a lane an expert 44 us.
+__global__ __launch_bounds__(1024) void balance_join_kernel(BalanceArgs a) {
+  __shared__ double red[16];
+  __shared__ int full[16];
+  const int tid = threadIdx.x, pairs = a.B * a.E;
+  int lp = 1;
+  while (lp < 32 && pairs * lp * 2 <= 2048) lp *= 2;
   double loss = 0.0;
   int filled = 0;
-  for (int seq = 0; seq < a.B; ++seq) {
+  auto rows = [&](int seq) {
     const int t0 = a.cu ? seq_start(a.cu, seq, a.T) : 0;
-    const int n = (a.cu ? max(seq_start(a.cu, seq + 1, a.T), t0) : a.T) - t0;
-    filled += n > 0;
-    for (int e = tid; e < a.E; e += 256) {
-      double s = 0.0;
-      int64_t c = 0;
-      for (int p = 0; p < a.parts; ++p) {
-        const int64_t at = ((int64_t)seq * a.parts + p) * a.E + e;
-        s += (double)a.part_sum[at];
-        c += a.part_count[at];
-      }
-      a.counts[(int64_t)seq * a.E + e] = c;
-      if (n > 0) loss += (double)c / n * (s / n);
+    return (a.cu ? max(seq_start(a.cu, seq + 1, a.T), t0) : a.T) - t0;
+  };
+  for (int i = tid; i < a.B; i += 1024) filled += rows(i) > 0;
+  const int sub = tid % lp;
+  for (int pair0 = 0; pair0 < pairs; pair0 += 1024 / lp) {  // uniform: every lane takes part in the sums
+    const int pair = pair0 + tid / lp;
+    const bool live = pair < pairs;
+    const int seq = live ? pair / a.E : 0, e = live ? pair % a.E : 0;
+    const int64_t at = (int64_t)seq * a.parts * a.E + e;
+    double s = 0.0;
+    int64_t c = 0;
+#pragma unroll 4
+    for (int p = live ? sub : a.parts; p < a.parts; p += lp) {
+      s += (double)a.part_sum[at + (int64_t)p * a.E];
+      c += a.part_count[at + (int64_t)p * a.E];
     }
+    for (int o = lp / 2; o > 0; o >>= 1) {
+      s += __shfl_xor(s, o, 64);
+      c += __shfl_xor(c, o, 64);
+    }
+    if (!live || sub != 0) continue;
+    a.counts[pair] = c;
+    const int n = rows(seq);
+    if (n > 0) loss += (double)c / n * (s / n);
   }
-  for (int o = 32; o > 0; o >>= 1) loss += __shfl_xor(loss, o, 64);
-  if ((tid & 63) == 0) red[tid >> 6] = loss;
+  for (int o = 32; o > 0; o >>= 1) {
+    loss += __shfl_xor(loss, o, 64);
+    filled += __shfl_xor(filled, o, 64);
+  }
+  if ((tid & 63) == 0) {
+    red[tid >> 6] = loss;
+    full[tid >> 6] = filled;
+  }
   __syncthreads();
   if (tid != 0) return;
-  const double total = (red[0] + red[1]) + (red[2] + red[3]);
-  a.loss[0] = filled ? (float)((double)a.coef * a.E * total / filled) : 0.f;
-  a.filled[0] = filled;
+  double total = 0.0;
+  int n = 0;
+  for (int w = 0; w < 16; ++w) {
+    total += red[w];
+    n += full[w];
+  }
+  a.loss[0] = n ? (float)((double)a.coef * a.E * total / n) : 0.f;
+  a.filled[0] = n;
 }
 
 template <int DT>
@@ -355,10 +383,10 @@ hipError_t launch_preference(const PreferenceArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-// Ranges a sequence's rows are cut into: two workgroups a CU over all, of 64 rows or more.
+// Ranges a sequence's rows are cut into: two workgroups a CU over all, of 128 rows or more.
 int balance_parts(int64_t T, int B) {
   int64_t want = 2 * (int64_t)device_cus() / (B > 0 ? B : 1);
-  const int64_t most = T / (64 * (int64_t)(B > 0 ? B : 1)) + 1;
+  const int64_t most = T / (128 * (int64_t)(B > 0 ? B : 1)) + 1;
   if (want > most) want = most;
   return want < 1 ? 1 : (int)want;
 }
@@ -370,7 +398,7 @@ hipError_t launch_balance(const BalanceArgs& a, hipStream_t s) {
 #undef RUN
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
-  balance_join_kernel<<<dim3(1), 256, 0, s>>>(a);
+  balance_join_kernel<<<dim3(1), 1024, 0, s>>>(a);
   return hipGetLastError();
 }
 hipError_t launch_balance_bwd(const BalanceArgs& a, hipStream_t s) {
