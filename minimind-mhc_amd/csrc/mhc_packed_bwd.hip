@@ -221,25 +221,29 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
   }
 }
 
-// dK and dV: one 4-wave workgroup per 128 keys of one kv head, 32 keys a wave, whose rows
-// of K and V stay in registers; the query rows that see them, of every head of the group,
+// dK and dV: one workgroup per 128 keys of one kv head, 32 keys a wave (head_dim 128: 16, or
+// the sums would leave one wave a SIMD), whose rows of K and V stay in registers; the query rows that see them, of every head of the group,
 // pass through LDS 32 at a time.  S = Q K^T and dP = G V^T put a lane's values all in one
 // key, and P and dS, rounded, are the operands of dV^T = G^T P and dK^T = Q^T dS.
 // An fp16 P is 2^14 times as large, which is taken out of dS as it is formed and of dV at the
 // end: a row of many keys has probabilities below fp16's smallest normal number.  dS has
 // no bound and stays as it is: its terms under 2^-14 round at 2^-25, as any fp16 gradient does.
 // KS = 2: four more waves take every second tile of rows, and the halves add up at the end.
+template <int HD>
+constexpr int packed_dkv_waves = HD == 128 ? 8 : 4;
+
 template <bool F16, int HD, int KS>
-__global__ __launch_bounds__(256 * KS, HD <= 96 ? 2 : 1) void packed_dkv_kernel(PackedAttnArgs a) {
+__global__ __launch_bounds__(64 * packed_dkv_waves<HD> * KS, 2) void packed_dkv_kernel(PackedAttnArgs a) {
   constexpr int NC = HD / 32, ND = HD / 16, QT = 32, KW = 128;
   constexpr int S = 4;                     // stages
   constexpr int TILE = QT * HD;            // elements
-  constexpr int UW = TILE * 2 / 1024 / 2;  // 1 KiB units a wave loads: waves 0 and 1 q, 2 and 3 g
+  constexpr int NW = packed_dkv_waves<HD>, KU = KW / NW / 16;  // waves of a half, 16-key parts of a wave
+  constexpr int UW = TILE * 2 / 1024 / (NW / 2);  // 1 KiB units a wave loads: half of the waves q, half g
   constexpr float kUp = F16 ? 14.f : 0.f, kDown = F16 ? 0x1p-14f : 1.f;
   __shared__ __align__(16) uint16_t lds_[KS][S][2 * TILE + 128];  // q, g, and the rows' 32 log sums and 32 D (fp32)
-  static_assert(KS == 1 || sizeof(lds_) >= 4 * 64 * 4 * ND * 16, "the second half's sums take the tiles' place");
-  const int tid = threadIdx.x & 255;
-  const int half = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  static_assert(KS == 1 || sizeof(lds_) >= NW * 64 * 2 * KU * ND * 16, "the second half's sums take the tiles' place");
+  const int tid = threadIdx.x & (64 * NW - 1);
+  const int half = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * NW));
   auto& lds = lds_[half];
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 15, g = lane >> 4;
@@ -251,7 +255,7 @@ __global__ __launch_bounds__(256 * KS, HD <= 96 ? 2 : 1) void packed_dkv_kernel(
   const PackedKeys kk{t.start, t.used};
   const int rep = a.heads / a.kv_heads;
   const int k0 = t.first - t.start;       // first key of the tile, in the sequence
-  const int kb0 = k0 + wave * 32;         // of the wave
+  const int kb0 = k0 + wave * 16 * KU;    // of the wave
   const int shift = kk.len - qq.len;      // query x of the sequence sees the keys up to x + shift
   const int q_first = max(k0 - shift, 0);
   const int n_rows = t.seq < a.B && k0 < kk.len ? max(qq.len - q_first, 0) : 0;
@@ -259,8 +263,8 @@ __global__ __launch_bounds__(256 * KS, HD <= 96 ? 2 : 1) void packed_dkv_kernel(
   const int nt = per_head * rep;          // tiles of rows, of all heads
   const int mine = (nt - half + KS - 1) / KS, steps = (nt + KS - 1) / KS;
 
-  const bool loads_g = wave >= 2;
-  const int u0 = (wave & 1) * UW;
+  const bool loads_g = wave >= NW / 2;
+  const int u0 = wave % (NW / 2) * UW;
   const int64_t row_st = loads_g ? (int64_t)a.heads * HD : a.qs_t, head_st = loads_g ? HD : a.qs_h;
   const uint16_t* src = static_cast<const uint16_t*>(loads_g ? a.g_out : a.q) + qq.start * row_st +
                         (int64_t)kvh * rep * head_st;
@@ -293,9 +297,9 @@ __global__ __launch_bounds__(256 * KS, HD <= 96 ? 2 : 1) void packed_dkv_kernel(
 #pragma unroll
   for (int i = 0; i < S - 1; ++i)
     if (i < mine) issue(lds[i]);
-  U32x4 kb[2][NC], vb[2][NC];
+  U32x4 kb[KU][NC], vb[KU][NC];
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
+  for (int u = 0; u < KU; ++u) {
     const int64_t row = kk.start + max(min(kb0 + u * 16 + r, kk.len - 1), 0);
     const uint16_t* kp = static_cast<const uint16_t*>(a.k) + row * a.ks_t + kvh * a.ks_h + 8 * g;
     const uint16_t* vp = static_cast<const uint16_t*>(a.v) + row * a.vs_t + kvh * a.vs_h + 8 * g;
@@ -306,9 +310,9 @@ __global__ __launch_bounds__(256 * KS, HD <= 96 ? 2 : 1) void packed_dkv_kernel(
     }
   }
   const float scale = a.scale * kPackedLog2e;
-  f32x4_t dk[2][ND], dv[2][ND];
+  f32x4_t dk[KU][ND], dv[KU][ND];
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
+  for (int u = 0; u < KU; ++u)
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
       dk[u][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -321,8 +325,8 @@ __global__ __launch_bounds__(256 * KS, HD <= 96 ? 2 : 1) void packed_dkv_kernel(
     const uint16_t* gs = qs + TILE;
     if (kb0 >= kk.len || q0 + QT - 1 + shift < kb0) return;  // no keys, or none that these rows see
     // the diagonal, and the sequence's last rows, behind which lie copies of the last
-    const bool edge = q0 + shift < kb0 + 31 || q0 + QT > qq.len;
-    f32x4_t s[2][2], dp[2][2];  // [16 query rows][16 keys]
+    const bool edge = q0 + shift < kb0 + 16 * KU - 1 || q0 + QT > qq.len;
+    f32x4_t s[2][KU], dp[2][KU];  // [16 query rows][16 keys]
     constexpr int QS = HD == 96 ? 1 : 2;  // 16-row parts read ahead together (registers)
 #pragma unroll
     for (int q0_ = 0; q0_ < 2; q0_ += QS) {
@@ -338,7 +342,7 @@ __global__ __launch_bounds__(256 * KS, HD <= 96 ? 2 : 1) void packed_dkv_kernel(
 #pragma unroll
       for (int q = q0_; q < q0_ + QS; ++q)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < KU; ++u) {
           s[q][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
           dp[q][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         }
@@ -347,7 +351,7 @@ __global__ __launch_bounds__(256 * KS, HD <= 96 ? 2 : 1) void packed_dkv_kernel(
 #pragma unroll
         for (int q = 0; q < QS; ++q)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
+          for (int u = 0; u < KU; ++u) {
             s[q0_ + q][u] = mfma16<F16>(qa[q][c], kb[u][c], s[q0_ + q][u]);
             dp[q0_ + q][u] = mfma16<F16>(ga[q][c], vb[u][c], dp[q0_ + q][u]);
           }
@@ -367,7 +371,7 @@ __global__ __launch_bounds__(256 * KS, HD <= 96 ? 2 : 1) void packed_dkv_kernel(
 #pragma unroll
       for (int q = 0; q < 2; ++q)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < KU; ++u)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int row = q0 + q * 16 + 4 * g + i;
@@ -377,11 +381,11 @@ __global__ __launch_bounds__(256 * KS, HD <= 96 ? 2 : 1) void packed_dkv_kernel(
             }
           }
     }
-    U32x4 pf[2], df[2];
+    U32x4 pf[KU], df[KU];
 #pragma unroll
     for (int q = 0; q < 2; ++q)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < KU; ++u) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[q][u][i] = exp2_f(fmaf(s[q][u][i], scale, kUp - l4[q][i]));
         pf[u].v[2 * q] = pack2<F16>(s[q][u][0], s[q][u][1]);
@@ -391,7 +395,7 @@ __global__ __launch_bounds__(256 * KS, HD <= 96 ? 2 : 1) void packed_dkv_kernel(
 #pragma unroll
       for (int q = 0; q < 2; ++q)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < KU; ++u) {
           float ds[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i)
@@ -411,7 +415,7 @@ __global__ __launch_bounds__(256 * KS, HD <= 96 ? 2 : 1) void packed_dkv_kernel(
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) dv[u][d] = mfma16<F16>(gc[d], pf[u], dv[u][d]);
+        for (int u = 0; u < KU; ++u) dv[u][d] = mfma16<F16>(gc[d], pf[u], dv[u][d]);
     };
     if constexpr (HD == 96) {  // with dV's products beside dS the registers spill
       terms();
@@ -422,16 +426,16 @@ __global__ __launch_bounds__(256 * KS, HD <= 96 ? 2 : 1) void packed_dkv_kernel(
       values();
       terms();
 #pragma unroll
-      for (int x = 0; x < 2 * ND; ++x) {
+      for (int x = 0; x < KU * ND; ++x) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x402, ND == 4 ? 5 : 4, 0);
+        __builtin_amdgcn_sched_group_barrier(0x402, ND == 4 ? 5 : 3, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) dk[u][d] = mfma16<F16>(qc[d], df[u], dk[u][d]);
+      for (int u = 0; u < KU; ++u) dk[u][d] = mfma16<F16>(qc[d], df[u], dk[u][d]);
   };
   int stage = 0, ch = 0, cq = 0;  // head and row tile of this step
   if (nt > 0) forth(half, ch, cq);
@@ -447,24 +451,24 @@ __global__ __launch_bounds__(256 * KS, HD <= 96 ? 2 : 1) void packed_dkv_kernel(
   }
   if constexpr (KS == 2) {
     __syncthreads();
-    float* x = reinterpret_cast<float*>(lds_) + wave * 64 * (4 * ND * 4) + lane * 4;
+    float* x = reinterpret_cast<float*>(lds_) + wave * 64 * (2 * KU * ND * 4) + lane * 4;
     if (half == 1) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < KU; ++u)
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
           *reinterpret_cast<f32x4_t*>(x + (u * ND + d) * 256) = dk[u][d];
-          *reinterpret_cast<f32x4_t*>(x + (2 * ND + u * ND + d) * 256) = dv[u][d];
+          *reinterpret_cast<f32x4_t*>(x + (KU * ND + u * ND + d) * 256) = dv[u][d];
         }
     }
     __syncthreads();
     if (half == 1) return;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < KU; ++u)
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
         const f32x4_t y = *reinterpret_cast<const f32x4_t*>(x + (u * ND + d) * 256);
-        const f32x4_t z = *reinterpret_cast<const f32x4_t*>(x + (2 * ND + u * ND + d) * 256);
+        const f32x4_t z = *reinterpret_cast<const f32x4_t*>(x + (KU * ND + u * ND + d) * 256);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           dk[u][d][i] += y[i];
@@ -474,7 +478,7 @@ __global__ __launch_bounds__(256 * KS, HD <= 96 ? 2 : 1) void packed_dkv_kernel(
   }
   // every row of the slot is written: those behind its length with zeros
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
+  for (int u = 0; u < KU; ++u) {
     const int key = kb0 + u * 16 + r;
     const int row = t.start + key;
     if (row >= t.end) continue;
@@ -509,10 +513,10 @@ hipError_t packed_bwd_hd(PackedAttnArgs a, hipStream_t s) {
   }
   if (a.Tk == 0) return hipSuccess;
   const dim3 kgrid((unsigned)(packed_tiles(a.Tk, a.B, 128) * a.kv_heads));
-  if (HD <= 96 && packed_halves(kgrid.x))  // at 128 eight waves do not fit the registers
+  if (HD <= 96 && packed_halves(kgrid.x))  // at 128 a workgroup has eight waves as it is
     packed_dkv_kernel<F16, HD <= 96 ? HD : 64, 2><<<kgrid, 512, 0, s>>>(a);
   else
-    packed_dkv_kernel<F16, HD, 1><<<kgrid, 256, 0, s>>>(a);
+    packed_dkv_kernel<F16, HD, 1><<<kgrid, 64 * packed_dkv_waves<HD>, 0, s>>>(a);
   return hipGetLastError();
 }
 
