@@ -576,13 +576,16 @@ int mhc_packed_attn_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, c
 
 /* Gradients g_q [Tq, heads, head_dim], g_k and g_v [Tk, kv_heads, head_dim]
  * (contiguous; every row is written) for g_out, contiguous as out.  out, rest and lse
- * are the forward's; delta [heads, Tq] fp32 is scratch.  No atomics: the same bits on every
- * run. */
+ * are the forward's.  No atomics: the same bits on every run.  Its workspace holds
+ * D = g_out . out of each row and, where few workgroups have long chains, parts of
+ * the sums; mhc_packed_attn_bwd_workspace_bytes gives its size (or -1). */
+int64_t mhc_packed_attn_bwd_workspace_bytes(int B, int64_t Tq, int64_t Tk, int heads, int kv_heads,
+                                            int head_dim);
 int mhc_packed_attn_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
                         int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
                         int64_t v_stride_h, const int* cu_q, const int* cu_k, const int* key_lengths,
-                        const void* out, const void* rest, const float* lse, const void* g_out, float* delta, void* g_q,
-                        void* g_k, void* g_v, int B, int64_t Tq, int64_t Tk, int heads, int kv_heads,
+                        const void* out, const void* rest, const float* lse, const void* g_out, void* g_q,
+                        void* g_k, void* g_v, void* workspace, int64_t workspace_bytes, int B, int64_t Tq, int64_t Tk, int heads, int kv_heads,
                         int head_dim, int dtype, float scale, hipStream_t stream);
 
 /* ------------------------------------------------------------------- losses

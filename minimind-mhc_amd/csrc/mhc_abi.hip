@@ -773,6 +773,15 @@ int64_t mhc_packed_attn_workspace_bytes(int B, int64_t Tq, int64_t Tk, int heads
   return mhc::packed_attn_workspace(a);
 }
 
+int64_t mhc_packed_attn_bwd_workspace_bytes(int B, int64_t Tq, int64_t Tk, int heads, int kv_heads, int head_dim) {
+  mhc::PackedAttnArgs a = packed_args(nullptr, 0, 0, nullptr, 0, 0, nullptr, 0, 0, nullptr, nullptr, nullptr, B, Tq,
+                                      Tk, heads, kv_heads, head_dim, mhc::kBF16, 1.f);
+  if (check_packed(a, Tq, Tk, mhc::kBF16, "mhc_packed_attn_bwd_workspace_bytes")) return -1;
+  mhc::packed_bwd_plan(a);
+  int64_t sums;
+  return mhc::packed_bwd_workspace(a, &sums);
+}
+
 int mhc_packed_attn_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
                         int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
                         int64_t v_stride_h, const int* cu_q, const int* cu_k, const int* key_lengths,
@@ -799,8 +808,8 @@ int mhc_packed_attn_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, c
 int mhc_packed_attn_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
                         int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
                         int64_t v_stride_h, const int* cu_q, const int* cu_k, const int* key_lengths,
-                        const void* out, const void* rest, const float* lse, const void* g_out, float* delta, void* g_q,
-                        void* g_k, void* g_v, int B, int64_t Tq, int64_t Tk, int heads, int kv_heads,
+                        const void* out, const void* rest, const float* lse, const void* g_out, void* g_q,
+                        void* g_k, void* g_v, void* workspace, int64_t workspace_bytes, int B, int64_t Tq, int64_t Tk, int heads, int kv_heads,
                         int head_dim, int dtype, float scale, hipStream_t stream) {
   const char* fn = "mhc_packed_attn_bwd";
   mhc::PackedAttnArgs a = packed_args(q, q_stride_t, q_stride_h, k, k_stride_t, k_stride_h, v, v_stride_t, v_stride_h,
@@ -814,8 +823,14 @@ int mhc_packed_attn_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, c
     for (const void* p : {k, v, (const void*)g_k, (const void*)g_v})
       if (!p || !aligned16(p)) return fail(hipErrorInvalidValue, "%s: null or unaligned pointer", fn);
   if (!cu_q || !cu_k) return fail(hipErrorInvalidValue, "%s: the sequences' bounds are required", fn);
-  if (Tq > 0 && (!lse || !delta)) return fail(hipErrorInvalidValue, "%s: lse and delta are required", fn);
-  a.out = const_cast<void*>(out); a.rest = const_cast<void*>(rest); a.lse = const_cast<float*>(lse); a.g_out = g_out; a.delta = delta;
+  if (Tq > 0 && !lse) return fail(hipErrorInvalidValue, "%s: lse is required", fn);
+  mhc::packed_bwd_plan(a);
+  int64_t sums;
+  const int64_t need = mhc::packed_bwd_workspace(a, &sums);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(hipErrorInvalidValue, "%s: workspace of %lld bytes needed (got %lld)", fn, (long long)need, (long long)workspace_bytes);
+  a.out = const_cast<void*>(out); a.rest = const_cast<void*>(rest); a.lse = const_cast<float*>(lse); a.g_out = g_out;
+  a.delta = static_cast<float*>(workspace); a.work = a.delta + sums;
   a.g_q = g_q; a.g_k = g_k; a.g_v = g_v;
   return hip_status(mhc::launch_packed_attn_bwd(a, stream), fn);
 }

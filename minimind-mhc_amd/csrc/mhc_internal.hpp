@@ -317,6 +317,7 @@ struct PackedAttnArgs {
   // backward
   const void* g_out;
   float* delta;  // [heads, Tq]
+  int ranges;    // packed_bwd_plan: of the query rows of a key tile; their sums go to `work`
   void* g_q;
   void* g_k;
   void* g_v;
@@ -324,6 +325,9 @@ struct PackedAttnArgs {
 void packed_attn_plan(PackedAttnArgs& a);
 int64_t packed_attn_workspace(const PackedAttnArgs& a);
 hipError_t launch_packed_attn(const PackedAttnArgs& a, hipStream_t s);
+void packed_bwd_plan(PackedAttnArgs& a);
+// Bytes, and the sums' place in it (floats behind delta, which is at its beginning).
+int64_t packed_bwd_workspace(const PackedAttnArgs& a, int64_t* sums);
 hipError_t launch_packed_attn_bwd(const PackedAttnArgs& a, hipStream_t s);
 
 // Log-probabilities of labels under rows of logits [T, V] (rows `stride` elements apart).

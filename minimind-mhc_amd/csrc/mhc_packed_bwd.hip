@@ -229,6 +229,8 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
 // end: a row of many keys has probabilities below fp16's smallest normal number.  dS has
 // no bound and stays as it is: its terms under 2^-14 round at 2^-25, as any fp16 gradient does.
 // KS = 2: four more waves take every second tile of rows, and the halves add up at the end.
+// With a.ranges > 1 a workgroup takes one range of the rows' tiles and leaves its sums in fp32
+// for packed_dkv_join_kernel.
 template <int HD>
 constexpr int packed_dkv_waves = HD == 128 ? 8 : 4;
 
@@ -250,7 +252,8 @@ __global__ __launch_bounds__(64 * packed_dkv_waves<HD> * KS, 2) void packed_dkv_
   const int kvh = blockIdx.x % a.kv_heads;
   PackedTile t;
   PackedKeys qq;  // the sequence's query rows
-  packed_rank<true>(a.cu_k, a.B, a.Tk, KW, 0, blockIdx.x / a.kv_heads, a.cu_q, a.Tq, a.k_len, nullptr, t, qq);
+  const int range = blockIdx.x / a.kv_heads % a.ranges;
+  packed_rank<true>(a.cu_k, a.B, a.Tk, KW, 0, blockIdx.x / a.kv_heads / a.ranges, a.cu_q, a.Tq, a.k_len, nullptr, t, qq);
   if (t.first >= t.end) return;
   const PackedKeys kk{t.start, t.used};
   const int rep = a.heads / a.kv_heads;
@@ -260,7 +263,9 @@ __global__ __launch_bounds__(64 * packed_dkv_waves<HD> * KS, 2) void packed_dkv_
   const int q_first = max(k0 - shift, 0);
   const int n_rows = t.seq < a.B && k0 < kk.len ? max(qq.len - q_first, 0) : 0;
   const int per_head = (n_rows + QT - 1) / QT;
-  const int nt = per_head * rep;          // tiles of rows, of all heads
+  const int all = per_head * rep;         // tiles of rows, of all heads
+  const int first = (int)((int64_t)all * range / a.ranges);
+  const int nt = (int)((int64_t)all * (range + 1) / a.ranges) - first;  // of the range
   const int mine = (nt - half + KS - 1) / KS, steps = (nt + KS - 1) / KS;
 
   const bool loads_g = wave >= NW / 2;
@@ -281,7 +286,11 @@ __global__ __launch_bounds__(64 * packed_dkv_waves<HD> * KS, 2) void packed_dkv_
       hh += over;
     }
   };
-  if (nt > 0) forth(half, ih, iq);
+  if (nt > 0) {
+    ih = first / per_head;
+    iq = first % per_head;
+    forth(half, ih, iq);
+  }
   auto issue = [&](uint16_t* __restrict__ d) {
     const int q0 = q_first + iq * QT;
     const uint16_t* p0 = src + ih * head_st + q0 * row_st;
@@ -437,8 +446,8 @@ __global__ __launch_bounds__(64 * packed_dkv_waves<HD> * KS, 2) void packed_dkv_
 #pragma unroll
       for (int u = 0; u < KU; ++u) dk[u][d] = mfma16<F16>(qc[d], df[u], dk[u][d]);
   };
-  int stage = 0, ch = 0, cq = 0;  // head and row tile of this step
-  if (nt > 0) forth(half, ch, cq);
+  int stage = 0, ch = 0, cq = nt > 0 ? first % per_head : 0;  // head and row tile of this step
+  forth(half, ch, cq);
   for (int it = 0; it < steps; ++it) {
     if (it + S - 1 <= mine) tile_wait<(S - 2) * (UW + 1)>();
     else if (it + S - 2 <= mine) tile_wait<(S - 3) * (UW + 1)>();
@@ -484,19 +493,45 @@ __global__ __launch_bounds__(64 * packed_dkv_waves<HD> * KS, 2) void packed_dkv_
     if (row >= t.end) continue;
     const bool used = key < kk.len;
     const int64_t at = ((int64_t)row * a.kv_heads + kvh) * HD + 4 * g;
+    const int64_t size = (int64_t)a.Tk * a.kv_heads * HD;
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
-      uint2 w = make_uint2(0, 0), x = w;
+      f32x4_t x = {0.f, 0.f, 0.f, 0.f}, y = x;
       if (used) {
-        w.x = pack2<F16>(dk[u][d][0] * a.scale, dk[u][d][1] * a.scale);
-        w.y = pack2<F16>(dk[u][d][2] * a.scale, dk[u][d][3] * a.scale);
-        x.x = pack2<F16>(dv[u][d][0] * kDown, dv[u][d][1] * kDown);
-        x.y = pack2<F16>(dv[u][d][2] * kDown, dv[u][d][3] * kDown);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i] = dk[u][d][i] * a.scale;
+          y[i] = dv[u][d][i] * kDown;
+        }
       }
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.g_k) + at + 16 * d) = w;
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.g_v) + at + 16 * d) = x;
+      if (a.ranges > 1) {
+        float* part = a.work + 2 * range * size + at + 16 * d;
+        *reinterpret_cast<f32x4_t*>(part) = x;
+        *reinterpret_cast<f32x4_t*>(part + size) = y;
+      } else {
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.g_k) + at + 16 * d) =
+            make_uint2(pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3]));
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.g_v) + at + 16 * d) =
+            make_uint2(pack2<F16>(y[0], y[1]), pack2<F16>(y[2], y[3]));
+      }
     }
   }
+}
+
+// The ranges' sums, in order, four elements of dK or dV a thread.
+template <bool F16>
+__global__ __launch_bounds__(256) void packed_dkv_join_kernel(PackedAttnArgs a) {
+  const int64_t size = (int64_t)a.Tk * a.kv_heads * a.head_dim;
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;  // of dK, then of dV
+  if (i >= 2 * size) return;
+  f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.work + i);
+  for (int n = 1; n < a.ranges; ++n) {
+    const f32x4_t y = *reinterpret_cast<const f32x4_t*>(a.work + 2 * n * size + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] += y[j];
+  }
+  uint16_t* out = i < size ? static_cast<uint16_t*>(a.g_k) + i : static_cast<uint16_t*>(a.g_v) + (i - size);
+  *reinterpret_cast<uint2*>(out) = make_uint2(pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3]));
 }
 
 template <bool F16, int HD>
@@ -512,15 +547,38 @@ hipError_t packed_bwd_hd(PackedAttnArgs a, hipStream_t s) {
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
   if (a.Tk == 0) return hipSuccess;
-  const dim3 kgrid((unsigned)(packed_tiles(a.Tk, a.B, 128) * a.kv_heads));
+  const dim3 kgrid((unsigned)(packed_tiles(a.Tk, a.B, 128) * a.kv_heads * a.ranges));
   if (HD <= 96 && packed_halves(kgrid.x))  // at 128 a workgroup has eight waves as it is
     packed_dkv_kernel<F16, HD <= 96 ? HD : 64, 2><<<kgrid, 512, 0, s>>>(a);
   else
     packed_dkv_kernel<F16, HD, 1><<<kgrid, 64 * packed_dkv_waves<HD>, 0, s>>>(a);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess || a.ranges == 1) return e;
+  const int64_t quads = (int64_t)a.Tk * a.kv_heads * HD / 2;
+  packed_dkv_join_kernel<F16><<<dim3((unsigned)((quads + 255) / 256)), 256, 0, s>>>(a);
   return hipGetLastError();
 }
 
 }  // namespace
+
+// Ranges that the query rows of a key tile are cut into: up to four workgroups a CU, none of
+// under 32 tiles of rows, so that the ranges' sums (8 bytes an element each way) stay small
+// beside the products.  A step of 2 sequences of 8000 tokens together, 8 / 2 heads of 128: 522 us
+// with 4 ranges and 1120 with one; of 2 of 16000, 16 / 2 heads of 64: 1540 with 4, 2136 with 2, 2496
+// with one; of 3 of 16001, 8 / 8 heads of 64 (four workgroups a CU as it is): 688 with 2, 664 with one.
+void packed_bwd_plan(PackedAttnArgs& a) {
+  const int64_t groups = (int64_t)a.Tk * a.kv_heads / 128 + 1;  // workgroups with work, about
+  const int64_t chain = (int64_t)a.Tq / (a.B > 0 ? a.B : 1) * (a.heads / a.kv_heads) / 32;  // tiles of the longest, about
+  int64_t want = 4 * (int64_t)device_cus() / groups;
+  if (want > chain / 32) want = chain / 32;
+  if (want > 8) want = 8;
+  a.ranges = want < 1 ? 1 : (int)want;
+}
+// D, and the ranges' sums of dK and dV.
+int64_t packed_bwd_workspace(const PackedAttnArgs& a, int64_t* sums) {
+  const int64_t delta = ((int64_t)a.heads * a.Tq + 3) / 4 * 4;
+  *sums = delta;
+  return (delta + (a.ranges > 1 ? 2 * a.ranges * (int64_t)a.Tk * a.kv_heads * a.head_dim : 0)) * 4;
+}
 
 hipError_t launch_packed_attn_bwd(const PackedAttnArgs& a, hipStream_t s) { MHC_PACKED_HD(packed_bwd_hd, a, s) }
 

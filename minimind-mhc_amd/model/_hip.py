@@ -113,12 +113,13 @@ _SIGNATURES = {
                                  _P, _P, _P, _P, _I64,             # k_out, v_out, out, workspace, bytes
                                  _I64, _I, _I, _I, _I, _I, _F, _F, _P]),
     "mhc_packed_attn_workspace_bytes": (_I64, [_I, _I64, _I64, _I, _I, _I]),
+    "mhc_packed_attn_bwd_workspace_bytes": (_I64, [_I, _I64, _I64, _I, _I, _I]),
     "mhc_packed_attn_fwd": (_I, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64,  # q, k, v and their strides
                                  _P, _P, _P, _P, _P, _P, _P, _I64,  # cu_q, cu_k, key_lengths, out, rest, lse, workspace
                                  _I, _I64, _I64, _I, _I, _I, _I, _F, _P]),
     "mhc_packed_attn_bwd": (_I, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64,
-                                 _P, _P, _P, _P, _P, _P, _P, _P,  # cu_q, cu_k, key_lengths, out, rest, lse, g_out, delta
-                                 _P, _P, _P,                      # g_q, g_k, g_v
+                                 _P, _P, _P, _P, _P, _P, _P,      # cu_q, cu_k, key_lengths, out, rest, lse, g_out
+                                 _P, _P, _P, _P, _I64,            # g_q, g_k, g_v, workspace, bytes
                                  _I, _I64, _I64, _I, _I, _I, _I, _F, _P]),
     "mhc_logprobs_fwd": (_I, [_P, _I64, _I, _P, _I64, _P, _P, _I64, _I, _P]),
     "mhc_logprobs_bwd": (_I, [_P, _I64, _I, _P, _I64, _P, _P, _P, _I64, _I, _P]),

@@ -94,13 +94,15 @@ class _PackedAttention(torch.autograd.Function):
         dev, new = q.device, torch.empty
         g_q = new((Tq, heads, hd), dtype=q.dtype, device=dev)
         g_k, g_v = (new((Tk, kv, hd), dtype=q.dtype, device=dev) for _ in range(2))
-        delta = new((heads, Tq), dtype=torch.float32, device=dev)
+        B, lib = cu_q.numel() - 1, H.load()
         with _ops.launch_device(q):
-            H.check(H.load().mhc_packed_attn_bwd(
+            nbytes = lib.mhc_packed_attn_bwd_workspace_bytes(B, Tq, Tk, heads, kv, hd)
+            ws = new(max(nbytes, 0), dtype=torch.uint8, device=dev)
+            H.check(lib.mhc_packed_attn_bwd(
                 q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs, cu_q.data_ptr(),
                 cu_k.data_ptr(), H.ptr(used), out.data_ptr(), rest.data_ptr(), lse.data_ptr(), g.data_ptr(),
-                delta.data_ptr(), g_q.data_ptr(), g_k.data_ptr(), g_v.data_ptr(), cu_q.numel() - 1,
-                Tq, Tk, heads, kv, hd, H.dtype_tag(q), ctx.scale, H.stream(dev)), "mhc_packed_attn_bwd")
+                g_q.data_ptr(), g_k.data_ptr(), g_v.data_ptr(), ws.data_ptr(), max(nbytes, 0), B, Tq, Tk,
+                heads, kv, hd, H.dtype_tag(q), ctx.scale, H.stream(dev)), "mhc_packed_attn_bwd")
         return g_q, g_k, g_v, None, None, None, None
 
 

@@ -85,7 +85,9 @@ TRAIN = [
     (96, 8, 4, BF, [1]), (96, 8, 4, BF, [63, 1, 65]), (96, 4, 2, F16, [128, 0, 127, 129]),
     (64, 4, 4, BF, [257, 31, 33]), (64, 3, 1, F16, [64, 64, 1, 1, 95]), (128, 8, 2, BF, [200, 311]),
     (128, 4, 1, F16, [32, 1, 0, 0, 160]), (96, 6, 2, BF, [5] * 70), (64, 12, 4, BF, [1] * 130 + [300]),
-    (128, 2, 2, BF, [0, 0]), (96, 16, 1, BF, [77, 130])]
+    (128, 2, 2, BF, [0, 0]), (96, 16, 1, BF, [77, 130]),
+    # long chains on few key tiles: dK and dV from several ranges of rows
+    (64, 8, 1, BF, [1100, 37]), (128, 8, 1, F16, [900, 300]), (96, 8, 1, BF, [0, 1300, 1])]
 
 
 @pytest.mark.gpu
