@@ -839,7 +839,7 @@ int mhc_packed_attn_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, c
 
 static int check_logits(const void* logits, int64_t stride, int dtype, const int64_t* labels, int64_t T, int V,
                         const char* fn) {
-  if (T < 0 || T > 1 << 30 || V < 1 || stride < 0)
+  if (T < 0 || T > 1 << 30 || V < 1 || V > 1 << 30 || stride < 0)
     return fail(hipErrorInvalidValue, "%s: bad shape (T=%lld V=%d stride=%lld)", fn, (long long)T, V, (long long)stride);
   if (!dtype_ok(dtype)) return fail(hipErrorInvalidValue, "%s: bad dtype %d", fn, dtype);
   if (T > 0 && (!logits || !labels || reinterpret_cast<uintptr_t>(logits) % mhc::dtype_bytes(dtype)))

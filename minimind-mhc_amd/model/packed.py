@@ -129,7 +129,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     of keys that no query sees.  The bounds stay on the device (no synchronisation; a
     captured graph takes other lengths on its next replay): they are clamped to the tensors,
     and bounds that decrease give unspecified rows.  Differentiable once; the gradients are
-    the same bits on every run.
+    the same bits on every run.  Not-finite keys or values of a token may turn earlier rows of
+    its own sequence into NaN, as a dense product under a mask does.
     """
     if torch.is_autocast_enabled("cuda"):
         low = torch.get_autocast_dtype("cuda")

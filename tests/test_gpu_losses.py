@@ -239,3 +239,22 @@ def test_balance_ignores_foreign_experts(dev):
     want = torch.bincount(index[:, 0], minlength=8)
     index[:, 1] = torch.tensor([-1, 8, 2 ** 40, -2 ** 40, 1 << 32], device=dev).repeat(10)
     assert torch.equal(balance_loss(x, index, 1.0)[1], want)
+
+
+@pytest.mark.gpu
+def test_logits_past_32_bits(dev):
+    """Rows past 2^31 elements, both ways."""
+    V = 65536
+    T = (1 << 31) // V + 6
+    x = torch.zeros(T, V, dtype=BF, device=dev)
+    tail = torch.randn(4, V, device=dev).to(BF)
+    x[-4:] = tail
+    labels = torch.full((T,), IGN, device=dev)
+    labels[-4:] = torch.tensor([0, 5, V - 1, 77], device=dev)
+    want, dwant = _exact_logprobs(tail, labels[-4:])
+    x.requires_grad_()
+    lp = token_logprobs(x, labels)
+    _lp_close(lp[-4:], want)
+    g, = torch.autograd.grad(lp.sum(), x)
+    _grad_close(g[-4:], dwant, torch.ones(4, 1, dtype=torch.float64), BF)
+    assert not bool(g[:100].any())

@@ -87,7 +87,9 @@ TRAIN = [
     (128, 4, 1, F16, [32, 1, 0, 0, 160]), (96, 6, 2, BF, [5] * 70), (64, 12, 4, BF, [1] * 130 + [300]),
     (128, 2, 2, BF, [0, 0]), (96, 16, 1, BF, [77, 130]),
     # long chains on few key tiles: dK and dV from several ranges of rows
-    (64, 8, 1, BF, [1100, 37]), (128, 8, 1, F16, [900, 300]), (96, 8, 1, BF, [0, 1300, 1])]
+    (64, 8, 1, BF, [1100, 37]), (128, 8, 1, F16, [900, 300]), (96, 8, 1, BF, [0, 1300, 1]),
+    # more sequences than the tiles are ranked for
+    (64, 2, 1, BF, [3] * 300 + [150]), (128, 2, 2, F16, [1, 0, 2] * 120)]
 
 
 @pytest.mark.gpu
@@ -168,3 +170,92 @@ def test_strides(dev):
     assert torch.equal(got[0], full[0])
     for a, b in zip(got[1:], full[1:]):
         assert torch.equal(a, b.sum(1, keepdim=True))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 40])
+def test_offsets_past_32_bits(dev, new):
+    """The second sequence's keys lie past 2^31 elements."""
+    kv, hd, n = 4, 96, 500
+    rows = (1 << 31) // (kv * hd) + 3000
+    torch.manual_seed(0)
+    q, g = (torch.randn(2 * new, 8, hd, device=dev).to(BF) for _ in range(2))
+    small = [torch.randn(10 + n, kv, hd, device=dev).to(BF) for _ in range(2)]
+    big = [torch.empty(rows, kv, hd, dtype=BF, device=dev) for _ in range(2)]
+    for b, s in zip(big, small):
+        b[:10], b[-n:] = s[:10], s[10:]
+    used = torch.tensor([10, n], dtype=torch.int32, device=dev)
+    res = []
+    for kvs, ends in ((small, [0, 10, 10 + n]), (big, [0, rows - n, rows])):
+        leaves = [t.requires_grad_() for t in (q.clone(), *kvs)]
+        out = packed_attention(*leaves, _cu([new, new], dev), key_lengths=used,
+                               cu_seqlens_k=torch.tensor(ends, dtype=torch.int32, device=dev))
+        gq, gk, gv = torch.autograd.grad(out, leaves, g)
+        res.append([out, gq, gk[:10], gv[:10], gk[-n:], gv[-n:]])
+        if kvs is big:
+            assert not bool(gk[10:1000].any()) and not bool(gv[-n - 1000:-n].any())
+    (want, size) = exact(q, *small, [new, new], [10, n], [10, n], hd ** -0.5)
+    for r in res:  # the key ranges may be cut otherwise
+        close(r[0], want[0], size[0], BF, OUT)
+    for a, b in zip(res[0][1:], res[1][1:]):
+        assert float((a.float() - b.float()).norm()) <= 2.0 ** -6 * float(a.float().norm())
+
+
+@pytest.mark.gpu
+def test_bounds_that_make_no_sense(dev):
+    """Bounds outside the tensors, and decreasing ones, are cut to them: such a call ends, and
+    the next one is right."""
+    T = 200
+    q, k, v, g = _make(dev, BF, T, T, 4, 2, 64)
+    good = packed_attention(q, k, v, _cu([120, 80], dev))
+    for ends in ([-5, 500, 2 ** 31 - 1], [0, 150, 20], [0, -2 ** 31, 200], [9, 9, 9]):
+        cu = torch.tensor(ends, dtype=torch.int32, device=dev)
+        for more in ({}, {"cu_seqlens_k": cu.flip(0).contiguous()},
+                     {"key_lengths": torch.tensor([-7, 2 ** 31 - 1], dtype=torch.int32, device=dev)}):
+            leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+            out = packed_attention(*leaves, cu, **more)
+            assert out.shape == q.shape
+            assert [x.shape for x in torch.autograd.grad(out, leaves, g)] == [q.shape, k.shape, v.shape]
+            packed_attention(q[:2], k, v, cu, **{"cu_seqlens_k": cu, **more})
+    assert torch.equal(packed_attention(q, k, v, _cu([120, 80], dev)), good)
+
+
+def hd_scale(hd):
+    return 1.01 * hd ** -0.5  # and the roundings of the products with it
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,keys,bounds", [(0, 0, [0]), (0, 5, [0, 0]), (7, 7, [0]), (3, 0, [0, 3]), (1, 1, [0, 1])])
+def test_smallest(dev, rows, keys, bounds):
+    q, k, v, g = _make(dev, BF, rows, keys, 4, 2, 64)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    cu = torch.tensor(bounds, dtype=torch.int32, device=dev)
+    ends = torch.tensor(bounds, dtype=torch.int32, device=dev).clamp_max(keys)
+    out = packed_attention(*leaves, cu, cu_seqlens_k=ends)
+    grads = torch.autograd.grad(out, leaves, g)
+    if (rows, keys) == (1, 1):  # one key: its value, whatever the score
+        assert torch.equal(out, v.repeat_interleave(2, 1))
+        # dS = G . v - D, the same sum of 64 products in fp32 twice, in two orders: each is
+        # within 64 half steps (2^-24) of its absolute sum, so dS is under 2^-17 of it
+        bar = 2.0 ** -17 * (g.float() * out.float()).abs().sum(-1, keepdim=True) * hd_scale(64)
+        assert bool((grads[0].float().abs() <= bar * k.float().abs().repeat_interleave(2, 1)).all())
+        assert bool((grads[1].float().abs() <= (bar * q.float().abs()).view(1, 2, 2, 64).sum(2)).all())
+    else:
+        assert not any(bool(t.any()) for t in (out, *grads))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,dtype", [(96, BF), (64, F16)])
+def test_extreme_scores(dev, hd, dtype):
+    """Rows of hugely negative, hugely positive and of equal scores: a maximum that is far
+    from 0 loses nothing."""
+    q, k, v, _ = _make(dev, dtype, 90, 90, 2, 2, hd)
+    big = 2.0 ** (60 if dtype == BF else 7)
+    q[:30], k[:, 0] = big, -big       # head 0: every score the same, far below 0
+    q[30:60] = -big                   # far above
+    q[60:] = 0.0
+    k[:, 1] = big
+    out = packed_attention(q, k, v, _cu([90], dev))
+    want = v.double().cumsum(0) / torch.arange(1, 91, device=dev, dtype=torch.float64)[:, None, None]
+    size = v.double().abs().cumsum(0) / torch.arange(1, 91, device=dev, dtype=torch.float64)[:, None, None]
+    close(out, want.cpu(), (size.cpu(), torch.zeros_like(size).cpu()), dtype, OUT)
