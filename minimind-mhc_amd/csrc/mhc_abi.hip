@@ -944,7 +944,7 @@ int mhc_balance_bwd(const int* cu, const int64_t* counts, const int* filled, con
   if (!dtype_ok(dtype)) return fail(hipErrorInvalidValue, "%s: bad dtype %d", fn, dtype);
   if (!cu && B != 1) return fail(hipErrorInvalidValue, "%s: bad shape (B=%d)", fn, B);
   if (T == 0) return 0;
-  if (!counts || !filled || !g_loss || !g_scores) return fail(hipErrorInvalidValue, "%s: null pointer", fn);
+  if ((B > 0 && !counts) || !filled || !g_loss || !g_scores) return fail(hipErrorInvalidValue, "%s: null pointer", fn);
   mhc::BalanceArgs a{};
   a.cu = cu; a.counts = const_cast<int64_t*>(counts); a.filled = const_cast<int*>(filled); a.g_loss = g_loss;
   a.g_scores = g_scores; a.dtype = dtype; a.T = (int)T; a.E = E; a.B = B; a.coef = coef;

@@ -6,6 +6,7 @@ model/model_minimind.py:290-297 and :421-425).
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
@@ -40,30 +41,30 @@ def _labels(labels: torch.Tensor, logits: torch.Tensor) -> torch.Tensor:
 
 
 def _scalar(g: torch.Tensor) -> torch.Tensor:
-    return g.to(torch.float32).contiguous()
+    return g if g.dtype == torch.float32 else g.to(torch.float32)
 
 
 def _stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _logprobs(x, labels, ignore, want_lse):
-    T, V = x.shape
-    lp = torch.empty(T, dtype=torch.float32, device=x.device)
-    lse = torch.empty((T, 2), dtype=torch.float32, device=x.device) if want_lse else None
-    with _ops.launch_device(x):
-        H.check(H.load().mhc_logprobs_fwd(x.data_ptr(), _stride(x), H.dtype_tag(x), labels.data_ptr(),
-                                          ignore, lp.data_ptr(), H.ptr(lse), T, V, H.stream(x.device)),
-                "mhc_logprobs_fwd")
-    return lp, lse
+def _logprobs(x, labels, ignore, lp: int, lse: Optional[int]):
+    """Writes the log-probabilities (and the rows' sums) to these addresses."""
+    H.check(H.load().mhc_logprobs_fwd(x.data_ptr(), _stride(x), H.dtype_tag(x), labels.data_ptr(), ignore,
+                                      lp, lse, x.shape[0], x.shape[1], H.stream(x.device)), "mhc_logprobs_fwd")
 
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, labels, ignore):
-        lp, lse = _logprobs(x, labels, ignore, True)
-        ctx.save_for_backward(x, labels, lse)
-        ctx.ignore = ignore
+        T, dev = x.shape[0], x.device
+        lp = torch.empty(T, dtype=torch.float32, device=dev)
+        lse = torch.empty((T, 2), dtype=torch.float32, device=dev) if ctx is not None else None
+        with _ops.launch_device(x):
+            _logprobs(x, labels, ignore, lp.data_ptr(), H.ptr(lse))
+        if ctx is not None:
+            ctx.save_for_backward(x, labels, lse)
+            ctx.ignore = ignore
         return lp
 
     @staticmethod
@@ -93,29 +94,29 @@ def token_logprobs(logits: torch.Tensor, labels: torch.Tensor,
     if _ops.wants_graph(logits):
         lp = _TokenLogprobs.apply(x, y, int(ignore_index))
     else:
-        lp = _logprobs(x, y, int(ignore_index), False)[0]
+        lp = _TokenLogprobs.forward(None, x, y, int(ignore_index))
     return lp.view(labels.shape)
 
 
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, labels, cu, reference, beta, smoothing, average, ignore, graph):
-        lp, lse = _logprobs(x, labels, ignore, graph)
-        T, P = x.shape[0], reference.numel() // 2
-        new = torch.empty
-        loss = new((), dtype=torch.float32, device=x.device)
-        rewards = new((2, P), dtype=torch.float32, device=x.device)
-        g_seq = new(2 * P, dtype=torch.float32, device=x.device)
-        scratch = new(P, dtype=torch.float64, device=x.device)
+    def forward(ctx, x, labels, cu, reference, beta, smoothing, average, ignore):
+        T, P, dev = x.shape[0], reference.numel() // 2, x.device
+        new, f32 = torch.empty, torch.float32
+        loss, rewards = new((), dtype=f32, device=dev), new((2, P), dtype=f32, device=dev)
+        rows = new((3 if ctx is not None else 1) * T, dtype=f32, device=dev)  # log-probabilities, and their sums
+        seqs = new(4 * P, dtype=f32, device=dev)  # g_seq, and the pairs' losses (64 bits)
+        lse = rows.data_ptr() + 4 * T if ctx is not None else None
+        r, g = rewards.data_ptr(), seqs.data_ptr()
         with _ops.launch_device(x):
+            _logprobs(x, labels, ignore, rows.data_ptr(), lse)
             H.check(H.load().mhc_preference_fwd(
-                lp.data_ptr(), labels.data_ptr(), ignore, cu.data_ptr(), reference.data_ptr(),
-                loss.data_ptr(), rewards[0].data_ptr(), rewards[1].data_ptr(), g_seq.data_ptr(),
-                scratch.data_ptr(), T, P, beta, smoothing, int(average), H.stream(x.device)),
-                "mhc_preference_fwd")
+                rows.data_ptr(), labels.data_ptr(), ignore, cu.data_ptr(), reference.data_ptr(),
+                loss.data_ptr(), r, r + 4 * P, g, g + 8 * P, T, P, beta, smoothing, int(average),
+                H.stream(dev)), "mhc_preference_fwd")
         chosen, rejected = rewards.unbind(0)
-        if graph:
-            ctx.save_for_backward(x, labels, cu, lse, g_seq)
+        if ctx is not None:
+            ctx.save_for_backward(x, labels, cu, rows, seqs)
             ctx.ignore = ignore
             ctx.mark_non_differentiable(chosen, rejected)
             ctx.set_materialize_grads(False)
@@ -125,17 +126,17 @@ class _PreferenceLoss(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g, *_):
         if g is None:
-            return (None,) * 9
-        x, labels, cu, lse, g_seq = ctx.saved_tensors
+            return (None,) * 8
+        x, labels, cu, rows, seqs = ctx.saved_tensors
         T, V = x.shape
         g = _scalar(g)
         out = torch.empty((T, V), dtype=x.dtype, device=x.device)
         with _ops.launch_device(x):
             H.check(H.load().mhc_preference_bwd(
-                x.data_ptr(), _stride(x), H.dtype_tag(x), labels.data_ptr(), ctx.ignore, lse.data_ptr(),
-                cu.data_ptr(), g_seq.data_ptr(), g.data_ptr(), out.data_ptr(), T, V, g_seq.numel() // 2,
-                H.stream(x.device)), "mhc_preference_bwd")
-        return (out,) + (None,) * 8
+                x.data_ptr(), _stride(x), H.dtype_tag(x), labels.data_ptr(), ctx.ignore,
+                rows.data_ptr() + 4 * T, cu.data_ptr(), seqs.data_ptr(), g.data_ptr(), out.data_ptr(), T, V,
+                seqs.numel() // 4, H.stream(x.device)), "mhc_preference_bwd")
+        return (out,) + (None,) * 7
 
 
 def preference_loss(logits: torch.Tensor, labels: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -168,8 +169,13 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, cu_seqlens: torc
     ref = reference.detach().to(torch.float32).contiguous()
     args = (x, y, cu, ref, float(beta), float(label_smoothing), bool(average), int(ignore_index))
     if _ops.wants_graph(logits):
-        return _PreferenceLoss.apply(*args, True)
-    return _PreferenceLoss.forward(None, *args, False)
+        return _PreferenceLoss.apply(*args)
+    return _PreferenceLoss.forward(None, *args)
+
+
+@functools.lru_cache(maxsize=1024)
+def _balance_workspace(T: int, E: int, B: int) -> int:
+    return max(H.load().mhc_balance_workspace_bytes(T, E, B), 0)
 
 
 class _BalanceLoss(torch.autograd.Function):
@@ -179,17 +185,16 @@ class _BalanceLoss(torch.autograd.Function):
         B = 1 if cu is None else cu.numel() - 1
         dev, new, lib = scores.device, torch.empty, H.load()
         loss = new((), dtype=torch.float32, device=dev)
-        counts = new((B, E), dtype=torch.int64, device=dev)
-        filled = new((), dtype=torch.int32, device=dev)
+        counts = new(E if cu is None else (B, E), dtype=torch.int64, device=dev)
         with _ops.launch_device(scores):
-            nbytes = lib.mhc_balance_workspace_bytes(T, E, B)
-            ws = new(max(nbytes, 0), dtype=torch.uint8, device=dev)
+            nbytes = _balance_workspace(T, E, B)
+            ws = new(nbytes + 16, dtype=torch.uint8, device=dev)  # the sequences with rows, then the partial sums
             H.check(lib.mhc_balance_fwd(
                 scores.data_ptr(), _stride(scores), H.dtype_tag(scores), index.data_ptr(), H.ptr(cu),
-                loss.data_ptr(), counts.data_ptr(), filled.data_ptr(), ws.data_ptr(), max(nbytes, 0),
+                loss.data_ptr(), counts.data_ptr(), ws.data_ptr(), ws.data_ptr() + 16, nbytes,
                 T, E, index.shape[1], B, coef, H.stream(dev)), "mhc_balance_fwd")
         if ctx is not None:
-            ctx.save_for_backward(cu, counts, filled)
+            ctx.save_for_backward(cu, counts, ws)
             ctx.shape, ctx.dtype, ctx.coef = (T, E), scores.dtype, coef
             ctx.mark_non_differentiable(counts)
             ctx.set_materialize_grads(False)
@@ -200,13 +205,13 @@ class _BalanceLoss(torch.autograd.Function):
     def backward(ctx, g, *_):
         if g is None:
             return (None,) * 4
-        cu, counts, filled = ctx.saved_tensors
+        cu, counts, ws = ctx.saved_tensors
         (T, E), g = ctx.shape, _scalar(g)
         out = torch.empty((T, E), dtype=ctx.dtype, device=counts.device)
         with _ops.launch_device(counts):
             H.check(H.load().mhc_balance_bwd(
-                H.ptr(cu), counts.data_ptr(), filled.data_ptr(), g.data_ptr(), out.data_ptr(),
-                H.dtype_tag(out), T, E, counts.shape[0], ctx.coef, H.stream(counts.device)),
+                H.ptr(cu), counts.data_ptr(), ws.data_ptr(), g.data_ptr(), out.data_ptr(),
+                H.dtype_tag(out), T, E, counts.numel() // E, ctx.coef, H.stream(counts.device)),
                 "mhc_balance_bwd")
         return out, None, None, None
 
@@ -233,7 +238,5 @@ def balance_loss(scores: torch.Tensor, index: torch.Tensor, coef: float,
     idx = index.reshape(-1, index.shape[-1]).contiguous()
     cu = None if cu_seqlens is None else _bounds("cu_seqlens", cu_seqlens, None, dev)
     if _ops.wants_graph(scores):
-        loss, counts = _BalanceLoss.apply(x, idx, cu, float(coef))
-    else:
-        loss, counts = _BalanceLoss.forward(None, x, idx, cu, float(coef))
-    return loss, counts if cu is not None else counts[0]
+        return _BalanceLoss.apply(x, idx, cu, float(coef))
+    return _BalanceLoss.forward(None, x, idx, cu, float(coef))

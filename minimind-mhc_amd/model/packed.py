@@ -6,6 +6,7 @@ No reference counterpart: the reference pads (model/model_minimind.py:161-256).
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional
 
@@ -55,6 +56,14 @@ def _dims(q, k, v):
     return Tq, heads, hd, Tk, kv
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace(backward: bool, *sizes) -> int:
+    """Bytes, which the sizes alone decide: asked of the library once for each (1.5 us)."""
+    lib = H.load()
+    ask = lib.mhc_packed_attn_bwd_workspace_bytes if backward else lib.mhc_packed_attn_workspace_bytes
+    return max(ask(*sizes), 0)
+
+
 def _forward(q, k, v, cu_q, cu_k, used, scale, graph):
     (q, *qs), (k, *ks), (v, *vs) = _strided(q), _strided(k), _strided(v)
     Tq, heads, hd = q.shape
@@ -64,11 +73,11 @@ def _forward(q, k, v, cu_q, cu_k, used, scale, graph):
     rest = torch.empty_like(out) if graph else None
     lse = torch.empty((heads, Tq), dtype=torch.float32, device=dev) if graph else None
     with _ops.launch_device(q):
-        nbytes = lib.mhc_packed_attn_workspace_bytes(B, Tq, Tk, heads, kv, hd)
+        nbytes = _workspace(False, B, Tq, Tk, heads, kv, hd)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
         H.check(lib.mhc_packed_attn_fwd(
             q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs, cu_q.data_ptr(), cu_k.data_ptr(),
-            H.ptr(used), out.data_ptr(), H.ptr(rest), H.ptr(lse), H.ptr(ws), max(nbytes, 0), B, Tq, Tk,
+            H.ptr(used), out.data_ptr(), H.ptr(rest), H.ptr(lse), H.ptr(ws), nbytes, B, Tq, Tk,
             heads, kv, hd, H.dtype_tag(q), scale, H.stream(dev)), "mhc_packed_attn_fwd")
     return out, rest, lse
 
@@ -96,12 +105,12 @@ class _PackedAttention(torch.autograd.Function):
         g_k, g_v = (new((Tk, kv, hd), dtype=q.dtype, device=dev) for _ in range(2))
         B, lib = cu_q.numel() - 1, H.load()
         with _ops.launch_device(q):
-            nbytes = lib.mhc_packed_attn_bwd_workspace_bytes(B, Tq, Tk, heads, kv, hd)
-            ws = new(max(nbytes, 0), dtype=torch.uint8, device=dev)
+            nbytes = _workspace(True, B, Tq, Tk, heads, kv, hd)
+            ws = new(nbytes, dtype=torch.uint8, device=dev)
             H.check(lib.mhc_packed_attn_bwd(
                 q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs, cu_q.data_ptr(),
                 cu_k.data_ptr(), H.ptr(used), out.data_ptr(), rest.data_ptr(), lse.data_ptr(), g.data_ptr(),
-                g_q.data_ptr(), g_k.data_ptr(), g_v.data_ptr(), ws.data_ptr(), max(nbytes, 0), B, Tq, Tk,
+                g_q.data_ptr(), g_k.data_ptr(), g_v.data_ptr(), ws.data_ptr(), nbytes, B, Tq, Tk,
                 heads, kv, hd, H.dtype_tag(q), ctx.scale, H.stream(dev)), "mhc_packed_attn_bwd")
         return g_q, g_k, g_v, None, None, None, None
 

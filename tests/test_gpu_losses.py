@@ -242,6 +242,25 @@ def test_balance_ignores_foreign_experts(dev):
 
 
 @pytest.mark.gpu
+def test_no_rows_and_no_sequences(dev):
+    x, y = torch.zeros(0, 10, device=dev, requires_grad=True), torch.zeros(0, dtype=torch.int64, device=dev)
+    lp = token_logprobs(x, y)
+    assert lp.shape == (0,) and torch.autograd.grad(lp.sum(), x)[0].shape == (0, 10)
+    cu, ref = torch.zeros(3, dtype=torch.int32, device=dev), torch.tensor([1.0, 3.0], device=dev)
+    loss, c, r = preference_loss(x, y, cu, ref, 0.5)
+    assert abs(float(loss) - math.log1p(math.exp(-1.0))) <= 2.0 ** -22 and float(c) == -0.5 and float(r) == -1.5
+    assert torch.autograd.grad(loss, x)[0].shape == (0, 10)
+    s = torch.rand(7, 4, device=dev, requires_grad=True)
+    k = torch.zeros(7, 1, dtype=torch.int64, device=dev)
+    for bounds in ([0], [0, 0, 0]):
+        loss, counts = balance_loss(s, k, 1.0, torch.tensor(bounds, dtype=torch.int32, device=dev))
+        assert float(loss) == 0.0 and counts.shape == (len(bounds) - 1, 4) and not bool(counts.any())
+        assert not bool(torch.autograd.grad(loss, s)[0].any())
+    loss, counts = balance_loss(s[:0], k[:0], 1.0)
+    assert float(loss) == 0.0 and not bool(counts.any())
+
+
+@pytest.mark.gpu
 def test_logits_past_32_bits(dev):
     """Rows past 2^31 elements, both ways."""
     V = 65536
