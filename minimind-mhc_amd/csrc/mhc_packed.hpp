@@ -187,8 +187,8 @@ __device__ __forceinline__ void packed_rank(const int* cu, int B, int T, int M, 
 // Whether a workgroup is two halves of four waves that share its tiles: where the launch has
 // about one workgroup a CU, so the longest chain of tiles sets its time.  Forward: one sequence
 // of 4096 tokens, 8 / 4 heads of 96 (264 workgroups), 71 us and 91 without; 12 sequences of 8192
-// tokens together (564), 52 and 47.  dK and dV of those (308): 102 and 139; of 3 sequences of
-// 16001 tokens, 8 heads of 64 (1032): 372 and 350.
+// tokens together (564), 52 and 47.  dK and dV of those in one range (308): 102 and 139; of 3
+// sequences of 16001 tokens, 8 heads of 64 (1032): 372 and 350.
 inline bool packed_halves(unsigned workgroups) { return workgroups <= (unsigned)device_cus() * 5 / 4; }
 // Tile numbers of T rows in B sequences.
 inline int64_t packed_tiles(int64_t T, int64_t B, int M) { return T / M + B + 1; }

@@ -561,15 +561,16 @@ hipError_t packed_bwd_hd(PackedAttnArgs a, hipStream_t s) {
 }  // namespace
 
 // Ranges that the query rows of a key tile are cut into: up to four workgroups a CU, none of
-// under 32 tiles of rows, so that the ranges' sums (8 bytes an element each way) stay small
-// beside the products.  A step of 2 sequences of 8000 tokens together, 8 / 2 heads of 128: 522 us
+// under 8 tiles of rows (on average), beside whose products the ranges' sums (8 bytes an element
+// each way) are small.  A step of 12 sequences of 8192 tokens together, 8 / 4 heads of 96: 179 us with
+// 3 ranges, 206 with one, 219 with 8; of 30 of 10000, 12 / 4 heads: 194, 231 and 254; of 2 sequences of 8000 tokens together, 8 / 2 heads of 128: 522 us
 // with 4 ranges and 1120 with one; of 2 of 16000, 16 / 2 heads of 64: 1540 with 4, 2136 with 2, 2496
 // with one; of 3 of 16001, 8 / 8 heads of 64 (four workgroups a CU as it is): 688 with 2, 664 with one.
 void packed_bwd_plan(PackedAttnArgs& a) {
   const int64_t groups = (int64_t)a.Tk * a.kv_heads / 128 + 1;  // workgroups with work, about
   const int64_t chain = (int64_t)a.Tq / (a.B > 0 ? a.B : 1) * (a.heads / a.kv_heads) / 32;  // tiles of the longest, about
   int64_t want = 4 * (int64_t)device_cus() / groups;
-  if (want > chain / 32) want = chain / 32;
+  if (want > chain / 8) want = chain / 8;
   if (want > 8) want = 8;
   a.ranges = want < 1 ? 1 : (int)want;
 }
