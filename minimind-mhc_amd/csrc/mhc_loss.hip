@@ -55,7 +55,9 @@ __device__ __forceinline__ U32x4 pack16(const float (&x)[kPer16<DT>]) {
 // --------------------------------------------------- log-probabilities of labels
 // One workgroup a row, one pass: each thread keeps a running maximum and sum.  A row may
 // begin anywhere: the elements before its first 16-byte boundary and behind its last go one
-// by one.  Rows whose label does not count are not read.
+// by one.  Rows whose label does not count are not read.  16384 x 6400 bf16 rows, a quarter of them
+// uncounted, 157 MB: 30 us, 5.2 TB/s, the rate of a copy; 2047 x 50257 fp32 55 us, 5.6 TB/s.  (Cached
+// instead of non-temporal loads 34 us.)
 template <int DT>
 __global__ __launch_bounds__(256) void logprob_kernel(LogitArgs a) {
   constexpr int PER = kPer16<DT>;
@@ -135,6 +137,9 @@ __device__ __forceinline__ float row_factor(const LogitArgs& a, int64_t row) {
   return lo < a.B ? a.g_seq[lo] * a.g_loss[0] : 0.f;
 }
 
+// One workgroup a row again: p from the stored maximum and sum, and the gradient, zeros where
+// the label does not count.  16384 x 6400 bf16, 367 MB: 54 us, 6.8 TB/s with part of the logits still in
+// the memory-side cache; 2047 x 50257 fp32, 720 MB: 138 to 173 us.
 template <int DT>
 __global__ __launch_bounds__(256) void logprob_bwd_kernel(LogitArgs a) {
   constexpr int PER = kPer16<DT>;
@@ -186,7 +191,8 @@ __device__ __forceinline__ double softplus(double t) { return fmax(t, 0.0) + log
 __device__ __forceinline__ double sigmoid_d(double t) { return 1.0 / (1.0 + exp(-t)); }
 
 // One workgroup a pair: both sequences' sums in 64 bits (a sequence's sum is hundreds of
-// units, the rewards' difference less than one), the pair's loss and its rows' factors.
+// units, the rewards' difference less than one), the pair's loss and its rows' factors.  16
+// pairs of 16384 rows: 5.4 us, latency.
 __global__ __launch_bounds__(256) void preference_kernel(PreferenceArgs a) {
   __shared__ double part[2][4];
   __shared__ int cnt[2][4];
@@ -237,7 +243,7 @@ __global__ __launch_bounds__(64) void preference_mean_kernel(PreferenceArgs a) {
 // -------------------------------------------------------------- balance loss
 // Each workgroup sums a range of one sequence's rows into partials; columns of scores in
 // registers (thread = column of a row group), counts by LDS integers (their order changes
-// nothing).  A second launch adds the ranges in order.
+// nothing).  A second launch adds the ranges in order.  16384 x 8 bf16: 3.7 us, latency.
 template <int DT>
 __global__ __launch_bounds__(256) void balance_kernel(BalanceArgs a) {
   extern __shared__ float sums[];  // [256] then int counts [E]
@@ -330,6 +336,7 @@ __global__ __launch_bounds__(1024) void balance_join_kernel(BalanceArgs a) {
   a.filled[0] = n;
 }
 
+// coef E f_e / T for every row: 16384 x 8 bf16 3.0 us, 8191 x 64 fp32 5.0 us, launch and divisions.
 template <int DT>
 __global__ __launch_bounds__(256) void balance_bwd_kernel(BalanceArgs a) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;

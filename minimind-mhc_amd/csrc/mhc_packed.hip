@@ -17,7 +17,13 @@ namespace {
 //     one query row, and S^T's registers, rounded, are P^T's operand as they stand.  V^T comes
 //     from the row-major tile by the transposing LDS load.
 //   * K and V tiles of 64 keys come through a ring of LDS stages by direct-to-LDS loads,
-//     one tile (head_dim 128) or two ahead.
+//     one tile (head_dim 128) or two ahead: through registers 0.5 us of a 1.7 us step was waiting.
+//   * The second half's softmax stands between the first half's output products, so the
+//     matrix cores and the VALU of a wave work side by side there.
+// Two fp16 sequences of 11903 and 4480 tokens, 8 / 2 heads of 128: 336 to 395 us, 840 to 990 TFLOP/s
+// (an 8192^3 product of the library 1268); matrix cores busy 49% of the time, the VALU 52%. Three
+// of 16001 together, 8 heads of 64: 201 us, 650 TFLOP/s, 43% and 61%: the exponentials bound it. 16 prompts
+// of 8192 together, 8 / 4 heads of 96: 37 us, of which the longest prompt's chain is 28.
 template <bool F16, int HD, int HP, int KS>
 __global__ __launch_bounds__(256 * KS, 2) void packed_fwd_kernel(PackedAttnArgs a) {
   constexpr int NC = HD / 32, ND = HD / 16, KT = 64;
@@ -274,8 +280,10 @@ __global__ __launch_bounds__(256 * KS, 2) void packed_fwd_kernel(PackedAttnArgs 
 
 // --------------------------------------------------------------- few queries, many keys
 // A workgroup takes up to 16 rows (tokens times query heads of one kv head) and a range of
-// the keys; its four waves take the range's 64-key tiles in turn, each with sums and LDS of
-// its own, and join at the end.
+// the keys; its four waves take the range's 32-key tiles in turn, each with sums and LDS of
+// its own (no barrier in the loop), and join at the end.  Bound by the cache's bytes, each
+// read once: 64 single tokens over slots of 2176 rows, 4 kv heads of 96, 144 MB, 33 us, 4.4 TB/s
+// (the first keys arrive some 5 us after the launch; 5.5 TB/s then).
 template <bool F16, int HD>
 __global__ __launch_bounds__(256) void packed_few_kernel(PackedAttnArgs a) {
   constexpr int NC = HD / 32, ND = HD / 16, KT = 32;
@@ -555,30 +563,38 @@ hipError_t packed_fwd_hd(const PackedAttnArgs& a, hipStream_t s) {
 
 }  // namespace
 
-// Which kernel, how many heads a workgroup takes and into how many ranges the keys go.
-// Only the totals are known here; the sequences' own lengths are read on the device.
+// Which kernel, how many heads a workgroup takes and into how many ranges the keys go. Only
+// the totals are known here; the sequences' own lengths are read on the device.
+//   * The kernel for few rows up to 8 rows (tokens times query heads of a kv head) a sequence on
+//     average: 64 sequences over 2176-row slots, 8 / 4 heads of 96, 1 new token each 36.3 us (the other
+//     kernel 38.5), 4 tokens 37.1 and 39.4, 8 tokens 51.5 and 40.8.
+//   * Ranges: two workgroups a CU, none of under 128 (512) keys on average. Those 64 single tokens
+//     in 1, 2, 4 and 8 ranges: 41.4, 36.3, 37.0, 41.4 us; 4 sequences of 4 tokens over 8000-row slots in 8, 16,
+//     32 and 64: 23.5, 23.0, 22.8, 23.0; one chunk of 512 tokens over 60000 rows, 16 / 2 heads of 128, in 4, 8, 16 and
+//     32: 180, 108, 109, 123; 8 of 128 over 4096 rows in 4, 8 and 16: 34.2, 32.5, 43.0.
 void packed_attn_plan(PackedAttnArgs& a) {
   const int rep = a.heads / a.kv_heads;
   const int B = a.B > 0 ? a.B : 1;
-  a.few = (int64_t)a.Tq * rep <= 16 * (int64_t)B;
-  int64_t units;
-  int tile;
+  a.few = (int64_t)a.Tq * rep <= 8 * (int64_t)B;
+  int groups, rows;
   if (a.few) {
     const int nb = (rep + 15) / 16;
     a.row_heads = (rep + nb - 1) / nb;
-    a.qtiles = (int)packed_tiles(a.Tq, a.B, 16 / a.row_heads);
-    const int64_t full = (a.Tq + 16 / a.row_heads - 1) / (16 / a.row_heads);  // tiles with rows, about
-    units = (full > B ? full : B < a.Tq ? B : a.Tq) * a.kv_heads * nb;
-    tile = 128;
+    groups = a.kv_heads * nb;
+    rows = 16 / a.row_heads;
   } else {
     a.row_heads = rep % 2 == 0 ? 2 : 1;
-    a.qtiles = (int)packed_tiles(a.Tq, a.B, 128 / a.row_heads);
-    units = ((int64_t)a.Tq * a.row_heads / 128 + 1) * (a.heads / a.row_heads);
-    tile = 512;
+    groups = a.heads / a.row_heads;
+    rows = 128 / a.row_heads;
   }
+  a.qtiles = (int)packed_tiles(a.Tq, a.B, rows);
+  // workgroups with rows, about: at least one a sequence
+  const int64_t full = ((int64_t)a.Tq + rows - 1) / rows, some = B < a.Tq ? B : a.Tq;
+  const int64_t units = (full > some ? full : some) * groups;
   const int64_t keys = a.Tk / B;  // of a sequence, on average
-  int64_t want = units > 0 ? (int64_t)device_cus() * (a.few ? 4 : 2) / units : 1;
-  if (want > keys / tile) want = keys / tile;
+  int64_t want = units > 0 ? (int64_t)device_cus() * 2 / units : 1;
+  const int least = a.few ? 128 : 512;
+  if (want > keys / least) want = keys / least;
   if (want > 128) want = 128;
   a.splits = want < 1 ? 1 : (int)want;
 }

@@ -12,7 +12,9 @@ namespace {
 
 // dQ: as the forward, one 4-wave workgroup per 128 query rows of one kv head, 32 rows a
 // wave.  S^T = K Q^T and dP^T = V G^T put a lane's values all in one query row, and dS^T,
-// rounded, is the operand of dQ^T = K^T dS^T as it stands.
+// rounded, is the operand of dQ^T = K^T dS^T as it stands.  Tiles and stages as there.
+// Three sequences of 16001 tokens together, 8 heads of 64: 229 us, 860 TFLOP/s of its three products
+// (matrix cores busy 44%, VALU 59%); 12 of 8192, 8 / 4 heads of 96: 54 us.
 template <bool F16, int HD, int HP>
 __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
   constexpr int NC = HD / 32, ND = HD / 16, KT = 64;
@@ -228,6 +230,8 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
 // An fp16 P is 2^14 times as large, which is taken out of dS as it is formed and of dV at the
 // end: a row of many keys has probabilities below fp16's smallest normal number.  dS has
 // no bound and stays as it is: its terms under 2^-14 round at 2^-25, as any fp16 gradient does.
+// Three sequences of 16001 tokens together, 8 heads of 64: 346 us, 760 TFLOP/s of its four products
+// (matrix cores busy 38%, VALU 50%); 12 of 8192, 8 / 4 heads of 96: 67 us and 14 for the join.
 // KS = 2: four more waves take every second tile of rows, and the halves add up at the end.
 // With a.ranges > 1 a workgroup takes one range of the rows' tiles and leaves its sums in fp32
 // for packed_dkv_join_kernel.
