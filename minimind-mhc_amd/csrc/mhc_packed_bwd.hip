@@ -12,18 +12,21 @@ namespace {
 
 // dQ: as the forward, one 4-wave workgroup per 128 query rows of one kv head, 32 rows a
 // wave.  S^T = K Q^T and dP^T = V G^T put a lane's values all in one query row, and dS^T,
-// rounded, is the operand of dQ^T = K^T dS^T as it stands.  Tiles and stages as there.
+// rounded, is the operand of dQ^T = K^T dS^T as it stands.  Tiles, stages and halves as there.
 // Three sequences of 16001 tokens together, 8 heads of 64: 229 us, 860 TFLOP/s of its three products
 // (matrix cores busy 44%, VALU 59%); 12 of 8192, 8 / 4 heads of 96: 54 us.
-template <bool F16, int HD, int HP>
-__global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
+template <bool F16, int HD, int HP, int KS>
+__global__ __launch_bounds__(256 * KS, 2) void packed_dq_kernel(PackedAttnArgs a) {
   constexpr int NC = HD / 32, ND = HD / 16, KT = 64;
   constexpr int PW = 128 / HP;
   constexpr int S = HD == 128 ? 2 : 3;     // stages
   constexpr int TILE = KT * HD;            // elements
   constexpr int UW = TILE * 2 / 1024 / 4;  // 1 KiB units of a tile a wave loads
-  __shared__ __align__(16) uint16_t lds[S][2][TILE];
-  const int tid = threadIdx.x;
+  __shared__ __align__(16) uint16_t lds_[KS][S][2][TILE];
+  static_assert(KS == 1 || sizeof(lds_) >= 4 * 64 * 2 * ND * 16, "the second half's sums take the tiles' place");
+  const int tid = threadIdx.x & 255;
+  const int half = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  auto& lds = lds_[half];
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 15, g = lane >> 4;
   const int groups = a.heads / HP;
@@ -37,7 +40,8 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
   const int pb = t.first + (HP == 2 ? (wave & 1) * 32 : wave * 32);
   const int shift = kk.len - t.end;
   const int last = min(t.first + PW, t.end) - 1 + shift;
-  const int nt = last < 0 ? 0 : last / KT + 1;
+  const int nt_all = last < 0 ? 0 : last / KT + 1;
+  const int nt = (nt_all - half + KS - 1) / KS, steps = (nt_all + KS - 1) / KS;  // this half's tiles
 
   const int64_t ks_t = a.ks_t, vs_t = a.vs_t;
   const uint16_t* kg = static_cast<const uint16_t*>(a.k) + kk.start * ks_t + kvh * a.ks_h;
@@ -46,9 +50,9 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
   kl.init(wave * UW, ks_t);
   vl.init(wave * UW, vs_t);
   auto issue = [&](int i, uint16_t* __restrict__ kd, uint16_t* __restrict__ vd) {
-    const int left = kk.len - i * KT;
-    kl.issue(kd, kg + (int64_t)i * KT * ks_t, wave * UW, ks_t, KT, left);
-    vl.issue(vd, vg + (int64_t)i * KT * vs_t, wave * UW, vs_t, KT, left);
+    const int kt = i * KS + half, left = kk.len - kt * KT;
+    kl.issue(kd, kg + (int64_t)kt * KT * ks_t, wave * UW, ks_t, KT, left);
+    vl.issue(vd, vg + (int64_t)kt * KT * vs_t, wave * UW, vs_t, KT, left);
   };
   U32x4 qb[2][NC], gb[2][NC];
   float lse[2], delta[2];
@@ -77,7 +81,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
     d += xor_lane32(d);
     delta[u] = d;
     lse[u] = a.lse[(int64_t)h * a.Tq + at];
-    if (g == 0 && row < t.end) a.delta[(int64_t)h * a.Tq + row] = d;
+    if (half == 0 && g == 0 && row < t.end) a.delta[(int64_t)h * a.Tq + row] = d;
   }
 #pragma unroll
   for (int i = 0; i < S - 1; ++i)
@@ -94,9 +98,9 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
   // step i: the tile in ks and vs, while one lands in kd and vd (which differ: restrict)
   auto step = [&](int i, const uint16_t* __restrict__ ks, const uint16_t* __restrict__ vs, uint16_t* __restrict__ kd,
                   uint16_t* __restrict__ vd) {
-    const int s0 = i * KT;
+    const int s0 = (i * KS + half) * KT;
     if (i + S - 1 < nt) issue(i + S - 1, kd, vd);
-    if (pb >= t.end || s0 > pb + 31 + shift) return;
+    if (i >= nt || pb >= t.end || s0 > pb + 31 + shift) return;
     const bool diagonal = s0 + KT - 1 > pb + shift;
     f32x4_t s[2][2][2], dp[2][2][2];  // [half of the tile][16 query rows][16 keys]
     U32x4 kc[2][ND], pf[2][2];
@@ -200,13 +204,33 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(PackedAttnArgs a) {
     }
   };
   int stage = 0;
-  for (int i = 0; i < nt; ++i) {
+  for (int i = 0; i < steps; ++i) {
     if (S > 2 && i + S - 1 <= nt) tile_wait<(S - 2) * 2 * UW>();
     else tile_wait<0>();
     tile_barrier();
     const int next = stage == 0 ? S - 1 : stage - 1;
     step(i, lds[stage][0], lds[stage][1], lds[next][0], lds[next][1]);
     stage = stage == S - 1 ? 0 : stage + 1;
+  }
+  if constexpr (KS == 2) {
+    __syncthreads();
+    float* x = reinterpret_cast<float*>(lds_) + wave * 64 * (2 * ND * 4) + lane * 4;
+    if (half == 1) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4_t*>(x + (u * ND + d) * 256) = dq[u][d];
+    }
+    __syncthreads();
+    if (half == 1) return;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const f32x4_t y = *reinterpret_cast<const f32x4_t*>(x + (u * ND + d) * 256);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dq[u][d][j] += y[j];
+      }
   }
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -544,10 +568,14 @@ hipError_t packed_bwd_hd(PackedAttnArgs a, hipStream_t s) {
   a.qtiles = (int)packed_tiles(a.Tq, a.B, 128 / hp);
   const dim3 grid((unsigned)((int64_t)a.qtiles * (a.heads / hp)));
   if (a.Tq > 0) {
-    if (hp == 2)
-      packed_dq_kernel<F16, HD, 2><<<grid, 256, 0, s>>>(a);
-    else
-      packed_dq_kernel<F16, HD, 1><<<grid, 256, 0, s>>>(a);
+    const bool halves = packed_halves(grid.x);
+    if (hp == 2) {
+      if (halves) packed_dq_kernel<F16, HD, 2, 2><<<grid, 512, 0, s>>>(a);
+      else packed_dq_kernel<F16, HD, 2, 1><<<grid, 256, 0, s>>>(a);
+    } else {
+      if (halves) packed_dq_kernel<F16, HD, 1, 2><<<grid, 512, 0, s>>>(a);
+      else packed_dq_kernel<F16, HD, 1, 1><<<grid, 256, 0, s>>>(a);
+    }
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
   if (a.Tk == 0) return hipSuccess;
