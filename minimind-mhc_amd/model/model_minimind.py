@@ -460,11 +460,8 @@ class MiniMindForCausalLM(nn.Module):
         labels, fp32 [n]: what preference_loss takes from its reference model.  Sums in 64 bits."""
         y = packed.next_labels(labels)[0]
         lp = self._token_logprobs(self(input_ids, packed=packed).logits[0], y)
-        at = packed.cu_seqlens.long()
-        def sums(t):  # noqa: E306
-            return F.pad(t.double().cumsum(0), (1, 0))[at].diff()
-        total = sums(lp)
-        return (total / sums(y != -100).clamp_min(1) if average else total).float()
+        total = packed.sums(lp)
+        return (total / packed.sums(y != -100).clamp_min(1) if average else total).float()
 
     def preference_loss(self, input_ids, labels, packed, reference, beta=0.1, label_smoothing=0.0,
                         average=False):

@@ -205,6 +205,14 @@ class PackedBatch:
         moved = torch.cat([labels[:, 1:], labels[:, :1]], 1)
         return moved.masked_fill((after != self.sequence) | (self.sequence == n), ignore_index)
 
+    def sums(self, t: torch.Tensor) -> torch.Tensor:
+        """The sum of t [rows] over each sequence, [n], in 64 bits and in the same order on every
+        run.  Each by itself: differences of one running sum would carry a value that is not
+        finite into every later sequence."""
+        at = self.cu_seqlens.long().clamp(0, self.rows)  # as the kernels take the bounds
+        at = torch.cat([at.new_zeros(1), at[1:]]).cummax(0).values
+        return torch.segment_reduce(t.double(), "sum", offsets=at, initial=0.0, unsafe=True)
+
 
 class PackedCache:
     """Keys and values of n sequences that grow in place, each in a slot of `capacity` rows

@@ -1,0 +1,70 @@
+"""Packed sequences without a GPU, where a call's sequences, rows, types and lengths are not
+the usual ones: values that are not finite, rows behind the last sequence, bounds past the
+rows, caches of another type, slots that fill up unevenly."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from model.model_minimind import MiniMindForCausalLM
+from model.packed import PackedBatch
+from tests.test_packed import _ints, _model
+
+
+# ------------------------------------------------- log-probabilities of sequences
+
+def _rows_of(m, monkeypatch, lp):
+    """m, whose rows' log-probabilities are lp wherever a label counts."""
+    monkeypatch.setattr(MiniMindForCausalLM, "_token_logprobs",
+                        staticmethod(lambda logits, y: torch.where(y != -100, lp, 0.0)))
+    return m
+
+
+@pytest.mark.parametrize("average", [False, True])
+@pytest.mark.parametrize("bad", [-math.inf, math.nan])
+def test_sequence_logprobs_keep_to_their_sequence(monkeypatch, bad, average):
+    lengths = [3, 0, 4, 1, 5]
+    b = PackedBatch.from_lengths(lengths, rows=15, device="cpu")
+    lp = -torch.rand(15)
+    lp[4] = bad  # of the third
+    got = _rows_of(_model(), monkeypatch, lp).sequence_logprobs(
+        torch.zeros(1, 15, dtype=torch.int64), torch.zeros(1, 15, dtype=torch.int64), b, average)
+    want, at = [], 0
+    for n in lengths:  # a sequence's last row predicts nothing
+        s = sum(float(x) for x in lp[at:at + max(n - 1, 0)])
+        want.append(s / max(n - 1, 1) if average else s)
+        at += n
+    assert got.dtype == torch.float32
+    # 64-bit sums, rounded once
+    torch.testing.assert_close(got, torch.tensor(want, dtype=torch.float64).float(), rtol=2.0 ** -23, atol=0.0,
+                               equal_nan=True)
+    assert torch.isfinite(got[[0, 1, 3, 4]]).all() and not math.isfinite(got[2])
+
+
+@pytest.mark.parametrize("cu", [(0, 5, 20), (0, -3, 12), (0, 9, 4)])
+def test_sequence_logprobs_of_bounds_past_the_rows(monkeypatch, cu):
+    """Clamped to the rows, as everywhere (the last: decreasing, any values, but no error)."""
+    b = PackedBatch(_ints(*cu), 12)
+    lp = -torch.rand(12)
+    ids = torch.zeros(1, 12, dtype=torch.int64)
+    got = _rows_of(_model(), monkeypatch, lp).sequence_logprobs(ids, ids, b)
+    assert got.shape == (2,)
+    if cu[1] == 5:
+        torch.testing.assert_close(got, torch.stack([lp[:4].double().sum(), lp[5:11].double().sum()]).float())
+
+
+def test_sequence_logprobs_gradient():
+    m = _model()
+    b = PackedBatch.from_lengths([4, 1, 6], rows=13, device="cpu")
+    ids = torch.randint(0, 50, (1, 13))
+    s = m.sequence_logprobs(ids, ids, b)
+    got = torch.autograd.grad((s * torch.tensor([1.0, 5.0, -2.0])).sum(), list(m.parameters()))
+    ref = []
+    for a, n in ((0, 4), (5, 6)):
+        lp = torch.log_softmax(m(ids[:, a:a + n]).logits[0], -1)
+        ref.append(lp[:-1].gather(1, ids[0, a + 1:a + n, None]).sum())
+    want = torch.autograd.grad(ref[0] - 2.0 * ref[1], list(m.parameters()))
+    for x, y in zip(got, want):
+        torch.testing.assert_close(x, y, rtol=1e-3, atol=1e-4)
