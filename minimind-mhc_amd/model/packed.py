@@ -254,7 +254,6 @@ class PackedCall:
         if batch.longest is not None:
             if cache._most + batch.longest > cap:
                 raise ValueError(f"mhc_amd: {cache._most} + {batch.longest} tokens may not fit slots of {cap} rows")
-            cache._most += batch.longest
         seq = batch.sequence.clamp_max(n - 1)
         self.positions = cache.lengths[seq] + batch.positions
         room = (batch.sequence < n) & (self.positions < cap)
@@ -262,8 +261,14 @@ class PackedCall:
         self.lengths = (cache.lengths + batch.cu_seqlens.diff()).clamp_max_(cap)
 
     def done(self) -> None:
-        if self.cache is not None:
-            self.cache.lengths.copy_(self.lengths)
+        """The call has stored its tokens: the lengths move on (those that the host keeps too, unless
+        the call was only captured)."""
+        if self.cache is None:
+            return
+        self.cache.lengths.copy_(self.lengths)
+        if self.batch.longest is not None and not (
+                self.lengths.is_cuda and torch.cuda.is_current_stream_capturing()):
+            self.cache._most += self.batch.longest
 
     def attention(self, q, k, v, layer: int, dropout: float = 0.0) -> torch.Tensor:
         """q [1, rows, heads, head_dim], k, v [1, rows, kv heads, head_dim] of the new tokens:

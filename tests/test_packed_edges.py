@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from model.model_minimind import MiniMindForCausalLM
-from model.packed import PackedBatch
+from model.packed import PackedBatch, PackedCache
 from tests.test_packed import _ints, _model
 
 
@@ -68,3 +68,25 @@ def test_sequence_logprobs_gradient():
     want = torch.autograd.grad(ref[0] - 2.0 * ref[1], list(m.parameters()))
     for x, y in zip(got, want):
         torch.testing.assert_close(x, y, rtol=1e-3, atol=1e-4)
+
+
+# ------------------------------------------------- slots that fill up unevenly
+
+def _step(m, cache, lengths, **kw):
+    b = PackedBatch.from_lengths(lengths, device="cpu") if not isinstance(lengths, PackedBatch) else lengths
+    with torch.no_grad():
+        return m(torch.zeros(1, b.rows, dtype=torch.int64), packed=b, past_key_values=cache, **kw)
+
+
+def test_failed_calls_take_no_room(monkeypatch):
+    m = _model().eval()
+    cache = PackedCache(m.config, 2, 10, torch.float32, "cpu")
+    _step(m, cache, [2, 1])
+    with monkeypatch.context() as c:
+        c.setattr(m.model.layers[1].mlp, "forward", lambda z: 1 / 0)
+        for _ in range(3):
+            with pytest.raises(ZeroDivisionError):
+                _step(m, cache, [8, 4])
+    assert cache.lengths.tolist() == [2, 1]
+    _step(m, cache, [8, 8])
+    assert cache.lengths.tolist() == [10, 9]
