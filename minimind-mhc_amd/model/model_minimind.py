@@ -412,7 +412,7 @@ class MiniMindModel(nn.Module):
             raise ValueError("packed sequences take no attention_mask: nothing of them is padding")
         if cache is not None and not isinstance(cache, PackedCache):
             raise ValueError("packed sequences need a PackedCache as past_key_values")
-        return PackedCall(packed, cache), cache, None
+        return PackedCall(packed, cache, slots=True), cache, None
 
 
 class MiniMindForCausalLM(nn.Module):

@@ -172,7 +172,8 @@ class PackedBatch:
     def __init__(self, cu_seqlens: torch.Tensor, rows: int):
         self.cu_seqlens = _bounds("cu_seqlens", cu_seqlens, None, cu_seqlens.device)
         self.rows = int(rows)
-        self.longest: Optional[int] = None  # of the sequences, where the host knows
+        self.lengths: Optional[list] = None  # of the sequences, where the host knows
+        self.longest: Optional[int] = None
         r = torch.arange(self.rows, dtype=torch.int32, device=cu_seqlens.device)
         self.sequence = torch.searchsorted(self.cu_seqlens[1:], r, right=True)  # n behind the last
         self.positions = (r - self.cu_seqlens[self.sequence]).long()
@@ -189,7 +190,8 @@ class PackedBatch:
         if rows < ends[-1]:
             raise ValueError(f"mhc_amd: {ends[-1]} tokens do not fit {rows} rows")
         b = cls(torch.tensor(ends, dtype=torch.int32, device=device), rows)
-        b.longest = max(lengths, default=0)
+        b.lengths = [int(n) for n in lengths]
+        b.longest = max(b.lengths, default=0)
         return b
 
     def __len__(self) -> int:
@@ -232,18 +234,22 @@ class PackedCache:
         self.slots = torch.arange(sequences + 1, dtype=torch.int32, device=device) * capacity
         self.lengths = torch.zeros(sequences, dtype=torch.int32, device=device)
         self.sequences, self.capacity = sequences, capacity
-        self._most = 0  # a bound on the lengths, as far as the host has seen
+        self._seen = [0] * sequences  # the slots' lengths, as far as the host has seen them
 
     def clear(self) -> None:
         """Empties every slot."""
         self.lengths.zero_()
-        self._most = 0
+        self._seen = [0] * self.sequences
 
 
 class PackedCall:
-    """One model call on a PackedBatch: positions, and with a cache where rows go."""
+    """One model call on a PackedBatch: positions, and with a cache where rows go.
 
-    def __init__(self, batch: PackedBatch, cache: Optional[PackedCache] = None):
+    A batch whose lengths the host knows is refused where its longest sequence would not fit
+    behind the longest slot; with `slots` (as the model calls it) only where a sequence would not
+    fit its own."""
+
+    def __init__(self, batch: PackedBatch, cache: Optional[PackedCache] = None, slots: bool = False):
         self.batch, self.cache = batch, cache
         self.positions, self.lengths, self.rows = batch.positions, None, None
         if cache is None:
@@ -251,9 +257,12 @@ class PackedCall:
         n, cap = cache.sequences, cache.capacity
         if len(batch) != n:
             raise ValueError(f"mhc_amd: a batch of {len(batch)} sequences on a cache of {n}")
-        if batch.longest is not None:
-            if cache._most + batch.longest > cap:
-                raise ValueError(f"mhc_amd: {cache._most} + {batch.longest} tokens may not fit slots of {cap} rows")
+        if batch.lengths is not None:
+            have, more = max(cache._seen), batch.longest
+            if slots and have + more > cap:
+                have, more = max(zip(cache._seen, batch.lengths), key=sum)
+            if have + more > cap:
+                raise ValueError(f"mhc_amd: {have} + {more} tokens may not fit slots of {cap} rows")
         seq = batch.sequence.clamp_max(n - 1)
         self.positions = cache.lengths[seq] + batch.positions
         room = (batch.sequence < n) & (self.positions < cap)
@@ -266,9 +275,9 @@ class PackedCall:
         if self.cache is None:
             return
         self.cache.lengths.copy_(self.lengths)
-        if self.batch.longest is not None and not (
+        if self.batch.lengths is not None and not (
                 self.lengths.is_cuda and torch.cuda.is_current_stream_capturing()):
-            self.cache._most += self.batch.longest
+            self.cache._seen = [a + b for a, b in zip(self.cache._seen, self.batch.lengths)]
 
     def attention(self, q, k, v, layer: int, dropout: float = 0.0) -> torch.Tensor:
         """q [1, rows, heads, head_dim], k, v [1, rows, kv heads, head_dim] of the new tokens:

@@ -78,6 +78,22 @@ def _step(m, cache, lengths, **kw):
         return m(torch.zeros(1, b.rows, dtype=torch.int64), packed=b, past_key_values=cache, **kw)
 
 
+def test_uneven_batches_that_fit():
+    m = _model().eval()
+    cache = PackedCache(m.config, 2, 10, torch.float32, "cpu")
+    _step(m, cache, [8, 1])
+    _step(m, cache, [1, 8])
+    _step(m, cache, [1, 0])
+    assert cache.lengths.tolist() == [10, 9]
+    for lengths in ([1, 0], [0, 2]):
+        with pytest.raises(ValueError, match="10 rows"):
+            _step(m, cache, lengths)
+    _step(m, cache, [0, 1])
+    assert cache.lengths.tolist() == [10, 10]
+    cache.clear()
+    _step(m, cache, [10, 10])
+
+
 def test_failed_calls_take_no_room(monkeypatch):
     m = _model().eval()
     cache = PackedCache(m.config, 2, 10, torch.float32, "cpu")
@@ -90,3 +106,15 @@ def test_failed_calls_take_no_room(monkeypatch):
     assert cache.lengths.tolist() == [2, 1]
     _step(m, cache, [8, 8])
     assert cache.lengths.tolist() == [10, 9]
+
+
+def test_batches_of_unknown_lengths_between():
+    """What the host has not seen refuses nothing; what it has seen still does."""
+    m = _model().eval()
+    cache = PackedCache(m.config, 2, 10, torch.float32, "cpu")
+    _step(m, cache, [6, 2])
+    _step(m, cache, PackedBatch(_ints(0, 1, 4), 4))
+    _step(m, cache, [3, 5])
+    assert cache.lengths.tolist() == [10, 10]
+    with pytest.raises(ValueError, match="10 rows"):
+        _step(m, cache, [2, 0])
