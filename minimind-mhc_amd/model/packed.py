@@ -181,17 +181,16 @@ class PackedBatch:
     @classmethod
     def from_lengths(cls, lengths, rows: Optional[int] = None, device="cuda") -> "PackedBatch":
         """Of these lengths; rows: their sum, or more."""
-        ends = [0]
+        lengths, ends = [int(n) for n in lengths], [0]
         for n in lengths:
             if n < 0:
                 raise ValueError(f"mhc_amd: a sequence of {n} tokens")
-            ends.append(ends[-1] + int(n))
+            ends.append(ends[-1] + n)
         rows = ends[-1] if rows is None else rows
         if rows < ends[-1]:
             raise ValueError(f"mhc_amd: {ends[-1]} tokens do not fit {rows} rows")
         b = cls(torch.tensor(ends, dtype=torch.int32, device=device), rows)
-        b.lengths = [int(n) for n in lengths]
-        b.longest = max(b.lengths, default=0)
+        b.lengths, b.longest = lengths, max(lengths, default=0)
         return b
 
     def __len__(self) -> int:

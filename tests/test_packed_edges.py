@@ -118,3 +118,9 @@ def test_batches_of_unknown_lengths_between():
     assert cache.lengths.tolist() == [10, 10]
     with pytest.raises(ValueError, match="10 rows"):
         _step(m, cache, [2, 0])
+
+
+def test_lengths_from_an_iterator():
+    b = PackedBatch.from_lengths((n for n in (3, 5)), device="cpu")
+    assert b.longest == 5 and b.cu_seqlens.tolist() == [0, 3, 8]
+    assert PackedBatch.from_lengths(torch.tensor([3, 5]), device="cpu").longest == 5
