@@ -383,7 +383,8 @@ class MiniMindModel(nn.Module):
         if call is None:
             pos = (self.freqs_cos[start:start + seq_len], self.freqs_sin[start:start + seq_len])
         else:  # each row's position in its own sequence (rows of none: any)
-            at = call.positions.clamp(0, self.freqs_cos.shape[0] - 1)
+            table = self.freqs_cos.shape[0]
+            at = call.positions.clamp(0, table - 1)
             pos = (self.freqs_cos[at], self.freqs_sin[at])
         more = {} if call is None else {"packed": call}
         presents = []
@@ -398,6 +399,9 @@ class MiniMindModel(nn.Module):
             h = self.norm[0](h, out_norm=self.norm[1], chain=chain)
         else:
             h = self.norm(h)
+        if call is not None and call.most > table:  # nothing is right there, and the host cannot tell
+            past = (call.positions >= table) & (packed.sequence < len(packed))
+            h = h.masked_fill(past[None, :, None], math.nan)
         aux = sum([l.mlp.aux_loss for l in self.layers if isinstance(l.mlp, MOEFeedForward)],
                   h.new_zeros(1).squeeze())
         return h, presents, aux
@@ -412,7 +416,10 @@ class MiniMindModel(nn.Module):
             raise ValueError("packed sequences take no attention_mask: nothing of them is padding")
         if cache is not None and not isinstance(cache, PackedCache):
             raise ValueError("packed sequences need a PackedCache as past_key_values")
-        return PackedCall(packed, cache, slots=True), cache, None
+        call, table = PackedCall(packed, cache, slots=True), self.freqs_cos.shape[0]
+        if call.reach > table:
+            raise ValueError(f"a packed sequence reaches {call.reach} positions, max_position_embeddings is {table}")
+        return call, cache, None
 
 
 class MiniMindForCausalLM(nn.Module):

@@ -251,6 +251,8 @@ class PackedCall:
     def __init__(self, batch: PackedBatch, cache: Optional[PackedCache] = None, slots: bool = False):
         self.batch, self.cache = batch, cache
         self.positions, self.lengths, self.rows = batch.positions, None, None
+        # positions that the host knows the sequences reach, and a bound on those they may reach
+        self.reach, self.most = batch.longest or 0, batch.rows if batch.longest is None else batch.longest
         if cache is None:
             return
         n, cap = cache.sequences, cache.capacity
@@ -262,6 +264,8 @@ class PackedCall:
                 have, more = max(zip(cache._seen, batch.lengths), key=sum)
             if have + more > cap:
                 raise ValueError(f"mhc_amd: {have} + {more} tokens may not fit slots of {cap} rows")
+            self.reach = max((a + b for a, b in zip(cache._seen, batch.lengths) if b), default=0)
+        self.most = cap
         seq = batch.sequence.clamp_max(n - 1)
         self.positions = cache.lengths[seq] + batch.positions
         room = (batch.sequence < n) & (self.positions < cap)

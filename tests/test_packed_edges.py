@@ -124,3 +124,48 @@ def test_lengths_from_an_iterator():
     b = PackedBatch.from_lengths((n for n in (3, 5)), device="cpu")
     assert b.longest == 5 and b.cu_seqlens.tolist() == [0, 3, 8]
     assert PackedBatch.from_lengths(torch.tensor([3, 5]), device="cpu").longest == 5
+
+
+# ------------------------------------------------- positions past the rotary table
+
+def test_positions_past_the_table_are_refused():
+    """Where the host knows the lengths; the dense call raises too."""
+    m = _model(max_position_embeddings=16).eval()
+    ids = torch.randint(0, 50, (1, 20))
+    with pytest.raises(RuntimeError):
+        m(ids)
+    for lengths in ([17, 3], [3, 17]):
+        with pytest.raises(ValueError, match="17 positions.*16"):
+            m(ids, packed=PackedBatch.from_lengths(lengths, device="cpu"))
+    b = PackedBatch.from_lengths([16, 1], rows=20, device="cpu")  # 3 rows of no sequence
+    torch.testing.assert_close(m(ids, packed=b).logits[:, :16], m(ids[:, :16]).logits, rtol=1e-4, atol=1e-4)
+
+
+def test_cached_positions_past_the_table_are_refused():
+    m = _model(max_position_embeddings=16).eval()
+    cache = PackedCache(m.config, 2, 20, torch.float32, "cpu")
+    ids = torch.randint(0, 50, (1, 14))
+    with torch.no_grad():
+        m(ids, packed=PackedBatch.from_lengths([10, 4], device="cpu"), past_key_values=cache)
+        with pytest.raises(ValueError, match="17 positions.*16"):
+            m(ids[:, :10], packed=PackedBatch.from_lengths([7, 3], device="cpu"), past_key_values=cache)
+        assert cache.lengths.tolist() == [10, 4]
+        out = m(ids[:, :10], packed=PackedBatch.from_lengths([6, 4], device="cpu"), past_key_values=cache)
+    assert cache.lengths.tolist() == [16, 8] and torch.isfinite(out.logits).all()
+
+
+def test_positions_the_host_does_not_know():
+    """Not a number behind the table's end instead of the last position's angles again: in that
+    sequence alone."""
+    m = _model(max_position_embeddings=16).eval()
+    ids = torch.randint(0, 50, (1, 40))
+    out = m(ids, packed=PackedBatch(_ints(0, 9, 29), 40)).logits[0]  # the second has 20 tokens
+    torch.testing.assert_close(out[:9], m(ids[:, :9]).logits[0], rtol=1e-4, atol=1e-4)
+    assert out[25:29].isnan().all() and torch.isfinite(out[29:]).all()
+    cache = PackedCache(m.config, 2, 20, torch.float32, "cpu")
+    with torch.no_grad():
+        for n in (9, 7):
+            out = m(ids[:, :n + 1], packed=PackedBatch(_ints(0, n, n + 1), n + 1), past_key_values=cache).logits[0]
+            assert torch.isfinite(out).all()
+        out = m(ids[:, :3], packed=PackedBatch(_ints(0, 2, 3), 3), past_key_values=cache).logits[0]
+    assert out[:2].isnan().all() and torch.isfinite(out[2]).all()
