@@ -270,17 +270,28 @@ class MOEFeedForward(nn.Module):
     def _balance(self, scores, idx, b, l, cu_seqlens):
         """(balance loss, the experts' counts): on the kernels for fp32 scores on the GPU, as
         the trainers' autocast gives, and for the loss of each sequence (cu_seqlens, or the
-        batch's rows); else one loss over all tokens on torch ops."""
+        batch's rows); else one loss over all tokens (with cu_seqlens: of the sequences) on torch
+        ops."""
         cfg = self.config
         each = getattr(cfg, "router_aux_loss_per_sequence", False)
         if each and cu_seqlens is None:
             cu_seqlens = torch.arange(b + 1, dtype=torch.int32, device=scores.device) * l
+        elif cu_seqlens is not None and not each:  # one stretch of rows: none behind the last sequence
+            cu_seqlens = torch.cat([cu_seqlens.new_zeros(1), cu_seqlens[-1:]])
         if scores.is_cuda and (each or scores.dtype == torch.float32) and _ops.eager_call():
-            return losses.balance_loss(scores, idx, cfg.router_aux_loss_coef, cu_seqlens if each else None)
+            loss, counts = losses.balance_loss(scores, idx, cfg.router_aux_loss_coef, cu_seqlens)
+            return loss, counts if each or cu_seqlens is None else counts[0]
         hot = F.one_hot(idx, cfg.num_experts)
-        if not each:
+        if cu_seqlens is None:
             load = hot.float().mean(0)
             return (load * scores.mean(0)).sum() * cfg.num_experts * cfg.router_aux_loss_coef, None
+        if not each:
+            rows = scores.shape[0]
+            inside = (torch.arange(rows, device=scores.device) < cu_seqlens[1])[:, None]
+            tokens = cu_seqlens[1].clamp(1, max(rows, 1))
+            load = (hot.sum(1) * inside).sum(0).float() / tokens
+            mean = torch.where(inside, scores.float(), 0.0).sum(0) / tokens
+            return (load * mean).sum() * cfg.num_experts * cfg.router_aux_loss_coef, None
         ends = cu_seqlens.tolist()
         parts = [(hot[i:j].float().sum((0, 1)) / (j - i) * scores[i:j].float().mean(0)).sum()
                  for i, j in zip(ends, ends[1:]) if j > i]

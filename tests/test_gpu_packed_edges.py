@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from model.packed import PackedBatch
+from tests.test_gpu_packed_model import _model
 
 BF, F16 = torch.bfloat16, torch.float16
 
@@ -45,3 +46,32 @@ def test_sums_of_sequences(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, eager)
+
+
+# ------------------------------------------------- the router's balance loss
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("each", [False, True])
+@pytest.mark.parametrize("lengths", [[60, 1, 33], [0, 5, 0], [0]])
+def test_rows_of_no_sequence_are_not_balanced(dev, lengths, each):
+    """Whatever the rows behind the sequences hold: the loss, counts and gradients are those of
+    a batch without such rows (to the sums' order)."""
+    m = _model(dev, torch.float32, use_moe=True, num_experts_per_tok=2, use_mhc=0, router_aux_loss_coef=0.5,
+               router_aux_loss_per_sequence=each).train()
+    moe, n = m.model.layers[0].mlp, sum(lengths)
+    ids = torch.randint(0, 500, (1, n + 70), device=dev)
+    res = []
+    for tail in (0, 70, 70):
+        x = torch.cat([ids[:, :n], torch.randint(0, 500, (1, tail), device=dev)], 1)
+        if x.numel() == 0:
+            continue
+        m.zero_grad()
+        m(x, packed=PackedBatch.from_lengths(lengths, rows=x.shape[1], device=dev)).aux_loss.backward()
+        assert moe.expert_counts.shape == ((len(lengths), 4) if each else (4,))
+        assert int(moe.expert_counts.sum()) == 2 * n
+        res.append((moe.aux_loss.detach().clone(), moe.expert_counts, moe.gate.weight.grad.clone()))
+    for other in res[1:]:
+        assert torch.equal(res[0][1], other[1])
+        torch.testing.assert_close(res[0][0], other[0], rtol=1e-5, atol=0.0)
+        torch.testing.assert_close(res[0][2], other[2], rtol=1e-3, atol=1e-3 * float(res[0][2].abs().max()))
+    assert n or (float(res[0][0]) == 0.0 and float(res[0][2].abs().max()) == 0.0)

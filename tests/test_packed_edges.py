@@ -169,3 +169,31 @@ def test_positions_the_host_does_not_know():
             assert torch.isfinite(out).all()
         out = m(ids[:, :3], packed=PackedBatch(_ints(0, 2, 3), 3), past_key_values=cache).logits[0]
     assert out[:2].isnan().all() and torch.isfinite(out[2]).all()
+
+
+# ------------------------------------------------- the router's balance loss
+
+@pytest.mark.parametrize("lengths", [[3], [6, 6], [0, 4, 0], []])
+def test_rows_of_no_sequence_are_not_balanced(lengths):
+    """The loss over all tokens takes the sequences' tokens alone: the same loss and
+    gradients whatever the rows behind them hold, and those of the sequences without such rows."""
+    m = _model(use_moe=True, num_experts_per_tok=2, router_aux_loss_coef=0.5).train()
+    moe, n = m.model.layers[0].mlp, sum(lengths)
+    res = []
+    ids = torch.randint(0, 50, (1, n + 8))
+    for rows, seed in ((n + 8, 1), (n + 8, 2), (n, None)):
+        x = ids.clone()
+        if seed is not None:
+            x[0, n:] = torch.randint(0, 50, (8,), generator=torch.Generator().manual_seed(seed))
+        m.zero_grad()
+        if rows == 0:
+            continue
+        out = m(x[:, :rows], packed=PackedBatch.from_lengths(lengths, rows=rows, device="cpu"))
+        out.aux_loss.backward()
+        res.append((out.aux_loss.detach(), moe.gate.weight.grad.clone()))
+    for other in res[1:]:
+        # other numbers of rows add up in other orders: 64 terms of a product 64 x 2^-24, some four
+        # products one after another before the gate's gradient, whose elements also cancel
+        for a, b in zip(res[0], other):
+            torch.testing.assert_close(a, b, rtol=0.0, atol=2.0 ** -16 * float(a.abs().max()))
+    assert n or (float(res[0][0]) == 0.0 and float(res[0][1].abs().max()) == 0.0)
