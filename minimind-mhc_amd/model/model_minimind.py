@@ -238,7 +238,8 @@ class MOEFeedForward(nn.Module):
         self.experts = nn.ModuleList([FeedForward(config, config.moe_intermediate_size)
                                       for _ in range(config.num_experts)])
         self.aux_loss = None
-        self.expert_counts = None  # of the last training call: tokens each expert got (by sequence)
+        # tokens each expert got (by sequence) in the last call, where that formed a balance loss
+        self.expert_counts = None
 
     def forward(self, x, cu_seqlens=None):
         b, l, d = x.shape
@@ -249,7 +250,7 @@ class MOEFeedForward(nn.Module):
             y = _ops.moe_experts(self.experts, xf, scores, self.config.num_experts_per_tok,
                                  self.config.norm_topk_prob, zero=aux)
             if y is not None:
-                self.aux_loss = aux
+                self.aux_loss, self.expert_counts = aux, None
                 return y.view(b, l, d)
         w, idx = torch.topk(scores, k=self.config.num_experts_per_tok, dim=-1, sorted=False)
         if self.config.norm_topk_prob:
@@ -263,7 +264,7 @@ class MOEFeedForward(nn.Module):
         if self.training and self.config.router_aux_loss_coef > 0:
             self.aux_loss, self.expert_counts = self._balance(scores, idx, b, l, cu_seqlens)
         else:
-            self.aux_loss = scores.new_zeros(1).squeeze()
+            self.aux_loss, self.expert_counts = scores.new_zeros(1).squeeze(), None
         return y.view(b, l, d)
 
 
@@ -284,14 +285,15 @@ class MOEFeedForward(nn.Module):
         hot = F.one_hot(idx, cfg.num_experts)
         if cu_seqlens is None:
             load = hot.float().mean(0)
-            return (load * scores.mean(0)).sum() * cfg.num_experts * cfg.router_aux_loss_coef, None
+            return (load * scores.mean(0)).sum() * cfg.num_experts * cfg.router_aux_loss_coef, hot.sum((0, 1))
         if not each:
             rows = scores.shape[0]
             inside = (torch.arange(rows, device=scores.device) < cu_seqlens[1])[:, None]
             tokens = cu_seqlens[1].clamp(1, max(rows, 1))
-            load = (hot.sum(1) * inside).sum(0).float() / tokens
+            counts = (hot.sum(1) * inside).sum(0)
             mean = torch.where(inside, scores.float(), 0.0).sum(0) / tokens
-            return (load * mean).sum() * cfg.num_experts * cfg.router_aux_loss_coef, None
+            loss = (counts.float() / tokens * mean).sum()
+            return loss * cfg.num_experts * cfg.router_aux_loss_coef, counts
         ends = cu_seqlens.tolist()
         parts = [(hot[i:j].float().sum((0, 1)) / (j - i) * scores[i:j].float().mean(0)).sum()
                  for i, j in zip(ends, ends[1:]) if j > i]

@@ -197,3 +197,15 @@ def test_rows_of_no_sequence_are_not_balanced(lengths):
         for a, b in zip(res[0], other):
             torch.testing.assert_close(a, b, rtol=0.0, atol=2.0 ** -16 * float(a.abs().max()))
     assert n or (float(res[0][0]) == 0.0 and float(res[0][1].abs().max()) == 0.0)
+
+
+def test_expert_counts_belong_to_their_call():
+    """Counted wherever the balance loss is formed, and none of an earlier call elsewhere."""
+    m = _model(use_moe=True, num_experts_per_tok=2).train()
+    ids = torch.randint(0, 50, (3, 7))
+    moe = m.model.layers[1].mlp
+    m(ids)
+    assert moe.expert_counts.dtype == torch.int64
+    assert moe.expert_counts.shape == (4,) and int(moe.expert_counts.sum()) == 42
+    m.eval()(ids)
+    assert moe.expert_counts is None
