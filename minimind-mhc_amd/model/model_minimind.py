@@ -294,7 +294,7 @@ class MOEFeedForward(nn.Module):
             mean = torch.where(inside, scores.float(), 0.0).sum(0) / tokens
             loss = (counts.float() / tokens * mean).sum()
             return loss * cfg.num_experts * cfg.router_aux_loss_coef, counts
-        ends = cu_seqlens.tolist()
+        ends = [0, *(min(max(e, 0), scores.shape[0]) for e in cu_seqlens.tolist()[1:])]  # as the kernels do
         parts = [(hot[i:j].float().sum((0, 1)) / (j - i) * scores[i:j].float().mean(0)).sum()
                  for i, j in zip(ends, ends[1:]) if j > i]
         counts = torch.stack([hot[i:j].sum((0, 1)) for i, j in zip(ends, ends[1:])])

@@ -209,3 +209,14 @@ def test_expert_counts_belong_to_their_call():
     assert moe.expert_counts.shape == (4,) and int(moe.expert_counts.sum()) == 42
     m.eval()(ids)
     assert moe.expert_counts is None
+
+
+@pytest.mark.parametrize("cu", [(0, 5, 20), (0, -3, 12)])
+def test_balance_of_each_sequence_clamps_its_bounds(cu):
+    m = _model(use_moe=True, num_experts_per_tok=2, router_aux_loss_per_sequence=True, router_aux_loss_coef=0.5).train()
+    ids = torch.randint(0, 50, (1, 12))
+    got = m(ids, packed=PackedBatch(_ints(*cu), 12))
+    lengths = [5, 7] if cu[1] == 5 else [0, 12]
+    assert m.model.layers[0].mlp.expert_counts.sum(1).tolist() == [2 * n for n in lengths]
+    want = m(ids, packed=PackedBatch.from_lengths(lengths, device="cpu"))
+    torch.testing.assert_close(got.aux_loss, want.aux_loss, rtol=1e-6, atol=0.0)
