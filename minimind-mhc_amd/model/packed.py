@@ -286,7 +286,7 @@ class PackedCall:
         """q [1, rows, heads, head_dim], k, v [1, rows, kv heads, head_dim] of the new tokens:
         [1, rows, heads * head_dim], over their sequences' keys so far."""
         q, k, v, cu = q[0], k[0], v[0], self.batch.cu_seqlens
-        cu_k, used = cu, None
+        cu_k, used, dtype = cu, None, q.dtype
         if self.cache is not None:
             if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
                 raise RuntimeError("mhc_amd: a cache is for inference; call under torch.no_grad()")
@@ -299,6 +299,8 @@ class PackedCall:
             out = packed_attention(q, k, v, cu, cu_seqlens_k=cu_k, key_lengths=used)
         else:
             out = _plain_attention(q, k, v, cu, cu_k, used, dropout)
+        if self.cache is not None and not torch.is_autocast_enabled(q.device.type):
+            out = out.to(dtype)  # the layer's, whatever the cache keeps; under autocast any type will do
         return out.reshape(1, out.shape[0], -1)
 
 

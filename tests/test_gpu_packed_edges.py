@@ -3,13 +3,14 @@ usual ones: values that are not finite, rows behind the last sequence, caches of
 type, gradients of very different sizes."""
 from __future__ import annotations
 
+import copy
 import math
 
 import pytest
 import torch
 
-from model.packed import PackedBatch
-from tests.test_gpu_packed_model import _model
+from model.packed import PackedBatch, PackedCache
+from tests.test_gpu_packed_model import _far, _model, _taken
 
 BF, F16 = torch.bfloat16, torch.float16
 
@@ -75,3 +76,27 @@ def test_rows_of_no_sequence_are_not_balanced(dev, lengths, each):
         torch.testing.assert_close(res[0][0], other[0], rtol=1e-5, atol=0.0)
         torch.testing.assert_close(res[0][2], other[2], rtol=1e-3, atol=1e-3 * float(res[0][2].abs().max()))
     assert n or (float(res[0][0]) == 0.0 and float(res[0][2].abs().max()) == 0.0)
+
+
+# ------------------------------------------------- a cache of another type than the model
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, BF, F16])
+@pytest.mark.parametrize("kept", [torch.float32, BF, F16, None])
+def test_cache_of_another_type(dev, monkeypatch, dtype, kept):
+    """A model takes a cache of any type (None: the default), on the kernels where that has 16
+    bits; its outputs stay in its own type."""
+    m = _model(dev).eval()
+    wide = copy.deepcopy(m).float()
+    m = m.to(dtype)
+    cache = PackedCache(m.config, 2, 64, device=dev, **({} if kept is None else {"dtype": kept}))
+    ids = torch.randint(0, 500, (1, 52), device=dev)
+    seen = _taken(monkeypatch)
+    with torch.inference_mode():
+        m(ids[:, :50], packed=PackedBatch.from_lengths([20, 30], device=dev), past_key_values=cache)
+        out = m(ids[:, 50:], packed=PackedBatch.from_lengths([1, 1], device=dev), past_key_values=cache).logits
+        ref = wide(ids[:, [*range(20), 50]]).logits[0, -1], wide(ids[:, [*range(20, 50), 51]]).logits[0, -1]
+    assert len(seen) == (0 if kept == torch.float32 else 4) and out.dtype == dtype
+    # some 20 roundings of 2^-8 one after another are 0.08, other keys than the right ones are of order 1
+    for got, want in zip(out[0], ref):
+        assert _far(got, want) < 0.1

@@ -220,3 +220,23 @@ def test_balance_of_each_sequence_clamps_its_bounds(cu):
     assert m.model.layers[0].mlp.expert_counts.sum(1).tolist() == [2 * n for n in lengths]
     want = m(ids, packed=PackedBatch.from_lengths(lengths, device="cpu"))
     torch.testing.assert_close(got.aux_loss, want.aux_loss, rtol=1e-6, atol=0.0)
+
+
+# ------------------------------------------------- a cache of another type than the model
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kept", [torch.float32, torch.bfloat16, torch.float16, None])
+def test_cache_of_another_type(dtype, kept):
+    """A model takes a cache of any type (None: the default): its outputs stay in its own."""
+    m = _model().to(dtype).eval()
+    cache = PackedCache(m.config, 2, 8, device="cpu", **({} if kept is None else {"dtype": kept}))
+    ids = torch.randint(0, 50, (1, 8))
+    with torch.no_grad():
+        out = m(ids[:, :6], packed=PackedBatch.from_lengths([2, 4], device="cpu"), past_key_values=cache)
+        out = m(ids[:, 6:], packed=PackedBatch.from_lengths([1, 1], device="cpu"), past_key_values=cache)
+        ref = m(ids[:, [0, 1, 6]]).logits[0, -1], m(ids[:, [2, 3, 4, 5, 7]]).logits[0, -1]
+    assert out.logits.dtype == dtype and cache.layers[0][0].dtype == (kept or torch.bfloat16)
+    assert float(cache.layers[0][0].float().abs().sum()) > 0
+    # the right tokens' keys: some 20 roundings of 2^-8 one after another are 0.08, other keys are of order 1
+    for got, want in zip(out.logits[0], ref):
+        assert float((got - want).float().norm() / want.float().norm()) < 0.1
