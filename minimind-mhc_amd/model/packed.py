@@ -6,6 +6,7 @@ No reference counterpart: the reference pads (model/model_minimind.py:161-256).
 """
 from __future__ import annotations
 
+import contextlib
 import functools
 import math
 from typing import Optional
@@ -17,6 +18,10 @@ from . import _hip as H
 from . import _ops
 
 HEAD_DIMS = _ops.ATTN_HEAD_DIMS
+
+
+def _autocast() -> bool:
+    return torch.is_autocast_enabled("cuda")
 
 
 def _bounds(name: str, t, n: Optional[int], dev: torch.device) -> torch.Tensor:
@@ -141,7 +146,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     the same bits on every run.  Not-finite keys or values of a token may turn earlier rows of
     its own sequence into NaN, as a dense product under a mask does.
     """
-    if torch.is_autocast_enabled("cuda"):
+    if _autocast():
         low = torch.get_autocast_dtype("cuda")
         q, k, v = q.to(low), k.to(low), v.to(low)
     dev = H.require_device(q, k, v)
@@ -294,9 +299,12 @@ class PackedCall:
             ck.index_copy_(0, self.rows, k.to(ck.dtype))
             cv.index_copy_(0, self.rows, v.to(cv.dtype))
             q, k, v, cu_k, used = q.to(ck.dtype), ck, cv, self.cache.slots, self.lengths
-        half = q.dtype in _ops.HALF or torch.is_autocast_enabled("cuda")
+        half = q.dtype in _ops.HALF or _autocast()
         if q.is_cuda and half and q.shape[2] in HEAD_DIMS and dropout == 0.0 and _ops.eager_call():
-            out = packed_attention(q, k, v, cu, cu_seqlens_k=cu_k, key_lengths=used)
+            # the cache's 16-bit type goes before an autocast's, which would copy every slot
+            slots = self.cache is not None and k.dtype in _ops.HALF
+            with torch.autocast("cuda", enabled=False) if slots and _autocast() else contextlib.nullcontext():
+                out = packed_attention(q, k, v, cu, cu_seqlens_k=cu_k, key_lengths=used)
         else:
             out = _plain_attention(q, k, v, cu, cu_k, used, dropout)
         if self.cache is not None and not torch.is_autocast_enabled(q.device.type):

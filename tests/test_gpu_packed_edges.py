@@ -9,6 +9,7 @@ import math
 import pytest
 import torch
 
+from model import packed
 from model.packed import PackedBatch, PackedCache
 from tests.test_gpu_packed_model import _far, _model, _taken
 
@@ -100,3 +101,21 @@ def test_cache_of_another_type(dev, monkeypatch, dtype, kept):
     # some 20 roundings of 2^-8 one after another are 0.08, other keys than the right ones are of order 1
     for got, want in zip(out[0], ref):
         assert _far(got, want) < 0.1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cast", [BF, F16])
+def test_cache_is_read_in_place_under_autocast(dev, monkeypatch, cast):
+    """Also where the autocast's type is not the cache's: no step copies the slots."""
+    m = _model(dev, torch.float32).eval()
+    cache = PackedCache(m.config, 2, 64, BF, dev)
+    read, run = [], packed._forward
+    monkeypatch.setattr(packed, "_forward", lambda q, k, v, *a: read.append((k.data_ptr(), v.data_ptr())) or run(q, k, v, *a))
+    ids = torch.randint(0, 500, (1, 52), device=dev)
+    with torch.inference_mode(), torch.autocast("cuda", cast):
+        m(ids[:, :50], packed=PackedBatch.from_lengths([20, 30], device=dev), past_key_values=cache)
+        out = m(ids[:, 50:], packed=PackedBatch.from_lengths([1, 1], device=dev), past_key_values=cache).logits
+    assert read == 2 * [(k.data_ptr(), v.data_ptr()) for k, v in cache.layers]
+    with torch.inference_mode():
+        for i, rows in enumerate(([*range(20), 50], [*range(20, 50), 51])):
+            assert _far(out[0, i], m(ids[:, rows]).logits[0, -1]) < 0.1  # as above
