@@ -124,21 +124,27 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogitArgs a) {
   }
 }
 
-// The factor of row t's gradient: its own, or that of its sequence in the preference loss
-// (lower bound over the sequences' ends).
-__device__ __forceinline__ float row_factor(const LogitArgs& a, int64_t row) {
-  if (!a.cu) return a.g_row[row];
+// The factor of a row's gradient: its own, or that of its sequence in the preference loss
+// (lower bound over the sequences' ends).  False for a row behind the last sequence: zeros then,
+// whatever its logits hold.
+__device__ __forceinline__ bool row_factor(const LogitArgs& a, int64_t row, float& f) {
+  if (!a.cu) {
+    f = a.g_row[row];
+    return true;
+  }
   int lo = 0, hi = a.B;  // the sequence with start <= row < end
   while (lo < hi) {
     const int mid = (lo + hi) / 2;
     if (min(max(a.cu[mid + 1], 0), (int)a.T) <= row) lo = mid + 1;
     else hi = mid;
   }
-  return lo < a.B ? a.g_seq[lo] * a.g_loss[0] : 0.f;
+  if (lo >= a.B) return false;
+  f = a.g_seq[lo] * a.g_loss[0];
+  return true;
 }
 
 // One workgroup a row again: p from the stored maximum and sum, and the gradient, zeros where
-// the label does not count.  16384 x 6400 bf16, 367 MB: 54 us, 6.8 TB/s with part of the logits still in
+// the row does not count.  16384 x 6400 bf16, 367 MB: 54 us, 6.8 TB/s with part of the logits still in
 // the memory-side cache; 2047 x 50257 fp32, 720 MB: 138 to 173 us.
 template <int DT>
 __global__ __launch_bounds__(256) void logprob_bwd_kernel(LogitArgs a) {
@@ -148,8 +154,8 @@ __global__ __launch_bounds__(256) void logprob_bwd_kernel(LogitArgs a) {
   const int64_t row = a.T - 1 - blockIdx.x;
   const int64_t label = a.labels[row];
   const int tid = threadIdx.x;
-  const bool counts = label != a.ignore;
-  const float f = counts ? row_factor(a, row) : 0.f;
+  float f = 0.f;
+  const bool counts = label != a.ignore && row_factor(a, row, f);
   const char* base = static_cast<const char*>(a.logits) + row * a.stride * EB;
   char* out = static_cast<char*>(a.g_logits) + row * a.V * EB;
   const float m = counts ? a.lse[2 * row] : 0.f, ls = counts ? a.lse[2 * row + 1] : 0.f;

@@ -10,6 +10,7 @@ import pytest
 import torch
 
 from model import packed
+from model.losses import preference_loss
 from model.packed import PackedBatch, PackedCache
 from tests.test_gpu_packed_model import _far, _model, _taken
 
@@ -119,3 +120,29 @@ def test_cache_is_read_in_place_under_autocast(dev, monkeypatch, cast):
     with torch.inference_mode():
         for i, rows in enumerate(([*range(20), 50], [*range(20, 50), 51])):
             assert _far(out[0, i], m(ids[:, rows]).logits[0, -1]) < 0.1  # as above
+
+
+# ------------------------------------------------- the preference loss
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, BF, F16])
+@pytest.mark.parametrize("V", [33, 500])
+def test_preference_rows_behind_the_last_sequence(dev, dtype, V):
+    """Count for nothing, though their labels count and their logits are no numbers: the same
+    bits as without them, and zeros as their gradients."""
+    torch.manual_seed(0)
+    ends, rows = [0, 7, 20, 21, 40], 46
+    x = torch.randn(rows, V, device=dev).to(dtype)
+    y = torch.randint(0, V, (rows,), device=dev)
+    cu = torch.tensor(ends, dtype=torch.int32, device=dev)
+    ref = torch.randn(4, device=dev)
+    short = x[:40].clone().requires_grad_()
+    want = preference_loss(short, y[:40], cu, ref)
+    g, = torch.autograd.grad(want[0], short)
+    x[40:], x[41], x[42, 3] = math.nan, -math.inf, math.inf
+    y[44] = V + 5
+    x.requires_grad_()
+    got = preference_loss(x, y, cu, ref)
+    d, = torch.autograd.grad(got[0], x)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(d[:40], g) and torch.equal(d[40:], torch.zeros_like(d[40:]))
