@@ -348,7 +348,9 @@ __global__ __launch_bounds__(256) void packed_few_kernel(PackedAttnArgs a) {
   const float scale = a.scale * kPackedLog2e;
   constexpr float kHead = packed_head<F16>;
   const int limit = live ? row + shift : -1;  // last key the lane's row sees
-  float m = kNoScore, l = 0.f;
+  float m = kNoScore;
+  f32x4_t l = {0.f, 0.f, 0.f, 0.f};  // sums of the rounded probabilities, as in the tiles of many queries
+  const U32x4 ones = packed_ones<F16>();
   f32x4_t o[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -397,7 +399,8 @@ __global__ __launch_bounds__(256) void packed_few_kernel(PackedAttnArgs a) {
       mx = fmaxf(mx - kHead, m);
       const float f = exp2_f(m - mx);
       m = mx;
-      l *= f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) l[i] *= f;
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -408,13 +411,11 @@ __global__ __launch_bounds__(256) void packed_few_kernel(PackedAttnArgs a) {
     for (int st = 0; st < 2; ++st) {
       float p[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        p[i] = exp2_f(fmaf(s[st][i], scale, -m));
-        l += p[i];
-      }
+      for (int i = 0; i < 4; ++i) p[i] = exp2_f(fmaf(s[st][i], scale, -m));
       pf.v[2 * st] = pack2<F16>(p[0], p[1]);
       pf.v[2 * st + 1] = pack2<F16>(p[2], p[3]);
     }
+    l = mfma16<F16>(ones, pf, l);
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
       U32x4 va;
@@ -429,8 +430,6 @@ __global__ __launch_bounds__(256) void packed_few_kernel(PackedAttnArgs a) {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     __builtin_amdgcn_wave_barrier();
   }
-  l += xor_lane16(l);
-  l += xor_lane32(l);
   // the waves' sums meet in LDS: [16 rows][HD] and then each row's maximum and sum
   __syncthreads();
   float* mine = reinterpret_cast<float*>(lds[wave]);
@@ -438,7 +437,7 @@ __global__ __launch_bounds__(256) void packed_few_kernel(PackedAttnArgs a) {
   for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4_t*>(mine + r * HD + 16 * d + 4 * g) = o[d];
   if (g == 0) {
     mine[16 * HD + r] = m;
-    mine[16 * HD + 16 + r] = l;
+    mine[16 * HD + 16 + r] = l[0];
   }
   __syncthreads();
   // thread (row of 16, 1/16 of the columns)

@@ -146,3 +146,24 @@ def test_preference_rows_behind_the_last_sequence(dev, dtype, V):
     d, = torch.autograd.grad(got[0], x)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert torch.equal(d[:40], g) and torch.equal(d[40:], torch.zeros_like(d[40:]))
+
+
+# ------------------------------------------------- attention
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("hd", [64, 96, 128])
+@pytest.mark.parametrize("new,keys", [(1, 32), (1, 2000), (3, 1000), (60, 60), (200, 333)])
+def test_weights_add_up_to_one(dev, dtype, hd, new, keys):
+    """Values of 1 everywhere come out as 1: the sums are those of the probabilities as the
+    product takes them, rounded.  Here all but a sequence's first are just under half a step above
+    a number of the type, so sums of the unrounded ones would be off by nearly that.  (fp32 sums of n terms
+    are off by n 2^-24 at most, under the half step below 1, 2^-9 and 2^-12, for these lengths.)"""
+    n, step = 24, 2.0 ** -7 if dtype == BF else 2.0 ** -10
+    q, k = torch.zeros(n * new, 8, hd, device=dev), torch.zeros(n, keys, 4, hd, device=dev)
+    q[..., 0], k[:, 1:, :, 0] = 1.0, -1.0
+    k = k.flatten(0, 1).to(dtype)
+    cu, ck = (torch.arange(n + 1, dtype=torch.int32, device=dev) * m for m in (new, keys))
+    out = packed.packed_attention(q.to(dtype), k, torch.ones_like(k), cu, cu_seqlens_k=ck,
+                                  scale=-math.log(0.5 * (1.0 + 0.49 * step)))
+    assert torch.equal(out, torch.ones_like(out))
