@@ -576,9 +576,9 @@ int mhc_packed_attn_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, c
 
 /* Gradients g_q [Tq, heads, head_dim], g_k and g_v [Tk, kv_heads, head_dim]
  * (contiguous; every row is written) for g_out, contiguous as out.  out, rest and lse
- * are the forward's.  No atomics: the same bits on every run.  Its workspace holds
- * D = g_out . out of each row and, where few workgroups have long chains, parts of
- * the sums; mhc_packed_attn_bwd_workspace_bytes gives its size (or -1). */
+ * are the forward's.  The same bits on every run (sums without atomics).  Its workspace
+ * holds D = g_out . out of each row, the longest rows of v and g_out, and, where few
+ * workgroups have long chains, parts of the sums; mhc_packed_attn_bwd_workspace_bytes gives its size (or -1). */
 int64_t mhc_packed_attn_bwd_workspace_bytes(int B, int64_t Tq, int64_t Tk, int heads, int kv_heads,
                                             int head_dim);
 int mhc_packed_attn_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,

@@ -778,8 +778,7 @@ int64_t mhc_packed_attn_bwd_workspace_bytes(int B, int64_t Tq, int64_t Tk, int h
                                       Tk, heads, kv_heads, head_dim, mhc::kBF16, 1.f);
   if (check_packed(a, Tq, Tk, mhc::kBF16, "mhc_packed_attn_bwd_workspace_bytes")) return -1;
   mhc::packed_bwd_plan(a);
-  int64_t sums;
-  return mhc::packed_bwd_workspace(a, &sums);
+  return mhc::packed_bwd_workspace(a, nullptr);
 }
 
 int mhc_packed_attn_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
@@ -825,12 +824,10 @@ int mhc_packed_attn_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, c
   if (!cu_q || !cu_k) return fail(hipErrorInvalidValue, "%s: the sequences' bounds are required", fn);
   if (Tq > 0 && !lse) return fail(hipErrorInvalidValue, "%s: lse is required", fn);
   mhc::packed_bwd_plan(a);
-  int64_t sums;
-  const int64_t need = mhc::packed_bwd_workspace(a, &sums);
+  const int64_t need = mhc::packed_bwd_workspace(a, static_cast<float*>(workspace));
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(hipErrorInvalidValue, "%s: workspace of %lld bytes needed (got %lld)", fn, (long long)need, (long long)workspace_bytes);
   a.out = const_cast<void*>(out); a.rest = const_cast<void*>(rest); a.lse = const_cast<float*>(lse); a.g_out = g_out;
-  a.delta = static_cast<float*>(workspace); a.work = a.delta + sums;
   a.g_q = g_q; a.g_k = g_k; a.g_v = g_v;
   return hip_status(mhc::launch_packed_attn_bwd(a, stream), fn);
 }

@@ -317,6 +317,8 @@ struct PackedAttnArgs {
   // backward
   const void* g_out;
   float* delta;  // [heads, Tq]
+  float* v_top;  // [kv_heads, tiles of 128 key rows]: the largest squared length of a row of v
+  float* g_top;  // [kv_heads, blocks of query rows]: of g_out, in a group of heads
   int ranges;    // packed_bwd_plan: of the query rows of a key tile; their sums go to `work`
   void* g_q;
   void* g_k;
@@ -326,8 +328,8 @@ void packed_attn_plan(PackedAttnArgs& a);
 int64_t packed_attn_workspace(const PackedAttnArgs& a);
 hipError_t launch_packed_attn(const PackedAttnArgs& a, hipStream_t s);
 void packed_bwd_plan(PackedAttnArgs& a);
-// Bytes, and the sums' place in it (floats behind delta, which is at its beginning).
-int64_t packed_bwd_workspace(const PackedAttnArgs& a, int64_t* sums);
+// Its bytes; lays out delta, v_top, g_top and work in it, where one is given.
+int64_t packed_bwd_workspace(PackedAttnArgs& a, float* workspace);
 hipError_t launch_packed_attn_bwd(const PackedAttnArgs& a, hipStream_t s);
 
 // Log-probabilities of labels under rows of logits [T, V] (rows `stride` elements apart).

@@ -191,7 +191,7 @@ __device__ __forceinline__ void packed_rank(const int* cu, int B, int T, int M, 
 // sequences of 16001 tokens, 8 heads of 64 (1032): 372 and 350.
 inline bool packed_halves(unsigned workgroups) { return workgroups <= (unsigned)device_cus() * 5 / 4; }
 // Tile numbers of T rows in B sequences.
-inline int64_t packed_tiles(int64_t T, int64_t B, int M) { return T / M + B + 1; }
+__host__ __device__ inline int64_t packed_tiles(int64_t T, int64_t B, int M) { return T / M + B + 1; }
 
 // An operand of ones: its product with the probabilities sums them on the matrix cores, over
 // all lanes at once, and sums what the outputs are formed of, the rounded ones.

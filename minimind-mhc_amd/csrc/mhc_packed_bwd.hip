@@ -3,12 +3,82 @@
 //   D_i = G_i . O_i,  dS_ij = P_ij (G_i . v_j - D_i),
 //   dQ_i = scale sum_j dS_ij k_j,  dK_j = scale sum_i dS_ij q_i,  dV_j = sum_i P_ij G_i.
 // One launch forms D and dQ by query tiles, a second dK and dV by key tiles, each summing
-// its own rows' terms in registers (fp32): no atomics, the same bits on every run.  P is
+// its own rows' terms in registers (fp32): no atomics on sums, the same bits on every run.  P is
 // formed twice for that: 7 products instead of 5.
+//
+// dS is an operand of products, so it is rounded to the tensors' type.  bf16 has fp32's range.
+// An fp16 dS is multiplied by a power of two first, which the result is divided by: P of many
+// keys times a gradient of 1e-3 lies below fp16's normal numbers (dQ was off by 4e-3 with 8192 keys,
+// by 4e-2 for gradients of 1e-4).  No dS exceeds half the longest row of v times the length of its row of g
+// (P_j sum_k P_k |dP_j - dP_k| <= P_j (1 - P_j) 2 |g| |v|), so the power that takes |g| |v| to 2^15 at most
+// cannot overflow, and leaves 28 binary digits of normal numbers below.  dQ takes |g| of its own row, dK the
+// longest row of g from the block of 1024 rows on where its keys are first seen.  This costs fp16 one
+// launch (16001 rows, 8 heads of 64: 4.8 us of 749 a step).
 #include "mhc_packed.hpp"
 
 namespace mhc {
 namespace {
+
+// Rows of a block of g_top: few enough blocks that one load a lane reads those of a long sequence.
+constexpr int kGradBlock = 1024;
+
+// The exponent e with sqrt(w) 2^e in [2^14, 2^15), w = |g|^2 |v|^2; 0 where that is no positive number.
+__device__ __forceinline__ int packed_exponent(float w) {
+  return w > 0.f && w < __builtin_inff() ? 15 - ((__builtin_amdgcn_frexp_expf(w) + 1) >> 1) : 0;
+}
+
+// v_top: the longest of a tile's rows in use; 16 lanes a row (12 of them load at head_dim 96).  Also
+// clears g_top, whose blocks the waves of the dQ kernel raise (a maximum: any order gives the same).
+// 16001 rows, 8 heads of 64: 4.7 us.
+template <int HD>
+__global__ __launch_bounds__(256) void packed_v_top_kernel(PackedAttnArgs a) {
+  __shared__ float top[4];
+  const int kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.kv_heads * packed_tiles(a.Tq, a.B, kGradBlock);
+       i += (int64_t)gridDim.x * 256)
+    a.g_top[i] = 0.f;
+  PackedTile t;
+  PackedKeys o;
+  packed_find(a.cu_k, a.B, a.Tk, 128, tile, a.cu_q, a.Tq, a.k_len, nullptr, t, o);
+  if (t.first >= t.end) return;
+  const int end = min(t.first + 128, t.start + t.used);
+  const int sub = threadIdx.x & 15, row0 = t.first + (int)(threadIdx.x >> 4);
+  U32x4 w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    w[i] = U32x4{};
+    const int row = row0 + 16 * i;
+    if (sub < HD / 8 && row < end)
+      w[i] = ld16(static_cast<const uint16_t*>(a.v) + row * a.vs_t + kvh * a.vs_h + 8 * sub);
+  }
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float x = elem_lo<true>(w[i].v[j]), y = elem_hi<true>(w[i].v[j]);
+      s = fmaf(x, x, fmaf(y, y, s));
+    }
+    s += dpp_f<kDppXor1>(s);
+    s += dpp_f<kDppXor2>(s);
+    s += dpp_f<kDppHalfMirror>(s);
+    s += dpp_f<kDppRowMirror>(s);
+    most = fmaxf(most, s);
+  }
+  most = wave_max(most);
+  if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = most;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    a.v_top[kvh * packed_tiles(a.Tk, a.B, 128) + tile] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+}
+// Of the first n keys of sequence seq, by one wave.
+__device__ __forceinline__ float packed_v_top(const PackedAttnArgs& a, int kvh, int seq, int start, int n) {
+  const float* p = a.v_top + kvh * packed_tiles(a.Tk, a.B, 128) + (start / 128 + seq);
+  float most = 0.f;
+  for (int i = __lane_id(); i < (n + 127) / 128; i += 64) most = fmaxf(most, p[i]);
+  return wave_max(most);
+}
 
 // dQ: as the forward, one 4-wave workgroup per 128 query rows of one kv head, 32 rows a
 // wave.  S^T = K Q^T and dP^T = V G^T put a lane's values all in one query row, and dS^T,
@@ -55,7 +125,7 @@ __global__ __launch_bounds__(256 * KS, 2) void packed_dq_kernel(PackedAttnArgs a
     vl.issue(vd, vg + (int64_t)kt * KT * vs_t, wave * UW, vs_t, KT, left);
   };
   U32x4 qb[2][NC], gb[2][NC];
-  float lse[2], delta[2];
+  float lse[2], delta[2], g2[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int row = pb + u * 16 + r;
@@ -65,7 +135,7 @@ __global__ __launch_bounds__(256 * KS, 2) void packed_dq_kernel(PackedAttnArgs a
     const uint16_t* go = static_cast<const uint16_t*>(a.g_out) + off;
     const uint16_t* oo = static_cast<const uint16_t*>(a.out) + off;
     const uint16_t* ro = static_cast<const uint16_t*>(a.rest) + off;
-    float d = 0.f;
+    float d = 0.f, n = 0.f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       qb[u][c] = ld16(q + 32 * c);
@@ -75,8 +145,14 @@ __global__ __launch_bounds__(256 * KS, 2) void packed_dq_kernel(PackedAttnArgs a
       for (int j = 0; j < 4; ++j) {
         d += elem_lo<F16>(gb[u][c].v[j]) * (elem_lo<F16>(o.v[j]) + elem_lo<F16>(rest.v[j]));
         d += elem_hi<F16>(gb[u][c].v[j]) * (elem_hi<F16>(o.v[j]) + elem_hi<F16>(rest.v[j]));
+        if constexpr (F16) {
+          const float x = elem_lo<F16>(gb[u][c].v[j]), y = elem_hi<F16>(gb[u][c].v[j]);
+          n = fmaf(x, x, fmaf(y, y, n));
+        }
       }
     }
+    n += xor_lane16(n);
+    g2[u] = n + xor_lane32(n);
     d += xor_lane16(d);
     d += xor_lane32(d);
     delta[u] = d;
@@ -86,6 +162,19 @@ __global__ __launch_bounds__(256 * KS, 2) void packed_dq_kernel(PackedAttnArgs a
 #pragma unroll
   for (int i = 0; i < S - 1; ++i)
     if (i < nt) issue(i, lds[i][0], lds[i][1]);
+  float out_scale[2] = {a.scale, a.scale};
+  int g_most = 0;
+  if constexpr (F16) {
+    const float v2 = packed_v_top(a, kvh, t.seq, kk.start, max(last + 1, 0));
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {  // P 2^e from here on
+      const int e = packed_exponent(g2[u] * v2);
+      lse[u] -= (float)e;
+      out_scale[u] = __builtin_amdgcn_ldexpf(a.scale, -e);
+    }
+    // rows behind the last are copies of it; no negative floats: their bits are in their order
+    g_most = __builtin_amdgcn_readfirstlane(__float_as_int(wave_max(fmaxf(g2[0], g2[1]))));
+  }
   const float scale = a.scale * kPackedLog2e;
   f32x4_t dq[2][ND];
 #pragma unroll
@@ -232,6 +321,10 @@ __global__ __launch_bounds__(256 * KS, 2) void packed_dq_kernel(PackedAttnArgs a
         for (int j = 0; j < 4; ++j) dq[u][d][j] += y[j];
       }
   }
+  if (F16 && pb < t.end && lane == 0)  // here: at the start the loop's first wait would be for it too
+    atomicMax(reinterpret_cast<int*>(a.g_top) + kvh * packed_tiles(a.Tq, a.B, kGradBlock) +
+                  (t.start / kGradBlock + t.seq + (pb - t.start) / kGradBlock),
+              g_most);
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int row = pb + u * 16 + r;
@@ -240,8 +333,8 @@ __global__ __launch_bounds__(256 * KS, 2) void packed_dq_kernel(PackedAttnArgs a
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
       uint2 w;
-      w.x = pack2<F16>(dq[u][d][0] * a.scale, dq[u][d][1] * a.scale);
-      w.y = pack2<F16>(dq[u][d][2] * a.scale, dq[u][d][3] * a.scale);
+      w.x = pack2<F16>(dq[u][d][0] * out_scale[u], dq[u][d][1] * out_scale[u]);
+      w.y = pack2<F16>(dq[u][d][2] * out_scale[u], dq[u][d][3] * out_scale[u]);
       *reinterpret_cast<uint2*>(out + 16 * d) = w;
     }
   }
@@ -251,9 +344,8 @@ __global__ __launch_bounds__(256 * KS, 2) void packed_dq_kernel(PackedAttnArgs a
 // the sums would leave one wave a SIMD), whose rows of K and V stay in registers; the query rows that see them, of every head of the group,
 // pass through LDS 32 at a time.  S = Q K^T and dP = G V^T put a lane's values all in one
 // key, and P and dS, rounded, are the operands of dV^T = G^T P and dK^T = Q^T dS.
-// An fp16 P is 2^14 times as large, which is taken out of dS as it is formed and of dV at the
-// end: a row of many keys has probabilities below fp16's smallest normal number.  dS has
-// no bound and stays as it is: its terms under 2^-14 round at 2^-25, as any fp16 gradient does.
+// An fp16 P is 2^14 times as large, which is taken out of dS as that gets its own power, and of
+// dV at the end: a row of many keys has probabilities below fp16's smallest normal number.
 // Three sequences of 16001 tokens together, 8 heads of 64: 346 us, 760 TFLOP/s of its four products
 // (matrix cores busy 38%, VALU 50%); 12 of 8192, 8 / 4 heads of 96: 67 us and 14 for the join.
 // KS = 2: four more waves take every second tile of rows, and the halves add up at the end.
@@ -346,6 +438,19 @@ __global__ __launch_bounds__(64 * packed_dkv_waves<HD> * KS, 2) void packed_dkv_
       vb[u][c] = ld16(vp + 32 * c);
     }
   }
+  float kd = 1.f, k_scale = a.scale;  // of dS, and of dK
+  if constexpr (F16) {
+    const float v2 = packed_v_top(a, kvh, t.seq, kk.start, kk.len);
+    float most = 0.f;
+    if (nt > 0) {
+      const float* p = a.g_top + kvh * packed_tiles(a.Tq, a.B, kGradBlock) + (qq.start / kGradBlock + t.seq);
+      for (int i = q_first / kGradBlock + lane; i <= (qq.len - 1) / kGradBlock; i += 64) most = fmaxf(most, p[i]);
+    }
+    most = wave_max(most);
+    const int e = __builtin_amdgcn_readfirstlane(packed_exponent(most * v2));
+    kd = __builtin_amdgcn_ldexpf(kDown, e);
+    k_scale = __builtin_amdgcn_ldexpf(a.scale, -e);
+  }
   const float scale = a.scale * kPackedLog2e;
   f32x4_t dk[KU][ND], dv[KU][ND];
 #pragma unroll
@@ -436,7 +541,7 @@ __global__ __launch_bounds__(64 * packed_dkv_waves<HD> * KS, 2) void packed_dkv_
           float ds[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            ds[i] = s[q][u][i] * (F16 ? fmaf(dp[q][u][i], kDown, -d4[q][i] * kDown) : dp[q][u][i] - d4[q][i]);
+            ds[i] = s[q][u][i] * (F16 ? fmaf(dp[q][u][i], kd, -d4[q][i] * kd) : dp[q][u][i] - d4[q][i]);
           df[u].v[2 * q] = pack2<F16>(ds[0], ds[1]);
           df[u].v[2 * q + 1] = pack2<F16>(ds[2], ds[3]);
         }
@@ -528,7 +633,7 @@ __global__ __launch_bounds__(64 * packed_dkv_waves<HD> * KS, 2) void packed_dkv_
       if (used) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          x[i] = dk[u][d][i] * a.scale;
+          x[i] = dk[u][d][i] * k_scale;
           y[i] = dv[u][d][i] * kDown;
         }
       }
@@ -567,6 +672,11 @@ hipError_t packed_bwd_hd(PackedAttnArgs a, hipStream_t s) {
   const int hp = (a.heads / a.kv_heads) % 2 == 0 ? 2 : 1;
   a.qtiles = (int)packed_tiles(a.Tq, a.B, 128 / hp);
   const dim3 grid((unsigned)((int64_t)a.qtiles * (a.heads / hp)));
+  if (F16 && a.Tq > 0 && a.Tk > 0) {
+    const dim3 tiles((unsigned)(packed_tiles(a.Tk, a.B, 128) * a.kv_heads));
+    packed_v_top_kernel<HD><<<tiles, 256, 0, s>>>(a);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  }
   if (a.Tq > 0) {
     const bool halves = packed_halves(grid.x);
     if (hp == 2) {
@@ -606,11 +716,19 @@ void packed_bwd_plan(PackedAttnArgs& a) {
   if (want > 8) want = 8;
   a.ranges = want < 1 ? 1 : (int)want;
 }
-// D, and the ranges' sums of dK and dV.
-int64_t packed_bwd_workspace(const PackedAttnArgs& a, int64_t* sums) {
-  const int64_t delta = ((int64_t)a.heads * a.Tq + 3) / 4 * 4;
-  *sums = delta;
-  return (delta + (a.ranges > 1 ? 2 * a.ranges * (int64_t)a.Tk * a.kv_heads * a.head_dim : 0)) * 4;
+// D, the longest rows of v and g by tiles, and the ranges' sums of dK and dV.
+int64_t packed_bwd_workspace(PackedAttnArgs& a, float* workspace) {
+  auto whole = [](int64_t n) { return (n + 3) / 4 * 4; };  // of 16 bytes
+  const int64_t v_top = whole((int64_t)a.heads * a.Tq);
+  const int64_t g_top = v_top + whole(packed_tiles(a.Tk, a.B, 128) * a.kv_heads);
+  const int64_t sums = g_top + whole(packed_tiles(a.Tq, a.B, kGradBlock) * a.kv_heads);
+  if (workspace) {
+    a.delta = workspace;
+    a.v_top = workspace + v_top;
+    a.g_top = workspace + g_top;
+    a.work = workspace + sums;
+  }
+  return (sums + (a.ranges > 1 ? 2 * a.ranges * (int64_t)a.Tk * a.kv_heads * a.head_dim : 0)) * 4;
 }
 
 hipError_t launch_packed_attn_bwd(const PackedAttnArgs& a, hipStream_t s) { MHC_PACKED_HD(packed_bwd_hd, a, s) }

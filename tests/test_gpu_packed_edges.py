@@ -12,6 +12,7 @@ import torch
 from model import packed
 from model.losses import preference_loss
 from model.packed import PackedBatch, PackedCache
+from tests.test_gpu_packed import _cu, exact
 from tests.test_gpu_packed_model import _far, _model, _taken
 
 BF, F16 = torch.bfloat16, torch.float16
@@ -167,3 +168,104 @@ def test_weights_add_up_to_one(dev, dtype, hd, new, keys):
     out = packed.packed_attention(q.to(dtype), k, torch.ones_like(k), cu, cu_seqlens_k=ck,
                                   scale=-math.log(0.5 * (1.0 + 0.49 * step)))
     assert torch.equal(out, torch.ones_like(out))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,slots,used,heads,kv,hd", [
+    ([64, 16], [8192, 3000], [8192, 2999], 2, 1, 64), ([300, 40], [4100, 90], [3500, 77], 2, 2, 96),
+    ([33], [6000], [5999], 4, 1, 128), ([1, 17, 64, 129, 300],) * 3 + (6, 2, 64), ([700, 90],) * 3 + (2, 1, 128),
+    ([1200, 5],) * 3 + (4, 2, 96)])
+@pytest.mark.parametrize("g_size,v_size", [(1.0, 1.0), (1e-2, 1.0), (1e-3, 1.0), (1e-4, 1.0), (1e-3, 2000.0),
+                                           (300.0, 1.0), (2.0, 1e-3)])
+def test_fp16_gradients_of_any_size(dev, new, slots, used, heads, kv, hd, g_size, v_size):
+    """The terms of dQ and dK keep fp16's 11 bits whatever the size of g and v, and however many
+    keys share a row's weight.  The bar is that of one rounding of each term and one of the result,
+    with no term that grows with the keys: half a step (2^-11) of the result, half of the smallest
+    number (2^-25), half a step of the terms' sizes; fp32 scores and sums are some 2^-18 of them."""
+    torch.manual_seed(0)
+    q, k, v, g = (torch.randn(rows, h, hd, device=dev) for rows, h in (
+        (sum(new), heads), (sum(slots), kv), (sum(slots), kv), (sum(new), heads)))
+    # gradients of very different sizes beside each other
+    g *= g_size * torch.exp2(torch.randint(-3, 4, (sum(new), heads, 1), device=dev).float())
+    q, k, v, g = (t.to(F16) for t in (q, k, v * v_size, g))
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    out = packed.packed_attention(*leaves, _cu(new, dev), cu_seqlens_k=_cu(slots, dev),
+                                  key_lengths=torch.tensor(used, dtype=torch.int32, device=dev))
+    grads = torch.autograd.grad(out, leaves, g)
+    want, size = exact(q, k, v, new, slots, used, 1.0 / math.sqrt(hd), g)
+    for name, got, ref, (sz, _) in zip("qkv", grads, want[1:], size[1:]):
+        got = got.double().cpu()
+        assert torch.isfinite(got).all()
+        bar = 2.0 ** -11 * ref.abs() + 2.0 ** -25 + (2.0 ** -11 + 2.0 ** -18) * sz
+        assert ((got - ref).abs() <= bar).all(), (name, float(((got - ref).abs() / bar).max()))
+        # over all of it the terms' roundings, each relative to a term, are as large as the result's
+        # in a sum of independent terms, so together 1.42 times the result's own
+        rms, own = float((got - ref).norm()), float((ref.half().double() - ref).norm())
+        assert rms <= 1.5 * own + 2.0 ** -18 * float(ref.norm()), (name, rms / own)
+
+
+@pytest.mark.gpu
+def test_fp16_gradients_captured(dev):
+    """A captured step replayed on gradients of other sizes: the eager bits, twice over."""
+    torch.manual_seed(0)
+    lengths = [1500, 0, 70, 1030]
+    q, k, v, g = (torch.randn(sum(lengths), h, 64, device=dev).to(F16) for h in (4, 2, 2, 4))
+    cu = _cu(lengths, dev)
+
+    def step(q, k, v, g):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        return torch.autograd.grad(packed.packed_attention(*leaves, cu), leaves, g)
+    state = [t.clone() for t in (q, k, v, g)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*state)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = step(*state)
+    for size in (1.0, 1e-4, 30.0, 1e-4):
+        state[3].copy_(g * size)
+        want = step(q, k, v, state[3])
+        assert all(torch.equal(a, b) for a, b in zip(want, step(q, k, v, state[3])))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(res, want)), size
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ends", [[-5, 500, 2 ** 31 - 1], [0, 150, 20], [0, -2 ** 31, 200], [9, 9, 9]])
+def test_fp16_bounds_that_make_no_sense(dev, ends):
+    """Such a backward pass ends, and the next one is right."""
+    torch.manual_seed(0)
+    q, k, v, g = (torch.randn(200, h, 64, device=dev).to(F16) for h in (4, 2, 2, 4))
+
+    def step(cu, **more):
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        return torch.autograd.grad(packed.packed_attention(*leaves, cu, **more), leaves, g)
+    good, cu = step(_cu([120, 80], dev)), torch.tensor(ends, dtype=torch.int32, device=dev)
+    for more in ({}, {"cu_seqlens_k": cu.flip(0).contiguous()},
+                 {"key_lengths": torch.tensor([-7, 2 ** 31 - 1], dtype=torch.int32, device=dev)}):
+        assert [t.shape for t in step(cu, **more)] == [q.shape, k.shape, v.shape]
+    assert all(torch.equal(a, b) for a, b in zip(step(_cu([120, 80], dev)), good))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["v", "g"])
+def test_fp16_gradients_beside_values_that_are_not_finite(dev, what):
+    """An infinite value or gradient in one sequence leaves the others' bits alone."""
+    torch.manual_seed(0)
+    lengths = [300, 200, 77]
+    q, k, v, g = (torch.randn(577, h, 64, device=dev).to(F16) for h in (4, 2, 2, 4))
+
+    def step():
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        return torch.autograd.grad(packed.packed_attention(*leaves, _cu(lengths, dev)), leaves, g)
+    good = step()
+    (v if what == "v" else g)[350, 0, 5] = math.inf
+    for a, b in zip(step(), good):
+        assert torch.equal(a[:300], b[:300]) and torch.equal(a[500:], b[500:])
+    (v if what == "v" else g)[350, 0, 5] = 0.0  # and none at all
+    q[300:500] = 0.0
+    g[300:500] = 0.0
+    assert not any(bool(t[300:500].any()) for t in step())
