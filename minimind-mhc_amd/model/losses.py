@@ -139,6 +139,13 @@ class _PreferenceLoss(torch.autograd.Function):
         return (out,) + (None,) * 7
 
 
+def _check_pairs(reference: torch.Tensor, label_smoothing: float) -> None:
+    if reference.dim() != 1 or reference.numel() < 2 or reference.numel() % 2:
+        raise ValueError(f"mhc_amd: reference must hold two values a pair, got {tuple(reference.shape)}")
+    if not 0.0 <= label_smoothing < 1.0:
+        raise ValueError(f"mhc_amd: label_smoothing must be in [0, 1), got {label_smoothing}")
+
+
 def preference_loss(logits: torch.Tensor, labels: torch.Tensor, cu_seqlens: torch.Tensor,
                     reference: torch.Tensor, beta: float = 0.1, label_smoothing: float = 0.0,
                     average: bool = False, ignore_index: int = IGNORE_INDEX):
@@ -161,10 +168,7 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, cu_seqlens: torc
     if logits.dim() != 2:
         raise ValueError(f"mhc_amd: logits must be [rows, V], got {tuple(logits.shape)}")
     x, y = _rows(logits, "logits"), _labels(labels, logits)
-    if reference.dim() != 1 or reference.numel() < 2 or reference.numel() % 2:
-        raise ValueError(f"mhc_amd: reference must hold two values a pair, got {tuple(reference.shape)}")
-    if not 0.0 <= label_smoothing < 1.0:
-        raise ValueError(f"mhc_amd: label_smoothing must be in [0, 1), got {label_smoothing}")
+    _check_pairs(reference, label_smoothing)
     cu = _bounds("cu_seqlens", cu_seqlens, reference.numel() + 1, dev)
     ref = reference.detach().to(torch.float32).contiguous()
     args = (x, y, cu, ref, float(beta), float(label_smoothing), bool(average), int(ignore_index))

@@ -480,18 +480,32 @@ class MiniMindForCausalLM(nn.Module):
         labels, fp32 [n]: what preference_loss takes from its reference model.  Sums in 64 bits."""
         y = packed.next_labels(labels)[0]
         lp = self._token_logprobs(self(input_ids, packed=packed).logits[0], y)
+        return self._sequence_sums(lp, y, packed, average).float()
+
+    @staticmethod
+    def _sequence_sums(lp, y, packed, average):
         total = packed.sums(lp)
-        return (total / packed.sums(y != -100).clamp_min(1) if average else total).float()
+        return total / packed.sums(y != -100).clamp_min(1) if average else total
 
     def preference_loss(self, input_ids, labels, packed, reference, beta=0.1, label_smoothing=0.0,
                         average=False):
         """The preference loss of packed pairs of answers (losses.preference_loss: the first
         half of the sequences chosen, the second rejected; labels -100 where a token does not
         count) plus the routers' balance loss, with the rewards."""
-        out = self(input_ids, packed=packed)
-        loss, chosen, rejected = losses.preference_loss(
-            out.logits[0], packed.next_labels(labels)[0], packed.cu_seqlens, reference, beta,
-            label_smoothing, average)
+        out, y = self(input_ids, packed=packed), packed.next_labels(labels)[0]
+        if out.logits.is_cuda and _ops.eager_call():
+            loss, chosen, rejected = losses.preference_loss(
+                out.logits[0], y, packed.cu_seqlens, reference, beta, label_smoothing, average)
+        else:
+            losses._check_pairs(reference, label_smoothing)
+            if reference.numel() != len(packed):
+                raise ValueError(f"mhc_amd: {reference.numel()} reference values for {len(packed)} sequences")
+            S = self._sequence_sums(self._token_logprobs(out.logits[0], y), y, packed, average)
+            reward = beta * (S - reference.detach().double())
+            chosen, rejected = reward.chunk(2)
+            z, e = chosen - rejected, label_smoothing
+            loss = -((1 - e) * F.logsigmoid(z) + e * F.logsigmoid(-z)).mean().float()
+            chosen, rejected = chosen.detach().float(), rejected.detach().float()
         return SimpleNamespace(loss=loss + out.aux_loss, aux_loss=out.aux_loss, chosen_rewards=chosen,
                                rejected_rewards=rejected, logits=out.logits)
 

@@ -240,3 +240,48 @@ def test_cache_of_another_type(dtype, kept):
     # the right tokens' keys: some 20 roundings of 2^-8 one after another are 0.08, other keys are of order 1
     for got, want in zip(out.logits[0], ref):
         assert float((got - want).float().norm() / want.float().norm()) < 0.1
+
+
+# ------------------------------------------------- the preference loss on torch ops
+
+@pytest.mark.parametrize("average", [False, True])
+@pytest.mark.parametrize("smoothing", [0.0, 0.2])
+def test_preference_loss_without_a_gpu(average, smoothing):
+    """The model's step on the torch path, against each sequence alone."""
+    m = _model()
+    lengths = [5, 3, 1, 7]
+    b = PackedBatch.from_lengths(lengths, rows=19, device="cpu")
+    ids = torch.randint(0, 50, (1, 19))
+    labels = ids.clone()
+    labels[0, :2] = -100
+    ref = torch.tensor([-12.0, -8.0, 0.5, -20.0])
+    out = m.preference_loss(ids, labels, b, ref, beta=0.2, label_smoothing=smoothing, average=average)
+    S, at = [], 0
+    for n in lengths:
+        lp = torch.log_softmax(m(ids[:, at:at + n]).logits[0], -1)
+        y = labels[0, at + 1:at + n]
+        rows = [lp[i, t] for i, t in enumerate(y) if t != -100]
+        S.append(sum(rows, torch.zeros(())) / (max(len(rows), 1) if average else 1))
+        at += n
+    r = 0.2 * (torch.stack(S) - ref)
+    z, ls = r[:2] - r[2:], torch.nn.functional.logsigmoid
+    want = -((1 - smoothing) * ls(z) + smoothing * ls(-z)).mean()
+    torch.testing.assert_close(out.loss, want, rtol=1e-5, atol=1e-6)
+    torch.testing.assert_close(torch.cat([out.chosen_rewards, out.rejected_rewards]), r.detach(), rtol=1e-4, atol=1e-5)
+    assert out.loss.dtype == torch.float32 and not out.chosen_rewards.requires_grad
+    got = torch.autograd.grad(out.loss, list(m.parameters()))
+    # sums of 64 terms in other orders, 2^-18 each, in up to 16 products one after another
+    for a, w in zip(got, torch.autograd.grad(want, list(m.parameters()))):
+        torch.testing.assert_close(a, w, rtol=0.0, atol=2.0 ** -14 * float(w.abs().max()))
+    for bad, kw in ((ref[:3], {}), (ref[:2], {}), (ref[None], {}), (ref, {"label_smoothing": 1.0})):
+        with pytest.raises(ValueError):
+            m.preference_loss(ids, labels, b, bad, **kw)
+
+
+def test_preference_loss_traces():
+    m = _model()
+    b = PackedBatch.from_lengths([5, 3], device="cpu")
+    ids = torch.randint(0, 50, (1, 8))
+    ref = torch.tensor([-12.0, -8.0])
+    got = torch.compile(lambda i: m.preference_loss(i, i, b, ref).loss, backend="eager")(ids)
+    torch.testing.assert_close(got, m.preference_loss(ids, ids, b, ref).loss, rtol=1e-5, atol=1e-6)
