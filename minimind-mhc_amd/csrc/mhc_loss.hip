@@ -231,7 +231,7 @@ __global__ __launch_bounds__(256) void preference_kernel(PreferenceArgs a) {
     reward[side] = (double)a.beta * (sum * each[side] - (double)a.reference[side * a.P + pair]);
   }
   const double z = reward[0] - reward[1], e = a.smoothing;
-  a.pair_loss[pair] = (1.0 - e) * softplus(-z) + e * softplus(z);
+  a.pair_loss[pair] = (1.0 - e) * softplus(-z) + (e > 0.0 ? e * softplus(z) : 0.0);  // z may be infinite
   const double dz = (e * sigmoid_d(z) - (1.0 - e) * sigmoid_d(-z)) * a.beta / a.P;
   a.chosen[pair] = (float)reward[0];
   a.rejected[pair] = (float)reward[1];

@@ -504,7 +504,8 @@ class MiniMindForCausalLM(nn.Module):
             reward = beta * (S - reference.detach().double())
             chosen, rejected = reward.chunk(2)
             z, e = chosen - rejected, label_smoothing
-            loss = -((1 - e) * F.logsigmoid(z) + e * F.logsigmoid(-z)).mean().float()
+            each = (1 - e) * F.logsigmoid(z) + (e * F.logsigmoid(-z) if e else 0.0)  # z may be infinite
+            loss = -each.mean().float()
             chosen, rejected = chosen.detach().float(), rejected.detach().float()
         return SimpleNamespace(loss=loss + out.aux_loss, aux_loss=out.aux_loss, chosen_rewards=chosen,
                                rejected_rewards=rejected, logits=out.logits)

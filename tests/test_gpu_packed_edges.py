@@ -269,3 +269,30 @@ def test_fp16_gradients_beside_values_that_are_not_finite(dev, what):
     q[300:500] = 0.0
     g[300:500] = 0.0
     assert not any(bool(t[300:500].any()) for t in step())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("smoothing", [0.0, 0.1])
+def test_preference_pairs_of_impossible_answers(dev, smoothing):
+    """A rejected answer that the model rules out (log-probability -inf) costs nothing without
+    label smoothing, and does not reach the other pairs; with it, and where the chosen answer
+    is ruled out, the loss is infinite."""
+    torch.manual_seed(0)
+    x, y = torch.randn(40, 50, device=dev), torch.randint(0, 50, (40,), device=dev)
+    cu = torch.tensor([0, 10, 20, 30, 40], dtype=torch.int32, device=dev)
+    ref = torch.randn(4, device=dev)
+    x[33].scatter_(0, y[33:34], -math.inf)  # of the second pair's rejected answer
+    leaf = x.clone().requires_grad_()
+    loss, chosen, rejected = preference_loss(leaf, y, cu, ref, label_smoothing=smoothing)
+    assert float(rejected[1]) == -math.inf and torch.isfinite(chosen).all()
+    first = preference_loss(torch.cat([x[:10], x[20:30]]), torch.cat([y[:10], y[20:30]]), cu[:3],
+                            ref[[0, 2]], label_smoothing=smoothing)[0]
+    if smoothing:
+        assert float(loss) == math.inf
+    else:
+        torch.testing.assert_close(loss.detach(), first / 2, rtol=2.0 ** -22, atol=0.0)
+        g, = torch.autograd.grad(loss, leaf)
+        assert torch.isfinite(g).all() and not bool(g[10:20].any()) and not bool(g[30:].any())
+    swapped = preference_loss(x[[*range(20, 40), *range(20)]], y[[*range(20, 40), *range(20)]], cu,
+                              ref[[2, 3, 0, 1]], label_smoothing=smoothing)[0]
+    assert float(swapped) == math.inf

@@ -285,3 +285,16 @@ def test_preference_loss_traces():
     ref = torch.tensor([-12.0, -8.0])
     got = torch.compile(lambda i: m.preference_loss(i, i, b, ref).loss, backend="eager")(ids)
     torch.testing.assert_close(got, m.preference_loss(ids, ids, b, ref).loss, rtol=1e-5, atol=1e-6)
+
+
+def test_preference_pairs_of_impossible_answers(monkeypatch):
+    """A rejected answer of log-probability -inf costs nothing without label smoothing."""
+    lp = -torch.rand(8)
+    lp[6] = -math.inf
+    m = _rows_of(_model(), monkeypatch, lp)
+    b, ids = PackedBatch.from_lengths([2] * 4, device="cpu"), torch.zeros(1, 8, dtype=torch.int64)
+    out = m.preference_loss(ids, ids, b, torch.zeros(4))
+    z = 0.1 * (lp[0] - lp[4])
+    torch.testing.assert_close(out.loss, -torch.nn.functional.logsigmoid(z) / 2)
+    assert float(out.rejected_rewards[1]) == -math.inf
+    assert float(m.preference_loss(ids, ids, b, torch.zeros(4), label_smoothing=0.1).loss) == math.inf
