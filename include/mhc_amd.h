@@ -612,11 +612,11 @@ int mhc_logprobs_bwd(const void* logits, int64_t stride, int dtype, const int64_
  * the chosen reward less the rejected one, loss (one element) = the mean of
  * -((1 - smoothing) log sigmoid(z) + smoothing log sigmoid(-z)).  g_seq [2 P]:
  * the loss's derivative by each logprob of a sequence.  scratch: 8 P bytes, 8-byte
- * aligned. */
+ * aligned.  flags: 1, average; 2, reference holds fp64 values instead of fp32 ones. */
 int mhc_preference_fwd(const float* logprobs, const int64_t* labels, int64_t ignore, const int* cu,
-                       const float* reference, float* loss, float* chosen, float* rejected,
+                       const void* reference, float* loss, float* chosen, float* rejected,
                        float* g_seq, void* scratch, int64_t T, int P, double beta,
-                       double smoothing, int average, hipStream_t stream);
+                       double smoothing, int flags, hipStream_t stream);
 
 /* g_logits [T, V] for g_loss (one element); rows of no sequence get zeros. */
 int mhc_preference_bwd(const void* logits, int64_t stride, int dtype, const int64_t* labels,

@@ -869,20 +869,20 @@ int mhc_logprobs_bwd(const void* logits, int64_t stride, int dtype, const int64_
 }
 
 int mhc_preference_fwd(const float* logprobs, const int64_t* labels, int64_t ignore, const int* cu,
-                       const float* reference, float* loss, float* chosen, float* rejected,
+                       const void* reference, float* loss, float* chosen, float* rejected,
                        float* g_seq, void* scratch, int64_t T, int P, double beta,
-                       double smoothing, int average, hipStream_t stream) {
+                       double smoothing, int flags, hipStream_t stream) {
   const char* fn = "mhc_preference_fwd";
   if (T < 0 || T > 1 << 30 || P < 1 || P > 1 << 29)
     return fail(hipErrorInvalidValue, "%s: bad shape (T=%lld pairs=%d)", fn, (long long)T, P);
   if ((T > 0 && (!logprobs || !labels)) || !cu || !reference || !loss || !chosen || !rejected || !g_seq || !scratch ||
-      reinterpret_cast<uintptr_t>(scratch) % 8)
+      reinterpret_cast<uintptr_t>(scratch) % 8 || reinterpret_cast<uintptr_t>(reference) % (flags & 2 ? 8 : 4))
     return fail(hipErrorInvalidValue, "%s: null or unaligned pointer", fn);
   mhc::PreferenceArgs a{};
   a.logprobs = logprobs; a.labels = labels; a.ignore = ignore; a.cu = cu; a.reference = reference;
   a.loss = loss; a.chosen = chosen; a.rejected = rejected; a.g_seq = g_seq;
   a.pair_loss = static_cast<double*>(scratch);
-  a.T = (int)T; a.P = P; a.beta = beta; a.smoothing = smoothing; a.average = average != 0;
+  a.T = (int)T; a.P = P; a.beta = beta; a.smoothing = smoothing; a.average = flags & 1; a.reference64 = flags & 2;
   return hip_status(mhc::launch_preference(a, stream), fn);
 }
 

@@ -355,7 +355,7 @@ struct PreferenceArgs {
   const float* logprobs;   // [T]
   const int64_t* labels;   // [T]
   const int* cu;           // [2 P + 1]
-  const float* reference;  // [2 P]
+  const void* reference;   // [2 P], fp32 or (reference64) fp64
   double* pair_loss;       // [P] scratch
   float* loss;             // one element
   float* chosen;           // [P] rewards
@@ -363,7 +363,7 @@ struct PreferenceArgs {
   float* g_seq;            // [2 P] d loss / d lp of a sequence's rows
   int64_t ignore;
   int T, P;
-  bool average;
+  bool average, reference64;
   double beta, smoothing;
 };
 hipError_t launch_preference(const PreferenceArgs& a, hipStream_t s);

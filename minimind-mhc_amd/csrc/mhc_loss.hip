@@ -228,7 +228,9 @@ __global__ __launch_bounds__(256) void preference_kernel(PreferenceArgs a) {
     const double sum = (part[side][0] + part[side][1]) + (part[side][2] + part[side][3]);
     const int count = cnt[side][0] + cnt[side][1] + cnt[side][2] + cnt[side][3];
     each[side] = a.average ? 1.0 / max(count, 1) : 1.0;
-    reward[side] = (double)a.beta * (sum * each[side] - (double)a.reference[side * a.P + pair]);
+    const int at = side * a.P + pair;
+    const double ref = a.reference64 ? static_cast<const double*>(a.reference)[at] : static_cast<const float*>(a.reference)[at];
+    reward[side] = a.beta * (sum * each[side] - ref);
   }
   const double z = reward[0] - reward[1], e = a.smoothing;
   a.pair_loss[pair] = (1.0 - e) * softplus(-z) + (e > 0.0 ? e * softplus(z) : 0.0);  // z may be infinite

@@ -125,7 +125,7 @@ _SIGNATURES = {
     "mhc_logprobs_bwd": (_I, [_P, _I64, _I, _P, _I64, _P, _P, _P, _I64, _I, _P]),
     "mhc_preference_fwd": (_I, [_P, _P, _I64, _P, _P,             # logprobs, labels, ignore, cu, reference
                                 _P, _P, _P, _P, _P,               # loss, chosen, rejected, g_seq, scratch
-                                _I64, _I, _D, _D, _I, _P]),
+                                _I64, _I, _D, _D, _I, _P]),       # T, P, beta, smoothing, flags
     "mhc_preference_bwd": (_I, [_P, _I64, _I, _P, _I64, _P, _P, _P, _P, _P, _I64, _I, _I, _P]),
     "mhc_balance_workspace_bytes": (_I64, [_I64, _I, _I]),
     "mhc_balance_fwd": (_I, [_P, _I64, _I, _P, _P,                # scores, stride, dtype, index, cu

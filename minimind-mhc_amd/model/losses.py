@@ -112,7 +112,8 @@ class _PreferenceLoss(torch.autograd.Function):
             _logprobs(x, labels, ignore, rows.data_ptr(), lse)
             H.check(H.load().mhc_preference_fwd(
                 rows.data_ptr(), labels.data_ptr(), ignore, cu.data_ptr(), reference.data_ptr(),
-                loss.data_ptr(), r, r + 4 * P, g, g + 8 * P, T, P, beta, smoothing, int(average),
+                loss.data_ptr(), r, r + 4 * P, g, g + 8 * P, T, P, beta, smoothing,
+                int(average) | (2 if reference.dtype == torch.float64 else 0),
                 H.stream(dev)), "mhc_preference_fwd")
         chosen, rejected = rewards.unbind(0)
         if ctx is not None:
@@ -156,7 +157,7 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, cu_seqlens: torc
     answers, the last n the rejected ones, in the same order; sequence i has the rows
     cu_seqlens[i] to cu_seqlens[i + 1], beginning with row 0, and rows behind the last count
     for nothing.  reference [2 n]: the reference model's sums (average: means) of the
-    sequences' token_logprobs.
+    sequences' token_logprobs, in 64 bits or taken to 32.
 
     With S a sequence's sum (mean over its counted rows) of token_logprobs, its reward is
     beta (S - reference); with z the chosen reward less the rejected one, the loss is the
@@ -170,7 +171,8 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, cu_seqlens: torc
     x, y = _rows(logits, "logits"), _labels(labels, logits)
     _check_pairs(reference, label_smoothing)
     cu = _bounds("cu_seqlens", cu_seqlens, reference.numel() + 1, dev)
-    ref = reference.detach().to(torch.float32).contiguous()
+    ref = reference.detach()
+    ref = (ref if ref.dtype == torch.float64 else ref.to(torch.float32)).contiguous()
     args = (x, y, cu, ref, float(beta), float(label_smoothing), bool(average), int(ignore_index))
     if _ops.wants_graph(logits):
         return _PreferenceLoss.apply(*args)

@@ -475,12 +475,14 @@ class MiniMindForCausalLM(nn.Module):
         y = packed.next_labels(labels)
         return -self._token_logprobs(logits[0], y[0]).sum() / (y != -100).sum()
 
-    def sequence_logprobs(self, input_ids, labels, packed, average=False):
+    def sequence_logprobs(self, input_ids, labels, packed, average=False, dtype=torch.float32):
         """The sum (average: mean) of the log-probabilities of each packed sequence's counted
-        labels, fp32 [n]: what preference_loss takes from its reference model.  Sums in 64 bits."""
+        labels, [n] in dtype: what preference_loss takes from its reference model.  Sums in 64 bits:
+        with dtype=torch.float64 they reach preference_loss as they are (a sum of some -5000 in 32
+        bits is up to 2.4e-4 off)."""
         y = packed.next_labels(labels)[0]
         lp = self._token_logprobs(self(input_ids, packed=packed).logits[0], y)
-        return self._sequence_sums(lp, y, packed, average).float()
+        return self._sequence_sums(lp, y, packed, average).to(dtype)
 
     @staticmethod
     def _sequence_sums(lp, y, packed, average):

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from model import packed
-from model.losses import preference_loss
+from model.losses import preference_loss, token_logprobs
 from model.packed import PackedBatch, PackedCache
 from tests.test_gpu_packed import _cu, exact
 from tests.test_gpu_packed_model import _far, _model, _taken
@@ -296,3 +296,34 @@ def test_preference_pairs_of_impossible_answers(dev, smoothing):
     swapped = preference_loss(x[[*range(20, 40), *range(20)]], y[[*range(20, 40), *range(20)]], cu,
                               ref[[2, 3, 0, 1]], label_smoothing=smoothing)[0]
     assert float(swapped) == math.inf
+
+
+@pytest.mark.gpu
+def test_preference_takes_64_bit_references(dev):
+    """A reference of 64 bits is not rounded: where it is the policy's own sums, the rewards are 0 up
+    to the order of 64-bit sums (2000 terms of 10 units).  In 32 bits half a step of a sum of -10000 is 5e-4."""
+    torch.manual_seed(0)
+    rows, V = 8000, 30
+    x, y = 5.0 * torch.randn(rows, V, device=dev), torch.randint(0, V, (rows,), device=dev)
+    b = PackedBatch.from_lengths([2000, 1999, 2001, 2000], device=dev)
+    own = b.sums(token_logprobs(x, y))
+    loss, chosen, rejected = preference_loss(x, y, b.cu_seqlens, own)
+    bar = 0.1 * 2000 * 2.0 ** -53 * float(own.abs().max())
+    assert chosen.dtype == torch.float32 and float(torch.cat([chosen, rejected]).abs().max()) <= bar
+    torch.testing.assert_close(float(loss), math.log(2.0), rtol=2.0 ** -23, atol=0.0)
+    low = preference_loss(x, y, b.cu_seqlens, own.float())
+    high = preference_loss(x, y, b.cu_seqlens, own.float().double())
+    assert all(torch.equal(a, c) for a, c in zip(low, high)) and float(low[1].abs().max()) > bar
+
+
+@pytest.mark.gpu
+def test_model_preference_in_64_bits(dev):
+    """sequence_logprobs hands its 64-bit sums on where it is asked to."""
+    m = _model(dev, torch.float32).eval()
+    b = PackedBatch.from_lengths([200, 150, 60, 90], device=dev)
+    ids = torch.randint(0, 500, (1, b.rows), device=dev)
+    with torch.no_grad():
+        own = m.sequence_logprobs(ids, ids, b, dtype=torch.float64)
+        assert own.dtype == torch.float64 and torch.equal(own.float(), m.sequence_logprobs(ids, ids, b))
+        out = m.preference_loss(ids, ids, b, own)
+    assert float(torch.cat([out.chosen_rewards, out.rejected_rewards]).abs().max()) <= 1e-10
