@@ -678,6 +678,30 @@ def wants_graph(*ts: torch.Tensor) -> bool:
     return not CAN_TELL or forward_ad._current_level >= 0 or any(t.requires_grad for t in ts)
 
 
+class _Once(torch.autograd.Function):
+    """The results of a backward pass as functions of its first input, so that differentiating
+    them again raises."""
+
+    @staticmethod
+    def forward(ctx, _, *ts):
+        return tuple(t.view_as(t) for t in ts)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("mhc_amd: this operator is differentiable once")
+
+
+def once(outs: tuple, *inputs: torch.Tensor) -> tuple:
+    """A backward pass's results, formed of these tensors by the library.  Under create_graph
+    they would pass for constants, also where an input wants a gradient, so a second derivative
+    through them raises instead."""
+    if torch.is_grad_enabled():
+        for t in inputs:
+            if t.requires_grad:
+                return _Once.apply(t, *(o.detach() for o in outs))
+    return outs
+
+
 def _function_modes() -> bool:
     """Whether one of the torch-function modes on the stack could see or replace the torch
     ops.  The one that torch.set_default_device and `with torch.device(...)` leave there

@@ -68,17 +68,16 @@ class _TokenLogprobs(torch.autograd.Function):
         return lp
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
+    def backward(ctx, grad):
         x, labels, lse = ctx.saved_tensors
         T, V = x.shape
-        g = g.to(torch.float32).contiguous()
+        g = grad.detach().to(torch.float32).contiguous()
         out = torch.empty((T, V), dtype=x.dtype, device=x.device)
         with _ops.launch_device(x):
             H.check(H.load().mhc_logprobs_bwd(
                 x.data_ptr(), _stride(x), H.dtype_tag(x), labels.data_ptr(), ctx.ignore, lse.data_ptr(),
                 g.data_ptr(), out.data_ptr(), T, V, H.stream(x.device)), "mhc_logprobs_bwd")
-        return out, None, None
+        return (*_ops.once((out,), x, grad), None, None)
 
 
 def token_logprobs(logits: torch.Tensor, labels: torch.Tensor,
@@ -124,20 +123,19 @@ class _PreferenceLoss(torch.autograd.Function):
         return loss, chosen, rejected
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, g, *_):
-        if g is None:
+    def backward(ctx, grad, *_):
+        if grad is None:
             return (None,) * 8
         x, labels, cu, rows, seqs = ctx.saved_tensors
         T, V = x.shape
-        g = _scalar(g)
+        g = _scalar(grad.detach())
         out = torch.empty((T, V), dtype=x.dtype, device=x.device)
         with _ops.launch_device(x):
             H.check(H.load().mhc_preference_bwd(
                 x.data_ptr(), _stride(x), H.dtype_tag(x), labels.data_ptr(), ctx.ignore,
                 rows.data_ptr() + 4 * T, cu.data_ptr(), seqs.data_ptr(), g.data_ptr(), out.data_ptr(), T, V,
                 seqs.numel() // 4, H.stream(x.device)), "mhc_preference_bwd")
-        return (out,) + (None,) * 7
+        return (*_ops.once((out,), x, grad),) + (None,) * 7
 
 
 def _check_pairs(reference: torch.Tensor, label_smoothing: float) -> None:

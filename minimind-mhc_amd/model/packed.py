@@ -12,7 +12,6 @@ import math
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _hip as H
 from . import _ops
@@ -96,8 +95,13 @@ class _PackedAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
+        with torch.no_grad():
+            grads = _PackedAttention._backward(ctx, g)
+        return (*_ops.once(grads, *ctx.saved_tensors[:3], g), None, None, None, None)
+
+    @staticmethod
+    def _backward(ctx, g):
         q, k, v, cu_q, cu_k, used, out, rest, lse = ctx.saved_tensors
         (q, *qs), (k, *ks), (v, *vs) = _strided(q), _strided(k), _strided(v)
         g = g.to(out.dtype).contiguous()
@@ -117,7 +121,7 @@ class _PackedAttention(torch.autograd.Function):
                 cu_k.data_ptr(), H.ptr(used), out.data_ptr(), rest.data_ptr(), lse.data_ptr(), g.data_ptr(),
                 g_q.data_ptr(), g_k.data_ptr(), g_v.data_ptr(), ws.data_ptr(), nbytes, B, Tq, Tk,
                 heads, kv, hd, H.dtype_tag(q), ctx.scale, H.stream(dev)), "mhc_packed_attn_bwd")
-        return g_q, g_k, g_v, None, None, None, None
+        return g_q, g_k, g_v
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,

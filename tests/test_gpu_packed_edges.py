@@ -327,3 +327,26 @@ def test_model_preference_in_64_bits(dev):
         assert own.dtype == torch.float64 and torch.equal(own.float(), m.sequence_logprobs(ids, ids, b))
         out = m.preference_loss(ids, ids, b, own)
     assert float(torch.cat([out.chosen_rewards, out.rejected_rewards]).abs().max()) <= 1e-10
+
+
+# ------------------------------------------------- second derivatives
+
+@pytest.mark.gpu
+def test_second_derivatives_raise(dev):
+    """A gradient penalty through what is differentiable once raises; the first derivatives are
+    the same with create_graph as without."""
+    torch.manual_seed(0)
+    q, k, g = (torch.randn(60, h, 64, device=dev).to(BF) for h in (4, 2, 4))
+    x, y = torch.randn(60, 50, device=dev), torch.randint(0, 50, (60,), device=dev)
+    cu = torch.tensor([0, 20, 60], dtype=torch.int32, device=dev)
+    calls = [(lambda q, k, v: (packed.packed_attention(q, k, v, cu) * g).sum(), (q, k, k.flip(0))),
+             (lambda x: token_logprobs(x, y).sum(), (x,)),
+             (lambda x: preference_loss(x, y, cu, torch.zeros(2, device=dev))[0], (x,))]
+    for call, inputs in calls:
+        w = [torch.ones((), device=dev, requires_grad=True) for _ in inputs]
+        leaves = [t.clone().requires_grad_() for t in inputs]
+        plain = torch.autograd.grad(call(*leaves), leaves)
+        grads = torch.autograd.grad(call(*[(t * s).to(t.dtype) for t, s in zip(leaves, w)]), leaves, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(grads, plain))
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            sum((d.float() ** 2).sum() for d in grads).backward()
