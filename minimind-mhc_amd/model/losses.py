@@ -10,13 +10,13 @@ import functools
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _hip as H
 from . import _ops
 from .packed import _bounds
 
 IGNORE_INDEX = -100
+MAX_EXPERTS = 4096  # of balance_loss
 
 
 def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -205,19 +205,21 @@ class _BalanceLoss(torch.autograd.Function):
         return loss, counts
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, g, *_):
-        if g is None:
+    def backward(ctx, grad, *_):
+        if grad is None:
             return (None,) * 4
         cu, counts, ws = ctx.saved_tensors
-        (T, E), g = ctx.shape, _scalar(g)
-        out = torch.empty((T, E), dtype=ctx.dtype, device=counts.device)
+        (T, E), g = ctx.shape, _scalar(grad.detach())
+        again = torch.is_grad_enabled() and grad.requires_grad  # the scores do not enter, only grad does
+        if again:
+            g = torch.ones_like(g)
+        out = torch.empty((T, E), dtype=torch.float32 if again else ctx.dtype, device=counts.device)
         with _ops.launch_device(counts):
             H.check(H.load().mhc_balance_bwd(
                 H.ptr(cu), counts.data_ptr(), ws.data_ptr(), g.data_ptr(), out.data_ptr(),
                 H.dtype_tag(out), T, E, counts.numel() // E, ctx.coef, H.stream(counts.device)),
                 "mhc_balance_bwd")
-        return out, None, None, None
+        return (out * grad).to(ctx.dtype) if again else out, None, None, None
 
 
 def balance_loss(scores: torch.Tensor, index: torch.Tensor, coef: float,
@@ -227,7 +229,7 @@ def balance_loss(scores: torch.Tensor, index: torch.Tensor, coef: float,
 
     scores [..., E] fp32, bf16 or fp16, the router's probabilities; index [..., k] int64, the
     experts each token went to.  counts [E] int64: how often each was taken.  loss: fp32,
-    differentiable once, in scores (counts are constants).
+    differentiable in scores, as often as wanted (counts are constants).
     cu_seqlens [n + 1] int32: the mean over the sequences (rows cu_seqlens[i] to
     cu_seqlens[i + 1], beginning with row 0) of each one's own loss instead, and counts
     [n, E].  Sequences without rows do not enter the mean; rows behind the last are
