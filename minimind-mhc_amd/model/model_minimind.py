@@ -279,7 +279,8 @@ class MOEFeedForward(nn.Module):
             cu_seqlens = torch.arange(b + 1, dtype=torch.int32, device=scores.device) * l
         elif cu_seqlens is not None and not each:  # one stretch of rows: none behind the last sequence
             cu_seqlens = torch.cat([cu_seqlens.new_zeros(1), cu_seqlens[-1:]])
-        if scores.is_cuda and (each or scores.dtype == torch.float32) and _ops.eager_call():
+        if (scores.is_cuda and (each or scores.dtype == torch.float32) and cfg.num_experts <= losses.MAX_EXPERTS
+                and _ops.eager_call()):
             loss, counts = losses.balance_loss(scores, idx, cfg.router_aux_loss_coef, cu_seqlens)
             return loss, counts if each or cu_seqlens is None else counts[0]
         hot = F.one_hot(idx, cfg.num_experts)

@@ -370,3 +370,19 @@ def test_balance_loss_in_a_gradient_penalty(dev, each):
     for a, b in zip(*res):
         # fp32 sums of 120 tokens and 192 dims in other orders, 2^-16, twice differentiated
         assert _far(a, b) <= 2.0 ** -13
+
+
+@pytest.mark.gpu
+def test_router_of_very_many_experts(dev):
+    """More experts than the kernels count: torch ops, as before."""
+    m = _model(dev, torch.float32, use_moe=True, num_experts_per_tok=2, use_mhc=0, router_aux_loss_coef=0.5)
+    moe = m.model.layers[0].mlp.train()
+    scores = torch.randn(20, 5000, device=dev).softmax(-1)
+    idx = scores.topk(2).indices
+    moe.config.num_experts = 5000
+    for each in (False, True):
+        moe.config.router_aux_loss_per_sequence = each
+        loss, counts = moe._balance(scores, idx, 2, 10, None)
+        want, n = moe._balance(scores.cpu(), idx.cpu(), 2, 10, None)
+        torch.testing.assert_close(loss.cpu(), want, rtol=1e-5, atol=0.0)
+        assert torch.equal(counts.cpu(), n)
