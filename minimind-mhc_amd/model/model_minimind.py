@@ -298,7 +298,8 @@ class MOEFeedForward(nn.Module):
         ends = [0, *(min(max(e, 0), scores.shape[0]) for e in cu_seqlens.tolist()[1:])]  # as the kernels do
         parts = [(hot[i:j].float().sum((0, 1)) / (j - i) * scores[i:j].float().mean(0)).sum()
                  for i, j in zip(ends, ends[1:]) if j > i]
-        counts = torch.stack([hot[i:j].sum((0, 1)) for i, j in zip(ends, ends[1:])])
+        counts = torch.cat([hot.new_zeros(0, cfg.num_experts),
+                            *(hot[i:j].sum((0, 1))[None] for i, j in zip(ends, ends[1:]))])
         loss = torch.stack(parts).mean() if parts else scores.float().sum() * 0.0
         return loss * cfg.num_experts * cfg.router_aux_loss_coef, counts
 

@@ -386,3 +386,16 @@ def test_router_of_very_many_experts(dev):
         want, n = moe._balance(scores.cpu(), idx.cpu(), 2, 10, None)
         torch.testing.assert_close(loss.cpu(), want, rtol=1e-5, atol=0.0)
         assert torch.equal(counts.cpu(), n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
+def test_batches_without_sequences(dev, dtype):
+    for each in (False, True):
+        m = _model(dev, dtype, use_moe=True, num_experts_per_tok=2, use_mhc=0, router_aux_loss_per_sequence=each).train()
+        b, ids = PackedBatch.from_lengths([], rows=5, device=dev), torch.randint(0, 500, (1, 5), device=dev)
+        out = m(ids, packed=b)
+        assert out.logits.shape == (1, 5, 500) and float(out.aux_loss.detach()) == 0.0
+        assert m.model.layers[0].mlp.expert_counts.shape == ((0, 4) if each else (4,))
+        assert m.sequence_logprobs(ids, ids, b).shape == (0,)
+        out.aux_loss.backward()

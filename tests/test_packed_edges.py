@@ -298,3 +298,14 @@ def test_preference_pairs_of_impossible_answers(monkeypatch):
     torch.testing.assert_close(out.loss, -torch.nn.functional.logsigmoid(z) / 2)
     assert float(out.rejected_rewards[1]) == -math.inf
     assert float(m.preference_loss(ids, ids, b, torch.zeros(4), label_smoothing=0.1).loss) == math.inf
+
+
+def test_batches_without_sequences():
+    for each in (False, True):
+        m = _model(use_moe=True, num_experts_per_tok=2, router_aux_loss_per_sequence=each).train()
+        b, ids = PackedBatch.from_lengths([], rows=5, device="cpu"), torch.randint(0, 50, (1, 5))
+        out = m(ids, packed=b)
+        assert out.logits.shape == (1, 5, 50) and float(out.aux_loss) == 0.0
+        assert m.model.layers[0].mlp.expert_counts.shape == ((0, 4) if each else (4,))
+        assert m.sequence_logprobs(ids, ids, b).shape == (0,)
+        out.aux_loss.backward()
