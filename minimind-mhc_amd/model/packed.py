@@ -330,9 +330,13 @@ def _plain_attention(q, k, v, cu_q, cu_k, used, dropout):
     inside = kp < torch.cat([have, new.new_zeros(1)])[ks]
     seen = (qs[:, None] == ks) & inside & (kp <= (qp + shift[qs])[:, None]) & (qs < n)[:, None]
     rep = q.shape[1] // k.shape[1]
-    k, v = (torch.where((inside & (ks < n))[:, None, None], t, 0).repeat_interleave(rep, 1).transpose(0, 1)
-            for t in (k, v))
+    # keys in use that are no numbers: a probability of 0 would not keep them from other rows
+    bad = ~(torch.isfinite(k).all(2) & torch.isfinite(v).all(2))
+    k, v = (torch.where((inside & (ks < n))[:, None, None] & ~bad[:, :, None], t, 0)
+            .repeat_interleave(rep, 1).transpose(0, 1) for t in (k, v))
     some = seen.any(1)
     out = torch.nn.functional.scaled_dot_product_attention(
         q.transpose(0, 1)[None], k[None], v[None], attn_mask=seen | ~some[:, None], dropout_p=dropout)
-    return torch.where(some[:, None, None], out[0].transpose(0, 1), 0)
+    out = torch.where(some[:, None, None], out[0].transpose(0, 1), 0)
+    hit = torch.matmul(seen.float(), bad.float()) > 0  # [rows, kv heads]
+    return out.masked_fill(hit.repeat_interleave(rep, 1)[:, :, None], math.nan)

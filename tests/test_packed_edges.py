@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from model.model_minimind import MiniMindForCausalLM
-from model.packed import PackedBatch, PackedCache
+from model.packed import PackedBatch, PackedCache, _plain_attention
 from tests.test_packed import _ints, _model
 
 
@@ -309,3 +309,24 @@ def test_batches_without_sequences():
         assert m.model.layers[0].mlp.expert_counts.shape == ((0, 4) if each else (4,))
         assert m.sequence_logprobs(ids, ids, b).shape == (0,)
         out.aux_loss.backward()
+
+
+# ------------------------------------------------- attention on torch ops
+
+@pytest.mark.parametrize("where", ["q", "k", "v"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_plain_attention_keeps_to_its_sequence(where, bad):
+    """Values that are not finite reach the rows that see them, and no other sequence."""
+    torch.manual_seed(0)
+    q, k, v = torch.randn(12, 4, 16), torch.randn(12, 2, 16), torch.randn(12, 2, 16)
+    cu = _ints(0, 4, 9, 11)
+    good = _plain_attention(q, k, v, cu, cu, None, 0.0)
+    t = {"q": q, "k": k, "v": v}[where].clone()
+    t[6, 0, 3] = bad
+    args = {"q": q, "k": k, "v": v, where: t.requires_grad_()}
+    out = _plain_attention(args["q"], args["k"], args["v"], cu, cu, None, 0.0)
+    keep = [0, 1, 2, 3, 4, 5, 9, 10, 11]
+    torch.testing.assert_close(out[keep], good[keep], rtol=1e-6, atol=1e-6)
+    assert not torch.isfinite(out[6, 0]).all()
+    g, = torch.autograd.grad(out[keep].sum(), t)
+    assert torch.isfinite(g[:4]).all() and torch.isfinite(g[9:]).all()
