@@ -17,6 +17,12 @@ from .packed import _bounds
 
 IGNORE_INDEX = -100
 MAX_EXPERTS = 4096  # of balance_loss
+_TYPES = (torch.float32, *_ops.HALF)
+
+
+def takes(t: torch.Tensor) -> bool:
+    """Whether the kernels take these logits or scores, in a call that nothing traces."""
+    return t.is_cuda and t.dtype in _TYPES and _ops.eager_call()
 
 
 def _rows(t: torch.Tensor, name: str) -> torch.Tensor:

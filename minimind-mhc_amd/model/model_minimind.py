@@ -279,8 +279,7 @@ class MOEFeedForward(nn.Module):
             cu_seqlens = torch.arange(b + 1, dtype=torch.int32, device=scores.device) * l
         elif cu_seqlens is not None and not each:  # one stretch of rows: none behind the last sequence
             cu_seqlens = torch.cat([cu_seqlens.new_zeros(1), cu_seqlens[-1:]])
-        if (scores.is_cuda and (each or scores.dtype == torch.float32) and cfg.num_experts <= losses.MAX_EXPERTS
-                and _ops.eager_call()):
+        if (each or scores.dtype == torch.float32) and cfg.num_experts <= losses.MAX_EXPERTS and losses.takes(scores):
             loss, counts = losses.balance_loss(scores, idx, cfg.router_aux_loss_coef, cu_seqlens)
             return loss, counts if each or cu_seqlens is None else counts[0]
         hot = F.one_hot(idx, cfg.num_experts)
@@ -466,7 +465,7 @@ class MiniMindForCausalLM(nn.Module):
 
     @staticmethod
     def _token_logprobs(logits, labels):
-        if logits.is_cuda and _ops.eager_call():
+        if losses.takes(logits):
             return losses.token_logprobs(logits, labels)
         return -F.cross_entropy(logits.float(), labels, ignore_index=-100, reduction="none")
 
@@ -497,7 +496,7 @@ class MiniMindForCausalLM(nn.Module):
         half of the sequences chosen, the second rejected; labels -100 where a token does not
         count) plus the routers' balance loss, with the rewards."""
         out, y = self(input_ids, packed=packed), packed.next_labels(labels)[0]
-        if out.logits.is_cuda and _ops.eager_call():
+        if losses.takes(out.logits):
             loss, chosen, rejected = losses.preference_loss(
                 out.logits[0], y, packed.cu_seqlens, reference, beta, label_smoothing, average)
         else:

@@ -399,3 +399,21 @@ def test_batches_without_sequences(dev, dtype):
         assert m.model.layers[0].mlp.expert_counts.shape == ((0, 4) if each else (4,))
         assert m.sequence_logprobs(ids, ids, b).shape == (0,)
         out.aux_loss.backward()
+
+
+@pytest.mark.gpu
+def test_model_of_64_bits(dev):
+    """No kernel takes fp64: the packed calls run on torch ops, as the dense ones do."""
+    m = _model(dev, torch.float64, use_moe=True, num_experts_per_tok=2, use_mhc=0,
+               router_aux_loss_per_sequence=True).train()
+    cpu = copy.deepcopy(m).cpu()
+    lengths = [20, 7, 1, 30]
+    ids, ref = torch.randint(0, 500, (1, 58)), torch.randn(4)
+    res = []
+    for net, d in ((m, dev), (cpu, "cpu")):
+        b = PackedBatch.from_lengths(lengths, device=d)
+        x = ids.to(d)
+        out = net.preference_loss(x, x, b, ref.to(d))
+        res.append((net(x, packed=b, labels=x).loss, net.sequence_logprobs(x, x, b), out.loss, out.aux_loss))
+    for a, w in zip(*res):  # the rows' log-probabilities are fp32
+        torch.testing.assert_close(a.detach().cpu().double(), w.detach().double(), rtol=1e-5, atol=1e-5)
