@@ -12,6 +12,7 @@ import torch
 from model import packed
 from model.losses import preference_loss, token_logprobs
 from model.packed import PackedBatch, PackedCache
+from tests.test_gpu_losses import EPS, F32, _exact_logprobs, _logits
 from tests.test_gpu_packed import _cu, exact
 from tests.test_gpu_packed_model import _far, _model, _taken
 
@@ -417,3 +418,74 @@ def test_model_of_64_bits(dev):
         res.append((net(x, packed=b, labels=x).loss, net.sequence_logprobs(x, x, b), out.loss, out.aux_loss))
     for a, w in zip(*res):  # the rows' log-probabilities are fp32
         torch.testing.assert_close(a.detach().cpu().double(), w.detach().double(), rtol=1e-5, atol=1e-5)
+
+
+# ------------------------------------------------- gradients of logits, each element by its own size
+
+def _each_close(got, dlp, f, dtype, factor=0.0):
+    """f ([hot] - p) element by element: half a step of the type, an error of the log-probability
+    (2^-15) on p and one of the factor on all, and at the label, where 1 - p is rounded, four half steps
+    of fp32.  (2^-25: half of fp16's smallest number; 2^-120: fp32's smallest exponentials are flushed.)"""
+    got, want = got.detach().double().cpu(), dlp * f
+    p = torch.where(dlp > 0, 1 - dlp, -dlp)  # 0 in rows that do not count, whose bar stays exact
+    bar = (EPS[dtype] + factor) * want.abs() + 2.0 ** -15 * p * f.abs() + (dlp > 0) * 2.0 ** -22 * f.abs() \
+        + (dlp != 0) * ((2.0 ** -25 if dtype == F16 else 0.0) + 2.0 ** -120)
+    bad = (got - want).abs() > bar
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[:5].tolist())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,V,dtype,pad,offset", [
+    (7, 7, F16, 0, 1), (5, 64, BF, 0, 3), (33, 6400, BF, 0, 0), (9, 6401, F16, 0, 0), (4, 6400, F32, 3, 1),
+    (6, 50257, F32, 0, 0), (5, 50257, BF, 0, 5), (300, 100, F16, 28, 0), (2, 131072, BF, 0, 0), (17, 2050, BF, 6, 7),
+    (3, 50257, F16, 3, 1), (2, 32001, F32, 1, 2)])
+def test_gradients_of_logits_each(dev, T, V, dtype, pad, offset):
+    x, labels = _logits(T, V, dtype, dev, pad=pad, offset=offset)
+    labels[0] = V - 1
+    dlp = _exact_logprobs(x, labels)[1]
+    x = x.detach().requires_grad_()
+    g = torch.randn(T) * (2.0 ** 12 if dtype == F16 else 1.0)
+    got, = torch.autograd.grad(token_logprobs(x, labels), x, g.to(dev))
+    _each_close(got, dlp, g.double()[:, None], dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V,dtype,offset", [(6400, BF, 0), (6401, F32, 1), (50257, F16, 3), (100, BF, 1)])
+def test_gradients_of_preference_each(dev, V, dtype, offset):
+    lengths, behind = [5, 9, 1, 12], 3
+    T = sum(lengths) + behind
+    x, labels = _logits(T, V, dtype, dev, offset=offset)
+    dlp = _exact_logprobs(x, labels)[1]
+    lp = _exact_logprobs(x, labels)[0]
+    ends = torch.tensor([0] + lengths).cumsum(0)
+    S = torch.stack([lp[a:b].sum() for a, b in zip(ends, ends[1:])])
+    ref = (S + torch.tensor([1.0, -2.0, 0.5, 3.0])).float()
+    r = 0.3 * (S - ref.double())
+    dz = -torch.sigmoid(r[2:] - r[:2]) * 0.3 / 2 * 2.0 ** 12
+    f = torch.cat([torch.cat([dz, -dz]).repeat_interleave(torch.tensor(lengths)), torch.zeros(behind)])[:, None]
+    x = x.detach().requires_grad_()
+    loss = preference_loss(x, labels, ends.to(dev, torch.int32), ref.to(dev), 0.3)[0]
+    got, = torch.autograd.grad(loss, x, torch.full((), 2.0 ** 12, device=dev))
+    dlp[-behind:] = 0.0
+    # z is off by 0.3 of 24 rows' errors of 2^-15, a sigmoid's relative slope is at most 1
+    _each_close(got, dlp, f, dtype, factor=0.3 * 24 * 2.0 ** -15 + 2.0 ** -22)
+
+
+@pytest.mark.gpu
+def test_routed_experts_of_packed_rows(dev):
+    """The routed layer of a packed inference call gives each sequence's rows what they get alone,
+    where the second and third expert are not a rounding apart (half a step of bf16 on scores of up to
+    1 is 2^-8 and less; 2^-5 leaves room for the gate's own)."""
+    m = _model(dev, use_moe=True, num_experts=6, num_experts_per_tok=2, use_mhc=0).eval()
+    moe, lengths = m.model.layers[0].mlp, [70, 1, 33, 150, 64]
+    torch.manual_seed(0)
+    moe.gate.weight.data.mul_(8.0)
+    x = torch.randn(1, sum(lengths), 192, device=dev).to(BF)
+    with torch.inference_mode():
+        top = (x[0].double() @ moe.gate.weight.double().t()).softmax(-1).topk(3).values
+        clear = top[:, 1] - top[:, 2] > 2.0 ** -5
+        got, alone = moe(x)[0], torch.cat([moe(t)[0] for t in x.split(lengths, 1)])
+    assert int(clear.sum()) > 150
+    # both round the same steps (two products, an activation, the weighted sum) to bf16: 4 of 2^-8 each
+    off = (got - alone).double().norm(dim=1) / alone.double().norm(dim=1)
+    assert float(off[clear].max()) <= 8 * 2.0 ** -8
