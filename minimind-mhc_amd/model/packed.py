@@ -338,5 +338,9 @@ def _plain_attention(q, k, v, cu_q, cu_k, used, dropout):
     out = torch.nn.functional.scaled_dot_product_attention(
         q.transpose(0, 1)[None], k[None], v[None], attn_mask=seen | ~some[:, None], dropout_p=dropout)
     out = torch.where(some[:, None, None], out[0].transpose(0, 1), 0)
-    hit = torch.matmul(seen.float(), bad.float()) > 0  # [rows, kv heads]
+    # [rows, kv heads]: whether one is among the keys a row sees, from its sequence's first to its own
+    upto = torch.cat([bad.new_zeros(1, bad.shape[1], dtype=torch.int32), bad.cumsum(0, dtype=torch.int32)])
+    first = cu_k.clamp(0, k.shape[1])[qs]
+    count = torch.minimum(qp + shift[qs] + 1, torch.cat([have, new.new_zeros(1)])[qs]).clamp_min(0)
+    hit = upto[(first + count).clamp_max(k.shape[1])] > upto[first]
     return out.masked_fill(hit.repeat_interleave(rep, 1)[:, :, None], math.nan)
