@@ -53,6 +53,14 @@ __device__ __forceinline__ U32x4 pack16(const float (&x)[kPer16<DT>]) {
 }
 
 // --------------------------------------------------- log-probabilities of labels
+// A workgroup a row, in as many lines of 2^22 of them as it takes: one dimension of a launch holds
+// less than 2^32 threads, and wraps without an error.
+constexpr int64_t kLaunchLine = 1 << 22;
+inline dim3 launch_rows(int64_t rows) {
+  return dim3((unsigned)(rows < kLaunchLine ? rows : kLaunchLine), (unsigned)((rows + kLaunchLine - 1) / kLaunchLine));
+}
+__device__ __forceinline__ int64_t launch_row() { return blockIdx.x + (int64_t)blockIdx.y * kLaunchLine; }
+
 // One workgroup a row, one pass: each thread keeps a running maximum and sum.  A row may
 // begin anywhere: the elements before its first 16-byte boundary and behind its last go one
 // by one.  Rows whose label does not count are not read.  16384 x 6400 bf16 rows, a quarter of them
@@ -62,7 +70,8 @@ template <int DT>
 __global__ __launch_bounds__(256) void logprob_kernel(LogitArgs a) {
   constexpr int PER = kPer16<DT>;
   __shared__ float sm[4], sl[4];
-  const int64_t row = blockIdx.x;
+  const int64_t row = launch_row();
+  if (row >= a.T) return;
   const int64_t label = a.labels[row];
   const int tid = threadIdx.x;
   const bool counts = label != a.ignore;
@@ -151,7 +160,8 @@ __global__ __launch_bounds__(256) void logprob_bwd_kernel(LogitArgs a) {
   constexpr int PER = kPer16<DT>;
   constexpr int EB = DT == kF32 ? 4 : 2;
   // from the last row back: the forward pass's last rows are still in the memory-side cache
-  const int64_t row = a.T - 1 - blockIdx.x;
+  const int64_t row = a.T - 1 - launch_row();
+  if (row < 0) return;
   const int64_t label = a.labels[row];
   const int tid = threadIdx.x;
   float f = 0.f;
@@ -380,13 +390,13 @@ __global__ __launch_bounds__(256) void balance_bwd_kernel(BalanceArgs a) {
 }  // namespace
 
 hipError_t launch_logprobs(const LogitArgs& a, hipStream_t s) {
-#define RUN(DT) logprob_kernel<DT><<<dim3((unsigned)a.T), 256, 0, s>>>(a)
+#define RUN(DT) logprob_kernel<DT><<<launch_rows(a.T), 256, 0, s>>>(a)
   MHC_LOSS_DT(a.dtype, RUN)
 #undef RUN
   return hipGetLastError();
 }
 hipError_t launch_logprobs_bwd(const LogitArgs& a, hipStream_t s) {
-#define RUN(DT) logprob_bwd_kernel<DT><<<dim3((unsigned)a.T), 256, 0, s>>>(a)
+#define RUN(DT) logprob_bwd_kernel<DT><<<launch_rows(a.T), 256, 0, s>>>(a)
   MHC_LOSS_DT(a.dtype, RUN)
 #undef RUN
   return hipGetLastError();

@@ -489,3 +489,23 @@ def test_routed_experts_of_packed_rows(dev):
     # both round the same steps (two products, an activation, the weighted sum) to bf16: 4 of 2^-8 each
     off = (got - alone).double().norm(dim=1) / alone.double().norm(dim=1)
     assert float(off[clear].max()) <= 8 * 2.0 ** -8
+
+
+# ------------------------------------------------- more rows than one dimension of a launch takes
+
+@pytest.mark.gpu
+def test_rows_past_the_launch_limit(dev):
+    """2^24 rows of 256 threads are 2^32 of them, one more than a dimension of a launch holds."""
+    T, V = (1 << 24) + 5, 3
+    torch.manual_seed(0)
+    part = torch.randn(1 << 10, V, device=dev).to(BF)
+    x = part.repeat(T // (1 << 10) + 1, 1)[:T].contiguous().requires_grad_()
+    y = torch.randint(0, V, (1 << 10,), device=dev).repeat(T // (1 << 10) + 1)[:T].contiguous()
+    small = x[:1 << 10].detach().requires_grad_()
+    want = token_logprobs(small, y[:1 << 10])
+    g, = torch.autograd.grad(want.sum(), small)
+    lp = token_logprobs(x, y)
+    got, = torch.autograd.grad(lp.sum(), x)
+    for t, w in ((lp.detach(), want.detach()), (got, g)):
+        assert torch.equal(t[:-5].view(-1, *w.shape), w.expand(T // (1 << 10), *w.shape))
+        assert torch.equal(t[-5:], w[:5])
