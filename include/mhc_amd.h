@@ -555,7 +555,8 @@ int mhc_linear_pays(const int* n, int count, int64_t M, int K, int glu);
  * sees the keys up to its own position.  Rows that see no key, and the rows
  * behind the last sequence, come out 0.  The bounds are clamped to the tensors;
  * bounds that decrease give unspecified rows.
- * Tq and Tk are at most 2^30.
+ * Tq and Tk are at most 2^30; shapes whose launches would need 2^32 threads are
+ * refused.
  */
 
 /* Bytes of workspace mhc_packed_attn_fwd needs (0: none), or -1 for a shape it

@@ -740,7 +740,7 @@ static int check_packed(const mhc::PackedAttnArgs& a, int64_t Tq, int64_t Tk, in
     return fail(hipErrorInvalidValue, "%s: bad shape (B=%d Tq=%lld Tk=%lld)", fn, a.B, (long long)Tq, (long long)Tk);
   if (int rc = check_attn(Tq, a.heads, a.kv_heads, a.head_dim, dtype, fn)) return rc;
   if (!(a.scale > 0.f) || a.scale > 3e38f) return fail(hipErrorInvalidValue, "%s: scale must be positive (got %g)", fn, (double)a.scale);
-  // the most workgroups of any of the launches: a tile number for every row and sequence
+  // a tile number for every row and sequence, as an int
   if ((Tq + a.B + 1) * a.heads > kMaxBlocks || (Tk / 64 + a.B + 1) * a.kv_heads > kMaxBlocks)
     return fail(hipErrorInvalidValue, "%s: too large", fn);
   for (int64_t st : {a.qs_t, a.qs_h, a.ks_t, a.ks_h, a.vs_t, a.vs_h})
@@ -748,6 +748,11 @@ static int check_packed(const mhc::PackedAttnArgs& a, int64_t Tq, int64_t Tk, in
   // a tile's rows are 32-bit byte offsets apart
   for (int64_t st : {a.qs_t, a.ks_t, a.vs_t})
     if (st >= 1 << 23) return fail(hipErrorInvalidValue, "%s: rows must be under 2^23 elements apart", fn);
+  return 0;
+}
+
+static int check_threads(int64_t threads, const char* fn) {
+  if (threads > mhc::kLaunchThreads) return fail(hipErrorInvalidValue, "%s: too large for a launch", fn);
   return 0;
 }
 
@@ -770,6 +775,7 @@ int64_t mhc_packed_attn_workspace_bytes(int B, int64_t Tq, int64_t Tk, int heads
   if (check_packed(a, Tq, Tk, mhc::kBF16, "mhc_packed_attn_workspace_bytes")) return -1;
   if (Tq == 0) return 0;
   mhc::packed_attn_plan(a);
+  if (check_threads(mhc::packed_attn_threads(a), "mhc_packed_attn_workspace_bytes")) return -1;
   return mhc::packed_attn_workspace(a);
 }
 
@@ -778,6 +784,7 @@ int64_t mhc_packed_attn_bwd_workspace_bytes(int B, int64_t Tq, int64_t Tk, int h
                                       Tk, heads, kv_heads, head_dim, mhc::kBF16, 1.f);
   if (check_packed(a, Tq, Tk, mhc::kBF16, "mhc_packed_attn_bwd_workspace_bytes")) return -1;
   mhc::packed_bwd_plan(a);
+  if (check_threads(mhc::packed_bwd_threads(a), "mhc_packed_attn_bwd_workspace_bytes")) return -1;
   return mhc::packed_bwd_workspace(a, nullptr);
 }
 
@@ -797,6 +804,7 @@ int mhc_packed_attn_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, c
   if (!cu_q || !cu_k) return fail(hipErrorInvalidValue, "%s: the sequences' bounds are required", fn);
   if (!rest != !lse || !aligned16(rest)) return fail(hipErrorInvalidValue, "%s: rest and lse are both given, 16-byte aligned, or neither", fn);
   mhc::packed_attn_plan(a);
+  if (int rc = check_threads(mhc::packed_attn_threads(a), fn)) return rc;
   const int64_t need = mhc::packed_attn_workspace(a);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(hipErrorInvalidValue, "%s: workspace of %lld bytes needed (got %lld)", fn, (long long)need, (long long)workspace_bytes);
@@ -824,6 +832,7 @@ int mhc_packed_attn_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, c
   if (!cu_q || !cu_k) return fail(hipErrorInvalidValue, "%s: the sequences' bounds are required", fn);
   if (Tq > 0 && !lse) return fail(hipErrorInvalidValue, "%s: lse is required", fn);
   mhc::packed_bwd_plan(a);
+  if (int rc = check_threads(mhc::packed_bwd_threads(a), fn)) return rc;
   const int64_t need = mhc::packed_bwd_workspace(a, static_cast<float*>(workspace));
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(hipErrorInvalidValue, "%s: workspace of %lld bytes needed (got %lld)", fn, (long long)need, (long long)workspace_bytes);
@@ -873,8 +882,9 @@ int mhc_preference_fwd(const float* logprobs, const int64_t* labels, int64_t ign
                        float* g_seq, void* scratch, int64_t T, int P, double beta,
                        double smoothing, int flags, hipStream_t stream) {
   const char* fn = "mhc_preference_fwd";
-  if (T < 0 || T > 1 << 30 || P < 1 || P > 1 << 29)
+  if (T < 0 || T > 1 << 30 || P < 1)
     return fail(hipErrorInvalidValue, "%s: bad shape (T=%lld pairs=%d)", fn, (long long)T, P);
+  if (int rc = check_threads((int64_t)P * 256, fn)) return rc;
   if ((T > 0 && (!logprobs || !labels)) || !cu || !reference || !loss || !chosen || !rejected || !g_seq || !scratch ||
       reinterpret_cast<uintptr_t>(scratch) % 8 || reinterpret_cast<uintptr_t>(reference) % (flags & 2 ? 8 : 4))
     return fail(hipErrorInvalidValue, "%s: null or unaligned pointer", fn);
@@ -905,7 +915,7 @@ static int check_balance(int64_t T, int E, int B, const char* fn) {
   if (T < 0 || T > 1 << 30 || E < 1 || E > mhc::kBalanceMaxExperts || B < 0 || (int64_t)B * E > kMaxBlocks ||
       T * E / 256 >= kMaxBlocks)
     return fail(hipErrorInvalidValue, "%s: bad shape (T=%lld E=%d B=%d)", fn, (long long)T, E, B);
-  return 0;
+  return check_threads((int64_t)B * mhc::balance_parts(T, B) * 256, fn);
 }
 
 int64_t mhc_balance_workspace_bytes(int64_t T, int E, int B) {

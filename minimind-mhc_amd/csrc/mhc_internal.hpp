@@ -324,10 +324,15 @@ struct PackedAttnArgs {
   void* g_k;
   void* g_v;
 };
+// A dimension of a launch holds less than 2^32 threads and wraps without an error.
+constexpr int64_t kLaunchThreads = 0xffffffff;
 void packed_attn_plan(PackedAttnArgs& a);
+// Threads of the largest launch.
+int64_t packed_attn_threads(const PackedAttnArgs& a);
 int64_t packed_attn_workspace(const PackedAttnArgs& a);
 hipError_t launch_packed_attn(const PackedAttnArgs& a, hipStream_t s);
 void packed_bwd_plan(PackedAttnArgs& a);
+int64_t packed_bwd_threads(const PackedAttnArgs& a);
 // Its bytes; lays out delta, v_top, g_top and work in it, where one is given.
 int64_t packed_bwd_workspace(PackedAttnArgs& a, float* workspace);
 hipError_t launch_packed_attn_bwd(const PackedAttnArgs& a, hipStream_t s);

@@ -357,7 +357,7 @@ __global__ __launch_bounds__(1024) void balance_join_kernel(BalanceArgs a) {
 // coef E f_e / T for every row: 16384 x 8 bf16 3.0 us, 8191 x 64 fp32 5.0 us, launch and divisions.
 template <int DT>
 __global__ __launch_bounds__(256) void balance_bwd_kernel(BalanceArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = launch_row() * 256 + threadIdx.x;
   if (i >= (int64_t)a.T * a.E) return;
   const int t = (int)(i / a.E), e = (int)(i % a.E);
   int seq = 0, n = a.T;
@@ -428,7 +428,7 @@ hipError_t launch_balance(const BalanceArgs& a, hipStream_t s) {
 }
 hipError_t launch_balance_bwd(const BalanceArgs& a, hipStream_t s) {
   const int64_t blocks = ((int64_t)a.T * a.E + 255) / 256;
-#define RUN(DT) balance_bwd_kernel<DT><<<dim3((unsigned)blocks), 256, 0, s>>>(a)
+#define RUN(DT) balance_bwd_kernel<DT><<<launch_rows(blocks), 256, 0, s>>>(a)
   MHC_LOSS_DT(a.dtype, RUN)
 #undef RUN
   return hipGetLastError();

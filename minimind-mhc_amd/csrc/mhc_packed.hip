@@ -537,14 +537,18 @@ __global__ __launch_bounds__(256) void packed_merge_kernel(PackedAttnArgs a) {
   if (a.lse && c == 0) a.lse[at % a.heads * a.Tq + at / a.heads] = packed_lse(m, ls);
 }
 
+int64_t few_blocks(const PackedAttnArgs& a) {
+  const int nb = (a.heads / a.kv_heads + a.row_heads - 1) / a.row_heads;
+  return ((int64_t)a.qtiles * a.splits + 7) / 8 * 8 * a.kv_heads * nb;
+}
+int64_t tile_blocks(const PackedAttnArgs& a) { return (int64_t)a.qtiles * a.splits * (a.heads / a.row_heads); }
+
 template <bool F16, int HD>
 hipError_t packed_fwd_hd(const PackedAttnArgs& a, hipStream_t s) {
   if (a.few) {
-    const int nb = (a.heads / a.kv_heads + a.row_heads - 1) / a.row_heads;
-    const int64_t ranges = ((int64_t)a.qtiles * a.splits + 7) / 8 * 8;
-    packed_few_kernel<F16, HD><<<dim3((unsigned)(ranges * a.kv_heads * nb)), 256, 0, s>>>(a);
+    packed_few_kernel<F16, HD><<<dim3((unsigned)few_blocks(a)), 256, 0, s>>>(a);
   } else {
-    const dim3 grid((unsigned)((int64_t)a.qtiles * a.splits * (a.heads / a.row_heads)));
+    const dim3 grid((unsigned)tile_blocks(a));
     const bool halves = packed_halves(grid.x);
     if (a.row_heads == 2) {
       if (halves) packed_fwd_kernel<F16, HD, 2, 2><<<grid, 512, 0, s>>>(a);
@@ -596,6 +600,11 @@ void packed_attn_plan(PackedAttnArgs& a) {
   if (want > keys / least) want = keys / least;
   if (want > 128) want = 128;
   a.splits = want < 1 ? 1 : (int)want;
+}
+int64_t packed_attn_threads(const PackedAttnArgs& a) {
+  const int64_t tiles = 256 * (a.few ? few_blocks(a) : tile_blocks(a));
+  const int64_t merge = a.splits > 1 ? 256 * (int64_t)a.Tq * a.heads : 0;
+  return tiles > merge ? tiles : merge;
 }
 int64_t packed_attn_workspace(const PackedAttnArgs& a) {
   return a.splits > 1 ? (int64_t)a.splits * a.Tq * a.heads * (a.head_dim + 2) * 4 : 0;

@@ -716,6 +716,12 @@ void packed_bwd_plan(PackedAttnArgs& a) {
   if (want > 8) want = 8;
   a.ranges = want < 1 ? 1 : (int)want;
 }
+int64_t packed_bwd_threads(const PackedAttnArgs& a) {
+  const int hp = (a.heads / a.kv_heads) % 2 == 0 ? 2 : 1;
+  const int64_t dq = 256 * packed_tiles(a.Tq, a.B, 128 / hp) * (a.heads / hp);
+  const int64_t dkv = 512 * packed_tiles(a.Tk, a.B, 128) * a.kv_heads * a.ranges;
+  return dq > dkv ? dq : dkv;  // the join has fewer: several ranges are for some 10^5 keys at most
+}
 // D, the longest rows of v and g by tiles, and the ranges' sums of dK and dV.
 int64_t packed_bwd_workspace(PackedAttnArgs& a, float* workspace) {
   auto whole = [](int64_t n) { return (n + 3) / 4 * 4; };  // of 16 bytes

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from model import packed
-from model.losses import preference_loss, token_logprobs
+from model.losses import balance_loss, preference_loss, token_logprobs
 from model.packed import PackedBatch, PackedCache
 from tests.test_gpu_losses import EPS, F32, _exact_logprobs, _logits
 from tests.test_gpu_packed import _cu, exact
@@ -509,3 +509,19 @@ def test_rows_past_the_launch_limit(dev):
     for t, w in ((lp.detach(), want.detach()), (got, g)):
         assert torch.equal(t[:-5].view(-1, *w.shape), w.expand(T // (1 << 10), *w.shape))
         assert torch.equal(t[-5:], w[:5])
+
+
+@pytest.mark.gpu
+def test_balance_gradient_past_the_launch_limit(dev):
+    """2^32 scores and some: every row's gradient."""
+    E, T = 256, (1 << 24) + 3
+    torch.manual_seed(0)
+    row = torch.rand(1, E, device=dev).to(BF)
+    index = torch.randint(0, E, (T, 1), device=dev)
+    x = row.expand(T, E).requires_grad_()
+    loss, counts = balance_loss(x, index, 1e6)
+    g, = torch.autograd.grad(loss, x)
+    assert torch.equal(counts, torch.bincount(index[:, 0], minlength=E))
+    want = (1e6 * E * (counts.double() / T) / T).to(BF)  # the same of every row, rounded once
+    torch.testing.assert_close(g[0], want, rtol=2.0 ** -7, atol=0.0)
+    assert bool((g == g[0]).all())

@@ -330,3 +330,30 @@ def test_plain_attention_keeps_to_its_sequence(where, bad):
     assert not torch.isfinite(out[6, 0]).all()
     g, = torch.autograd.grad(out[keep].sum(), t)
     assert torch.isfinite(g[:4]).all() and torch.isfinite(g[9:]).all()
+
+
+# ------------------------------------------------- launches of 2^32 threads
+
+def test_library_refuses_what_a_launch_cannot_hold():
+    """Such a launch would wrap without an error.  Nothing of these calls reaches a device."""
+    import ctypes
+    from model import _hip
+    lib, p = _hip.load(), ctypes.c_void_p(16)
+
+    def refused(rc):
+        return rc != 0 and b"too large" in lib.mhc_last_error()
+    for B, Tq, heads, kv in ((1 << 24, 8, 2, 1), (1 << 22, 1 << 22, 16, 16), (1 << 21, 1 << 23, 32, 32)):
+        sizes = (B, Tq, Tq, heads, kv, 64)
+        assert lib.mhc_packed_attn_workspace_bytes(*sizes) == -1
+        assert lib.mhc_packed_attn_bwd_workspace_bytes(*sizes) == -1
+        assert refused(lib.mhc_packed_attn_fwd(p, 64, 64, p, 64, 64, p, 64, 64, p, p, None, p, None, None, p, 1 << 60,
+                                               *sizes, 1, 0.1, None))
+        assert refused(lib.mhc_packed_attn_bwd(p, 64, 64, p, 64, 64, p, 64, 64, p, p, None, p, p, p, p, p, p, p, p,
+                                               1 << 60, *sizes, 1, 0.1, None))
+    assert refused(lib.mhc_preference_fwd(p, p, -100, p, p, p, p, p, p, p, 4, 1 << 24, 0.1, 0.0, 0, None))
+    assert lib.mhc_balance_workspace_bytes(4, 1, 1 << 24) == -1
+    assert refused(lib.mhc_balance_fwd(p, 1, 0, p, p, p, p, p, p, 1 << 60, 4, 1, 1, 1 << 24, 0.1, None))
+    # the largest that are not
+    assert lib.mhc_packed_attn_workspace_bytes(1 << 20, 1 << 20, 1 << 20, 8, 4, 64) >= 0
+    assert lib.mhc_packed_attn_bwd_workspace_bytes(1 << 20, 1 << 20, 1 << 20, 8, 4, 64) > 0
+    assert lib.mhc_balance_workspace_bytes(1 << 20, 64, 1 << 20) > 0
