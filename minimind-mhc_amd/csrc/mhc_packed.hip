@@ -568,13 +568,16 @@ hipError_t packed_fwd_hd(const PackedAttnArgs& a, hipStream_t s) {
 
 // Which kernel, how many heads a workgroup takes and into how many ranges the keys go. Only
 // the totals are known here; the sequences' own lengths are read on the device.
+// Times of the launches, join included:
 //   * The kernel for few rows up to 8 rows (tokens times query heads of a kv head) a sequence on
-//     average: 64 sequences over 2176-row slots, 8 / 4 heads of 96, 1 new token each 36.3 us (the other
-//     kernel 38.5), 4 tokens 37.1 and 39.4, 8 tokens 51.5 and 40.8.
-//   * Ranges: two workgroups a CU, none of under 128 (512) keys on average. Those 64 single tokens
-//     in 1, 2, 4 and 8 ranges: 41.4, 36.3, 37.0, 41.4 us; 4 sequences of 4 tokens over 8000-row slots in 8, 16,
-//     32 and 64: 23.5, 23.0, 22.8, 23.0; one chunk of 512 tokens over 60000 rows, 16 / 2 heads of 128, in 4, 8, 16 and
-//     32: 180, 108, 109, 123; 8 of 128 over 4096 rows in 4, 8 and 16: 34.2, 32.5, 43.0.
+//     average: 64 sequences over 2176-row slots, 8 / 4 heads of 96, 1 new token each 36.4 us (the other
+//     kernel 39.4), 4 tokens 36.8 and 39.3, 8 tokens 54.3 and 39.4.
+//   * Ranges: two workgroups a CU, none of under 128 (512) keys on average, 128 at most. Those 64 single
+//     tokens in 1, 2, 4 and 8 ranges: 39.7, 36.7, 37.5, 42.1 us; 4 sequences of 4 tokens over 8000 keys each in 8, 16,
+//     32 and 64: 23.6, 22.5, 18.0, 20.8; one token over 65001 keys, 16 / 2 heads of 128, in 64, 128, 256 and 512:
+//     26.2, 20.8, 21.4, 29.4 (the join 3.9, 3.8, 5.2, 8.7 of them: hence the 128); one chunk of 512 tokens over
+//     60000 keys, 16 / 2 heads of 128, in 2, 4, 8 and 16: 463, 262, 270, 277 (the products 960 TFLOP/s in 8); 8 of 128
+//     over 4096 keys in 1, 4, 8 and 16: 64.3, 36.4, 35.9, 51.1.
 void packed_attn_plan(PackedAttnArgs& a) {
   const int rep = a.heads / a.kv_heads;
   const int B = a.B > 0 ? a.B : 1;

@@ -704,7 +704,10 @@ hipError_t packed_bwd_hd(PackedAttnArgs a, hipStream_t s) {
 
 // Ranges that the query rows of a key tile are cut into: up to four workgroups a CU, none of
 // under 8 tiles of rows (on average), beside whose products the ranges' sums (8 bytes an element
-// each way) are small.  A step of 12 sequences of 8192 tokens together, 8 / 4 heads of 96: 179 us with
+// each way) are small; 8 at most, which keeps the workspace to 64 bytes an element of k. (More would be
+// faster where key tiles are few: dK, dV and their join of one sequence of 4096 tokens, 8 / 1 heads of 64, in 4, 8, 16
+// and 31 ranges 154, 86, 72 and 70 us; of 2000 and 1000 tokens, 16 / 1 heads of 96, in 8 and 32 108 and 72; of one of
+// 16000, 8 / 1 heads of 64, in 2, 4 and 8 1067, 849 and 611.)  A step of 12 sequences of 8192 tokens together, 8 / 4 heads of 96: 179 us with
 // 3 ranges, 206 with one, 219 with 8; of 30 of 10000, 12 / 4 heads: 194, 231 and 254; of 2 sequences of 8000 tokens together, 8 / 2 heads of 128: 522 us
 // with 4 ranges and 1120 with one; of 2 of 16000, 16 / 2 heads of 64: 1540 with 4, 2136 with 2, 2496
 // with one; of 3 of 16001, 8 / 8 heads of 64 (four workgroups a CU as it is): 688 with 2, 664 with one.
