@@ -8,8 +8,8 @@
 //
 // dS is an operand of products, so it is rounded to the tensors' type.  bf16 has fp32's range.
 // An fp16 dS is multiplied by a power of two first, which the result is divided by: P of many
-// keys times a gradient of 1e-3 lies below fp16's normal numbers (dQ was off by 4e-3 with 8192 keys,
-// by 4e-2 for gradients of 1e-4).  No dS exceeds half the longest row of v times the length of its row of g
+// keys times a gradient of 1e-3 lies below fp16's normal numbers (dQ over 8192 keys was off by 1e-2,
+// for gradients of 1e-4 by 0.1).  No dS exceeds half the longest row of v times the length of its row of g
 // (P_j sum_k P_k |dP_j - dP_k| <= P_j (1 - P_j) 2 |g| |v|), so the power that takes |g| |v| to 2^15 at most
 // cannot overflow, and leaves 28 binary digits of normal numbers below.  dQ takes |g| of its own row, dK the
 // longest row of g from the block of 1024 rows on where its keys are first seen.  This costs fp16 one

@@ -176,7 +176,8 @@ class PackedBatch:
 
     cu_seqlens [n + 1] int32: sequence i has the rows cu_seqlens[i] to cu_seqlens[i + 1] of
     `rows`, beginning with row 0; rows behind the last belong to none (their outputs mean
-    nothing).  Everything stays on cu_seqlens' device, without a synchronisation."""
+    nothing).  Everything stays on cu_seqlens' device, without a synchronisation; rows' places
+    are formed here, so other bounds need another batch (in a captured graph: formed inside it)."""
 
     def __init__(self, cu_seqlens: torch.Tensor, rows: int):
         self.cu_seqlens = _bounds("cu_seqlens", cu_seqlens, None, cu_seqlens.device)
@@ -231,7 +232,9 @@ class PackedCache:
     A call appends its sequences' tokens and moves `lengths` on (on the device, so a captured
     decode step can be replayed).  Tokens that a slot has no room for are not stored, and
     their sequence's outputs mean nothing from then on; a batch made from_lengths is refused
-    before that.  Rows of no sequence change nothing."""
+    before that, as far as the host has seen the slots fill up.  Rows of no sequence change
+    nothing.  dtype may differ from the model's: 16-bit slots are read by the kernels, under any
+    autocast."""
 
     def __init__(self, config, sequences: int, capacity: int, dtype=torch.bfloat16, device="cuda"):
         if sequences < 1 or capacity < 1:
