@@ -96,13 +96,13 @@ class _PackedAttention(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
+        saved = ctx.saved_tensors  # once: checkpointing hands them out a single time
         with torch.no_grad():
-            grads = _PackedAttention._backward(ctx, g)
-        return (*_ops.once(grads, *ctx.saved_tensors[:3], g), None, None, None, None)
+            grads = _PackedAttention._backward(ctx.scale, g, *saved)
+        return (*_ops.once(grads, *saved[:3], g), None, None, None, None)
 
     @staticmethod
-    def _backward(ctx, g):
-        q, k, v, cu_q, cu_k, used, out, rest, lse = ctx.saved_tensors
+    def _backward(scale, g, q, k, v, cu_q, cu_k, used, out, rest, lse):
         (q, *qs), (k, *ks), (v, *vs) = _strided(q), _strided(k), _strided(v)
         g = g.to(out.dtype).contiguous()
         if g.data_ptr() % 16:  # a caller's view; the kernels load 16 bytes
@@ -120,7 +120,7 @@ class _PackedAttention(torch.autograd.Function):
                 q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs, cu_q.data_ptr(),
                 cu_k.data_ptr(), H.ptr(used), out.data_ptr(), rest.data_ptr(), lse.data_ptr(), g.data_ptr(),
                 g_q.data_ptr(), g_k.data_ptr(), g_v.data_ptr(), ws.data_ptr(), nbytes, B, Tq, Tk,
-                heads, kv, hd, H.dtype_tag(q), ctx.scale, H.stream(dev)), "mhc_packed_attn_bwd")
+                heads, kv, hd, H.dtype_tag(q), scale, H.stream(dev)), "mhc_packed_attn_bwd")
         return g_q, g_k, g_v
 
 

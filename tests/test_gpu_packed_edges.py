@@ -525,3 +525,23 @@ def test_balance_gradient_past_the_launch_limit(dev):
     want = (1e6 * E * (counts.double() / T) / T).to(BF)  # the same of every row, rounded once
     torch.testing.assert_close(g[0], want, rtol=2.0 ** -7, atol=0.0)
     assert bool((g == g[0]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_recomputed_in_the_backward_pass(dev, dtype):
+    """Under activation checkpointing (which lets a saved tensor be asked for once): the same bits."""
+    from torch.utils.checkpoint import checkpoint
+    torch.manual_seed(0)
+    q, k, g = (torch.randn(60, h, 64, device=dev).to(dtype) for h in (4, 2, 4))
+    x, y = torch.randn(60, 50, device=dev), torch.randint(0, 50, (60,), device=dev)
+    s, index = torch.rand(60, 8, device=dev), torch.randint(0, 8, (60, 2), device=dev)
+    cu = torch.tensor([0, 20, 60], dtype=torch.int32, device=dev)
+
+    def call(q, k, v, x, s):
+        return ((packed.packed_attention(q, k, v, cu) * g).float().sum() + token_logprobs(x, y).sum()
+                + preference_loss(x * 2, y, cu, torch.zeros(2, device=dev))[0] + balance_loss(s, index, 1.0, cu)[0])
+    leaves = [t.clone().requires_grad_() for t in (q, k, k.flip(0), x, s)]
+    want = torch.autograd.grad(call(*leaves), leaves)
+    got = torch.autograd.grad(checkpoint(call, *leaves, use_reentrant=False), leaves)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
