@@ -180,11 +180,13 @@ class PackedBatch:
     are formed here, so other bounds need another batch (in a captured graph: formed inside it)."""
 
     def __init__(self, cu_seqlens: torch.Tensor, rows: int):
-        self.cu_seqlens = _bounds("cu_seqlens", cu_seqlens, None, cu_seqlens.device)
+        cu = _bounds("cu_seqlens", cu_seqlens, None, cu_seqlens.device)
         self.rows = int(rows)
+        # from row 0, within the rows, not decreasing: no place formed of them lies outside a tensor
+        self.cu_seqlens = torch.cat([cu.new_zeros(1), cu[1:].clamp(0, self.rows)]).cummax(0).values
         self.lengths: Optional[list] = None  # of the sequences, where the host knows
         self.longest: Optional[int] = None
-        r = torch.arange(self.rows, dtype=torch.int32, device=cu_seqlens.device)
+        r = torch.arange(self.rows, dtype=torch.int32, device=cu.device)
         self.sequence = torch.searchsorted(self.cu_seqlens[1:], r, right=True)  # n behind the last
         self.positions = (r - self.cu_seqlens[self.sequence]).long()
 
@@ -220,9 +222,7 @@ class PackedBatch:
         """The sum of t [rows] over each sequence, [n], in 64 bits and in the same order on every
         run.  Each by itself: differences of one running sum would carry a value that is not
         finite into every later sequence."""
-        at = self.cu_seqlens.long().clamp(0, self.rows)  # as the kernels take the bounds
-        at = torch.cat([at.new_zeros(1), at[1:]]).cummax(0).values
-        return torch.segment_reduce(t.double(), "sum", offsets=at, initial=0.0, unsafe=True)
+        return torch.segment_reduce(t.double(), "sum", offsets=self.cu_seqlens.long(), initial=0.0, unsafe=True)
 
 
 class PackedCache:

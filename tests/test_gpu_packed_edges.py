@@ -545,3 +545,38 @@ def test_recomputed_in_the_backward_pass(dev, dtype):
     want = torch.autograd.grad(call(*leaves), leaves)
     got = torch.autograd.grad(checkpoint(call, *leaves, use_reentrant=False), leaves)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_batch_formed_inside_a_graph(dev):
+    """A captured call takes other lengths on its next replay where its batch is formed inside:
+    forward, losses and the cache's places, also of bounds that make no sense."""
+    m = _model(dev).eval()
+    cache = PackedCache(m.config, 3, 120, BF, dev)
+    ids = torch.randint(0, 500, (1, 90), device=dev)
+    cu = torch.tensor([0, 30, 60, 90], dtype=torch.int32, device=dev)
+
+    def call():
+        b = PackedBatch(cu, 90)
+        out = m(ids, packed=b, labels=ids)
+        cache.clear()
+        kept = m(ids, packed=b, past_key_values=cache).logits
+        return out.logits, out.loss, m.sequence_logprobs(ids, ids, b), kept, cache.lengths.clone()
+    with torch.inference_mode():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            res = call()
+        for ends in ([0, 1, 2, 90], [0, 0, 45, 80], [0, 30, 60, 90], [7, 50, 20, 300], [0, -9, 2 ** 31 - 1, 5]):
+            cu.copy_(torch.tensor(ends, dtype=torch.int32))
+            want = call()
+            graph.replay()
+            torch.cuda.synchronize()
+            used = min(max(ends[-1], 0), 90) if ends[1:] == sorted(ends[1:]) else 0
+            for a, w in zip(res, want):
+                a, w = (t[:, :used] if t.dim() == 3 else t for t in (a, w))  # rows of no sequence: anything
+                assert torch.equal(a.nan_to_num(), w.nan_to_num()), ends

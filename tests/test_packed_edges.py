@@ -357,3 +357,32 @@ def test_library_refuses_what_a_launch_cannot_hold():
     assert lib.mhc_packed_attn_workspace_bytes(1 << 20, 1 << 20, 1 << 20, 8, 4, 64) >= 0
     assert lib.mhc_packed_attn_bwd_workspace_bytes(1 << 20, 1 << 20, 1 << 20, 8, 4, 64) > 0
     assert lib.mhc_balance_workspace_bytes(1 << 20, 64, 1 << 20) > 0
+
+
+# ------------------------------------------------- bounds that make no sense, and the cache
+
+@pytest.mark.parametrize("ends", [(9, 9, 9), (3, 5, 8), (0, 150, 20), (-5, 500, 2 ** 31 - 1), (0, -2 ** 31, 8), (0, 6, 2)])
+def test_cache_under_bounds_that_make_no_sense(ends):
+    """They are taken as the kernels take them: no row lands outside its slots, no length leaves
+    them, and the next call is right."""
+    m = _model().eval()
+    cache = PackedCache(m.config, 2, 10, torch.float32, "cpu")
+    ids = torch.randint(0, 50, (1, 8))
+    with torch.no_grad():
+        for _ in range(3):
+            m(ids, packed=PackedBatch(_ints(*ends), 8), past_key_values=cache)
+            assert 0 <= int(cache.lengths.min()) and int(cache.lengths.max()) <= 10
+        m(ids, packed=PackedBatch(_ints(*ends), 8), labels=ids)
+        cache.clear()
+        out = m(ids, packed=PackedBatch.from_lengths([5, 3], device="cpu"), past_key_values=cache).logits[0]
+        torch.testing.assert_close(out[:5], m(ids[:, :5]).logits[0], rtol=1e-4, atol=1e-4)
+    assert cache.lengths.tolist() == [5, 3]
+
+
+def test_batch_takes_bounds_as_the_kernels_do():
+    b = PackedBatch(_ints(3, 5, 500), 8)
+    assert b.cu_seqlens.tolist() == [0, 5, 8] and b.positions.tolist() == [0, 1, 2, 3, 4, 0, 1, 2]
+    cu = _ints(0, 2, 4)
+    b = PackedBatch(cu, 4)
+    cu.fill_(1)  # a batch keeps its own
+    assert b.cu_seqlens.tolist() == [0, 2, 4]
