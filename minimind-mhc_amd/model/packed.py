@@ -233,24 +233,34 @@ class PackedCache:
     decode step can be replayed).  Tokens that a slot has no room for are not stored, and
     their sequence's outputs mean nothing from then on; a batch made from_lengths is refused
     before that, as far as the host has seen the slots fill up.  Rows of no sequence change
-    nothing.  dtype may differ from the model's: 16-bit slots are read by the kernels, under any
+    nothing.  `lengths` may be set from outside, to free a slot or roll it back.  dtype may differ from the model's: 16-bit slots are read by the kernels, under any
     autocast."""
 
     def __init__(self, config, sequences: int, capacity: int, dtype=torch.bfloat16, device="cuda"):
         if sequences < 1 or capacity < 1:
             raise ValueError(f"mhc_amd: a cache of {sequences} slots of {capacity} rows")
         shape = (sequences * capacity + 1, config.num_key_value_heads, config.head_dim)  # the last: what is dropped
-        self.layers = [tuple(torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
-                       for _ in range(config.num_hidden_layers)]
-        self.slots = torch.arange(sequences + 1, dtype=torch.int32, device=device) * capacity
-        self.lengths = torch.zeros(sequences, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):  # ordinary tensors: a cache outlives the mode it is made in
+            self.layers = [tuple(torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
+                           for _ in range(config.num_hidden_layers)]
+            self.slots = torch.arange(sequences + 1, dtype=torch.int32, device=device) * capacity
+            self.lengths = torch.zeros(sequences, dtype=torch.int32, device=device)
         self.sequences, self.capacity = sequences, capacity
-        self._seen = [0] * sequences  # the slots' lengths, as far as the host has seen them
+        self._count()
 
     def clear(self) -> None:
         """Empties every slot."""
         self.lengths.zero_()
-        self._seen = [0] * self.sequences
+        self._count()
+
+    def _count(self, seen: Optional[list] = None) -> None:
+        """The slots' lengths as far as the host has seen them, of the tensor as it stands now."""
+        self._seen, self._of = seen or [0] * self.sequences, self.lengths._version
+
+    def seen(self) -> list:
+        if self._of != self.lengths._version:  # set from outside since
+            self._count()
+        return self._seen
 
 
 class PackedCall:
@@ -271,12 +281,13 @@ class PackedCall:
         if len(batch) != n:
             raise ValueError(f"mhc_amd: a batch of {len(batch)} sequences on a cache of {n}")
         if batch.lengths is not None:
-            have, more = max(cache._seen), batch.longest
+            seen = cache.seen()
+            have, more = max(seen), batch.longest
             if slots and have + more > cap:
-                have, more = max(zip(cache._seen, batch.lengths), key=sum)
+                have, more = max(zip(seen, batch.lengths), key=sum)
             if have + more > cap:
                 raise ValueError(f"mhc_amd: {have} + {more} tokens may not fit slots of {cap} rows")
-            self.reach = max((a + b for a, b in zip(cache._seen, batch.lengths) if b), default=0)
+            self.reach = max((a + b for a, b in zip(seen, batch.lengths) if b), default=0)
         self.most = cap
         seq = batch.sequence.clamp_max(n - 1)
         self.positions = cache.lengths[seq] + batch.positions
@@ -289,10 +300,12 @@ class PackedCall:
         the call was only captured)."""
         if self.cache is None:
             return
+        seen = self.cache.seen()
         self.cache.lengths.copy_(self.lengths)
         if self.batch.lengths is not None and not (
                 self.lengths.is_cuda and torch.cuda.is_current_stream_capturing()):
-            self.cache._seen = [a + b for a, b in zip(self.cache._seen, self.batch.lengths)]
+            seen = [a + b for a, b in zip(seen, self.batch.lengths)]
+        self.cache._count(seen)
 
     def attention(self, q, k, v, layer: int, dropout: float = 0.0) -> torch.Tensor:
         """q [1, rows, heads, head_dim], k, v [1, rows, kv heads, head_dim] of the new tokens:

@@ -386,3 +386,39 @@ def test_batch_takes_bounds_as_the_kernels_do():
     b = PackedBatch(cu, 4)
     cu.fill_(1)  # a batch keeps its own
     assert b.cu_seqlens.tolist() == [0, 2, 4]
+
+
+def test_slots_that_are_freed_or_rolled_back():
+    """lengths may be set from outside: what the host has counted no longer refuses anything."""
+    m = _model().eval()
+    cache = PackedCache(m.config, 2, 10, torch.float32, "cpu")
+    ids = torch.randint(0, 50, (1, 9))
+    with torch.no_grad():
+        m(ids, packed=PackedBatch.from_lengths([8, 1], device="cpu"), past_key_values=cache)
+        cache.lengths[0] = 0  # another conversation takes the slot
+        out = m(ids, packed=PackedBatch.from_lengths([9, 0], device="cpu"), past_key_values=cache).logits[0]
+        torch.testing.assert_close(out, m(ids).logits[0], rtol=1e-4, atol=1e-4)
+        assert cache.lengths.tolist() == [9, 1]
+        for _ in range(12):  # the last token of both, again and again
+            m(ids[:, :2], packed=PackedBatch.from_lengths([1, 1], device="cpu"), past_key_values=cache)
+            cache.lengths.sub_(1)
+        assert cache.lengths.tolist() == [9, 1]
+        m(ids[:, :2], packed=PackedBatch.from_lengths([1, 1], device="cpu"), past_key_values=cache)
+        m(ids[:, :8], packed=PackedBatch.from_lengths([0, 8], device="cpu"), past_key_values=cache)
+        with pytest.raises(ValueError, match="10 rows"):  # counted anew since then: 1 and 1 + 8, and 9 more
+            m(ids, packed=PackedBatch.from_lengths([0, 9], device="cpu"), past_key_values=cache)
+
+
+def test_cache_made_in_inference_mode():
+    """Is a cache as any other: used outside, and its lengths set from outside."""
+    m = _model().eval()
+    ids = torch.randint(0, 50, (1, 9))
+    b = PackedBatch.from_lengths([8, 1], device="cpu")
+    with torch.inference_mode():
+        cache = PackedCache(m.config, 2, 10, torch.float32, "cpu")
+        for _ in range(3):
+            m(ids, packed=b, past_key_values=cache)
+            cache.lengths.zero_()
+    with torch.no_grad():
+        m(ids, packed=b, past_key_values=cache)
+    assert cache.lengths.tolist() == [8, 1]
