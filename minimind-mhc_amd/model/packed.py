@@ -182,13 +182,14 @@ class PackedBatch:
     def __init__(self, cu_seqlens: torch.Tensor, rows: int):
         cu = _bounds("cu_seqlens", cu_seqlens, None, cu_seqlens.device)
         self.rows = int(rows)
-        # from row 0, within the rows, not decreasing: no place formed of them lies outside a tensor
-        self.cu_seqlens = torch.cat([cu.new_zeros(1), cu[1:].clamp(0, self.rows)]).cummax(0).values
         self.lengths: Optional[list] = None  # of the sequences, where the host knows
         self.longest: Optional[int] = None
-        r = torch.arange(self.rows, dtype=torch.int32, device=cu.device)
-        self.sequence = torch.searchsorted(self.cu_seqlens[1:], r, right=True)  # n behind the last
-        self.positions = (r - self.cu_seqlens[self.sequence]).long()
+        with torch.inference_mode(False):  # ordinary tensors: a batch outlives the mode it is made in
+            # from row 0, within the rows, not decreasing: no place formed of them lies outside a tensor
+            r = torch.arange(self.rows, dtype=torch.int32, device=cu.device)
+            self.cu_seqlens = torch.cat([r.new_zeros(1), cu[1:].clamp(0, self.rows)]).cummax(0).values
+            self.sequence = torch.searchsorted(self.cu_seqlens[1:], r, right=True)  # n behind the last
+            self.positions = (r - self.cu_seqlens[self.sequence]).long()
 
     @classmethod
     def from_lengths(cls, lengths, rows: Optional[int] = None, device="cuda") -> "PackedBatch":

@@ -580,3 +580,15 @@ def test_batch_formed_inside_a_graph(dev):
             for a, w in zip(res, want):
                 a, w = (t[:, :used] if t.dim() == 3 else t for t in (a, w))  # rows of no sequence: anything
                 assert torch.equal(a.nan_to_num(), w.nan_to_num()), ends
+
+
+@pytest.mark.gpu
+def test_batch_made_in_inference_mode(dev):
+    """Serves a training step afterwards: the reference model's pass comes first."""
+    m = _model(dev, use_moe=True, num_experts_per_tok=2, use_mhc=0, router_aux_loss_per_sequence=True).train()
+    ids = torch.randint(0, 500, (1, 160), device=dev)
+    with torch.inference_mode():
+        b = PackedBatch.from_lengths([50, 30, 10, 70], device=dev)
+        ref = m.sequence_logprobs(ids, ids, b)
+    m.preference_loss(ids, ids, b, ref).loss.backward()
+    m(ids, packed=b, labels=ids).loss.backward()

@@ -422,3 +422,16 @@ def test_cache_made_in_inference_mode():
     with torch.no_grad():
         m(ids, packed=b, past_key_values=cache)
     assert cache.lengths.tolist() == [8, 1]
+
+
+def test_batch_made_in_inference_mode():
+    """Serves a training step afterwards: the reference model's pass comes first."""
+    m = _model(use_moe=True, num_experts_per_tok=2).train()
+    ids = torch.randint(0, 50, (1, 16))
+    with torch.inference_mode():
+        b = PackedBatch.from_lengths([5, 3, 1, 7], device="cpu")
+        c = PackedBatch(_ints(0, 5, 8, 9, 16), 16)
+        ref = m.sequence_logprobs(ids, ids, b)
+    for batch in (b, c):
+        m.preference_loss(ids, ids, batch, ref).loss.backward()
+        m(ids, packed=batch, labels=ids).loss.backward()
