@@ -625,7 +625,7 @@ int mhc_preference_bwd(const void* logits, int64_t stride, int dtype, const int6
                        const float* g_loss, void* g_logits, int64_t T, int V, int P,
                        hipStream_t stream);
 
-/* Balance loss of a router over T tokens, E <= 4096 experts: scores [T, E],
+/* Balance loss of a router over T tokens, E <= 4096 experts (B E <= 2^30): scores [T, E],
  * index [T, K] (int64, contiguous) the experts of each token (others than 0 .. E -
  * 1 are not counted).  loss (one element) = coef E sum_e (count_e / T) mean_e.  cu (NULL, or
  * [B + 1]): the mean of the losses of B sequences, over those with rows.  counts [B, E]

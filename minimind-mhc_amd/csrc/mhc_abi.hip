@@ -912,7 +912,7 @@ int mhc_preference_bwd(const void* logits, int64_t stride, int dtype, const int6
 }
 
 static int check_balance(int64_t T, int E, int B, const char* fn) {
-  if (T < 0 || T > 1 << 30 || E < 1 || E > mhc::kBalanceMaxExperts || B < 0 || (int64_t)B * E > kMaxBlocks ||
+  if (T < 0 || T > 1 << 30 || E < 1 || E > mhc::kBalanceMaxExperts || B < 0 || (int64_t)B * E > 1 << 30 ||
       T * E / 256 >= kMaxBlocks)
     return fail(hipErrorInvalidValue, "%s: bad shape (T=%lld E=%d B=%d)", fn, (long long)T, E, B);
   return check_threads((int64_t)B * mhc::balance_parts(T, B) * 256, fn);

@@ -435,3 +435,11 @@ def test_batch_made_in_inference_mode():
     for batch in (b, c):
         m.preference_loss(ids, ids, batch, ref).loss.backward()
         m(ids, packed=batch, labels=ids).loss.backward()
+
+
+def test_library_refuses_more_experts_and_sequences_than_are_joined():
+    """2^31 less 128 pairs of them: the join counts in 32 bits, some past the last."""
+    from model import _hip
+    lib = _hip.load()
+    assert lib.mhc_balance_workspace_bytes(4, 128, (1 << 24) - 1) == -1
+    assert lib.mhc_balance_workspace_bytes(4, 64, 1 << 23) > 0
