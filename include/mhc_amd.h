@@ -589,6 +589,85 @@ int mhc_packed_attn_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, c
                         void* g_k, void* g_v, void* workspace, int64_t workspace_bytes, int B, int64_t Tq, int64_t Tk, int heads, int kv_heads,
                         int head_dim, int dtype, float scale, hipStream_t stream);
 
+/* -------------------------------------------------------- rotary positions
+ * Pairs (a, b) of a head's first rotary_dim elements, half layout (d, d +
+ * rotary_dim / 2), interleaved (flags 1) (2 d, 2 d + 1): a' = a c - b s, b' =
+ * b c + a s; flags 2: the transposed map, which gradients take.  Elements behind
+ * rotary_dim (even, at most head_dim) stay.  cos, sin: table_rows rows (a position each,
+ * table_stride elements apart) of rotary_dim / 2 values, fp32, bf16 or fp16; the pairs of a
+ * row whose position lies outside them are NaN.
+ */
+
+/* q [T, heads, head_dim], k [T, kv_heads, head_dim] (fp32, bf16 or fp16; either may have 0
+ * heads) at the given strides to contiguous q_out, k_out; positions [T] int32 or int64
+ * (positions_bytes). */
+int mhc_rotary(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+               int64_t k_stride_t, int64_t k_stride_h, const void* cos, const void* sin,
+               int64_t table_stride, int64_t table_rows, int table_dtype, const void* positions,
+               int positions_bytes, void* q_out, void* k_out, int64_t T, int heads, int kv_heads,
+               int head_dim, int rotary_dim, int flags, int dtype, hipStream_t stream);
+
+/* ---------------------------------------------------------- cache of pages
+ * Key x of sequence i lies in page page_table[i, x / page] (int32 [B, width]), row x % page; a
+ * page has a power of two of 16 to 2^20 rows, a sequence at most width * page <= 2^30 keys.  cu [B + 1]:
+ * sequence i has the new rows cu[i] .. cu[i + 1], the first entry taken as 0; lengths [B]: the keys
+ * before them, behind which those of the new rows stand.  All are device data: bounds and lengths are
+ * clamped, keys of a page number outside 0 .. pages - 1 are not there.  Strides of pages, rows and heads
+ * are in elements, multiples of 8, those of rows under 2^23.  16-bit tensors of one dtype, T <= 2^30.
+ */
+
+/* Stores k and v of the new rows and rotates q: with gains ([head_dim], fp32, bf16 or fp16; either may be NULL)
+ * after a per-head RMSNorm, positions lengths + depths [T] (NULL: lengths + place in the sequence).  q_out contiguous; rows
+ * of no sequence get zeros there and are not stored, nor are rows without a page. */
+int mhc_paged_append(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+                     int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
+                     int64_t v_stride_h, const void* q_gain, const void* k_gain, int gain_dtype,
+                     float eps, const void* cos, const void* sin, int64_t table_stride,
+                     int64_t table_rows, int table_dtype, const int* cu, const int* lengths,
+                     const int* depths, const int* page_table, void* q_out, void* k_pages,
+                     int64_t kp_stride_p, int64_t kp_stride_t, int64_t kp_stride_h, void* v_pages,
+                     int64_t vp_stride_p, int64_t vp_stride_t, int64_t vp_stride_h, int64_t T, int B,
+                     int heads, int kv_heads, int head_dim, int rotary_dim, int width, int pages,
+                     int page, int flags, int dtype, hipStream_t stream);
+
+/* Bytes of workspace mhc_paged_attn_fwd needs (0: none), or -1 for a shape it does not take. */
+int64_t mhc_paged_attn_workspace_bytes(int B, int64_t Tq, int heads, int kv_heads, int head_dim);
+
+/* out [Tq, heads, head_dim] (contiguous) = softmax(scale q k^T) v, scale > 0, head_dim 64, 96 or 128.  A
+ * row sees the lengths[i] keys before, and of its sequence's new rows those up to itself or, with tree [Tq,
+ * tree_words], those whose bit is set (row j: bit j % 64 of word j / 64).  Rows that see no key, and
+ * rows of no sequence, come out 0. */
+int mhc_paged_attn_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_pages,
+                       int64_t kp_stride_p, int64_t kp_stride_t, int64_t kp_stride_h,
+                       const void* v_pages, int64_t vp_stride_p, int64_t vp_stride_t,
+                       int64_t vp_stride_h, const int* page_table, const int* lengths, const int* cu,
+                       const int64_t* tree, int tree_words, void* out, void* workspace,
+                       int64_t workspace_bytes, int B, int64_t Tq, int heads, int kv_heads,
+                       int head_dim, int width, int pages, int page, int dtype, float scale,
+                       hipStream_t stream);
+
+/* Keys lengths + path[cu + j] move to lengths + j, j < kept [B], in each of `planes` arrays of pages
+ * ([pages, page, row_bytes], plane_bytes apart; sizes in multiples of 16); path entries below j, or no row of the
+ * sequence, move nothing.  new_lengths [B] = lengths + kept, at most width * page. */
+int mhc_paged_keep(void* planes_at, const int* page_table, const int* lengths, const int* cu,
+                   const int* kept, const int* path, int* new_lengths, int64_t T, int B, int planes,
+                   int64_t plane_bytes, int64_t row_bytes, int width, int pages, int page,
+                   hipStream_t stream);
+
+/* ---------------------------------------------------------- drafted tokens
+ * Rows cu[i] .. cu[i + 1] of sequence i are a tree: its first row its last token, the others drafted,
+ * parents [T] (places in the sequence, before the row's own; NULL: the row before).  probs [T, V]: the target's
+ * probabilities after each row; draft_probs [T, V] of one dtype with it, or NULL: those that a row's children were drawn
+ * from.  At a node, a = 0, c = 1, its children in turn (token x, uniform u): accepted if u q(x) c < max(p(x) - a
+ * q(x), 0), else a += c, c = sum max(p - a q, 0).  Without draft_probs: if u c < p(x), else c -= p(x), p(x) = 0.
+ * Without uniforms [T]: if x is the first of the largest p.  kept [B]: rows accepted, the first among them; path [T]:
+ * their places, then -1; next [B]: the first token whose cumulated remaining p exceeds the first row's uniform
+ * times the total (of p itself where nothing remains), or the first of the largest; -1 where there is none.
+ * Probabilities that are not positive finite numbers count as 0. */
+int mhc_verify_drafts(const void* probs, const void* draft_probs, int dtype, const int64_t* tokens,
+                      const int* parents, const float* uniforms, const int* cu, int* kept, int* path,
+                      int64_t* next, int64_t T, int V, int B, hipStream_t stream);
+
 /* ------------------------------------------------------------------- losses
  * Logits and scores are fp32, bf16 or fp16; sums and log-probabilities fp32 or
  * wider.  Row strides are in elements; rows may begin at any element.

@@ -3,6 +3,7 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <initializer_list>
 #include <mutex>
 
 #include "mhc_amd.h"
@@ -839,6 +840,181 @@ int mhc_packed_attn_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, c
   a.out = const_cast<void*>(out); a.rest = const_cast<void*>(rest); a.lse = const_cast<float*>(lse); a.g_out = g_out;
   a.g_q = g_q; a.g_k = g_k; a.g_v = g_v;
   return hip_status(mhc::launch_packed_attn_bwd(a, stream), fn);
+}
+
+// ------------------------------------------- rotary positions, cache of pages
+
+static int check_rotary(const mhc::RotaryArgs& a, const char* fn) {
+  if (a.T < 0 || a.T > 1 << 30 || a.heads < 0 || a.kv_heads < 0 || a.heads > 1 << 20 || a.kv_heads > 1 << 20 || a.hd < 1 ||
+      a.hd > 1 << 20 || (int64_t)a.T * (a.heads + a.kv_heads) * a.hd > int64_t(1) << 40)
+    return fail(hipErrorInvalidValue, "%s: bad shape (T=%lld heads=%d kv_heads=%d head_dim=%d)", fn, (long long)a.T, a.heads, a.kv_heads, a.hd);
+  if (a.rd < 0 || a.rd % 2 != 0 || a.rd > a.hd)
+    return fail(hipErrorInvalidValue, "%s: rotary_dim must be even and at most head_dim (got %d)", fn, a.rd);
+  if (!dtype_ok(a.dtype) || !dtype_ok(a.table_dtype)) return fail(hipErrorInvalidValue, "%s: bad dtype %d or %d", fn, a.dtype, a.table_dtype);
+  if (a.table_stride < 0 || a.table_rows < 0) return fail(hipErrorInvalidValue, "%s: bad tables", fn);
+  if (a.T > 0 && a.rd > 0 && a.table_rows > 0 && (!a.cos || !a.sin)) return fail(hipErrorInvalidValue, "%s: null tables", fn);
+  return 0;
+}
+
+int mhc_rotary(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t, int64_t k_stride_h,
+               const void* cos, const void* sin, int64_t table_stride, int64_t table_rows, int table_dtype,
+               const void* positions, int positions_bytes, void* q_out, void* k_out, int64_t T, int heads, int kv_heads,
+               int head_dim, int rotary_dim, int flags, int dtype, hipStream_t stream) {
+  const char* fn = "mhc_rotary";
+  mhc::RotaryArgs a{};
+  a.x[0] = q; a.xs_t[0] = q_stride_t; a.xs_h[0] = q_stride_h; a.y[0] = q_out;
+  a.x[1] = k; a.xs_t[1] = k_stride_t; a.xs_h[1] = k_stride_h; a.y[1] = k_out;
+  a.cos = cos; a.sin = sin; a.table_stride = table_stride; a.table_rows = table_rows; a.table_dtype = table_dtype;
+  a.positions = positions; a.wide_positions = positions_bytes == 8;
+  a.T = T; a.heads = heads; a.kv_heads = kv_heads; a.hd = head_dim; a.rd = rotary_dim; a.dtype = dtype;
+  a.interleaved = flags & 1; a.back = flags & 2;
+  if (int rc = check_rotary(a, fn)) return rc;
+  if (positions_bytes != 4 && positions_bytes != 8) return fail(hipErrorInvalidValue, "%s: positions of %d bytes", fn, positions_bytes);
+  if (T == 0 || heads + kv_heads == 0) return 0;
+  if ((heads > 0 && (!q || !q_out)) || (kv_heads > 0 && (!k || !k_out)) || !positions)
+    return fail(hipErrorInvalidValue, "%s: null pointer", fn);
+  return hip_status(mhc::launch_rotary(a, false, stream), fn);
+}
+
+// Shared checks of the entry points on pages; gives the shift of the page size.
+static int check_pages(int64_t T, int B, int width, int pages, int page, int* shift, const char* fn) {
+  if (T < 0 || T > 1 << 30 || B < 0 || width < 0 || pages < 0)
+    return fail(hipErrorInvalidValue, "%s: bad shape (T=%lld B=%d width=%d pages=%d)", fn, (long long)T, B, width, pages);
+  if (page < 16 || page > 1 << 20 || (page & (page - 1)) != 0)
+    return fail(hipErrorInvalidValue, "%s: a page must have a power of two of 16 to 2^20 rows (got %d)", fn, page);
+  if ((int64_t)width * page > 1 << 30) return fail(hipErrorInvalidValue, "%s: at most 2^30 keys a sequence", fn);
+  *shift = __builtin_ctz((unsigned)page);
+  return 0;
+}
+static int check_page_strides(std::initializer_list<int64_t> all, std::initializer_list<int64_t> rows, const char* fn) {
+  for (int64_t st : all)
+    if (st < 0 || st % 8 != 0) return fail(hipErrorInvalidValue, "%s: strides must be multiples of 8 elements", fn);
+  for (int64_t st : rows)
+    if (st >= 1 << 23) return fail(hipErrorInvalidValue, "%s: rows must be under 2^23 elements apart", fn);
+  return 0;
+}
+
+int mhc_paged_append(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
+                     int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h, const void* q_gain,
+                     const void* k_gain, int gain_dtype, float eps, const void* cos, const void* sin, int64_t table_stride,
+                     int64_t table_rows, int table_dtype, const int* cu, const int* lengths, const int* depths,
+                     const int* page_table, void* q_out, void* k_pages, int64_t kp_stride_p, int64_t kp_stride_t,
+                     int64_t kp_stride_h, void* v_pages, int64_t vp_stride_p, int64_t vp_stride_t, int64_t vp_stride_h,
+                     int64_t T, int B, int heads, int kv_heads, int head_dim, int rotary_dim, int width, int pages, int page,
+                     int flags, int dtype, hipStream_t stream) {
+  const char* fn = "mhc_paged_append";
+  mhc::RotaryArgs a{};
+  a.x[0] = q; a.xs_t[0] = q_stride_t; a.xs_h[0] = q_stride_h; a.y[0] = q_out;
+  a.x[1] = k; a.xs_t[1] = k_stride_t; a.xs_h[1] = k_stride_h; a.y[1] = k_pages;
+  a.x[2] = v; a.xs_t[2] = v_stride_t; a.xs_h[2] = v_stride_h; a.y[2] = v_pages;
+  a.ys_p[1] = kp_stride_p; a.ys_t[1] = kp_stride_t; a.ys_h[1] = kp_stride_h;
+  a.ys_p[2] = vp_stride_p; a.ys_t[2] = vp_stride_t; a.ys_h[2] = vp_stride_h;
+  a.cos = cos; a.sin = sin; a.table_stride = table_stride; a.table_rows = table_rows; a.table_dtype = table_dtype;
+  a.q_gain = q_gain; a.k_gain = k_gain; a.gain_dtype = gain_dtype; a.eps = eps;
+  a.cu = cu; a.lengths = lengths; a.depths = depths; a.page_table = page_table;
+  a.T = T; a.heads = heads; a.kv_heads = kv_heads; a.hd = head_dim; a.rd = rotary_dim; a.dtype = dtype;
+  a.B = B; a.width = width; a.pages = pages;
+  a.interleaved = flags & 1;
+  if (int rc = check_rotary(a, fn)) return rc;
+  if (int rc = check_pages(T, B, width, pages, page, &a.page_shift, fn)) return rc;
+  if (heads < 1 || kv_heads < 1) return fail(hipErrorInvalidValue, "%s: bad shape (heads=%d kv_heads=%d)", fn, heads, kv_heads);
+  if (dtype == mhc::kF32) return fail(hipErrorInvalidValue, "%s: dtype must be bf16 or fp16 (got %d)", fn, dtype);
+  if ((q_gain || k_gain) && !dtype_ok(gain_dtype)) return fail(hipErrorInvalidValue, "%s: bad gain dtype %d", fn, gain_dtype);
+  if (int rc = check_page_strides({kp_stride_p, kp_stride_t, kp_stride_h, vp_stride_p, vp_stride_t, vp_stride_h},
+                                  {kp_stride_t, vp_stride_t}, fn)) return rc;
+  if (T == 0) return 0;
+  if (!q || !k || !v || !q_out || !cu || (B > 0 && (!lengths || (width > 0 && !page_table))) ||
+      (pages > 0 && (!k_pages || !v_pages)))
+    return fail(hipErrorInvalidValue, "%s: null pointer", fn);
+  return hip_status(mhc::launch_rotary(a, true, stream), fn);
+}
+
+static int check_paged(const mhc::PagedAttnArgs& a, int64_t Tq, int dtype, const char* fn) {
+  if (int rc = check_attn(Tq, a.heads, a.kv_heads, a.head_dim, dtype, fn)) return rc;
+  if (!(a.scale > 0.f) || a.scale > 3e38f) return fail(hipErrorInvalidValue, "%s: scale must be positive (got %g)", fn, (double)a.scale);
+  if ((Tq + a.B + 2) * a.heads > kMaxBlocks) return fail(hipErrorInvalidValue, "%s: too large", fn);
+  return 0;
+}
+
+int64_t mhc_paged_attn_workspace_bytes(int B, int64_t Tq, int heads, int kv_heads, int head_dim) {
+  const char* fn = "mhc_paged_attn_workspace_bytes";
+  mhc::PagedAttnArgs a{};
+  a.B = B; a.Tq = (int)Tq; a.heads = heads; a.kv_heads = kv_heads; a.head_dim = head_dim; a.scale = 1.f;
+  if (B < 0 || Tq < 0 || Tq > 1 << 30 || check_paged(a, Tq, mhc::kBF16, fn)) return -1;
+  if (Tq == 0) return 0;
+  mhc::paged_attn_plan(a);
+  if (check_threads(mhc::paged_attn_threads(a), fn)) return -1;
+  return mhc::paged_attn_workspace(a);
+}
+
+int mhc_paged_attn_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_pages, int64_t kp_stride_p,
+                       int64_t kp_stride_t, int64_t kp_stride_h, const void* v_pages, int64_t vp_stride_p,
+                       int64_t vp_stride_t, int64_t vp_stride_h, const int* page_table, const int* lengths, const int* cu,
+                       const int64_t* tree, int tree_words, void* out, void* workspace, int64_t workspace_bytes, int B,
+                       int64_t Tq, int heads, int kv_heads, int head_dim, int width, int pages, int page, int dtype,
+                       float scale, hipStream_t stream) {
+  const char* fn = "mhc_paged_attn_fwd";
+  mhc::PagedAttnArgs a{};
+  a.q = q; a.qs_t = q_stride_t; a.qs_h = q_stride_h;
+  a.k = k_pages; a.ks_p = kp_stride_p; a.ks_t = kp_stride_t; a.ks_h = kp_stride_h;
+  a.v = v_pages; a.vs_p = vp_stride_p; a.vs_t = vp_stride_t; a.vs_h = vp_stride_h;
+  a.page_table = page_table; a.lengths = lengths; a.cu = cu;
+  a.tree = reinterpret_cast<const uint64_t*>(tree); a.words = tree_words;
+  a.B = B; a.heads = heads; a.kv_heads = kv_heads; a.head_dim = head_dim; a.width = width; a.pages = pages;
+  a.f16 = dtype == mhc::kF16; a.scale = scale;
+  if (int rc = check_pages(Tq, B, width, pages, page, &a.page_shift, fn)) return rc;
+  a.Tq = (int)Tq;
+  if (int rc = check_paged(a, Tq, dtype, fn)) return rc;
+  if (int rc = check_page_strides({q_stride_t, q_stride_h, kp_stride_p, kp_stride_t, kp_stride_h, vp_stride_p, vp_stride_t, vp_stride_h},
+                                  {q_stride_t, kp_stride_t, vp_stride_t}, fn)) return rc;
+  if (tree && (tree_words < 1 || tree_words > 1 << 24)) return fail(hipErrorInvalidValue, "%s: a tree of %d words a row", fn, tree_words);
+  if (Tq == 0) return 0;
+  if (!q || !out || !aligned16(q) || !aligned16(out) || !cu || (B > 0 && (!lengths || (width > 0 && !page_table))) ||
+      (pages > 0 && (!k_pages || !v_pages || !aligned16(k_pages) || !aligned16(v_pages))))
+    return fail(hipErrorInvalidValue, "%s: null or unaligned pointer", fn);
+  mhc::paged_attn_plan(a);
+  if (int rc = check_threads(mhc::paged_attn_threads(a), fn)) return rc;
+  const int64_t need = mhc::paged_attn_workspace(a);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(hipErrorInvalidValue, "%s: workspace of %lld bytes needed (got %lld)", fn, (long long)need, (long long)workspace_bytes);
+  a.out = out; a.work = static_cast<float*>(workspace);
+  return hip_status(mhc::launch_paged_attn(a, stream), fn);
+}
+
+int mhc_paged_keep(void* planes_at, const int* page_table, const int* lengths, const int* cu, const int* kept, const int* path,
+                   int* new_lengths, int64_t T, int B, int planes, int64_t plane_bytes, int64_t row_bytes, int width, int pages,
+                   int page, hipStream_t stream) {
+  const char* fn = "mhc_paged_keep";
+  mhc::KeepArgs a{};
+  if (int rc = check_pages(T, B, width, pages, page, &a.page_shift, fn)) return rc;
+  if (planes < 0 || row_bytes < 16 || row_bytes % 16 != 0 || row_bytes > 1 << 24 || plane_bytes < 0 || plane_bytes % 16 != 0)
+    return fail(hipErrorInvalidValue, "%s: rows of %lld bytes, planes of %lld: multiples of 16", fn, (long long)row_bytes, (long long)plane_bytes);
+  if (B == 0) return 0;
+  if ((planes > 0 && pages > 0 && (!planes_at || !aligned16(planes_at))) || !lengths || !cu || !kept || (T > 0 && !path) ||
+      !new_lengths || (width > 0 && !page_table))
+    return fail(hipErrorInvalidValue, "%s: null or unaligned pointer", fn);
+  a.pages_at = planes_at; a.page_table = page_table; a.lengths = lengths; a.cu = cu; a.kept = kept; a.path = path;
+  a.new_lengths = new_lengths; a.plane_bytes = plane_bytes; a.row_bytes = row_bytes;
+  a.planes = planes; a.row16 = (int)(row_bytes / 16); a.B = B; a.T = (int)T; a.width = width; a.pages = pages;
+  if (int rc = check_threads(((int64_t)planes * a.row16 + 256), fn)) return rc;
+  return hip_status(mhc::launch_keep(a, stream), fn);
+}
+
+int mhc_verify_drafts(const void* probs, const void* draft_probs, int dtype, const int64_t* tokens, const int* parents,
+                      const float* uniforms, const int* cu, int* kept, int* path, int64_t* next, int64_t T, int V, int B,
+                      hipStream_t stream) {
+  const char* fn = "mhc_verify_drafts";
+  if (T < 0 || T > 1 << 30 || V < 1 || V > 1 << 30 || B < 0 || B > 1 << 22)
+    return fail(hipErrorInvalidValue, "%s: bad shape (T=%lld V=%d B=%d)", fn, (long long)T, V, B);
+  if (!dtype_ok(dtype)) return fail(hipErrorInvalidValue, "%s: bad dtype %d", fn, dtype);
+  if (draft_probs && !uniforms) return fail(hipErrorInvalidValue, "%s: draft probabilities without random numbers", fn);
+  if (B == 0) return 0;
+  if ((T > 0 && (!probs || !tokens || !path)) || !cu || !kept || !next || !aligned16(probs) || !aligned16(draft_probs))
+    return fail(hipErrorInvalidValue, "%s: null or unaligned pointer", fn);
+  mhc::VerifyArgs a{};
+  a.probs = probs; a.draft = draft_probs; a.tokens = tokens; a.parents = parents; a.uniforms = uniforms; a.cu = cu;
+  a.kept = kept; a.path = path; a.next = next; a.T = T; a.V = V; a.B = B; a.dtype = dtype;
+  return hip_status(mhc::launch_verify(a, stream), fn);
 }
 
 // ------------------------------------------------------------------- losses

@@ -337,6 +337,96 @@ int64_t packed_bwd_threads(const PackedAttnArgs& a);
 int64_t packed_bwd_workspace(PackedAttnArgs& a, float* workspace);
 hipError_t launch_packed_attn_bwd(const PackedAttnArgs& a, hipStream_t s);
 
+// Rotary positions of q [T, heads, hd] and k [T, kv_heads, hd] (x[0], x[1]; rows and heads at the
+// given element strides) to contiguous y[0], y[1]; with `append` k and v (x[2]) go to the rows of
+// a cache of pages (y[1], y[2]) instead.  cos, sin: `table_rows` rows of rd / 2 angles.
+constexpr int kRotaryRows = 32;  // of a workgroup, at most
+struct RotaryArgs {
+  const void* x[3];
+  void* y[3];
+  int64_t xs_t[3], xs_h[3];
+  const void* cos;
+  const void* sin;
+  int64_t table_stride, table_rows;
+  int table_dtype;
+  bool table_wide;        // launch_rotary: the tables' rows lie on 16 bytes
+  const void* positions;  // [T] int32 or (wide_positions) int64; append: none
+  bool wide_positions;
+  int64_t T;
+  int heads, kv_heads, hd, rd, dtype;
+  bool interleaved, back;
+  int rows;               // launch_rotary: of a workgroup
+  // append
+  const void* q_gain;     // [hd] each, or null
+  const void* k_gain;
+  int gain_dtype;
+  float eps;
+  const int* cu;          // [B + 1]
+  const int* lengths;     // [B] keys before the new rows
+  const int* depths;      // [T] rows' positions behind those, or null: as they stand
+  const int* page_table;  // [B, width]
+  int64_t ys_p[3], ys_t[3], ys_h[3];
+  int B, width, pages, page_shift;
+  __host__ __device__ int x_heads(int which) const { return which == 0 ? heads : kv_heads; }
+};
+hipError_t launch_rotary(RotaryArgs a, bool append, hipStream_t s);
+
+// Drafted tokens of B sequences (T rows) against the target's probabilities [T, V].
+struct VerifyArgs {
+  const void* probs;
+  const void* draft;        // [T, V], or null: certain drafts
+  const int64_t* tokens;    // [T]
+  const int* parents;       // [T], or null: chains
+  const float* uniforms;    // [T], or null: greedy
+  const int* cu;            // [B + 1]
+  int* kept;                // [B]
+  int* path;                // [T]
+  int64_t* next;            // [B]
+  int64_t T;
+  int V, B, dtype;
+};
+hipError_t launch_verify(const VerifyArgs& a, hipStream_t s);
+
+// Moves the keys of accepted rows within the pages of every plane.
+struct KeepArgs {
+  void* pages_at;           // [planes, pages, page, row_bytes]
+  const int* page_table;    // [B, width]
+  const int* lengths;       // [B]
+  const int* cu;            // [B + 1]
+  const int* kept;          // [B]
+  const int* path;          // [T]
+  int* new_lengths;         // [B]
+  int64_t plane_bytes, row_bytes;
+  int planes, row16, B, T, width, pages, page_shift, seqs_line;
+};
+hipError_t launch_keep(KeepArgs a, hipStream_t s);
+
+// Attention over a cache of pages: q, out [Tq, heads, head_dim]; k, v rows at the given element
+// strides of a page, of a row in it and of a head.  tree [Tq, words]: bits of the sequence's new
+// rows that each row sees (null: causal).
+struct PagedAttnArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  const int* page_table;   // [B, width]
+  const int* lengths;      // [B] keys before the new rows
+  const int* cu;           // [B + 1]
+  const uint64_t* tree;
+  void* out;               // contiguous
+  float* work;
+  int64_t qs_t, qs_h, ks_p, ks_t, ks_h, vs_p, vs_t, vs_h;
+  int B, Tq, heads, kv_heads, head_dim, width, pages, page_shift, words;
+  bool f16;
+  float scale;
+  // paged_attn_plan: rows of a workgroup; workgroups of a kv head that the keys are spread
+  // over (0: one a tile of rows), key tiles of a range at least, and the launch's units
+  int block_rows, slots, least, units;
+};
+void paged_attn_plan(PagedAttnArgs& a);
+int64_t paged_attn_workspace(const PagedAttnArgs& a);
+int64_t paged_attn_threads(const PagedAttnArgs& a);
+hipError_t launch_paged_attn(const PagedAttnArgs& a, hipStream_t s);
+
 // Log-probabilities of labels under rows of logits [T, V] (rows `stride` elements apart).
 struct LogitArgs {
   const void* logits;

@@ -121,6 +121,25 @@ _SIGNATURES = {
                                  _P, _P, _P, _P, _P, _P, _P,      # cu_q, cu_k, key_lengths, out, rest, lse, g_out
                                  _P, _P, _P, _P, _I64,            # g_q, g_k, g_v, workspace, bytes
                                  _I, _I64, _I64, _I, _I, _I, _I, _F, _P]),
+    "mhc_rotary": (_I, [_P, _I64, _I64, _P, _I64, _I64,       # q, k and their strides
+                        _P, _P, _I64, _I64, _I, _P, _I,       # cos, sin, stride, rows, dtype, positions, bytes
+                        _P, _P, _I64, _I, _I, _I, _I, _I, _I, _P]),
+    "mhc_paged_append": (_I, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64,  # q, k, v and their strides
+                              _P, _P, _I, _F,                 # gains, dtype, eps
+                              _P, _P, _I64, _I64, _I,         # cos, sin, stride, rows, dtype
+                              _P, _P, _P, _P, _P,             # cu, lengths, depths, page_table, q_out
+                              _P, _I64, _I64, _I64, _P, _I64, _I64, _I64,      # k_pages, v_pages and their strides
+                              _I64, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
+    "mhc_paged_attn_workspace_bytes": (_I64, [_I, _I64, _I, _I, _I]),
+    "mhc_paged_attn_fwd": (_I, [_P, _I64, _I64,               # q and its strides
+                                _P, _I64, _I64, _I64, _P, _I64, _I64, _I64,    # k_pages, v_pages and their strides
+                                _P, _P, _P, _P, _I,           # page_table, lengths, cu, tree, words
+                                _P, _P, _I64,                 # out, workspace, bytes
+                                _I, _I64, _I, _I, _I, _I, _I, _I, _I, _F, _P]),
+    "mhc_paged_keep": (_I, [_P, _P, _P, _P, _P, _P, _P,       # planes, page_table, lengths, cu, kept, path, new
+                            _I64, _I, _I, _I64, _I64, _I, _I, _I, _P]),
+    "mhc_verify_drafts": (_I, [_P, _P, _I, _P, _P, _P, _P,    # probs, draft, dtype, tokens, parents, uniforms, cu
+                               _P, _P, _P, _I64, _I, _I, _P]),
     "mhc_logprobs_fwd": (_I, [_P, _I64, _I, _P, _I64, _P, _P, _I64, _I, _P]),
     "mhc_logprobs_bwd": (_I, [_P, _I64, _I, _P, _I64, _P, _P, _P, _I64, _I, _P]),
     "mhc_preference_fwd": (_I, [_P, _P, _I64, _P, _P,             # logprobs, labels, ignore, cu, reference

@@ -1,0 +1,96 @@
+"""Verification of drafted tokens against a target model's probabilities.
+
+No reference counterpart: the reference decodes a token at a time
+(eval_llm.py, trainer/train_grpo.py).
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _hip as H
+from . import _ops
+from .packed import _bounds
+
+_TYPES = (torch.float32, *_ops.HALF)
+
+
+def _row_ints(name: str, t: torch.Tensor, rows: int, dtype: torch.dtype) -> torch.Tensor:
+    if t.dtype != dtype:
+        raise TypeError(f"mhc_amd: {name} must be {dtype}, got {t.dtype}")
+    if tuple(t.shape) != (rows,):
+        raise ValueError(f"mhc_amd: {name} must be [{rows}], got {tuple(t.shape)}")
+    return t.contiguous()
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """t in order and on 16 bytes, as the kernel reads it."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def verify_drafts(probs: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.Tensor,
+                  parents: Optional[torch.Tensor] = None, draft_probs: Optional[torch.Tensor] = None,
+                  uniforms: Optional[torch.Tensor] = None):
+    """(kept [n] int32, path [rows] int32, next [n] int64) of n packed sequences' drafts.
+
+    Sequence i has the rows cu_seqlens[i] to cu_seqlens[i + 1] (int32, beginning with row 0): its
+    last token first, then its drafted ones, a tree.  tokens [rows] int64.
+    parents [rows] int32: the place in its sequence of the token that a row follows, before its
+    own (the first row's does not count, any other without such a parent is never accepted); None:
+    each follows the one before it.
+    probs [rows, V] fp32, bf16 or fp16: the target's probabilities after each row's token (greedy:
+    logits will do).  draft_probs [rows, V]: those a row's children were drawn from, independently;
+    None: the drafts were certain (siblings then differ, as a draft's most probable tokens do).
+    uniforms [rows] in [0, 1): random numbers, one a drafted row and, in the first row, one for the
+    next token; None: greedy.
+
+    Sampled, kept rows and next token together are distributed as the target's own samples: at a
+    node, with target p and draft q, a = 0 and c = 1, its children in turn (token x, number u) are
+    accepted if u q(x) c < max(p(x) - a q(x), 0), else a += c and c = sum max(p - a q, 0); where none
+    is left, next is the first token whose cumulated max(p - a q, 0) exceeds the first row's number
+    times the total.  Certain drafts: accepted if u c < p(x), else c -= p(x), and x is out.  Greedy:
+    accepted if x is the first of the most probable tokens.  In 64 bits; probabilities that are not
+    positive finite numbers count as 0; where nothing is left next comes from p itself, and is -1
+    where p has nothing either.
+
+    kept: accepted rows of each sequence with the first one (0 without rows); path: their places
+    in the sequence, in order, then -1.  Rows behind the last sequence keep -1.  Not differentiable.
+    """
+    dev = H.require_device(probs, tokens, parents, draft_probs, uniforms)
+    if probs.dim() != 2 or probs.shape[1] < 1:
+        raise ValueError(f"mhc_amd: probs must be [rows, V], got {tuple(probs.shape)}")
+    T, V = probs.shape
+    for name, t in (("probs", probs), ("draft_probs", draft_probs)):
+        if t is not None and t.dtype not in _TYPES:
+            raise TypeError(f"mhc_amd: {name} must be fp32, bf16 or fp16, got {t.dtype}")
+    if draft_probs is not None:
+        if draft_probs.shape != probs.shape:
+            raise ValueError(f"mhc_amd: draft_probs {tuple(draft_probs.shape)} and probs {tuple(probs.shape)} differ")
+        if uniforms is None:
+            raise ValueError("mhc_amd: draft_probs need uniforms")
+    tokens = _row_ints("tokens", tokens, T, torch.int64)
+    if parents is not None:
+        parents = _row_ints("parents", parents, T, torch.int32)
+    if uniforms is not None:
+        if not uniforms.is_floating_point() or tuple(uniforms.shape) != (T,):
+            raise ValueError(f"mhc_amd: uniforms must be [{T}] floating point, got {tuple(uniforms.shape)} {uniforms.dtype}")
+        uniforms = uniforms.detach().to(torch.float32).contiguous()
+    cu = _bounds("cu_seqlens", cu_seqlens, None, dev)
+    probs, n = probs.detach(), cu.numel() - 1
+    if draft_probs is not None:
+        draft_probs = draft_probs.detach()
+        if draft_probs.dtype != probs.dtype:
+            probs, draft_probs = probs.float(), draft_probs.float()
+        draft_probs = _aligned(draft_probs)
+    probs = _aligned(probs)
+    kept = torch.empty(n, dtype=torch.int32, device=dev)
+    path = torch.empty(T, dtype=torch.int32, device=dev) if n else torch.full((T,), -1, dtype=torch.int32, device=dev)
+    following = torch.empty(n, dtype=torch.int64, device=dev)
+    with _ops.launch_device(probs):
+        H.check(H.load().mhc_verify_drafts(
+            probs.data_ptr(), H.ptr(draft_probs), H.dtype_tag(probs), tokens.data_ptr(), H.ptr(parents), H.ptr(uniforms),
+            cu.data_ptr(), kept.data_ptr(), path.data_ptr(), following.data_ptr(), T, V, n, H.stream(dev)),
+            "mhc_verify_drafts")
+    return kept, path, following
