@@ -613,7 +613,7 @@ int mhc_rotary(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void
  * sequence i has the new rows cu[i] .. cu[i + 1], the first entry taken as 0; lengths [B]: the keys
  * before them, behind which those of the new rows stand.  All are device data: bounds and lengths are
  * clamped, keys of a page number outside 0 .. pages - 1 are not there.  Strides of pages, rows and heads
- * are in elements, multiples of 8, those of rows under 2^23.  16-bit tensors of one dtype, T <= 2^30.
+ * (the same in k_pages and v_pages) are in elements, multiples of 8, those of rows under 2^23.  16-bit tensors of one dtype, T <= 2^30.
  */
 
 /* Stores k and v of the new rows and rotates q: with gains ([head_dim], fp32, bf16 or fp16; either may be NULL)
@@ -624,10 +624,8 @@ int mhc_paged_append(const void* q, int64_t q_stride_t, int64_t q_stride_h, cons
                      int64_t v_stride_h, const void* q_gain, const void* k_gain, int gain_dtype,
                      float eps, const void* cos, const void* sin, int64_t table_stride,
                      int64_t table_rows, int table_dtype, const int* cu, const int* lengths,
-                     const int* depths, const int* page_table, void* q_out, void* k_pages,
-                     int64_t kp_stride_p, int64_t kp_stride_t, int64_t kp_stride_h, void* v_pages,
-                     int64_t vp_stride_p, int64_t vp_stride_t, int64_t vp_stride_h, int64_t T, int B,
-                     int heads, int kv_heads, int head_dim, int rotary_dim, int width, int pages,
+                     const int* depths, const int* page_table, void* q_out, void* k_pages, void* v_pages,
+                     int64_t stride_p, int64_t stride_t, int64_t stride_h, int64_t T, int B, int heads, int kv_heads, int head_dim, int rotary_dim, int width, int pages,
                      int page, int flags, int dtype, hipStream_t stream);
 
 /* Bytes of workspace mhc_paged_attn_fwd needs (0: none), or -1 for a shape it does not take. */
@@ -638,9 +636,8 @@ int64_t mhc_paged_attn_workspace_bytes(int B, int64_t Tq, int heads, int kv_head
  * tree_words], those whose bit is set (row j: bit j % 64 of word j / 64).  Rows that see no key, and
  * rows of no sequence, come out 0. */
 int mhc_paged_attn_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_pages,
-                       int64_t kp_stride_p, int64_t kp_stride_t, int64_t kp_stride_h,
-                       const void* v_pages, int64_t vp_stride_p, int64_t vp_stride_t,
-                       int64_t vp_stride_h, const int* page_table, const int* lengths, const int* cu,
+                       const void* v_pages, int64_t stride_p, int64_t stride_t, int64_t stride_h,
+                       const int* page_table, const int* lengths, const int* cu,
                        const int64_t* tree, int tree_words, void* out, void* workspace,
                        int64_t workspace_bytes, int B, int64_t Tq, int heads, int kv_heads,
                        int head_dim, int width, int pages, int page, int dtype, float scale,

@@ -898,17 +898,15 @@ int mhc_paged_append(const void* q, int64_t q_stride_t, int64_t q_stride_h, cons
                      int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h, const void* q_gain,
                      const void* k_gain, int gain_dtype, float eps, const void* cos, const void* sin, int64_t table_stride,
                      int64_t table_rows, int table_dtype, const int* cu, const int* lengths, const int* depths,
-                     const int* page_table, void* q_out, void* k_pages, int64_t kp_stride_p, int64_t kp_stride_t,
-                     int64_t kp_stride_h, void* v_pages, int64_t vp_stride_p, int64_t vp_stride_t, int64_t vp_stride_h,
-                     int64_t T, int B, int heads, int kv_heads, int head_dim, int rotary_dim, int width, int pages, int page,
+                     const int* page_table, void* q_out, void* k_pages, void* v_pages, int64_t stride_p, int64_t stride_t,
+                     int64_t stride_h, int64_t T, int B, int heads, int kv_heads, int head_dim, int rotary_dim, int width, int pages, int page,
                      int flags, int dtype, hipStream_t stream) {
   const char* fn = "mhc_paged_append";
   mhc::RotaryArgs a{};
   a.x[0] = q; a.xs_t[0] = q_stride_t; a.xs_h[0] = q_stride_h; a.y[0] = q_out;
   a.x[1] = k; a.xs_t[1] = k_stride_t; a.xs_h[1] = k_stride_h; a.y[1] = k_pages;
   a.x[2] = v; a.xs_t[2] = v_stride_t; a.xs_h[2] = v_stride_h; a.y[2] = v_pages;
-  a.ys_p[1] = kp_stride_p; a.ys_t[1] = kp_stride_t; a.ys_h[1] = kp_stride_h;
-  a.ys_p[2] = vp_stride_p; a.ys_t[2] = vp_stride_t; a.ys_h[2] = vp_stride_h;
+  a.ys_p = stride_p; a.ys_t = stride_t; a.ys_h = stride_h;
   a.cos = cos; a.sin = sin; a.table_stride = table_stride; a.table_rows = table_rows; a.table_dtype = table_dtype;
   a.q_gain = q_gain; a.k_gain = k_gain; a.gain_dtype = gain_dtype; a.eps = eps;
   a.cu = cu; a.lengths = lengths; a.depths = depths; a.page_table = page_table;
@@ -920,8 +918,7 @@ int mhc_paged_append(const void* q, int64_t q_stride_t, int64_t q_stride_h, cons
   if (heads < 1 || kv_heads < 1) return fail(hipErrorInvalidValue, "%s: bad shape (heads=%d kv_heads=%d)", fn, heads, kv_heads);
   if (dtype == mhc::kF32) return fail(hipErrorInvalidValue, "%s: dtype must be bf16 or fp16 (got %d)", fn, dtype);
   if ((q_gain || k_gain) && !dtype_ok(gain_dtype)) return fail(hipErrorInvalidValue, "%s: bad gain dtype %d", fn, gain_dtype);
-  if (int rc = check_page_strides({kp_stride_p, kp_stride_t, kp_stride_h, vp_stride_p, vp_stride_t, vp_stride_h},
-                                  {kp_stride_t, vp_stride_t}, fn)) return rc;
+  if (int rc = check_page_strides({stride_p, stride_t, stride_h}, {stride_t}, fn)) return rc;
   if (T == 0) return 0;
   if (!q || !k || !v || !q_out || !cu || (B > 0 && (!lengths || (width > 0 && !page_table))) ||
       (pages > 0 && (!k_pages || !v_pages)))
@@ -947,17 +944,15 @@ int64_t mhc_paged_attn_workspace_bytes(int B, int64_t Tq, int heads, int kv_head
   return mhc::paged_attn_workspace(a);
 }
 
-int mhc_paged_attn_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_pages, int64_t kp_stride_p,
-                       int64_t kp_stride_t, int64_t kp_stride_h, const void* v_pages, int64_t vp_stride_p,
-                       int64_t vp_stride_t, int64_t vp_stride_h, const int* page_table, const int* lengths, const int* cu,
+int mhc_paged_attn_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_pages, const void* v_pages,
+                       int64_t stride_p, int64_t stride_t, int64_t stride_h, const int* page_table, const int* lengths, const int* cu,
                        const int64_t* tree, int tree_words, void* out, void* workspace, int64_t workspace_bytes, int B,
                        int64_t Tq, int heads, int kv_heads, int head_dim, int width, int pages, int page, int dtype,
                        float scale, hipStream_t stream) {
   const char* fn = "mhc_paged_attn_fwd";
   mhc::PagedAttnArgs a{};
   a.q = q; a.qs_t = q_stride_t; a.qs_h = q_stride_h;
-  a.k = k_pages; a.ks_p = kp_stride_p; a.ks_t = kp_stride_t; a.ks_h = kp_stride_h;
-  a.v = v_pages; a.vs_p = vp_stride_p; a.vs_t = vp_stride_t; a.vs_h = vp_stride_h;
+  a.k = k_pages; a.v = v_pages; a.s_p = stride_p; a.s_t = stride_t; a.s_h = stride_h;
   a.page_table = page_table; a.lengths = lengths; a.cu = cu;
   a.tree = reinterpret_cast<const uint64_t*>(tree); a.words = tree_words;
   a.B = B; a.heads = heads; a.kv_heads = kv_heads; a.head_dim = head_dim; a.width = width; a.pages = pages;
@@ -965,8 +960,7 @@ int mhc_paged_attn_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, co
   if (int rc = check_pages(Tq, B, width, pages, page, &a.page_shift, fn)) return rc;
   a.Tq = (int)Tq;
   if (int rc = check_paged(a, Tq, dtype, fn)) return rc;
-  if (int rc = check_page_strides({q_stride_t, q_stride_h, kp_stride_p, kp_stride_t, kp_stride_h, vp_stride_p, vp_stride_t, vp_stride_h},
-                                  {q_stride_t, kp_stride_t, vp_stride_t}, fn)) return rc;
+  if (int rc = check_page_strides({q_stride_t, q_stride_h, stride_p, stride_t, stride_h}, {q_stride_t, stride_t}, fn)) return rc;
   if (tree && (tree_words < 1 || tree_words > 1 << 24)) return fail(hipErrorInvalidValue, "%s: a tree of %d words a row", fn, tree_words);
   if (Tq == 0) return 0;
   if (!q || !out || !aligned16(q) || !aligned16(out) || !cu || (B > 0 && (!lengths || (width > 0 && !page_table))) ||

@@ -365,7 +365,7 @@ struct RotaryArgs {
   const int* lengths;     // [B] keys before the new rows
   const int* depths;      // [T] rows' positions behind those, or null: as they stand
   const int* page_table;  // [B, width]
-  int64_t ys_p[3], ys_t[3], ys_h[3];
+  int64_t ys_p, ys_t, ys_h;
   int B, width, pages, page_shift;
   __host__ __device__ int x_heads(int which) const { return which == 0 ? heads : kv_heads; }
 };
@@ -402,7 +402,7 @@ struct KeepArgs {
 hipError_t launch_keep(KeepArgs a, hipStream_t s);
 
 // Attention over a cache of pages: q, out [Tq, heads, head_dim]; k, v rows at the given element
-// strides of a page, of a row in it and of a head.  tree [Tq, words]: bits of the sequence's new
+// strides of a page, of a row in it and of a head (the same in both).  tree [Tq, words]: bits of the sequence's new
 // rows that each row sees (null: causal).
 struct PagedAttnArgs {
   const void* q;
@@ -414,13 +414,13 @@ struct PagedAttnArgs {
   const uint64_t* tree;
   void* out;               // contiguous
   float* work;
-  int64_t qs_t, qs_h, ks_p, ks_t, ks_h, vs_p, vs_t, vs_h;
+  int64_t qs_t, qs_h, s_p, s_t, s_h;
   int B, Tq, heads, kv_heads, head_dim, width, pages, page_shift, words;
   bool f16;
   float scale;
-  // paged_attn_plan: rows of a workgroup; workgroups of a kv head that the keys are spread
-  // over (0: one a tile of rows), key tiles of a range at least, and the launch's units
-  int block_rows, slots, least, units;
+  // paged_attn_plan: rows of a workgroup, waves that share its keys; workgroups of a kv head that the
+  // keys are spread over (0: one a block of rows), key tiles of a range at least, and the launch's units
+  int block_rows, key_waves, slots, least, units;
 };
 void paged_attn_plan(PagedAttnArgs& a);
 int64_t paged_attn_workspace(const PagedAttnArgs& a);

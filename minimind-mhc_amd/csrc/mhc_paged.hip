@@ -16,7 +16,7 @@ constexpr int kPagedSeqs = 256;  // up to so many, workgroups are dealt out by t
 // sequence, over part `split` of `splits` of the keys they see.
 struct PagedUnit {
   int seq, start, n, past, len;
-  int first, split, splits;
+  int first, split, splits, blocks;
 };
 struct PagedSeq {
   int start, n, past, len;
@@ -47,12 +47,16 @@ __device__ __forceinline__ double wave_total(double v) {
 
 // Unit number w of a kv head.  The keys of all sequences, times their blocks of rows, are cut
 // into about a.slots ranges of the same length; a sequence shorter than one is one unit a block.
-// Behind the sequences' units come those that clear the rows behind the last one (seq = B).
-// `row` >= 0: instead the first unit of the block with that row (of Tq), w is set to it.
+// The blocks of one range are neighbours.  Behind the sequences' units come those that clear the
+// rows behind the last one (seq = B).  Workgroup `at` of XCD `xcd` takes the at-th of an eighth of
+// the units: neighbours, which read the same keys, share its L2.
+// `row` >= 0: instead the first range's unit of the block with that row (of Tq), and the distance
+// to the next range's.
 template <int KT>
-__device__ __forceinline__ bool paged_find(const PagedAttnArgs& a, int& w, PagedUnit& u, int row) {
+__device__ __forceinline__ bool paged_find(const PagedAttnArgs& a, int xcd, int at_xcd, int& w, PagedUnit& u, int row) {
   const int lane = __lane_id(), rep = a.heads / a.kv_heads, RB = a.block_rows;
   if (a.B > kPagedSeqs) {  // sequence i has the unit numbers from start(i) rep / RB + i on
+    w = at_xcd * 8 + xcd;
     int lo = 0, hi = a.B + 1;
     while (hi - lo > 1) {
       const int step = (hi - lo - 1 + 63) / 64;
@@ -65,7 +69,7 @@ __device__ __forceinline__ bool paged_find(const PagedAttnArgs& a, int& w, Paged
     const bool in = lo < a.B;
     const int first = seq_start(a.cu, lo, a.Tq);
     const PagedSeq q = paged_seq(a, lo, first, in ? a.cu[lo + 1] : a.Tq, in ? a.lengths[lo] : 0);
-    u = PagedUnit{lo, q.start, q.n, q.past, q.len, 0, 0, 1};
+    u = PagedUnit{lo, q.start, q.n, q.past, q.len, 0, 0, 1, 1};
     const int64_t at = (w - ((int64_t)first * rep / RB + lo)) * RB;
     if (at < 0 || at >= (int64_t)q.n * rep) return false;
     u.first = (int)at;
@@ -73,7 +77,7 @@ __device__ __forceinline__ bool paged_find(const PagedAttnArgs& a, int& w, Paged
   }
   constexpr int C = kPagedSeqs / 64;
   PagedSeq q[C];
-  int blocks[C], units[C];
+  int blocks[C];
   double work = 0.0;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
@@ -88,18 +92,35 @@ __device__ __forceinline__ bool paged_find(const PagedAttnArgs& a, int& w, Paged
     }
   }
   int per = INT32_MAX;
-  if (a.slots > 0) per = max((int)fmin(wave_total(work) / a.slots, 1e9) + 1, a.least);
-  int before = 0;
+  if (a.slots > 0) {  // a block's last range is half one on average
+    int all = 0;
+#pragma unroll
+    for (int c = 0; c < C; ++c) all += blocks[c];
+    const double want = fmax(a.slots - 0.5 * wave_total(all), 0.5 * a.slots);
+    per = max((int)fmin(wave_total(work) / want, 1e9) + 1, a.least);
+  }
+  int splits[C], inc[C], all = 0;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    splits[c] = inc[c] = 0;
+    if (c * 64 < a.B) {
+      const int nt = (q[c].len + KT - 1) / KT;
+      splits[c] = nt > per ? (nt + per - 1) / per : 1;
+      inc[c] = all + wave_scan(blocks[c] * splits[c]);
+      all = __builtin_amdgcn_readlane(inc[c], 63);
+    }
+  }
+  const int end = seq_start(a.cu, a.B, a.Tq);
+  if (row < 0) {  // with the units of the rows behind the last sequence
+    const int eighth = (all + (int)(((int64_t)(a.Tq - end) * rep + RB - 1) / RB) + 7) / 8;
+    if (at_xcd >= eighth) return false;
+    w = xcd * eighth + at_xcd;
+  }
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     if (c * 64 >= a.B) break;
-    const int nt = (q[c].len + KT - 1) / KT;
-    const int splits = nt > per ? (nt + per - 1) / per : 1;
-    units[c] = blocks[c] * splits;
-    const int inc = wave_scan(units[c]);
-    bool mine;
-    if (row >= 0) mine = q[c].n > 0 && row >= q[c].start && row < q[c].start + q[c].n;
-    else mine = before + inc > w && before + inc - units[c] <= w;
+    const int first = inc[c] - blocks[c] * splits[c];
+    const bool mine = row >= 0 ? q[c].n > 0 && row >= q[c].start && row < q[c].start + q[c].n : first <= w && w < inc[c];
     const uint64_t who = __ballot(mine);
     if (who) {
       const int l = __ffsll((unsigned long long)who) - 1;
@@ -108,26 +129,25 @@ __device__ __forceinline__ bool paged_find(const PagedAttnArgs& a, int& w, Paged
       u.n = __builtin_amdgcn_readlane(q[c].n, l);
       u.past = __builtin_amdgcn_readlane(q[c].past, l);
       u.len = __builtin_amdgcn_readlane(q[c].len, l);
-      u.splits = __builtin_amdgcn_readlane(splits, l);
-      const int base = before + __builtin_amdgcn_readlane(inc - units[c], l);
+      u.splits = __builtin_amdgcn_readlane(splits[c], l);
+      u.blocks = __builtin_amdgcn_readlane(blocks[c], l);
+      const int base = __builtin_amdgcn_readlane(first, l);
       if (row >= 0) {
         u.split = 0;
         u.first = (row - u.start) * rep / RB * RB;
-        w = base + u.first / RB * u.splits;
+        w = base + u.first / RB;
       } else {
-        u.split = (w - base) % u.splits;
-        u.first = (w - base) / u.splits * RB;
+        u.split = (w - base) / u.blocks;
+        u.first = (w - base) % u.blocks * RB;
       }
       return true;
     }
-    before += __builtin_amdgcn_readlane(inc, 63);
   }
   if (row >= 0) return false;
   // the rows behind the last sequence
-  const int end = seq_start(a.cu, a.B, a.Tq);
-  const int64_t at = (int64_t)(w - before) * RB;
-  u = PagedUnit{a.B, end, a.Tq - end, 0, 0, 0, 0, 1};
-  if (at >= (int64_t)u.n * rep) return false;
+  const int64_t at = (int64_t)(w - all) * RB;
+  u = PagedUnit{a.B, end, a.Tq - end, 0, 0, 0, 0, 1, 1};
+  if (at < 0 || at >= (int64_t)u.n * rep) return false;
   u.first = (int)at;
   return true;
 }
@@ -138,17 +158,24 @@ __device__ __forceinline__ int scalar_int(const int* p) {
 }
 
 // A workgroup takes 16 U RW rows (tokens times the query heads of one kv head) over a range of the
-// keys.  RW waves share the tiles of KT keys, 16 U rows each; KW such groups take every KW-th
-// tile, and join in LDS at the end.  Tiles come by direct-to-LDS loads: a wave loads whole groups
-// of 16 keys, which lie in one page, so a page number is one scalar read a group.
+// keys.  RW waves share the tiles of KT keys, 16 U rows each; or (RW = 1) KW waves with the same rows
+// take every KW-th tile, each with a ring of its own and no barrier, and join in LDS at the end.
+// Tiles come by direct-to-LDS loads: a wave loads whole groups of 16 keys, which lie in one page, so
+// a page number is one scalar read a group.  No wave leaves a step early: with a way out, for tiles
+// that none of a wave's rows sees, the compiler spilled 56 registers at head_dim 128 (64 tokens over
+// 65001 keys, 16 / 2 heads: 117 us instead of 51).
+template <int HD, int RW, int KW, int S>
+constexpr int paged_waves =  // of a SIMD, as the tiles' LDS lets in: two at most
+    160 * 1024 / (KW * S * 4 * (RW == 1 ? 32 : 64) * HD) * RW * KW >= 8 ? 2 : 1;
 template <bool F16, int HD, int RW, int KW, int U, int S>
-__global__ __launch_bounds__(64 * RW * KW, RW == 4 ? 2 : 1) void paged_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(64 * RW * KW, (paged_waves<HD, RW, KW, S>)) void paged_kernel(PagedAttnArgs a) {
   constexpr int KT = RW == 1 ? 32 : 64;
   constexpr int NC = HD / 32, ND = HD / 16, NT = KT / 16, NH = KT / 32;
   constexpr int GW = NT / RW;               // groups of 16 keys that a wave loads of a tile
   constexpr int UG = HD / 32;               // 1 KiB units of a group
   constexpr int TILE = KT * HD;             // elements
   constexpr int WAVES = RW * KW, RB = 16 * U * RW;
+  static_assert(RW == 1 || KW == 1, "waves that share a tile take the same steps");
   __shared__ __align__(16) uint16_t lds[KW][S][2][TILE];
   static_assert(KW == 1 || sizeof(lds) >= WAVES * 16 * U * (HD + 2) * 4, "the waves' sums take the tiles' place");
   const int tid = threadIdx.x, lane = tid & 63;
@@ -160,9 +187,10 @@ __global__ __launch_bounds__(64 * RW * KW, RW == 4 ? 2 : 1) void paged_kernel(Pa
   // workgroups are dealt to the 8 XCDs in turn
   const int in = blockIdx.x % (8 * a.kv_heads);
   const int kvh = in / 8;
-  int w = blockIdx.x / (8 * a.kv_heads) * 8 + in % 8;
+  int w = 0;
   PagedUnit t;
-  if (w >= a.units || !paged_find<KT>(a, w, t, -1)) return;
+  if (!paged_find<KT>(a, in % 8, blockIdx.x / (8 * a.kv_heads), w, t, -1) || w >= a.units) return;
+  for (int* x : {&t.seq, &t.start, &t.n, &t.past, &t.len, &t.first, &t.split, &t.splits, &w}) *x = __builtin_amdgcn_readfirstlane(*x);
   const int rows = t.n * rep;
   const int last_token = (min(t.first + RB, rows) - 1) / rep;
   const bool causal = a.tree == nullptr;
@@ -170,66 +198,7 @@ __global__ __launch_bounds__(64 * RW * KW, RW == 4 ? 2 : 1) void paged_kernel(Pa
   const int nt_all = (seen + KT - 1) / KT;
   const int per = (nt_all + t.splits - 1) / t.splits;
   const int t0 = min(t.split * per, nt_all), t1 = min(t0 + per, nt_all);
-  const int steps = (t1 - t0 + KW - 1) / KW;
-
-  // ---- loading
-  const int* table = a.page_table + (int64_t)min(t.seq, a.B - 1) * a.width;
-  const int mask = (1 << a.page_shift) - 1;
-  const uint16_t* kg = static_cast<const uint16_t*>(a.k) + kvh * a.ks_h;
-  const uint16_t* vg = static_cast<const uint16_t*>(a.v) + kvh * a.vs_h;
-  uint32_t koff[GW * UG], voff[GW * UG];
-#pragma unroll
-  for (int i = 0; i < GW * UG; ++i) {
-    const int at = ((rw * GW) * UG + i) * 64 + lane, row = at / (HD / 8), col = tile_column<HD>(row, at % (HD / 8)) * 8;
-    koff[i] = (uint32_t)((row & 15) * a.ks_t + col) * 2;
-    voff[i] = (uint32_t)((row & 15) * a.vs_t + col) * 2;
-  }
-  const int last_group = (max(seen, 1) - 1) & ~15;
-  int page[NT];  // of the next tile to load
-  auto look = [&](int i) {
-    const int kt = min(t0 + i * KW + kw, t1 - 1);
-#pragma unroll
-    for (int x = 0; x < NT; ++x) page[x] = scalar_int(table + (min(kt * KT + 16 * x, last_group) >> a.page_shift));
-  };
-  uint64_t bad = 0;  // groups in no page, four bits a stage
-  auto issue = [&](int i, int stage, uint16_t* __restrict__ kd, uint16_t* __restrict__ vd) {
-    const int kt = min(t0 + i * KW + kw, t1 - 1);
-    uint32_t none = 0;
-#pragma unroll
-    for (int x = 0; x < NT; ++x) none |= (unsigned)page[x] >= (unsigned)a.pages ? 1u << x : 0u;
-    bad = (bad & ~(15ull << (4 * stage))) | ((uint64_t)none << (4 * stage));
-#pragma unroll
-    for (int y = 0; y < GW; ++y) {
-      const int x = rw * GW + y;
-      int p = page[0];
-#pragma unroll
-      for (int z = 1; z < NT; ++z)
-        if (x == z) p = page[z];
-      if ((unsigned)p >= (unsigned)a.pages) p = 0;
-      const int row = min(kt * KT + 16 * x, last_group) & mask;
-      const char* kp = reinterpret_cast<const char*>(kg + p * a.ks_p + row * a.ks_t);
-      const char* vp = reinterpret_cast<const char*>(vg + p * a.vs_p + row * a.vs_t);
-#pragma unroll
-      for (int i2 = 0; i2 < UG; ++i2) {
-        const int at = x * UG + i2;
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kp + koff[y * UG + i2]),
-                                         (__attribute__((address_space(3))) void*)(reinterpret_cast<char*>(kd) + at * 1024), 16, 0, 0);
-      }
-#pragma unroll
-      for (int i2 = 0; i2 < UG; ++i2) {
-        const int at = x * UG + i2;
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vp + voff[y * UG + i2]),
-                                         (__attribute__((address_space(3))) void*)(reinterpret_cast<char*>(vd) + at * 1024), 16, 0, 0);
-      }
-    }
-    if (i + 1 < steps) look(i + 1);
-  };
-  if (steps > 0) {
-    look(0);
-#pragma unroll
-    for (int i = 0; i < S - 1; ++i)
-      if (i < steps) issue(i, i, lds[kw][i][0], lds[kw][i][1]);
-  }
+  const int steps = max((t1 - t0 - kw + KW - 1) / KW, 0);  // of this wave
 
   // ---- rows
   U32x4 qb[U][NC];
@@ -244,9 +213,74 @@ __global__ __launch_bounds__(64 * RW * KW, RW == 4 ? 2 : 1) void paged_kernel(Pa
 #pragma unroll
     for (int c = 0; c < NC; ++c) qb[u][c] = ld16(q + 32 * c);
   }
-  const int wave_first = (t.first + rw * U * 16) / rep;  // tokens of the wave's rows
-  const int wave_last = (min(t.first + (rw + 1) * U * 16, rows) - 1) / rep;
-  const bool idle = t.first + rw * U * 16 >= rows;
+
+  // ---- loading
+  const int* table = a.page_table + (int64_t)min(t.seq, a.B - 1) * a.width;
+  const int mask = (1 << a.page_shift) - 1;
+  const char* kg = reinterpret_cast<const char*>(static_cast<const uint16_t*>(a.k) + kvh * a.s_h);
+  const char* vg = reinterpret_cast<const char*>(static_cast<const uint16_t*>(a.v) + kvh * a.s_h);
+  const int64_t page_b = 2 * a.s_p, row_b = 2 * a.s_t;  // of K and of V
+  const int g0 = rw * GW;                                 // the wave's first group
+  uint32_t off[GW * UG];
+#pragma unroll
+  for (int i = 0; i < GW * UG; ++i) {
+    const int at = (g0 * UG + i) * 64 + lane, row = at / (HD / 8);
+    off[i] = (uint32_t)((row & 15) * row_b + tile_column<HD>(row, at % (HD / 8)) * 16);
+  }
+  const int last_group = (max(seen, 1) - 1) & ~15;
+  int page[GW];  // of the next tile to load
+  auto look = [&](int i) {
+    const int kt = min(t0 + i * KW + kw, t1 - 1);
+#pragma unroll
+    for (int y = 0; y < GW; ++y) page[y] = scalar_int(table + (min(kt * KT + 16 * (g0 + y), last_group) >> a.page_shift));
+  };
+  auto issue = [&](int i, uint16_t* __restrict__ kd, uint16_t* __restrict__ vd) {
+    const int kt = min(t0 + i * KW + kw, t1 - 1);
+    auto fetch = [&](const char* from, int y, uint16_t* to) {
+#pragma unroll
+      for (int z = 0; z < UG; ++z)
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void*)(from + off[y * UG + z]),
+            (__attribute__((address_space(3))) void*)(reinterpret_cast<char*>(to) + ((g0 + y) * UG + z) * 1024), 16, 0, 0);
+    };
+#pragma unroll
+    for (int y = 0; y < GW; ++y) {
+      const int p = (unsigned)page[y] < (unsigned)a.pages ? page[y] : 0;
+      const int64_t from = p * page_b + (min(kt * KT + 16 * (g0 + y), last_group) & mask) * row_b;
+      fetch(kg + from, y, kd);
+      fetch(vg + from, y, vd);
+    }
+  };
+  auto arrived = [&] {  // waits for the queries: in the loop that would be a wait for every tile in flight
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        u32x4_t w = __builtin_bit_cast(u32x4_t, qb[u][c]);
+        asm volatile("" : "+v"(w));
+        qb[u][c] = __builtin_bit_cast(U32x4, w);
+      }
+  };
+  bool lost = false;  // whether a page of the range is none: then every tile looks which of its groups are
+  if (steps > 0) {
+    look(0);
+    const int p0 = t0 * KT >> a.page_shift, p1 = min(t1 * KT - 1, last_group) >> a.page_shift;
+    const int entry = table[min(p0 + lane, p1)];
+    issue(0, lds[kw][0][0], lds[kw][0][1]);
+    look(1);
+    arrived();
+    lost = __any((unsigned)entry >= (unsigned)a.pages);
+#pragma unroll
+    for (int i = 1; i < S - 1; ++i)
+      if (i < steps) {
+        issue(i, lds[kw][i][0], lds[kw][i][1]);
+        look(i + 1);
+      }
+    for (int p = p0 + 64; p <= p1; p += 64) lost |= __any((unsigned)table[min(p + lane, p1)] >= (unsigned)a.pages);
+  } else {
+    arrived();
+  }
+  const int wave_first = (t.first + rw * U * 16) / rep;  // token of the wave's first row
   const float scale = a.scale * kPackedLog2e;
   constexpr float kHead = packed_head<F16>;
   float m[U];
@@ -262,80 +296,114 @@ __global__ __launch_bounds__(64 * RW * KW, RW == 4 ? 2 : 1) void paged_kernel(Pa
   TileReads<HD> at;
   at.init(r, g);
 
-  auto step = [&](int i, int stage, int next, const uint16_t* __restrict__ ks, const uint16_t* __restrict__ vs,
-                  uint16_t* __restrict__ kd, uint16_t* __restrict__ vd) {
+  const int plain = min(t.len, t.past + (causal ? wave_first + 1 : 0));  // keys that all of the wave's rows see
+  // As restrict parameters the compiler sees that the stages differ; else it waits for every
+  // load in flight before it reads one.
+  auto step = [&](int i, const uint16_t* __restrict__ ks, const uint16_t* __restrict__ vs, uint16_t* __restrict__ kd,
+                  uint16_t* __restrict__ vd) {
     const int kt = t0 + i * KW + kw, s0 = kt * KT;
-    if (i + S - 1 < steps) issue(i + S - 1, next, kd, vd);
-    if (kt >= t1 || idle || (causal && s0 > t.past + wave_last)) return;
+    if (i + S - 1 < steps) issue(i + S - 1, kd, vd);
+    look(i + S);
+    uint32_t none = 0;  // groups in no page
+    if (lost) {
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+        none |= (unsigned)scalar_int(table + (min(s0 + 16 * x, last_group) >> a.page_shift)) >= (unsigned)a.pages ? 1u << x : 0u;
+    }
+    // Bits of the lane's 4 NT keys, 16 st + 4 g + x at 4 st + x: those that are there, and those that
+    // each row sees.  Formed here, before the products need the registers, and opaque: the compiler
+    // would keep a scalar mask of every comparison.
+    uint32_t there = ~0u, sees[U];
+    const bool holes = s0 + KT > t.len || none;
+    const bool edge = s0 + KT > plain || none;
+    if (edge) {
+      int g4 = 4 * g;  // opaque: what follows stays in this branch instead of in registers around the loop
+      asm volatile("" : "+v"(g4));
+#pragma unroll
+      for (int st = 0; st < NT; ++st) {
+        const int n = min(max(t.len - (s0 + 16 * st + g4), 0), 4);
+        there &= ~((none >> st & 1 ? 15u : 15u & (15u << n)) << (4 * st));
+      }
+      asm volatile("" : "+v"(there));
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        uint32_t see = there;
+        int tok = token[u];
+        asm volatile("" : "+v"(tok));
+        if (causal) {
+#pragma unroll
+          for (int st = 0; st < NT; ++st) {
+            const int n = min(max(t.past + tok + 1 - (s0 + 16 * st + g4), 0), 4);
+            see &= ~((15u & (15u << n)) << (4 * st));
+          }
+        } else {
+          const uint64_t* row = a.tree + (int64_t)(t.start + max(tok, 0)) * a.words;
+#pragma unroll
+          for (int st = 0; st < NT; ++st) {
+            const int j0 = s0 + 16 * st + g4 - t.past;  // of the sequence's rows
+            const int w0 = j0 >> 6, w1 = (j0 + 3) >> 6;
+            const uint64_t lo = w0 < 0 ? ~0ull : w0 < a.words ? row[w0] : 0, hi = w1 < 0 ? ~0ull : w1 < a.words ? row[w1] : 0;
+            const int sh = j0 & 63;  // four bits of the two words from there on
+            const uint32_t four = (uint32_t)(lo >> sh) | (w1 > w0 ? (uint32_t)(hi << (64 - sh)) : 0u);
+            see &= ~((15u & ~four) << (4 * st));
+          }
+        }
+        asm volatile("" : "+v"(see));
+        sees[u] = see;
+      }
+    }
     f32x4_t s[U][NT];
-    U32x4 ka[NT][NC];
-#pragma unroll
-    for (int st = 0; st < NT; ++st)
-#pragma unroll
-      for (int c = 0; c < NC; ++c) ka[st][c] = at.row16(ks, st, c);
-    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int st = 0; st < NT; ++st)
 #pragma unroll
       for (int u = 0; u < U; ++u) s[u][st] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    // Operands are read from LDS before their products; the barriers keep the compiler from
+    // sinking each read to its use, where every pair of products would wait.  At head_dim 128 half of
+    // the tile at a time: all of it does not fit the registers beside the outputs.
+    constexpr int KA = HD == 128 && NT > 2 ? 2 : NT;
 #pragma unroll
-    for (int sp = 0; sp < NT; sp += 2)
+    for (int s2 = 0; s2 < NT; s2 += KA) {
+      U32x4 ka[KA][NC];
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
+      for (int st = 0; st < KA; ++st)
 #pragma unroll
-        for (int st = sp; st < sp + 2; ++st)
+        for (int c = 0; c < NC; ++c) ka[st][c] = at.row16(ks, s2 + st, c);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int u = 0; u < U; ++u) s[u][st] = mfma16<F16>(ka[st][c], qb[u][c], s[u][st]);
+      for (int sp = 0; sp < KA; sp += 2)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int st = sp; st < sp + 2; ++st)
+#pragma unroll
+            for (int u = 0; u < U; ++u) s[u][s2 + st] = mfma16<F16>(ka[st][c], qb[u][c], s[u][s2 + st]);
+    }
     U32x4 va[NH][ND];
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int d = 0; d < ND; ++d) va[0][d] = at.columns32(vs, 0, d);
     __builtin_amdgcn_sched_barrier(0);
-    const uint32_t none = (uint32_t)(bad >> (4 * stage)) & 15u;
-    const bool edge = s0 + KT > t.past + (causal ? wave_first + 1 : 0) || none;  // uniform
-    if (edge) {
+    if (edge) {  // uniform
+      asm volatile("");  // a branch: as selects they would be part of every step
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int st = 0; st < NT; ++st) {
-          const int k0 = s0 + st * 16 + 4 * g, j0 = k0 - t.past;
-          uint32_t bits = 15;  // of the lane's four keys
-          if (causal) {
-            const int more = token[u] - j0;  // keys k0 .. k0 + more
-            bits = more >= 3 ? 15u : more < 0 ? 0u : (2u << more) - 1u;
-          } else if (j0 > -4) {
-            const uint64_t* row = a.tree + (int64_t)(t.start + max(token[u], 0)) * a.words;
-            bits = 0;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const int j = j0 + x;
-              const bool own = j < 0 || (j < 64 * a.words && (row[min(max(j, 0) >> 6, a.words - 1)] >> (j & 63) & 1));
-              bits |= own ? 1u << x : 0u;
-            }
-          }
-          if (none >> st & 1) bits = 0;
-          if (token[u] < 0) bits = 0;
+        for (int st = 0; st < NT; ++st)
 #pragma unroll
           for (int x = 0; x < 4; ++x)
-            if (!(bits >> x & 1) || k0 + x >= t.len) s[u][st][x] = -__builtin_inff();
-        }
+            if (!(sees[u] >> (4 * st + x) & 1)) s[u][st][x] = -__builtin_inff();
     }
     // V rows that are no keys: probability 0 times what lies there could be NaN
-    const bool holes = s0 + KT > t.len || none;  // uniform
     auto clear = [&](int hh) {
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        uint32_t keep[2];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int k0 = s0 + 32 * hh + 16 * q + 4 * g + 2 * x;
-          const bool no = none >> (2 * hh + q) & 1;
-          keep[x] = (no || k0 >= t.len ? 0u : 0xffffu) | (no || k0 + 1 >= t.len ? 0u : 0xffff0000u);
-        }
+        const uint32_t four = there >> (4 * (2 * hh + q));
+        const uint32_t k0 = (four & 1 ? 0xffffu : 0u) | (four & 2 ? 0xffff0000u : 0u);
+        const uint32_t k1 = (four & 4 ? 0xffffu : 0u) | (four & 8 ? 0xffff0000u : 0u);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-          va[hh][d].v[2 * q] &= keep[0];
-          va[hh][d].v[2 * q + 1] &= keep[1];
+          va[hh][d].v[2 * q] &= k0;
+          va[hh][d].v[2 * q + 1] &= k1;
         }
       }
     };
@@ -362,8 +430,7 @@ __global__ __launch_bounds__(64 * RW * KW, RW == 4 ? 2 : 1) void paged_kernel(Pa
       }
     }
     U32x4 pf[U][NH];
-#pragma unroll
-    for (int hh = 0; hh < NH; ++hh) {
+    auto softmax = [&](int hh) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -374,17 +441,35 @@ __global__ __launch_bounds__(64 * RW * KW, RW == 4 ? 2 : 1) void paged_kernel(Pa
           pf[u][hh].v[2 * q] = pack2<F16>(p[0], p[1]);
           pf[u][hh].v[2 * q + 1] = pack2<F16>(p[2], p[3]);
         }
-      if (hh > 0) {
-#pragma unroll
-        for (int d = 0; d < ND; ++d) va[hh][d] = at.columns32(vs, hh, d);
-      }
-      if (holes) clear(hh);
+    };
+    auto outputs = [&](int hh) {
 #pragma unroll
       for (int u = 0; u < U; ++u) l[u] = mfma16<F16>(ones, pf[u][hh], l[u]);
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int u = 0; u < U; ++u) o[u][d] = mfma16<F16>(va[hh][d], pf[u][hh], o[u][d]);
+    };
+    softmax(0);
+    if (holes) clear(0);
+    if constexpr (NH == 1) {
+      outputs(0);
+    } else {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int d = 0; d < ND; ++d) va[1][d] = at.columns32(vs, 1, d);
+      __builtin_amdgcn_sched_barrier(0);
+      // the first half's products with the second half's softmax between them
+      outputs(0);
+      softmax(1);
+#pragma unroll
+      for (int x = 0; x < U * ND + U; ++x) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x402, ND == 4 ? 4 : 3, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (holes) clear(1);
+      outputs(1);
     }
   };
   int stage = 0;
@@ -394,7 +479,7 @@ __global__ __launch_bounds__(64 * RW * KW, RW == 4 ? 2 : 1) void paged_kernel(Pa
     else tile_wait<0>();
     if (RW > 1) tile_barrier();  // the tile has landed for every wave, and all are done with the one before
     const int next = stage == 0 ? S - 1 : stage - 1;
-    step(i, stage, next, lds[kw][stage][0], lds[kw][stage][1], lds[kw][next][0], lds[kw][next][1]);
+    step(i, lds[kw][stage][0], lds[kw][stage][1], lds[kw][next][0], lds[kw][next][1]);
     stage = stage == S - 1 ? 0 : stage + 1;
   }
 
@@ -474,70 +559,117 @@ __global__ __launch_bounds__(64 * RW * KW, RW == 4 ? 2 : 1) void paged_kernel(Pa
   }
 }
 
-// Joins the ranges of one row and kv head: HD / 4 lanes take four columns each of a head.
-template <bool F16, int HD, int KT>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
+// Joins the ranges of a row: a lane takes four columns of one of its heads; with P = 4 the workgroup's
+// waves take every fourth range of the same 64 of them, and the sums meet in LDS.  64 rows of 16
+// heads of 128 from 64 ranges: 6 us (P = 1: 25); 1024 rows of 8 heads of 96 from one to three: 11 us (5).
+template <bool F16, int HD, int KT, int P>
+__global__ __launch_bounds__(P == 16 ? 1024 : 256) void paged_join_kernel(PagedAttnArgs a) {
+  __shared__ __align__(16) f32x4_t sums[P][64];
+  __shared__ float2 marks[P][64];
   const int rep = a.heads / a.kv_heads, RB = a.block_rows;
   const int row = blockIdx.x;
   const float* ml = a.work + (int64_t)a.units * a.kv_heads * RB * HD;
   PagedUnit u;
   int w = 0;
-  if (!paged_find<KT>(a, w, u, row) || u.splits == 1) return;
-  for (int x = threadIdx.x; x < a.heads * (HD / 4); x += 256) {
-    const int head = x / (HD / 4), col = x % (HD / 4) * 4, kvh = head / rep;
-    const int at = (row - u.start) * rep + head % rep;  // a head's row may begin the next block
-    const int first = w + (at / RB - u.first / RB) * u.splits;
-    if (first + u.splits > a.units) continue;  // bounds that decrease
-    float mx = kNoScore, l = 0.f;
-    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < u.splits; ++s) {
-      const int64_t part = ((int64_t)(first + s) * a.kv_heads + kvh) * RB + at % RB;
-      const float2 e = *reinterpret_cast<const float2*>(ml + 2 * part);
-      const f32x4_t v = *reinterpret_cast<const f32x4_t*>(a.work + part * HD + col);
-      const float mn = fmaxf(mx, e.x), f = exp2_f(mx - mn), k = exp2_f(e.x - mn);
-      mx = mn;
-      l = l * f + e.y * k;
+  if (!paged_find<KT>(a, 0, 0, w, u, row) || u.splits == 1) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int x = P == 1 ? blockIdx.z * 256 + threadIdx.x : blockIdx.z * 64 + lane;
+  const bool live = x < a.heads * (HD / 4);
+  const int head = live ? x / (HD / 4) : 0, col = live ? x % (HD / 4) * 4 : 0, kvh = head / rep;
+  const int at = (row - u.start) * rep + head % rep;  // a head's row may begin the next block
+  const int first = w + at / RB - u.first / RB;
+  const int splits = min(u.splits, (a.units - first + u.blocks - 1) / u.blocks);  // fewer: bounds that decrease
+  float mx = kNoScore, l = 0.f;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  auto add = [&](const float2& e, const f32x4_t& v) {
+    const float mn = fmaxf(mx, e.x), f = exp2_f(mx - mn), k = exp2_f(e.x - mn);
+    mx = mn;
+    l = l * f + e.y * k;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = o[j] * f + v[j] * k;
-    }
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    uint2 y;
-    y.x = pack2<F16>(o[0] * inv, o[1] * inv);
-    y.y = pack2<F16>(o[2] * inv, o[3] * inv);
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + ((int64_t)row * a.heads + head) * HD + col) = y;
+    for (int j = 0; j < 4; ++j) o[j] = o[j] * f + v[j] * k;
+  };
+#pragma unroll 4
+  for (int s = P == 1 ? 0 : wave; s < splits; s += P) {
+    const int64_t part = ((int64_t)(first + s * u.blocks) * a.kv_heads + kvh) * RB + at % RB;
+    add(*reinterpret_cast<const float2*>(ml + 2 * part), *reinterpret_cast<const f32x4_t*>(a.work + part * HD + col));
   }
+  if constexpr (P > 1) {
+    sums[wave][lane] = o;
+    marks[wave][lane] = make_float2(mx, l);
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int s = 1; s < P; ++s) add(marks[s][lane], sums[s][lane]);
+  }
+  if (!live) return;
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  uint2 y;
+  y.x = pack2<F16>(o[0] * inv, o[1] * inv);
+  y.y = pack2<F16>(o[2] * inv, o[3] * inv);
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + ((int64_t)row * a.heads + head) * HD + col) = y;
 }
 
+// Blocks of rows, at most.
+int64_t paged_row_blocks(const PagedAttnArgs& a) {
+  return (int64_t)a.Tq * (a.heads / a.kv_heads) / a.block_rows + (a.B > 0 ? a.B : 1);
+}
 int64_t paged_blocks(const PagedAttnArgs& a) { return ((int64_t)a.units + 7) / 8 * 8 * a.kv_heads; }
 
-template <bool F16, int HD, int RW, int KW, int U, int S>
+template <bool F16, int HD, int RW, int KW, int U>
 hipError_t run_paged(const PagedAttnArgs& a, hipStream_t s) {
-  paged_kernel<F16, HD, RW, KW, U, S><<<dim3((unsigned)paged_blocks(a)), 64 * RW * KW, 0, s>>>(a);
+  paged_kernel<F16, HD, RW, KW, U, 2><<<dim3((unsigned)paged_blocks(a)), 64 * RW * KW, 0, s>>>(a);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  if (a.slots > 0) paged_join_kernel<F16, HD, RW == 1 ? 32 : 64><<<dim3((unsigned)a.Tq), 256, 0, s>>>(a);
+  if (a.slots > 0) {
+    constexpr int KT = RW == 1 ? 32 : 64;
+    const int64_t most = ((int64_t)a.width << a.page_shift) / (KT * a.least);  // ranges that the pages have room for
+    if (most == 0) return hipGetLastError();
+    const int items = a.heads * (HD / 4);  // of a row
+    const dim3 grid((unsigned)a.Tq, 1, (unsigned)((items + 63) / 64));
+    if ((int64_t)a.Tq * items > 512 * (int64_t)device_cus())
+      paged_join_kernel<F16, HD, KT, 1><<<dim3(grid.x, 1, (unsigned)((items + 255) / 256)), 256, 0, s>>>(a);
+    else if (most < 64 || a.slots < 64 * paged_row_blocks(a))
+      paged_join_kernel<F16, HD, KT, 4><<<grid, 256, 0, s>>>(a);
+    else
+      paged_join_kernel<F16, HD, KT, 16><<<grid, 1024, 0, s>>>(a);
+  }
   return hipGetLastError();
 }
 
 template <bool F16, int HD>
 hipError_t paged_hd(const PagedAttnArgs& a, hipStream_t s) {
-  constexpr int S1 = HD == 128 ? 2 : 3;
   switch (a.block_rows) {
-    case 16: return run_paged<F16, HD, 1, 4, 1, S1>(a, s);
-    case 32: return run_paged<F16, HD, 1, 4, 2, S1>(a, s);
-    case 64: return run_paged<F16, HD, 2, 2, 2, 2>(a, s);
-    default: return run_paged<F16, HD, 4, 1, 2, S1>(a, s);
+    case 16: return a.key_waves == 4 ? run_paged<F16, HD, 1, 4, 1>(a, s) : run_paged<F16, HD, 1, 1, 1>(a, s);
+    case 32: return a.key_waves == 4 ? run_paged<F16, HD, 1, 4, 2>(a, s) : run_paged<F16, HD, 1, 1, 2>(a, s);
+    case 64: return run_paged<F16, HD, 2, 1, 2>(a, s);
+    default: return run_paged<F16, HD, 4, 1, 2>(a, s);
   }
 }
 
 }  // namespace
 
+// How the work is cut; only totals are known here, the sequences' own lengths are read on the device.
+// Microseconds a call in a captured graph, join included, for 1, 2, 3, 4 workgroups a CU:
+//   * Up to 32 rows a sequence and kv head, a wave each: 64 single tokens over 725 to 2175 keys, 8 / 4
+//     heads of 96: -, 38.6, 37.6, 36.0 (5: 35.8, 6: 40); trees of 16 nodes there -, 45.8, 45.4, 43.9 (5: 45.2).
+//     Where that would be more than 256 ranges of a sequence, four waves share one instead (one token
+//     over 65001 keys, 16 / 2 heads of 128: 34.5 with 512 ranges, 24.7 with 128 of four waves).
+//   * Up to 64 rows, two waves: 4 trees of 30 nodes over 8000 keys 23.7, 22.4, 23.8, 33.0; one of 32 over 65001
+//     keys 38.1, 33.1, 35.7, 42.5.
+//   * More, four waves: 6 chunks of 500 over 4100 keys, heads of 64: 82, 54, 49, 54; of 96: 97, 63, 70, -;
+//     one tree of 64 nodes over 65001 keys, 16 / 2 heads of 128: 67, 58, 67, 71.
 void paged_attn_plan(PagedAttnArgs& a) {
   const int rep = a.heads / a.kv_heads;
   const int64_t B = a.B > 0 ? a.B : 1, rows = (int64_t)a.Tq * rep, each = (rows + B - 1) / B;
   a.block_rows = each <= 16 ? 16 : each <= 32 ? 32 : each <= 64 ? 64 : 128;
-  const int64_t blocks = rows / a.block_rows + B;
-  const int64_t want = ((int64_t)device_cus() + a.kv_heads - 1) / a.kv_heads;
-  a.slots = a.B > kPagedSeqs || blocks >= 4 * want ? 0 : (int)want;
+  const int64_t blocks = paged_row_blocks(a);
+  const int cu = a.block_rows <= 32 ? 4 : a.block_rows == 128 && a.head_dim == 64 ? 3 : 2;
+  int64_t slots = ((int64_t)device_cus() * cu + a.kv_heads - 1) / a.kv_heads;
+  a.key_waves = 1;
+  if (a.block_rows <= 32 && slots > 256 * blocks) {
+    a.key_waves = 4;
+    slots /= 4;
+  }
+  a.slots = a.B > kPagedSeqs || blocks >= 4 * slots ? 0 : (int)slots;
   a.least = a.block_rows <= 32 ? 4 : 2;
   const int64_t units = a.slots + blocks + 2;
   a.units = units > INT32_MAX ? INT32_MAX : (int)units;

@@ -117,7 +117,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
         to = (t * a.heads + h) * a.hd;
       } else {
         if (p.page < 0) continue;
-        to = p.page * a.ys_p[which] + p.row * a.ys_t[which] + h * a.ys_h[which];
+        to = p.page * a.ys_p + p.row * a.ys_t + h * a.ys_h;
       }
     } else {
       position = a.wide_positions ? static_cast<const int64_t*>(a.positions)[t]
@@ -270,7 +270,7 @@ hipError_t launch_rotary(RotaryArgs a, bool append, hipStream_t s) {
       if (i == 1 && a.kv_heads == 0) continue;
       if (reinterpret_cast<uintptr_t>(a.x[i]) % bytes || reinterpret_cast<uintptr_t>(a.y[i]) % bytes) return false;
       if (a.xs_t[i] % v || a.xs_h[i] % v) return false;
-      if (append && i > 0 && (a.ys_p[i] % v || a.ys_t[i] % v || a.ys_h[i] % v)) return false;
+      if (append && i > 0 && (a.ys_p % v || a.ys_t % v || a.ys_h % v)) return false;
     }
     return true;
   };

@@ -128,11 +128,11 @@ _SIGNATURES = {
                               _P, _P, _I, _F,                 # gains, dtype, eps
                               _P, _P, _I64, _I64, _I,         # cos, sin, stride, rows, dtype
                               _P, _P, _P, _P, _P,             # cu, lengths, depths, page_table, q_out
-                              _P, _I64, _I64, _I64, _P, _I64, _I64, _I64,      # k_pages, v_pages and their strides
+                              _P, _P, _I64, _I64, _I64,       # k_pages, v_pages, their strides
                               _I64, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
     "mhc_paged_attn_workspace_bytes": (_I64, [_I, _I64, _I, _I, _I]),
     "mhc_paged_attn_fwd": (_I, [_P, _I64, _I64,               # q and its strides
-                                _P, _I64, _I64, _I64, _P, _I64, _I64, _I64,    # k_pages, v_pages and their strides
+                                _P, _P, _I64, _I64, _I64,     # k_pages, v_pages, their strides
                                 _P, _P, _P, _P, _I,           # page_table, lengths, cu, tree, words
                                 _P, _P, _I64,                 # out, workspace, bytes
                                 _I, _I64, _I, _I, _I, _I, _I, _I, _I, _F, _P]),

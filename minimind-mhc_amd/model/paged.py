@@ -42,6 +42,8 @@ def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, hd: Optional[int] = Non
     for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
         if t.stride(3) != 1 or any(s % 8 for s in t.stride()[:3]) or t.stride(1) >= 1 << 23 or t.data_ptr() % 16:
             raise ValueError(f"mhc_amd: {name} must have heads in order on 16 bytes (strides {t.stride()})")
+    if k_pages.stride() != v_pages.stride():
+        raise ValueError(f"mhc_amd: k_pages and v_pages lie differently (strides {k_pages.stride()} and {v_pages.stride()})")
     return n, page, kv, dim
 
 
@@ -75,8 +77,8 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
 
     q [rows, heads, head_dim], k and v [rows, kv heads, head_dim]: the projections, in the pages'
     type, any strides (those with a head's elements in order are read in place).
-    k_pages, v_pages [pages, page, kv heads, head_dim] bf16 or fp16, written in place: strides of
-    whole 16 bytes, a page a power of two of at least 16 rows.  page_table [n, width] int32: key x
+    k_pages, v_pages [pages, page, kv heads, head_dim] bf16 or fp16, written in place: the same strides,
+    of whole 16 bytes, a page a power of two of at least 16 rows.  page_table [n, width] int32: key x
     of sequence i lies in page page_table[i, x // page], row x % page.
     cu_seqlens [n + 1] int32: sequence i has the new rows cu_seqlens[i] to cu_seqlens[i + 1],
     beginning with row 0; lengths [n] int32: the keys it has before them.  Row j of them becomes key
@@ -124,8 +126,7 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
         H.check(H.load().mhc_paged_append(
             q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs, H.ptr(gains[0]), H.ptr(gains[1]), tag, float(eps),
             cos.data_ptr(), sin.data_ptr(), stride, cos.shape[0], H.dtype_tag(cos), cu.data_ptr(), lens.data_ptr(),
-            H.ptr(deep), table.data_ptr(), out.data_ptr(), k_pages.data_ptr(), *_strides(k_pages), v_pages.data_ptr(),
-            *_strides(v_pages), T, n, heads, kv, hd, 2 * cos.shape[1], table.shape[1], pages, page,
+            H.ptr(deep), table.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), *_strides(k_pages), T, n, heads, kv, hd, 2 * cos.shape[1], table.shape[1], pages, page,
             1 if interleaved else 0, H.dtype_tag(q), H.stream(dev)), "mhc_paged_append")
     _written(k_pages, v_pages)
     return out
@@ -187,7 +188,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         nbytes = _workspace(n, T, heads, kv, hd)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
         H.check(H.load().mhc_paged_attn_fwd(
-            q.data_ptr(), row, head, k_pages.data_ptr(), *_strides(k_pages), v_pages.data_ptr(), *_strides(v_pages),
+            q.data_ptr(), row, head, k_pages.data_ptr(), v_pages.data_ptr(), *_strides(k_pages),
             table.data_ptr(), lens.data_ptr(), cu.data_ptr(), H.ptr(tree), words, out.data_ptr(), H.ptr(ws), nbytes,
             n, T, heads, kv, hd, table.shape[1], pages, page, H.dtype_tag(q), scale, H.stream(dev)), "mhc_paged_attn_fwd")
     return out
