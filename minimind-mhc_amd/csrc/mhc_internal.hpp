@@ -340,7 +340,6 @@ hipError_t launch_packed_attn_bwd(const PackedAttnArgs& a, hipStream_t s);
 // Rotary positions of q [T, heads, hd] and k [T, kv_heads, hd] (x[0], x[1]; rows and heads at the
 // given element strides) to contiguous y[0], y[1]; with `append` k and v (x[2]) go to the rows of
 // a cache of pages (y[1], y[2]) instead.  cos, sin: `table_rows` rows of rd / 2 angles.
-constexpr int kRotaryRows = 32;  // of a workgroup, at most
 struct RotaryArgs {
   const void* x[3];
   void* y[3];
@@ -355,7 +354,6 @@ struct RotaryArgs {
   int64_t T;
   int heads, kv_heads, hd, rd, dtype;
   bool interleaved, back;
-  int rows;               // launch_rotary: of a workgroup
   // append
   const void* q_gain;     // [hd] each, or null
   const void* k_gain;

@@ -20,31 +20,28 @@ from .rotary import _rows, _tables, plain_rotary
 
 
 def _no_graph(what: str, *ts) -> None:
-    if any(t is not None and _ops.wants_graph(t) for t in ts):
+    if _ops.wants_graph(*(t for t in ts if t is not None)):
         raise RuntimeError(f"mhc_amd: {what} is for inference; call under torch.no_grad()")
 
 
-def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, hd: Optional[int] = None):
-    """(pages, page, kv heads, head_dim) of the cache's two tensors, which are read in place."""
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if t.dim() != 4:
-            raise ValueError(f"mhc_amd: {name} must be [pages, page, kv heads, head_dim], got {tuple(t.shape)}")
-    if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
-        raise ValueError(f"mhc_amd: k_pages {tuple(k_pages.shape)} {k_pages.dtype} and v_pages "
-                         f"{tuple(v_pages.shape)} {v_pages.dtype} differ")
+def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, hd: int):
+    """(pages, page, kv heads, strides of page, row and head) of the cache's two tensors."""
+    shape, strides = k_pages.shape, k_pages.stride()
+    if len(shape) != 4 or shape != v_pages.shape or k_pages.dtype != v_pages.dtype or strides != v_pages.stride():
+        raise ValueError(f"mhc_amd: k_pages {tuple(shape)} {k_pages.dtype} (strides {strides}) and v_pages "
+                         f"{tuple(v_pages.shape)} {v_pages.dtype} ({v_pages.stride()}) must be alike, "
+                         "[pages, page, kv heads, head_dim]")
     if k_pages.dtype not in _ops.HALF:
         raise TypeError(f"mhc_amd: pages hold bf16 or fp16, not {k_pages.dtype}")
-    n, page, kv, dim = k_pages.shape
+    n, page, kv, dim = shape
     if page < 16 or page & (page - 1):
         raise ValueError(f"mhc_amd: a page must have a power of two of at least 16 rows, got {page}")
-    if hd is not None and dim != hd:
+    if dim != hd:
         raise ValueError(f"mhc_amd: heads of {hd} and pages of {dim}")
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if t.stride(3) != 1 or any(s % 8 for s in t.stride()[:3]) or t.stride(1) >= 1 << 23 or t.data_ptr() % 16:
-            raise ValueError(f"mhc_amd: {name} must have heads in order on 16 bytes (strides {t.stride()})")
-    if k_pages.stride() != v_pages.stride():
-        raise ValueError(f"mhc_amd: k_pages and v_pages lie differently (strides {k_pages.stride()} and {v_pages.stride()})")
-    return n, page, kv, dim
+    p, t, h, one = strides
+    if one != 1 or (p | t | h) % 8 or t >= 1 << 23 or (k_pages.data_ptr() | v_pages.data_ptr()) % 16:
+        raise ValueError(f"mhc_amd: pages must have heads in order on 16 bytes (strides {strides})")
+    return n, page, kv, p, t, h
 
 
 def _written(*ts: torch.Tensor) -> None:
@@ -52,10 +49,6 @@ def _written(*ts: torch.Tensor) -> None:
     for t in ts:
         if not t.is_inference():
             torch.autograd.graph.increment_version(t)
-
-
-def _strides(t: torch.Tensor):
-    return t.stride()[:3]
 
 
 def _table(page_table: torch.Tensor, n: int, dev: torch.device) -> torch.Tensor:
@@ -94,11 +87,10 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
     """
     dev = H.require_device(q, k, v, k_pages, v_pages, cos, sin, depths, q_gain, k_gain)
     _no_graph("paged_append", q, k, v, k_pages, v_pages, q_gain, k_gain, cos, sin)
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 3:
-            raise ValueError(f"mhc_amd: {name} must be [rows, heads, head_dim], got {tuple(t.shape)}")
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError(f"mhc_amd: q and k must be [rows, heads, head_dim], got {tuple(q.shape)} and {tuple(k.shape)}")
     T, heads, hd = q.shape
-    pages, page, kv, _ = _pages(k_pages, v_pages, hd)
+    pages, page, kv, *strides = _pages(k_pages, v_pages, hd)
     if k.shape != v.shape or tuple(k.shape) != (T, kv, hd) or heads < 1:
         raise ValueError(f"mhc_amd: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} and pages "
                          f"{tuple(k_pages.shape)} do not belong together")
@@ -110,23 +102,25 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
     lens = _bounds("lengths", lengths, n, dev)
     deep = None if depths is None else _bounds("depths", depths, T, dev)
     table = _table(page_table, n, dev)
-    gains = []
-    for name, g in (("q_gain", q_gain), ("k_gain", k_gain)):
-        if g is not None and tuple(g.shape) != (hd,):
-            raise ValueError(f"mhc_amd: {name} must be [{hd}], got {tuple(g.shape)}")
-        gains.append(None if g is None else g.contiguous())
-    given = [g for g in gains if g is not None]
-    if len(given) == 2 and given[0].dtype != given[1].dtype:
-        gains = [g.float() for g in gains]
-    tag = H.dtype_tag(next(g for g in gains if g is not None)) if given else 0
-    cos, sin, stride = _tables(cos, sin, hd, dev)
-    (q, *qs), (k, *ks), (v, *vs) = _rows("q", q, T), _rows("k", k, T), _rows("v", v, T)
+    gains, tag = (None, None), 0
+    if q_gain is not None or k_gain is not None:
+        gains = [None if g is None else g.contiguous() for g in (q_gain, k_gain)]
+        given = [g for g in gains if g is not None]
+        for g in given:
+            if tuple(g.shape) != (hd,):
+                raise ValueError(f"mhc_amd: a gain must be [{hd}], got {tuple(g.shape)}")
+        if len({g.dtype for g in given}) > 1:
+            gains = [g.float() for g in gains]
+            given = gains
+        tag = H.dtype_tag(given[0])
+    cos, sin, stride = _tables(cos, sin, hd)
+    (q, *qs), (k, *ks), (v, *vs) = _rows(q, T), _rows(k, T), _rows(v, T)
     out = torch.empty((T, heads, hd), dtype=q.dtype, device=dev)
     with _ops.launch_device(q):
         H.check(H.load().mhc_paged_append(
             q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs, H.ptr(gains[0]), H.ptr(gains[1]), tag, float(eps),
             cos.data_ptr(), sin.data_ptr(), stride, cos.shape[0], H.dtype_tag(cos), cu.data_ptr(), lens.data_ptr(),
-            H.ptr(deep), table.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), *_strides(k_pages), T, n, heads, kv, hd, 2 * cos.shape[1], table.shape[1], pages, page,
+            H.ptr(deep), table.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), *strides, T, n, heads, kv, hd, 2 * cos.shape[1], table.shape[1], pages, page,
             1 if interleaved else 0, H.dtype_tag(q), H.stream(dev)), "mhc_paged_append")
     _written(k_pages, v_pages)
     return out
@@ -161,7 +155,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if q.dim() != 3:
         raise ValueError(f"mhc_amd: q must be [rows, heads, head_dim], got {tuple(q.shape)}")
     T, heads, hd = q.shape
-    pages, page, kv, _ = _pages(k_pages, v_pages, hd)
+    pages, page, kv, *strides = _pages(k_pages, v_pages, hd)
     if hd not in HEAD_DIMS:
         raise ValueError(f"mhc_amd: head_dim must be one of {HEAD_DIMS}, got {hd}")
     if kv < 1 or heads < 1 or heads % kv:
@@ -179,8 +173,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
     if not (0.0 < scale < 3e38):
         raise ValueError(f"mhc_amd: scale must be positive, got {scale}")
-    row, head = (q.stride(i) if q.shape[i] > 1 else 0 for i in (0, 1))
-    if q.stride(2) != 1 or row % 8 or head % 8 or row >= 1 << 23 or q.data_ptr() % 16:
+    row, head, one = q.stride()
+    row, head = row if T > 1 else 0, head if heads > 1 else 0
+    if one != 1 or (row | head) % 8 or row >= 1 << 23 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
         row, head = heads * hd, hd
     out = torch.empty((T, heads, hd), dtype=q.dtype, device=dev)
@@ -188,7 +183,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         nbytes = _workspace(n, T, heads, kv, hd)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
         H.check(H.load().mhc_paged_attn_fwd(
-            q.data_ptr(), row, head, k_pages.data_ptr(), v_pages.data_ptr(), *_strides(k_pages),
+            q.data_ptr(), row, head, k_pages.data_ptr(), v_pages.data_ptr(), *strides,
             table.data_ptr(), lens.data_ptr(), cu.data_ptr(), H.ptr(tree), words, out.data_ptr(), H.ptr(ws), nbytes,
             n, T, heads, kv, hd, table.shape[1], pages, page, H.dtype_tag(q), scale, H.stream(dev)), "mhc_paged_attn_fwd")
     return out

@@ -14,48 +14,48 @@ from . import _hip as H
 from . import _ops
 
 
-def _tables(cos: torch.Tensor, sin: torch.Tensor, head_dim: int, dev: torch.device):
+def _tables(cos: torch.Tensor, sin: torch.Tensor, head_dim: int):
     """(cos, sin, row stride) of tables [positions, rotary_dim / 2]."""
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != sin.dtype:
-        raise ValueError(f"mhc_amd: cos {tuple(cos.shape)} and sin {tuple(sin.shape)} must be alike, "
+    shape = cos.shape
+    if len(shape) != 2 or shape != sin.shape or cos.dtype != sin.dtype:
+        raise ValueError(f"mhc_amd: cos {tuple(shape)} and sin {tuple(sin.shape)} must be alike, "
                          "[positions, rotary_dim / 2]")
-    if 2 * cos.shape[1] > head_dim:
-        raise ValueError(f"mhc_amd: tables of {cos.shape[1]} angles for heads of {head_dim}")
-    if cos.get_device() != dev.index or sin.get_device() != dev.index:
-        raise RuntimeError(f"mhc_amd: the tables are on {cos.device} and {sin.device}, the tensors on {dev}")
+    if 2 * shape[1] > head_dim:
+        raise ValueError(f"mhc_amd: tables of {shape[1]} angles for heads of {head_dim}")
     H.dtype_tag(cos)
-    if cos.stride() != sin.stride() or cos.shape[1] > 1 and cos.stride(1) != 1:
+    stride = cos.stride()
+    if stride != sin.stride() or shape[1] > 1 and stride[1] != 1:
         cos, sin = cos.contiguous(), sin.contiguous()
-    return cos, sin, cos.stride(0) if cos.shape[0] > 1 else cos.shape[1]
+        stride = cos.stride()
+    return cos, sin, stride[0] if shape[0] > 1 else shape[1]
 
 
-def _rows(name: str, t: torch.Tensor, rows: int):
+def _rows(t: torch.Tensor, rows: int):
     """t [..., heads, head_dim] as (t [rows, heads, head_dim], row stride, head stride)."""
     if t.dim() != 3:
         try:
             t = t.view(rows, t.shape[-2], t.shape[-1])
         except RuntimeError:  # rows that no one stride joins
             t = t.reshape(rows, t.shape[-2], t.shape[-1])
-    if t.shape[2] > 1 and t.stride(2) != 1:
+    row, head, one = t.stride()
+    if one != 1 and t.shape[2] > 1:
         t = t.contiguous()
-    row, head = (t.stride(i) if t.shape[i] > 1 else 0 for i in (0, 1))
+        row, head, one = t.stride()
     return t, row, head
 
 
-def _turn(q, k, cos, sin, positions, flags):
-    rows = positions.numel()
-    (q3, *qs), out_q = _rows("q", q, rows), torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if k is None:
-        k3, ks, out_k, kv = None, (0, 0), None, 0
-    else:
-        (k3, *ks), out_k = _rows("k", k, rows), torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        kv = k.shape[-2]
-    cos, sin, stride = _tables(cos, sin, q.shape[-1], q.device)
+def _turn(q, k, cos, sin, stride, positions, flags):
+    rows, shape, dev = positions.numel(), q.shape, q.device
+    q3, *qs = _rows(q, rows)
+    out_q, out_k, k3, ks, kv = torch.empty(shape, dtype=q.dtype, device=dev), None, None, (0, 0), 0
+    if k is not None:
+        k3, *ks = _rows(k, rows)
+        out_k, kv = torch.empty(k.shape, dtype=q.dtype, device=dev), k.shape[-2]
     with _ops.launch_device(q):
         H.check(H.load().mhc_rotary(
             q3.data_ptr(), *qs, H.ptr(k3), *ks, cos.data_ptr(), sin.data_ptr(), stride, cos.shape[0],
             H.dtype_tag(cos), positions.data_ptr(), positions.element_size(), out_q.data_ptr(), H.ptr(out_k),
-            rows, q.shape[-2], kv, q.shape[-1], 2 * cos.shape[1], flags, H.dtype_tag(q), H.stream(q.device)),
+            rows, shape[-2], kv, shape[-1], 2 * cos.shape[1], flags, H.dtype_tag(q), H.stream(dev)),
             "mhc_rotary")
     return out_q, out_k
 
@@ -64,28 +64,28 @@ class _Rotary(torch.autograd.Function):
     """A linear map: its backward pass is the transposed one, itself a _Rotary."""
 
     @staticmethod
-    def forward(ctx, q, k, cos, sin, positions, flags):
+    def forward(ctx, q, k, cos, sin, stride, positions, flags):
         ctx.save_for_backward(cos, sin, positions)
-        ctx.flags = flags
+        ctx.stride, ctx.flags = stride, flags
         ctx.set_materialize_grads(False)
-        return _turn(q, k, cos, sin, positions, flags)
+        return _turn(q, k, cos, sin, stride, positions, flags)
 
     @staticmethod
     def backward(ctx, gq, gk):
         cos, sin, positions = ctx.saved_tensors
-        back = (cos, sin, positions, ctx.flags ^ 2)
+        back = (cos, sin, ctx.stride, positions, ctx.flags ^ 2)
         if gq is None:
             if gk is not None:
                 gk = _apply(gk, None, *back)[0]
         else:
             gq, gk = _apply(gq, gk, *back)
-        return gq, gk, None, None, None, None
+        return gq, gk, None, None, None, None, None
 
 
-def _apply(q, k, cos, sin, positions, flags):
-    if _ops.wants_graph(q) or k is not None and _ops.wants_graph(k):
-        return _Rotary.apply(q, k, cos, sin, positions, flags)
-    return _turn(q, k, cos, sin, positions, flags)
+def _apply(q, k, *args):
+    if _ops.wants_graph(q, q if k is None else k):
+        return _Rotary.apply(q, k, *args)
+    return _turn(q, k, *args)
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor,
@@ -114,9 +114,9 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, sin: t
         raise ValueError(f"mhc_amd: positions {tuple(positions.shape)} do not belong to q {tuple(q.shape)}")
     if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
         raise RuntimeError("mhc_amd: the tables of rotary are constants; detach them")
-    _tables(cos, sin, q.shape[-1], dev)
+    tables = _tables(cos, sin, q.shape[-1])
     positions = positions if positions.is_contiguous() else positions.contiguous()
-    return _apply(q, k, cos, sin, positions, 1 if interleaved else 0)
+    return _apply(q, k, *tables, positions, 1 if interleaved else 0)
 
 
 def plain_rotary(q, k, cos, sin, positions, interleaved: bool = False):
