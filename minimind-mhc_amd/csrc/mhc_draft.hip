@@ -15,6 +15,7 @@ namespace mhc {
 namespace {
 
 constexpr int kDraftNodes = 1024;  // of a sequence, whose numbers are fetched at a time
+constexpr int kDraftBlocks = 8;    // 16-byte blocks of a row that a lane keeps
 constexpr int kDraftGone = 64;     // rejected siblings that are kept at hand
 
 template <int DT>
@@ -30,32 +31,36 @@ struct ProbRow {
     base = static_cast<const char*>(p) + (at - off) * dtype_bytes(DT);
   }
   __device__ int blocks() const { return (V + off + PER - 1) / PER; }
-  // The PER elements of a block, 0 for those that are none of the row's.
-  __device__ __forceinline__ void load(int block, float (&x)[PER]) const {
+  // A block's 16 bytes, 0 for the elements that are none of the row's.
+  __device__ __forceinline__ U32x4 raw(int block) const {
     const int e0 = block * PER - off;
-    if (e0 >= 0 && e0 + PER <= V) {
-      const U32x4 w = ld16(base + (int64_t)block * 16);
+    if (e0 >= 0 && e0 + PER <= V) return ld16(base + (int64_t)block * 16);
+    uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (DT == kF32) {
-          x[j] = __uint_as_float(w.v[j]);
-        } else {
-          x[2 * j] = elem_lo<DT == kF16>(w.v[j]);
-          x[2 * j + 1] = elem_hi<DT == kF16>(w.v[j]);
-        }
+    for (int i = 0; i < PER; ++i)
+      if ((unsigned)(e0 + i) < (unsigned)V) {
+        if constexpr (DT == kF32) w[i] = reinterpret_cast<const uint32_t*>(base)[(int64_t)block * PER + i];
+        else w[i / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(base)[(int64_t)block * PER + i] << (16 * (i & 1));
       }
-    } else {
+    return U32x4{{w[0], w[1], w[2], w[3]}};
+  }
+  static __device__ __forceinline__ void open(const U32x4& w, float (&x)[PER]) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i)
-        x[i] = (unsigned)(e0 + i) < (unsigned)V ? ld_any(base, (int64_t)block * PER + i, DT) : 0.f;
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (DT == kF32) {
+        x[j] = __uint_as_float(w.v[j]);
+      } else {
+        x[2 * j] = elem_lo<DT == kF16>(w.v[j]);
+        x[2 * j + 1] = elem_hi<DT == kF16>(w.v[j]);
+      }
     }
   }
-  __device__ float at(int e) const { return ld_any(base, (int64_t)e + off, DT); }
 };
 
-// A probability: what is no positive finite number counts as 0.
+// A probability: what is no positive finite number counts as 0 (the maximum of NaN and 0 is 0).
 __device__ __forceinline__ double prob(float x) {
-  return x > 0.f && x < __builtin_inff() ? (double)x : 0.0;
+  x = fmaxf(x, 0.f);
+  return (double)(x < __builtin_inff() ? x : 0.f);
 }
 __device__ __forceinline__ double left_of(double p, double q, double a) { return fmax(p - a * q, 0.0); }
 
@@ -117,27 +122,45 @@ __global__ __launch_bounds__(64 * W) void verify_kernel(VerifyArgs a) {
   };
   // sum over the row of what is left, by each wave over a contiguous part of the blocks
   const int parts = (P.init(a.probs, start, V), (V + 2 * PER - 2) / PER + W - 1) / W;
-  auto weights = [&](int block, double (&w)[PER]) {
+  auto weights = [&](int block, const U32x4& pw, const U32x4& qw, double (&w)[PER]) {
     float p[PER], q[PER];
-    P.load(block, p);
-    if (a.draft) Q.load(block, q);
+    ProbRow<DT>::open(pw, p);
+    ProbRow<DT>::open(qw, q);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) w[i] = a.draft ? left_of(prob(p[i]), prob(q[i]), ratio) : prob(p[i]);
+    for (int i = 0; i < PER; ++i) w[i] = ratio > 0.0 ? left_of(prob(p[i]), prob(q[i]), ratio) : prob(p[i]);
     if (!a.draft && rejected > 0) {
 #pragma unroll
       for (int i = 0; i < PER; ++i)
         if (w[i] > 0.0 && gone(block * PER + i - P.off)) w[i] = 0.0;
     }
   };
-  auto total = [&]() {  // also leaves the waves' sums in s_sum
+  // The sum of that; also leaves the waves' sums in s_sum.  A row of up to G blocks a lane stays in
+  // registers for the node's next rejections.
+  constexpr int G = kDraftBlocks;
+  U32x4 pw[G], qw[G];
+  bool have_p = false, have_q = false;  // of the node
+  auto total = [&]() {
     const int nb = P.blocks(), b1 = min((wave + 1) * parts, nb);
+    const bool held = parts <= 64 * G;
     double s = 0.0;
-    for (int b = wave * parts + lane; b < b1; b += 64) {
-      double w[PER];
-      weights(b, w);
+    for (int b0 = wave * parts; b0 < b1; b0 += 64 * G) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) s += w[i];
+      for (int g = 0; g < G; ++g) {
+        const int b = b0 + g * 64 + lane;
+        if (!held || !have_p) pw[g] = b < b1 ? P.raw(b) : U32x4{};
+        if (ratio > 0.0 && (!held || !have_q)) qw[g] = b < b1 ? Q.raw(b) : U32x4{};
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        if (b0 + g * 64 >= b1) break;  // uniform
+        double w[PER];
+        weights(b0 + g * 64 + lane, pw[g], qw[g], w);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) s += w[i];
+      }
     }
+    have_p = true;
+    have_q = ratio > 0.0;
     s = wave_sum64(s);
     __syncthreads();
     if (lane == 0) s_sum[wave] = s;
@@ -151,15 +174,25 @@ __global__ __launch_bounds__(64 * W) void verify_kernel(VerifyArgs a) {
     const int nb = P.blocks();
     float m = -__builtin_inff();
     int at = INT32_MAX;
-    for (int b = tid; b < nb; b += TH) {
-      float p[PER];
-      P.load(b, p);
+    constexpr int G = 4;
+    for (int b0 = tid; b0 < nb; b0 += G * TH) {
+      U32x4 pw[G];
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int v = b * PER + i - P.off;
-        if ((unsigned)v < (unsigned)V && (p[i] > m || (p[i] == m && v < at))) {
-          m = p[i];
-          at = v;
+      for (int g = 0; g < G; ++g) {
+        pw[g] = U32x4{};
+        if (b0 + g * TH < nb) pw[g] = P.raw(b0 + g * TH);
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        float p[PER];
+        ProbRow<DT>::open(pw[g], p);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int v = (b0 + g * TH) * PER + i - P.off;
+          if ((unsigned)v < (unsigned)V && (p[i] > m || (p[i] == m && v < at))) {
+            m = p[i];
+            at = v;
+          }
         }
       }
     }
@@ -241,6 +274,7 @@ __global__ __launch_bounds__(64 * W) void verify_kernel(VerifyArgs a) {
       if (yes) {
         cur = j;
         rejected = 0;
+        have_p = have_q = false;
         if (tid == 0) a.path[start + kept] = j;
         ++kept;
         enter(j);
@@ -260,7 +294,7 @@ __global__ __launch_bounds__(64 * W) void verify_kernel(VerifyArgs a) {
     }
     return;
   }
-  double all = total();
+  double all = ratio > 0.0 ? norm : total();  // the last rejection's sum, and the waves' parts of it
   if (!(all > 0.0)) {  // nothing left: the target itself
     ratio = 0.0;
     rejected = 0;
@@ -288,7 +322,7 @@ __global__ __launch_bounds__(64 * W) void verify_kernel(VerifyArgs a) {
     double s = 0.0;
     for (int b = t0; b < t1; ++b) {
       double w[PER];
-      weights(b, w);
+      weights(b, P.raw(b), ratio > 0.0 ? Q.raw(b) : U32x4{}, w);
 #pragma unroll
       for (int i = 0; i < PER; ++i) s += w[i];
     }
@@ -306,7 +340,7 @@ __global__ __launch_bounds__(64 * W) void verify_kernel(VerifyArgs a) {
     int first = INT32_MAX, most = -1;  // the first past the border, the last with a weight
     for (int b = t0; b < t1; ++b) {
       double w[PER];
-      weights(b, w);
+      weights(b, P.raw(b), ratio > 0.0 ? Q.raw(b) : U32x4{}, w);
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         cum += w[i];
@@ -386,7 +420,8 @@ __global__ __launch_bounds__(256) void keep_kernel(KeepArgs a) {
 
 template <int DT>
 hipError_t launch_verify_dt(const VerifyArgs& a, hipStream_t s) {
-  if (a.V >= 16384) verify_kernel<DT, 16><<<dim3((unsigned)a.B), 1024, 0, s>>>(a);
+  // four waves hold a row of up to 2048 blocks in registers, sixteen one of 8192
+  if (a.V > 2048 * ProbRow<DT>::PER - 2 * ProbRow<DT>::PER) verify_kernel<DT, 16><<<dim3((unsigned)a.B), 1024, 0, s>>>(a);
   else verify_kernel<DT, 4><<<dim3((unsigned)a.B), 256, 0, s>>>(a);
   return hipGetLastError();
 }
