@@ -22,7 +22,9 @@ Differences from the reference, all outside the mHC path:
     neighbouring HIP launch; with autograd they run as separate ops in the
     reference's order (model/model_minimind.py:326-336, :365-370);
   * `packed` (a PackedBatch) says that the rows of a batch of one are several sequences one
-    after another; a PackedCache then takes the place of the caches that grow by copies;
+    after another; a PackedCache or a PagedCache then takes the place of the caches that grow by
+    copies; over a PagedCache `drafts` (a DraftTree) says that they are drafted tokens;
+  * rotary_dim and rope_interleaved of the config turn a part of each head, in neighbouring pairs;
   * one StreamChain per forward is passed to every mHC call, so each launch
     that writes the residual stream hands its rows' sums of squares to the
     next pre launch (used at n >= 8 or hidden > 1024).
@@ -36,12 +38,16 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from . import _hip as H
 from . import _ops, losses
 from ._ops import StreamChain
 from .mhc_common import MHCHead, StreamExpand
 from .mhc_fused import MHCConnection_Fused
 from .mhc_fused_no_hres import MHCConnection_FusedNoHres
 from .packed import PackedBatch, PackedCache, PackedCall
+from .paged import DraftTree, PagedCache, PagedCall
+from .rotary import plain_rotary, rotary
+from .speculative import plain_verify, verify_drafts
 
 
 class MiniMindConfig:
@@ -68,6 +74,11 @@ class MiniMindConfig:
         self.max_position_embeddings = kwargs.get("max_position_embeddings", 32768)
         self.rms_norm_eps = kwargs.get("rms_norm_eps", 1e-6)
         self.rope_theta = kwargs.get("rope_theta", 1e6)
+        # the first so many elements of a head turn, in halves or as neighbouring pairs
+        self.rotary_dim = kwargs.get("rotary_dim", self.head_dim)
+        self.rope_interleaved = kwargs.get("rope_interleaved", False)
+        assert 0 < self.rotary_dim <= self.head_dim and self.rotary_dim % 2 == 0 or self.rotary_dim == self.head_dim, \
+            f"rotary_dim must be even and at most head_dim, got {self.rotary_dim}"
         self.tie_word_embeddings = kwargs.get("tie_word_embeddings", True)
         self.inference_rope_scaling = kwargs.get("inference_rope_scaling", False)
         self.rope_scaling = {
@@ -151,13 +162,15 @@ class Attention(nn.Module):
         self.q_norm = nn.RMSNorm(self.head_dim, eps=config.rms_norm_eps)
         self.k_norm = nn.RMSNorm(self.head_dim, eps=config.rms_norm_eps)
         self.dropout = config.dropout
+        self.rope_interleaved = config.rope_interleaved
 
     def forward(self, x, position_embeddings, past_key_value=None, use_cache=False,
                 attention_mask=None, packed=None, layer_id=0):
         bsz, seq_len, _ = x.shape
         xq, xk, xv = (_ops.linears(x, self.q_proj, self.k_proj, self.v_proj)
                       or (self.q_proj(x), self.k_proj(x), self.v_proj(x)))
-        route = None if attention_mask is not None or packed is not None else _ops.attn_route(
+        own_pairs = len(position_embeddings) == 3  # tables and positions: not whole heads in halves
+        route = None if attention_mask is not None or packed is not None or own_pairs else _ops.attn_route(
             self, xq, xk, xv, position_embeddings, past_key_value)
         if route == "decode":
             out, past_kv = _ops.attn_decode(self, xq, xk, xv, position_embeddings,
@@ -170,9 +183,16 @@ class Attention(nn.Module):
         xq = xq.view(bsz, seq_len, self.n_local_heads, self.head_dim)
         xk = xk.view(bsz, seq_len, self.n_local_kv_heads, self.head_dim)
         xv = xv.view(bsz, seq_len, self.n_local_kv_heads, self.head_dim)
+        if isinstance(packed, PagedCall):
+            return _ops.linear(packed.attention(self, xq, xk, xv, position_embeddings, layer_id), self.o_proj), None
         xq, xk = self.q_norm(xq), self.k_norm(xk)
-        cos, sin = position_embeddings
-        xq, xk = apply_rotary_pos_emb(xq, xk, cos, sin)
+        if own_pairs:
+            cos, sin, positions = position_embeddings
+            takes = xq.is_cuda and xq.dtype == xk.dtype and xq.dtype in H._DTYPE_TAG and _ops.eager_call()
+            xq, xk = (rotary if takes else plain_rotary)(xq, xk, cos, sin, positions, self.rope_interleaved)
+        else:
+            cos, sin = position_embeddings
+            xq, xk = apply_rotary_pos_emb(xq, xk, cos, sin)
         if packed is not None:
             out = packed.attention(xq, xk, xv, layer_id, self.dropout if self.training else 0.0)
             return _ops.linear(out, self.o_proj), None
@@ -372,17 +392,20 @@ class MiniMindModel(nn.Module):
             self.embed_up_norm = nn.Identity()
             self.layers = nn.ModuleList([MiniMindBlock(i, config) for i in range(self.num_hidden_layers)])
             self.norm = nn.RMSNorm(D, eps=eps)
-        cos, sin = precompute_freqs_cis(config.head_dim, config.max_position_embeddings,
+        self.own_pairs = config.rotary_dim != config.head_dim or config.rope_interleaved
+        cos, sin = precompute_freqs_cis(config.rotary_dim, config.max_position_embeddings,
                                         config.rope_theta, config.rope_scaling)
         self.register_buffer("freqs_cos", cos, persistent=False)
         self.register_buffer("freqs_sin", sin, persistent=False)
 
     def forward(self, input_ids, attention_mask=None, past_key_values=None, use_cache=False,
-                packed=None, **kwargs):
+                packed=None, drafts=None, **kwargs):
         bsz, seq_len = input_ids.shape
         call, cache = None, None
         if packed is not None:
-            call, cache, past_key_values = self._packed_call(input_ids, attention_mask, past_key_values, packed)
+            call, cache, past_key_values = self._packed_call(input_ids, attention_mask, past_key_values, packed, drafts)
+        elif drafts is not None:
+            raise ValueError("drafts need packed sequences and a PagedCache")
         past_key_values = past_key_values or [None] * len(self.layers)
         start = past_key_values[0][0].shape[1] if past_key_values[0] is not None else 0
         h = self.dropout(self.embed_tokens(input_ids))
@@ -394,10 +417,22 @@ class MiniMindModel(nn.Module):
             h = self.embed_up_norm[1].forward_normed(h, self.embed_up_norm[0], chain=chain)
         else:
             h = self.embed_up_norm(h)
-        if call is None:
+        table = self.freqs_cos.shape[0]
+        if self.own_pairs and call is None and start + seq_len > table:
+            raise ValueError(f"{start + seq_len} positions, max_position_embeddings is {table}")
+        if isinstance(call, PagedCall) or self.own_pairs:  # whole tables, and where a rotation takes them the positions
+            half = self.freqs_cos.shape[1] // 2
+            pos = (self.freqs_cos[:, :half], self.freqs_sin[:, :half])
+            if isinstance(call, PagedCall):
+                if call.most > table:
+                    call.within(table)
+            else:
+                at = (torch.arange(start, start + seq_len, device=h.device) if call is None
+                      else call.positions.clamp(0, table - 1))
+                pos = (*pos, at.expand(bsz, seq_len))
+        elif call is None:
             pos = (self.freqs_cos[start:start + seq_len], self.freqs_sin[start:start + seq_len])
         else:  # each row's position in its own sequence (rows of none: any)
-            table = self.freqs_cos.shape[0]
             at = call.positions.clamp(0, table - 1)
             pos = (self.freqs_cos[at], self.freqs_sin[at])
         more = {} if call is None else {"packed": call}
@@ -421,16 +456,19 @@ class MiniMindModel(nn.Module):
         return h, presents, aux
 
 
-    def _packed_call(self, input_ids, attention_mask, cache, packed):
-        """(the PackedCall, its cache or None, past_key_values for the layers)."""
+    def _packed_call(self, input_ids, attention_mask, cache, packed, drafts):
+        """(the PackedCall or PagedCall, its cache or None, past_key_values for the layers)."""
         if not isinstance(packed, PackedBatch) or tuple(input_ids.shape) != (1, packed.rows):
             raise ValueError(f"packed must be a PackedBatch of input_ids' rows, [1, rows], not of "
                              f"{tuple(input_ids.shape)}")
         if attention_mask is not None:
             raise ValueError("packed sequences take no attention_mask: nothing of them is padding")
-        if cache is not None and not isinstance(cache, PackedCache):
-            raise ValueError("packed sequences need a PackedCache as past_key_values")
-        call, table = PackedCall(packed, cache, slots=True), self.freqs_cos.shape[0]
+        if cache is not None and not isinstance(cache, (PackedCache, PagedCache)):
+            raise ValueError("packed sequences need a PackedCache or a PagedCache as past_key_values")
+        if drafts is not None and not isinstance(cache, PagedCache):
+            raise ValueError("drafts need a PagedCache as past_key_values")
+        call = PagedCall(packed, cache, drafts) if isinstance(cache, PagedCache) else PackedCall(packed, cache, slots=True)
+        table = self.freqs_cos.shape[0]
         if call.reach > table:
             raise ValueError(f"a packed sequence reaches {call.reach} positions, max_position_embeddings is {table}")
         return call, cache, None
@@ -489,6 +527,26 @@ class MiniMindForCausalLM(nn.Module):
     def _sequence_sums(lp, y, packed, average):
         total = packed.sums(lp)
         return total / packed.sums(y != -100).clamp_min(1) if average else total
+
+    @torch.no_grad()
+    def verify_step(self, input_ids, packed, cache, parents=None, draft_probs=None, uniforms=None, temperature=1.0):
+        """One step of decoding with drafts: input_ids [1, rows], each packed sequence's last token
+        (not in the cache yet) and its drafted ones, a tree (parents, DraftTree) or a chain; cache: the
+        PagedCache of what came before.  Runs the model on all of them, keeps the accepted branch in
+        the cache (speculative.verify_drafts: draft_probs [rows, V] and uniforms [rows]; without
+        uniforms greedy, else the model's probabilities at that temperature) and gives kept [n], path
+        [rows], next_tokens [n], the sequences' new last tokens, and the logits."""
+        if not isinstance(cache, PagedCache):
+            raise ValueError("verify_step needs a PagedCache")
+        if not temperature > 0.0:
+            raise ValueError(f"mhc_amd: temperature must be positive, got {temperature} (greedy: no uniforms)")
+        drafts = DraftTree(packed, parents)
+        logits = self(input_ids, packed=packed, past_key_values=cache, drafts=drafts).logits[0]
+        probs = logits if uniforms is None else torch.softmax(logits.float() / temperature, -1)
+        kept, path, following = (verify_drafts if probs.is_cuda else plain_verify)(
+            probs, input_ids[0], packed.cu_seqlens, parents, draft_probs, uniforms)
+        cache.keep(packed, kept, path)
+        return SimpleNamespace(kept=kept, path=path, next_tokens=following, logits=logits[None])
 
     def preference_loss(self, input_ids, labels, packed, reference, beta=0.1, label_smoothing=0.0,
                         average=False):

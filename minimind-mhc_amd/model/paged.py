@@ -222,3 +222,279 @@ def paged_keep(planes: torch.Tensor, page_table: torch.Tensor, lengths: torch.Te
             "mhc_paged_keep")
     _written(planes)
     return new
+
+
+class DraftTree:
+    """Drafted tokens of a PackedBatch: each sequence's first row is its last token, the others a tree
+    behind it, parents before children.  A model call with drafts=DraftTree(...) over a PagedCache
+    stores them without moving the sequences on; PagedCache.keep then keeps a branch.
+
+    parents [rows] int32: the place in its sequence of the row that a row follows (the first row's
+    does not count; a row without a parent before it sees only itself and the past).  None: chains,
+    each row following the one before it.
+    mask [rows, words] int64 (None for chains): the rows that each row sees, as paged_attention takes
+    them; depths [rows] int32: their distance from the first row.  Both are formed here, on the
+    device, so other trees need another DraftTree (in a captured graph: formed inside it)."""
+
+    def __init__(self, batch: PackedBatch, parents: Optional[torch.Tensor] = None):
+        self.batch, self.parents, self.mask, self.depths = batch, parents, None, None
+        if parents is None:
+            return
+        rows, dev = batch.rows, batch.cu_seqlens.device
+        if parents.dtype != torch.int32 or tuple(parents.shape) != (rows,) or parents.device != dev:
+            raise ValueError(f"mhc_amd: parents must be int32 [{rows}] on {dev}, got {parents.dtype} "
+                             f"{tuple(parents.shape)} on {parents.device}")
+        most = rows if batch.longest is None else batch.longest
+        with torch.inference_mode(False):  # ordinary tensors, as the batch's
+            r, place = torch.arange(rows, device=dev), batch.positions
+            first = r - place
+            up = parents.long()
+            good = (up >= 0) & (up < place) & (batch.sequence < len(batch))
+            jump = torch.cat([torch.where(good, first + up, rows), r.new_full((1,), rows)])  # the last: none
+            mask = torch.zeros(rows + 1, max((most + 63) // 64, 1), dtype=torch.int64, device=dev)
+            inside = place < 64 * mask.shape[1]
+            word = torch.where(inside, place // 64, 0)
+            mask[r, word] = torch.where(inside, torch.ones_like(r) << (place % 64), 0)
+            depth = torch.cat([good.int(), r.new_zeros(1, dtype=torch.int32)])
+            step = 1
+            while step < most:  # each round doubles the ancestors that a row has joined with
+                mask |= mask[jump]
+                depth += depth[jump]
+                jump = jump[jump]
+                step *= 2
+            self.mask, self.depths = mask[:rows].contiguous(), depth[:rows].contiguous()
+
+
+class PagedCache:
+    """Keys and values of n sequences in pages that are handed out as the sequences grow: pass it as
+    past_key_values with a PackedBatch of n sequences.
+
+    capacity: the most keys a sequence may have; page: rows of a page, a power of two of at least
+    16; pages: how many there are for all sequences together (default: enough for every one to reach
+    its capacity).  The kernels read and write the pages in place; a sequence's pages stand in
+    page_table [n, width] (int32, -1: none), its keys in lengths [n] (int32), both on the device.
+
+    A call's new rows need pages before it: a call with a batch made from_lengths hands them out by
+    itself, as does reserve(), and raises where none are left.  The host counts what the sequences may
+    have at most; after keep(), which only the device knows the result of, it counts all of a tree's
+    rows, until settle() looks at the lengths and takes back the pages that are not needed.  A call that
+    is captured into a graph hands out none: reserve() what its replays will need before.  Rows that
+    have no page are dropped, and their sequence's outputs mean nothing from then on."""
+
+    def __init__(self, config, sequences: int, capacity: int, page: int = 64, pages: Optional[int] = None,
+                 dtype=torch.bfloat16, device="cuda"):
+        if sequences < 1 or capacity < 1:
+            raise ValueError(f"mhc_amd: a cache of {sequences} sequences of {capacity} keys")
+        if page < 16 or page & (page - 1):
+            raise ValueError(f"mhc_amd: a page must have a power of two of at least 16 rows, got {page}")
+        width = (capacity + page - 1) // page
+        pages = sequences * width if pages is None else pages
+        if pages < 1:
+            raise ValueError(f"mhc_amd: a cache of {pages} pages")
+        with torch.inference_mode(False):  # ordinary tensors: a cache outlives the mode it is made in
+            self.planes = torch.zeros(2 * config.num_hidden_layers, pages, page, config.num_key_value_heads,
+                                      config.head_dim, dtype=dtype, device=device)
+            self.page_table = torch.full((sequences, width), -1, dtype=torch.int32, device=device)
+            self.lengths = torch.zeros(sequences, dtype=torch.int32, device=device)
+        self.layers = [(self.planes[2 * i], self.planes[2 * i + 1]) for i in range(config.num_hidden_layers)]
+        self.sequences, self.capacity, self.page = sequences, capacity, page
+        self.clear()
+
+    def clear(self) -> None:
+        """Empties every sequence and takes all pages back."""
+        self.most = [0] * self.sequences  # keys that each sequence has at most
+        self.owned = [[] for _ in range(self.sequences)]
+        self.free_pages = list(range(self.planes.shape[1]))[::-1]
+        self.lengths.zero_()
+        self.page_table.fill_(-1)
+
+    def free(self, sequence: int) -> None:
+        """Empties a sequence and takes its pages back."""
+        self.free_pages += self.owned[sequence][::-1]
+        self.owned[sequence], self.most[sequence] = [], 0
+        self.lengths[sequence] = 0
+        self.page_table[sequence] = -1
+
+    def reserve(self, rows) -> None:
+        """Pages for so many more rows of each sequence (a number, or one for each): all of them or, with
+        an error, none."""
+        rows = [int(rows)] * self.sequences if not hasattr(rows, "__len__") else [int(n) for n in rows]
+        if len(rows) != self.sequences:
+            raise ValueError(f"mhc_amd: rows of {len(rows)} sequences for a cache of {self.sequences}")
+        need = []
+        for i, n in enumerate(rows):
+            if n and self.most[i] + n > self.capacity:
+                raise ValueError(f"mhc_amd: {self.most[i]} + {n} keys may not fit a sequence's {self.capacity}")
+            need.append(max(0, -(-(self.most[i] + n) // self.page) - len(self.owned[i])) if n else 0)
+        if sum(need) > len(self.free_pages):
+            raise RuntimeError(f"mhc_amd: {sum(need)} pages needed, {len(self.free_pages)} left")
+        if not any(need):
+            return
+        seqs, slots, numbers = [], [], []
+        for i, n in enumerate(need):
+            for _ in range(n):
+                seqs.append(i)
+                slots.append(len(self.owned[i]))
+                numbers.append(self.free_pages.pop())
+                self.owned[i].append(numbers[-1])
+        at = torch.tensor([seqs, slots], device=self.page_table.device)
+        self.page_table[at[0], at[1]] = torch.tensor(numbers, dtype=torch.int32, device=self.page_table.device)
+
+    def settle(self) -> None:
+        """Looks at the lengths (a synchronisation) and takes back the pages behind them."""
+        self.most = [min(max(n, 0), self.capacity) for n in self.lengths.tolist()]
+        seqs, slots = [], []
+        for i, n in enumerate(self.most):
+            keep = -(-n // self.page)
+            slots += range(keep, len(self.owned[i]))
+            seqs += [i] * (len(self.owned[i]) - keep)
+            self.free_pages += self.owned[i][keep:][::-1]
+            del self.owned[i][keep:]
+        if seqs:
+            self.page_table[seqs, slots] = -1
+
+    def grown(self, batch: PackedBatch) -> torch.Tensor:
+        """The lengths with the batch's rows, as far as there is room."""
+        return (self.lengths + batch.cu_seqlens.diff()).clamp_max_(self.page_table.shape[1] * self.page)
+
+    def keep(self, batch: PackedBatch, kept: torch.Tensor, path: torch.Tensor) -> None:
+        """Keeps the accepted rows of a call with drafts (verify_drafts' kept and path): moves their keys
+        and values together in every layer, and the lengths on."""
+        if len(batch) != self.sequences:
+            raise ValueError(f"mhc_amd: a batch of {len(batch)} sequences on a cache of {self.sequences}")
+        if self.planes.is_cuda:
+            new = paged_keep(self.planes, self.page_table, self.lengths, batch.cu_seqlens, kept, path)
+        else:
+            new = self._plain_keep(batch, kept, path)
+        self.lengths.copy_(new)
+        self._count(batch)
+
+    def _count(self, batch: PackedBatch) -> None:
+        """The rows of a call, as far as the host knows them (a captured call has stored none)."""
+        if self.lengths.is_cuda and torch.cuda.is_current_stream_capturing():
+            return
+        new = [batch.rows] * self.sequences if batch.lengths is None else batch.lengths
+        self.most = [min(a + b, self.capacity) for a, b in zip(self.most, new)]
+
+    def rows_of(self, sequence: torch.Tensor, key: torch.Tensor) -> torch.Tensor:
+        """Rows of a plane, its pages one after another, of keys of sequences; -1 where there is none."""
+        width, pages = self.page_table.shape[1], self.planes.shape[1]
+        inside = (sequence < self.sequences) & (key >= 0) & (key < width * self.page)
+        number = self.page_table[sequence.clamp_max(self.sequences - 1), (key // self.page).clamp(0, width - 1)]
+        inside &= (number >= 0) & (number < pages)
+        return torch.where(inside, number.long() * self.page + key % self.page, -1)
+
+    def _plain_keep(self, batch, kept, path):
+        seq, place = batch.sequence, batch.positions
+        count = batch.cu_seqlens.diff()
+        kept = torch.minimum(kept, count).clamp_min(0)
+        at = seq.clamp_max(self.sequences - 1)
+        go = (seq < self.sequences) & (place < kept[at]) & (path > place) & (path < count[at])
+        src = self.rows_of(at, (self.lengths[at] + path).long())
+        dst = self.rows_of(at, (self.lengths[at] + place).long())
+        go &= (src >= 0) & (dst >= 0)
+        flat = self.planes.flatten(1, 2)
+        flat[:, dst[go]] = flat[:, src[go]]
+        return (self.lengths + kept).clamp_max(self.page_table.shape[1] * self.page)
+
+
+class PagedCall:
+    """One model call on a PackedBatch over a PagedCache: where its rows stand."""
+
+    def __init__(self, batch: PackedBatch, cache: PagedCache, drafts: Optional[DraftTree] = None):
+        if len(batch) != cache.sequences:
+            raise ValueError(f"mhc_amd: a batch of {len(batch)} sequences on a cache of {cache.sequences}")
+        if drafts is not None and drafts.batch is not batch:
+            raise ValueError("mhc_amd: drafts of another batch")
+        self.batch, self.cache, self.drafts = batch, cache, drafts
+        capturing = cache.lengths.is_cuda and torch.cuda.is_current_stream_capturing()
+        # positions that the host knows the sequences reach, and a bound on those they may reach
+        self.reach, self.most = 0, cache.capacity
+        if batch.lengths is not None:
+            self.reach = max((n for n in batch.lengths), default=0)
+            if not capturing:
+                cache.reserve(batch.lengths)
+        self.depths = None if drafts is None else drafts.depths
+        deep = batch.positions if self.depths is None else self.depths.long()
+        self.past = cache.lengths[batch.sequence.clamp_max(cache.sequences - 1)]
+        self.positions = self.past + deep
+
+    def within(self, table: int) -> None:
+        """Rows past a table of so many positions take its last one (their outputs mean nothing; as NaN
+        they would reach the other rows of their sequences)."""
+        self.depths = (self.positions.clamp(0, table - 1) - self.past).int()
+
+    def done(self) -> None:
+        """The call has stored its rows: without drafts they stay."""
+        if self.drafts is None:
+            self.cache.lengths.copy_(self.cache.grown(self.batch))
+            self.cache._count(self.batch)
+
+    def attention(self, m, q, k, v, tables, layer: int) -> torch.Tensor:
+        """q [1, rows, heads, head_dim], k, v [1, rows, kv heads, head_dim], the projections of the
+        attention layer m: [1, rows, heads * head_dim]; tables: cos and sin, [positions, rotary_dim / 2]."""
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+            raise RuntimeError("mhc_amd: a cache is for inference; call under torch.no_grad()")
+        q, k, v, dtype = q[0], k[0], v[0], q.dtype
+        cache, cu, tree = self.cache, self.batch.cu_seqlens, self.drafts
+        kp, vp = cache.layers[layer]
+        if self._fused(m, q, kp):
+            q, k, v = (t if t.dtype == kp.dtype else t.to(kp.dtype) for t in (q, k, v))
+            q = paged_append(q, k, v, kp, vp, cache.page_table, cache.lengths, cu, *tables,
+                             depths=self.depths, q_gain=m.q_norm.weight,
+                             k_gain=m.k_norm.weight, eps=m.q_norm.eps, interleaved=m.rope_interleaved)
+            out = paged_attention(q, kp, vp, cache.page_table, cache.lengths, cu, tree=None if tree is None else tree.mask)
+        else:
+            at = self.positions if self.depths is None else self.past + self.depths
+            q, k = plain_rotary(m.q_norm(q), m.k_norm(k), *tables, at, m.rope_interleaved)
+            out = self._plain(q.to(kp.dtype), k.to(kp.dtype), v.to(kp.dtype), kp, vp, m.dropout if m.training else 0.0)
+        if out.dtype != dtype and not torch.is_autocast_enabled(out.device.type):
+            out = out.to(dtype)
+        return out.reshape(1, out.shape[0], -1)
+
+    @staticmethod
+    def _fused(m, q, pages) -> bool:
+        """Whether the kernels take this layer's norms and types, in a call that nothing traces."""
+        norms = (m.q_norm, m.k_norm)
+        return (q.is_cuda and pages.dtype in _ops.HALF and q.shape[2] in HEAD_DIMS and _ops.eager_call()
+                and not (m.training and m.dropout > 0)
+                and all(_ops.plain_module(n, torch.nn.RMSNorm) and n.weight is not None and n.eps is not None
+                        and n.weight.dtype in (torch.float32, *_ops.HALF) for n in norms)
+                and m.q_norm.eps == m.k_norm.eps)
+
+    def _plain(self, q, k, v, kp, vp, dropout):
+        """Storing and attention on torch ops, for what the kernels do not take: one attention under a
+        mask over all sequences' keys."""
+        cache, batch, tree = self.cache, self.batch, self.drafts
+        n, room = cache.sequences, cache.page_table.shape[1] * cache.page
+        seq, dev = batch.sequence, q.device
+        mine = seq.clamp_max(n - 1)
+        past = cache.lengths.clamp(0, room).long()
+        rows = cache.rows_of(seq, past[mine] + batch.positions)
+        there = rows >= 0
+        kf, vf = kp.flatten(0, 1), vp.flatten(0, 1)
+        kf[rows[there]], vf[rows[there]] = k[there], v[there]
+        have = torch.minimum(past + batch.cu_seqlens.diff(), past.new_full((), room))
+        owner = torch.arange(n, device=dev).repeat_interleave(room)
+        key = torch.arange(room, device=dev).repeat(n)
+        at = cache.rows_of(owner, key)
+        real = (at >= 0) & (key < have[owner])
+        fresh = key - past[owner]  # place among the new rows
+        seen = (seq[:, None] == owner) & real
+        if tree is None or tree.mask is None:
+            seen &= fresh <= batch.positions[:, None]
+        else:
+            bit = fresh.clamp(0, 64 * tree.mask.shape[1] - 1)
+            own = (tree.mask[:, bit // 64] >> (bit % 64)) & 1 == 1
+            seen &= (fresh < 0) | own & (fresh < 64 * tree.mask.shape[1])
+        rep = q.shape[1] // kp.shape[2]
+        kk, vv = (t[at.clamp_min(0)] for t in (kf, vf))
+        # keys that are no numbers: a probability of 0 would not keep them from other rows
+        bad = real[:, None] & ~(torch.isfinite(kk).all(2) & torch.isfinite(vv).all(2))
+        kk, vv = (torch.where((real[:, None] & ~bad)[:, :, None], t, 0).repeat_interleave(rep, 1).transpose(0, 1) for t in (kk, vv))
+        some = seen.any(1)
+        out = torch.nn.functional.scaled_dot_product_attention(
+            q.transpose(0, 1)[None], kk[None], vv[None], attn_mask=seen | ~some[:, None], dropout_p=dropout)
+        out = torch.where(some[:, None, None], out[0].transpose(0, 1), 0)
+        hit = torch.stack([(seen & b).any(1) for b in bad.unbind(1)], 1)
+        return out.masked_fill(hit.repeat_interleave(rep, 1)[:, :, None], math.nan)

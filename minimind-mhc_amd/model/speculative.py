@@ -94,3 +94,60 @@ def verify_drafts(probs: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.T
             cu.data_ptr(), kept.data_ptr(), path.data_ptr(), following.data_ptr(), T, V, n, H.stream(dev)),
             "mhc_verify_drafts")
     return kept, path, following
+
+
+def plain_verify(probs, tokens, cu_seqlens, parents=None, draft_probs=None, uniforms=None):
+    """verify_drafts on the host, a sequence at a time, for tensors that are on no GPU."""
+    T, V = probs.shape
+    ends = [0, *(min(max(e, 0), T) for e in cu_seqlens.tolist()[1:])]
+    tokens = tokens.tolist()
+    up = parents.tolist() if parents is not None else None
+    u = uniforms.float().double().tolist() if uniforms is not None else None
+    p_all, q_all = (None if t is None else torch.where((t > 0) & torch.isfinite(t), t, 0).double() for t in (probs, draft_probs))
+    path, kept, following = torch.full((T,), -1, dtype=torch.int32), [], []
+    for a, b in zip(ends, ends[1:]):
+        if b <= a:
+            kept.append(0)
+            following.append(-1)
+            continue
+        node, count, j = 0, 1, 0
+        path[a] = 0
+
+        def enter():
+            raw = probs[a + node].float()
+            best = int(torch.where(raw.isnan(), -float("inf"), raw).argmax()) if u is None and not raw.isnan().all() else -1
+            return best, p_all[a + node].clone(), None if q_all is None else q_all[a + node], 0.0, 1.0
+        best, p, q, ratio, norm = enter()
+        for j in range(1, b - a):
+            parent = j - 1 if up is None else up[a + j]
+            if parent != node:
+                continue
+            x = tokens[a + j]
+            inside = 0 <= x < V
+            if u is None:
+                good = inside and x == best
+            else:
+                px, qx = float(p[x]) if inside else 0.0, 1.0 if q is None else float(q[x]) if inside else 0.0
+                good = u[a + j] * qx * norm < max(px - ratio * (0.0 if q is None else qx), 0.0)
+            if good:
+                node = j
+                path[a + count] = j
+                count += 1
+                best, p, q, ratio, norm = enter()
+            elif q is not None:
+                ratio += norm
+                norm = float((p - ratio * q).clamp_min(0).sum())
+            elif u is not None and inside:
+                norm = max(norm - px, 0.0)
+                p[x] = 0.0
+        if u is not None:
+            w = p if q is None else (p - ratio * q).clamp_min(0)
+            if not float(w.sum()) > 0:
+                w = p_all[a + node]
+            run = w.cumsum(0)
+            past = ((run > u[a] * run[-1]) & (w > 0)).nonzero()
+            some = (w > 0).nonzero()
+            best = int(past[0]) if len(past) else int(some[-1]) if len(some) else -1
+        kept.append(count)
+        following.append(best)
+    return torch.tensor(kept, dtype=torch.int32), path, torch.tensor(following, dtype=torch.int64)
