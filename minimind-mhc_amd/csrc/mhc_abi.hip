@@ -998,7 +998,7 @@ int mhc_verify_drafts(const void* probs, const void* draft_probs, int dtype, con
                       const float* uniforms, const int* cu, int* kept, int* path, int64_t* next, int64_t T, int V, int B,
                       hipStream_t stream) {
   const char* fn = "mhc_verify_drafts";
-  if (T < 0 || T > 1 << 30 || V < 1 || V > 1 << 30 || B < 0 || B > 1 << 22)
+  if (T < 0 || T > 1 << 30 || V < 1 || V > 1 << 28 || B < 0 || B > 1 << 22)
     return fail(hipErrorInvalidValue, "%s: bad shape (T=%lld V=%d B=%d)", fn, (long long)T, V, B);
   if (!dtype_ok(dtype)) return fail(hipErrorInvalidValue, "%s: bad dtype %d", fn, dtype);
   if (draft_probs && !uniforms) return fail(hipErrorInvalidValue, "%s: draft probabilities without random numbers", fn);

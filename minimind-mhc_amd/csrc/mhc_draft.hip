@@ -21,28 +21,30 @@ constexpr int kDraftGone = 64;     // rejected siblings that are kept at hand
 template <int DT>
 struct ProbRow {
   static constexpr int PER = DT == kF32 ? 4 : 8;  // elements of 16 bytes
-  // The row's elements lie in the tensor's 16-byte blocks: element e of the row is at e + off.
-  const char* base;
+  // The row's elements lie in the tensor's 16-byte blocks: element e of the row is at e + off.  Blocks
+  // are loaded through a descriptor that ends with the row's last word, without a branch, so all of a lane's are in
+  // flight together.
+  __amdgpu_buffer_rsrc_t rsrc;
   int off, V;
   __device__ void init(const void* p, int64_t row, int V_) {
     V = V_;
     const int64_t at = row * V;
-    off = (int)(at % PER);
-    base = static_cast<const char*>(p) + (at - off) * dtype_bytes(DT);
+    off = __builtin_amdgcn_readfirstlane((int)(at % PER));
+    const int64_t base = wave_uniform(reinterpret_cast<int64_t>(p) + (at - off) * dtype_bytes(DT));
+    rsrc = make_rsrc(reinterpret_cast<const void*>(base), ((uint32_t)(off + V) * dtype_bytes(DT) + 3) & ~3u);
   }
   __device__ int blocks() const { return (V + off + PER - 1) / PER; }
-  // A block's 16 bytes, 0 for the elements that are none of the row's.
-  __device__ __forceinline__ U32x4 raw(int block) const {
+  // A block's 16 bytes (none: zeros), and 0 for the elements that are none of the row's.
+  __device__ __forceinline__ U32x4 raw(int block, bool there) const {
+    return buf_load16(rsrc, oob_unless(there, (uint32_t)block * 16));
+  }
+  __device__ __forceinline__ void trim(int block, U32x4& w) const {
     const int e0 = block * PER - off;
-    if (e0 >= 0 && e0 + PER <= V) return ld16(base + (int64_t)block * 16);
-    uint32_t w[4] = {0, 0, 0, 0};
+    if (e0 < 0 || e0 + PER > V) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if ((unsigned)(e0 + i) < (unsigned)V) {
-        if constexpr (DT == kF32) w[i] = reinterpret_cast<const uint32_t*>(base)[(int64_t)block * PER + i];
-        else w[i / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(base)[(int64_t)block * PER + i] << (16 * (i & 1));
-      }
-    return U32x4{{w[0], w[1], w[2], w[3]}};
+      for (int i = 0; i < PER; ++i)
+        if ((unsigned)(e0 + i) >= (unsigned)V) w.v[DT == kF32 ? i : i / 2] &= DT == kF32 ? 0u : i & 1 ? 0xffffu : 0xffff0000u;
+    }
   }
   static __device__ __forceinline__ void open(const U32x4& w, float (&x)[PER]) {
 #pragma unroll
@@ -61,6 +63,17 @@ struct ProbRow {
 __device__ __forceinline__ double prob(float x) {
   x = fmaxf(x, 0.f);
   return (double)(x < __builtin_inff() ? x : 0.f);
+}
+// The same of the element of 16 bytes' word w (bf16: half `high` of it) where all of them are known to be
+// finite and not negative, in two or three integer operations (a conversion takes four times as long): fp32's
+// exponent and mantissa moved to their places.  Zero becomes 2^-127 (and the smallest numbers, which have no
+// implicit one, up to twice as large): nothing beside a probability that counts.
+__device__ __forceinline__ double fast64(uint32_t f) {
+  return __builtin_bit_cast(double, (uint64_t)((f >> 3) + 0x38000000u) << 32 | (uint64_t)(f << 29));
+}
+__device__ __forceinline__ double fast64_bf16(uint32_t w, bool high) {
+  const uint32_t b = high ? w >> 16 : w & 0xffffu;
+  return __builtin_bit_cast(double, (uint64_t)((b << 13) + 0x38000000u) << 32);
 }
 __device__ __forceinline__ double left_of(double p, double q, double a) { return fmax(p - a * q, 0.0); }
 
@@ -147,8 +160,48 @@ __global__ __launch_bounds__(64 * W) void verify_kernel(VerifyArgs a) {
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const int b = b0 + g * 64 + lane;
-        if (!held || !have_p) pw[g] = b < b1 ? P.raw(b) : U32x4{};
-        if (ratio > 0.0 && (!held || !have_q)) qw[g] = b < b1 ? Q.raw(b) : U32x4{};
+        if (!held || !have_p) pw[g] = P.raw(b, b < b1);
+        if (ratio > 0.0 && (!held || !have_q)) qw[g] = Q.raw(b, b < b1);
+      }
+      const bool edge = b0 == 0 || b0 + 64 * G >= nb;  // uniform: the row's first or last block is among them
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        if (!edge || b0 + g * 64 >= b1) break;
+        P.trim(b0 + g * 64 + lane, pw[g]);
+        if (ratio > 0.0) Q.trim(b0 + g * 64 + lane, qw[g]);
+      }
+      // Rows are finite and not negative: seen from the largest of their bits, taken as whole numbers.
+      bool fast = DT != kF16 && ratio > 0.0;
+      if (fast) {
+        uint32_t top = 0;
+        typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (DT == kF32)
+              top = max(top, max(pw[g].v[j], qw[g].v[j]));
+            else
+              top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top),
+                                       __builtin_elementwise_max(__builtin_bit_cast(u16x2, pw[g].v[j]), __builtin_bit_cast(u16x2, qw[g].v[j]))));
+          }
+        fast = !__any(DT == kF32 ? top >= 0x7f800000u : (top >> 16) >= 0x7f80u || (top & 0xffffu) >= 0x7f80u);
+      }
+      if (fast) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          if (b0 + g * 64 >= b1) break;  // uniform
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (DT == kF32) {
+              s += left_of(fast64(pw[g].v[j]), fast64(qw[g].v[j]), ratio);
+            } else {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) s += left_of(fast64_bf16(pw[g].v[j], h), fast64_bf16(qw[g].v[j], h), ratio);
+            }
+          }
+        }
+        continue;
       }
 #pragma unroll
       for (int g = 0; g < G; ++g) {
@@ -174,24 +227,31 @@ __global__ __launch_bounds__(64 * W) void verify_kernel(VerifyArgs a) {
     const int nb = P.blocks();
     float m = -__builtin_inff();
     int at = INT32_MAX;
-    constexpr int G = 4;
     for (int b0 = tid; b0 < nb; b0 += G * TH) {
       U32x4 pw[G];
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        pw[g] = U32x4{};
-        if (b0 + g * TH < nb) pw[g] = P.raw(b0 + g * TH);
-      }
+      for (int g = 0; g < G; ++g) pw[g] = P.raw(b0 + g * TH, b0 + g * TH < nb);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        float p[PER];
+        const int b = b0 + g * TH, e0 = b * PER - P.off;
+        if (b - tid >= nb) break;  // uniform
+        float p[PER], t = -__builtin_inff();
         ProbRow<DT>::open(pw[g], p);
+        if (e0 < 0 || e0 + PER > V) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const int v = (b0 + g * TH) * PER + i - P.off;
-          if ((unsigned)v < (unsigned)V && (p[i] > m || (p[i] == m && v < at))) {
-            m = p[i];
-            at = v;
+          for (int i = 0; i < PER; ++i)
+            if ((unsigned)(e0 + i) >= (unsigned)V) p[i] = __builtin_nanf("");
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) t = fmaxf(t, p[i]);
+        if (t > m || at == INT32_MAX) {  // seldom: the place of the block's first largest
+          int first = INT32_MAX;
+#pragma unroll
+          for (int i = PER - 1; i >= 0; --i)
+            if (p[i] == t) first = e0 + i;
+          if (first != INT32_MAX) {
+            m = t;
+            at = first;
           }
         }
       }
@@ -322,7 +382,13 @@ __global__ __launch_bounds__(64 * W) void verify_kernel(VerifyArgs a) {
     double s = 0.0;
     for (int b = t0; b < t1; ++b) {
       double w[PER];
-      weights(b, P.raw(b), ratio > 0.0 ? Q.raw(b) : U32x4{}, w);
+      U32x4 pw = P.raw(b, true), qw{};
+      if (ratio > 0.0) {
+        qw = Q.raw(b, true);
+        Q.trim(b, qw);
+      }
+      P.trim(b, pw);
+      weights(b, pw, qw, w);
 #pragma unroll
       for (int i = 0; i < PER; ++i) s += w[i];
     }
@@ -340,7 +406,13 @@ __global__ __launch_bounds__(64 * W) void verify_kernel(VerifyArgs a) {
     int first = INT32_MAX, most = -1;  // the first past the border, the last with a weight
     for (int b = t0; b < t1; ++b) {
       double w[PER];
-      weights(b, P.raw(b), ratio > 0.0 ? Q.raw(b) : U32x4{}, w);
+      U32x4 pw = P.raw(b, true), qw{};
+      if (ratio > 0.0) {
+        qw = Q.raw(b, true);
+        Q.trim(b, qw);
+      }
+      P.trim(b, pw);
+      weights(b, pw, qw, w);
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         cum += w[i];
