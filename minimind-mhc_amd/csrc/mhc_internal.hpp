@@ -423,7 +423,7 @@ struct PagedAttnArgs {
 void paged_attn_plan(PagedAttnArgs& a);
 int64_t paged_attn_workspace(const PagedAttnArgs& a);
 int64_t paged_attn_threads(const PagedAttnArgs& a);
-hipError_t launch_paged_attn(const PagedAttnArgs& a, hipStream_t s);
+hipError_t launch_paged_attn(PagedAttnArgs a, hipStream_t s);
 
 // Log-probabilities of labels under rows of logits [T, V] (rows `stride` elements apart).
 struct LogitArgs {

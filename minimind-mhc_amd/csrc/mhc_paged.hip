@@ -572,21 +572,24 @@ __global__ __launch_bounds__(64 * RW * KW, (paged_waves<HD, RW, KW, S>)) void pa
   }
 }
 
-// Joins the ranges of a row: a lane takes four columns of one of its heads; with P = 4 the workgroup's
-// waves take every fourth range of the same 64 of them, and the sums meet in LDS.  64 rows of 16
+// Joins the ranges of a row: a lane takes four columns of one of its heads, a wave 64 such; with P > 1 the
+// workgroup's P waves take every P-th range of the same 64, and the sums meet in LDS.  64 rows of 16
 // heads of 128 from 64 ranges: 6 us (P = 1: 25); 1024 rows of 8 heads of 96 from one to three: 11 us (5).
 template <bool F16, int HD, int KT, int P>
 __global__ __launch_bounds__(P == 16 ? 1024 : 256) void paged_join_kernel(PagedAttnArgs a) {
   __shared__ __align__(16) f32x4_t sums[P][64];
   __shared__ float2 marks[P][64];
   const int rep = a.heads / a.kv_heads, RB = a.block_rows;
-  const int row = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned chunks = (a.heads * (HD / 4) + 63) / 64;  // Tq of them: under 2^31 with Tq * heads
+  const unsigned at_wave = P == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
+  const int row = at_wave / chunks;
+  if (row >= a.Tq) return;
   const float* ml = a.work + (int64_t)a.units * a.kv_heads * RB * HD;
   PagedUnit u;
   int w = 0;
   if (!paged_find<KT>(a, 0, 0, w, u, row) || u.splits == 1) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int x = P == 1 ? blockIdx.z * 256 + threadIdx.x : blockIdx.z * 64 + lane;
+  const int x = (int)(at_wave % chunks) * 64 + lane;
   const bool live = x < a.heads * (HD / 4);
   const int head = live ? x / (HD / 4) : 0, col = live ? x % (HD / 4) * 4 : 0, kvh = head / rep;
   const int at = (row - u.start) * rep + head % rep;  // a head's row may begin the next block
@@ -636,14 +639,13 @@ hipError_t run_paged(const PagedAttnArgs& a, hipStream_t s) {
     constexpr int KT = RW == 1 ? 32 : 64;
     const int64_t most = ((int64_t)a.width << a.page_shift) / (KT * a.least);  // ranges that the pages have room for
     if (most == 0) return hipGetLastError();
-    const int items = a.heads * (HD / 4);  // of a row
-    const dim3 grid((unsigned)a.Tq, 1, (unsigned)((items + 63) / 64));
-    if ((int64_t)a.Tq * items > 512 * (int64_t)device_cus())
-      paged_join_kernel<F16, HD, KT, 1><<<dim3(grid.x, 1, (unsigned)((items + 255) / 256)), 256, 0, s>>>(a);
+    const int64_t waves = (int64_t)a.Tq * ((a.heads * (HD / 4) + 63) / 64);
+    if (waves > 8 * (int64_t)device_cus())
+      paged_join_kernel<F16, HD, KT, 1><<<dim3((unsigned)((waves + 3) / 4)), 256, 0, s>>>(a);
     else if (most < 64 || a.slots < 64 * paged_row_blocks(a))
-      paged_join_kernel<F16, HD, KT, 4><<<grid, 256, 0, s>>>(a);
+      paged_join_kernel<F16, HD, KT, 4><<<dim3((unsigned)waves), 256, 0, s>>>(a);
     else
-      paged_join_kernel<F16, HD, KT, 16><<<grid, 1024, 0, s>>>(a);
+      paged_join_kernel<F16, HD, KT, 16><<<dim3((unsigned)waves), 1024, 0, s>>>(a);
   }
   return hipGetLastError();
 }
@@ -691,10 +693,19 @@ int64_t paged_attn_workspace(const PagedAttnArgs& a) {
   return a.slots > 0 ? (int64_t)a.units * a.kv_heads * a.block_rows * (a.head_dim + 2) * 4 : 0;
 }
 int64_t paged_attn_threads(const PagedAttnArgs& a) {
-  const int64_t tiles = 256 * paged_blocks(a), join = a.slots > 0 ? 256 * (int64_t)a.Tq : 0;
+  const int64_t tiles = 256 * paged_blocks(a);
+  const int64_t join = a.slots > 0 ? 256 * (int64_t)a.Tq * ((a.heads * (a.head_dim / 4) + 63) / 64) : 0;  // at most
   return tiles > join ? tiles : join;
 }
 
-hipError_t launch_paged_attn(const PagedAttnArgs& a, hipStream_t s) { MHC_PACKED_HD(paged_hd, a, s) }
+hipError_t launch_paged_attn(PagedAttnArgs a, hipStream_t s) {
+  // Few short sequences, as far as their pages have room: four waves share a range and nothing is joined
+  // (one token, 8 / 4 heads of 96, over 300 keys: 11.8 us in ranges, 8.0 so; over 900: 12.3 and 12.7).
+  if (a.block_rows <= 32 && (int64_t)a.width << a.page_shift <= 768 && paged_row_blocks(a) * a.kv_heads <= device_cus()) {
+    a.slots = 0;
+    a.key_waves = 4;
+  }
+  MHC_PACKED_HD(paged_hd, a, s)
+}
 
 }  // namespace mhc
