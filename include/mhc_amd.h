@@ -609,11 +609,11 @@ int mhc_rotary(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void
 
 /* ---------------------------------------------------------- cache of pages
  * Key x of sequence i lies in page page_table[i, x / page] (int32 [B, width]), row x % page; a
- * page has a power of two of 16 to 2^20 rows, a sequence at most width * page <= 2^30 keys.  cu [B + 1]:
+ * page has a power of two of 16 to 2^20 rows, a sequence at most width * page <= 2^29 keys.  cu [B + 1]:
  * sequence i has the new rows cu[i] .. cu[i + 1], the first entry taken as 0; lengths [B]: the keys
  * before them, behind which those of the new rows stand.  All are device data: bounds and lengths are
  * clamped, keys of a page number outside 0 .. pages - 1 are not there.  Strides of pages, rows and heads
- * (the same in k_pages and v_pages) are in elements, multiples of 8, those of rows under 2^23.  16-bit tensors of one dtype, T <= 2^30.
+ * (the same in k_pages and v_pages) are in elements, multiples of 8, those of rows under 2^23.  16-bit tensors of one dtype, T <= 2^29.
  */
 
 /* Stores k and v of the new rows and rotates q: with gains ([head_dim], fp32, bf16 or fp16; either may be NULL)

@@ -878,11 +878,12 @@ int mhc_rotary(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void
 
 // Shared checks of the entry points on pages; gives the shift of the page size.
 static int check_pages(int64_t T, int B, int width, int pages, int page, int* shift, const char* fn) {
-  if (T < 0 || T > 1 << 30 || B < 0 || width < 0 || pages < 0)
+  if (T < 0 || T > 1 << 29 || B < 0 || width < 0 || pages < 0)
     return fail(hipErrorInvalidValue, "%s: bad shape (T=%lld B=%d width=%d pages=%d)", fn, (long long)T, B, width, pages);
   if (page < 16 || page > 1 << 20 || (page & (page - 1)) != 0)
     return fail(hipErrorInvalidValue, "%s: a page must have a power of two of 16 to 2^20 rows (got %d)", fn, page);
-  if ((int64_t)width * page > 1 << 30) return fail(hipErrorInvalidValue, "%s: at most 2^30 keys a sequence", fn);
+  // positions and keys behind them are ints
+  if ((int64_t)width * page > 1 << 29) return fail(hipErrorInvalidValue, "%s: at most 2^29 keys a sequence", fn);
   *shift = __builtin_ctz((unsigned)page);
   return 0;
 }
@@ -937,7 +938,7 @@ int64_t mhc_paged_attn_workspace_bytes(int B, int64_t Tq, int heads, int kv_head
   const char* fn = "mhc_paged_attn_workspace_bytes";
   mhc::PagedAttnArgs a{};
   a.B = B; a.Tq = (int)Tq; a.heads = heads; a.kv_heads = kv_heads; a.head_dim = head_dim; a.scale = 1.f;
-  if (B < 0 || Tq < 0 || Tq > 1 << 30 || check_paged(a, Tq, mhc::kBF16, fn)) return -1;
+  if (B < 0 || Tq < 0 || Tq > 1 << 29 || check_paged(a, Tq, mhc::kBF16, fn)) return -1;
   if (Tq == 0) return 0;
   mhc::paged_attn_plan(a);
   if (check_threads(mhc::paged_attn_threads(a), fn)) return -1;
@@ -998,9 +999,10 @@ int mhc_verify_drafts(const void* probs, const void* draft_probs, int dtype, con
                       const float* uniforms, const int* cu, int* kept, int* path, int64_t* next, int64_t T, int V, int B,
                       hipStream_t stream) {
   const char* fn = "mhc_verify_drafts";
-  if (T < 0 || T > 1 << 30 || V < 1 || V > 1 << 28 || B < 0 || B > 1 << 22)
+  if (T < 0 || T > 1 << 30 || V < 1 || V > 1 << 28 || B < 0)
     return fail(hipErrorInvalidValue, "%s: bad shape (T=%lld V=%d B=%d)", fn, (long long)T, V, B);
   if (!dtype_ok(dtype)) return fail(hipErrorInvalidValue, "%s: bad dtype %d", fn, dtype);
+  if (int rc = check_threads((int64_t)B * 1024, fn)) return rc;
   if (draft_probs && !uniforms) return fail(hipErrorInvalidValue, "%s: draft probabilities without random numbers", fn);
   if (B == 0) return 0;
   if ((T > 0 && (!probs || !tokens || !path)) || !cu || !kept || !next || !aligned16(probs) || !aligned16(draft_probs))

@@ -139,8 +139,8 @@ __device__ __forceinline__ bool paged_find(const PagedAttnArgs& a, int xcd, int 
         u.first = (row - u.start) * rep / RB * RB;
         w = base + u.first / RB;
       } else {
-        u.split = (w - base) / u.blocks;
-        u.first = (w - base) % u.blocks * RB;
+        u.split = min(max((w - base) / u.blocks, 0), u.splits - 1);  // the bounds of both: where cu decreases
+        u.first = max((w - base) % u.blocks, 0) * RB;
       }
       return true;
     }

@@ -162,7 +162,7 @@ class Attention(nn.Module):
         self.q_norm = nn.RMSNorm(self.head_dim, eps=config.rms_norm_eps)
         self.k_norm = nn.RMSNorm(self.head_dim, eps=config.rms_norm_eps)
         self.dropout = config.dropout
-        self.rope_interleaved = config.rope_interleaved
+        self.rope_interleaved = getattr(config, "rope_interleaved", False)
 
     def forward(self, x, position_embeddings, past_key_value=None, use_cache=False,
                 attention_mask=None, packed=None, layer_id=0):
@@ -392,8 +392,9 @@ class MiniMindModel(nn.Module):
             self.embed_up_norm = nn.Identity()
             self.layers = nn.ModuleList([MiniMindBlock(i, config) for i in range(self.num_hidden_layers)])
             self.norm = nn.RMSNorm(D, eps=eps)
-        self.own_pairs = config.rotary_dim != config.head_dim or config.rope_interleaved
-        cos, sin = precompute_freqs_cis(config.rotary_dim, config.max_position_embeddings,
+        rotary_dim = getattr(config, "rotary_dim", config.head_dim)
+        self.own_pairs = rotary_dim != config.head_dim or getattr(config, "rope_interleaved", False)
+        cos, sin = precompute_freqs_cis(rotary_dim, config.max_position_embeddings,
                                         config.rope_theta, config.rope_scaling)
         self.register_buffer("freqs_cos", cos, persistent=False)
         self.register_buffer("freqs_sin", sin, persistent=False)

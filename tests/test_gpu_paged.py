@@ -424,3 +424,56 @@ def test_keep_senseless_paths_and_no_pages(dev):
     paged_keep(pool.planes, pool.table, ints([30], dev), ints([0, 8], dev), ints([4], dev), ints([1, 5, 6, 7, 0, 0, 0, 0], dev))
     pool.planes.flatten(1, 2)[:, pool.at(0, 30, 32)[:1]] = before.flatten(1, 2)[:, pool.at(0, 30, 32)[:1]]
     assert torch.equal(pool.planes, before)
+
+
+# ------------------------------------------------------------------- refusals
+
+@pytest.mark.gpu
+def test_refusals(dev):
+    """Wrong shapes, types and layouts raise, and write nothing."""
+    from model.rotary import rotary
+    from model.speculative import verify_drafts
+    pool, q = make(dev, BF, [20, 5], [3, 2], 16, 4, 2, 64)
+    k = torch.randn(5, 2, 64, device=dev).to(BF)
+    cu, lens, table = ints([0, 3, 5], dev), ints([20, 5], dev), pool.table
+    cos, sin = (t.to(dev) for t in tables(40, 64))
+    before = pool.planes.clone()
+
+    def app(q=q, k=k, v=k, kp=pool.k, vp=pool.v, table=table, lens=lens, cu=cu, cos=cos, sin=sin, **kw):
+        return paged_append(q, k, v, kp, vp, table, lens, cu, cos, sin, **kw)
+
+    def att(q=q, kp=pool.k, vp=pool.v, table=table, lens=lens, cu=cu, **kw):
+        return paged_attention(q, kp, vp, table, lens, cu, **kw)
+    odd = torch.empty(2 * 6 * 16 * 2 * 64 + 1, dtype=BF, device=dev)[1:].view(2, 6, 16, 2, 64)
+    grad = q.clone().requires_grad_()
+    wide = torch.zeros(6, 16, 2, 68, dtype=BF, device=dev)[..., :64]
+    bad = [
+        lambda: app(q=q.float()), lambda: app(k=k.to(F16)), lambda: app(v=k[:4]), lambda: app(q=q[:, :, :32]),
+        lambda: app(lens=lens.long()), lambda: app(lens=lens[:1]), lambda: app(cu=cu.cpu()), lambda: app(table=table[:1]),
+        lambda: app(table=table.long()), lambda: app(table=table[0]), lambda: app(cos=cos[0]), lambda: app(cos=cos[:, :16]),
+        lambda: app(sin=sin.to(BF)), lambda: app(depths=ints([0, 1], dev)), lambda: app(q_gain=torch.ones(32, device=dev)),
+        lambda: app(kp=odd[0], vp=odd[1]), lambda: app(kp=pool.k[:, :8], vp=pool.v[:, :8]), lambda: app(vp=pool.v[:2]),
+        lambda: app(kp=wide, vp=wide), lambda: app(q=grad), lambda: app(kp=pool.k.float(), vp=pool.v.float()),
+        lambda: att(q=q.float()), lambda: att(q=grad), lambda: att(q=q[:, :3]), lambda: att(q=q[0]), lambda: att(scale=0.0),
+        lambda: att(scale=-1.0), lambda: att(scale=math.nan), lambda: att(tree=torch.ones(5, 1, dtype=torch.int32, device=dev)),
+        lambda: att(tree=torch.ones(4, 1, dtype=torch.int64, device=dev)), lambda: att(tree=torch.ones(5, 0, dtype=torch.int64, device=dev)),
+        lambda: att(tree=torch.ones(5, 1, dtype=torch.int64)), lambda: att(kp=pool.k[..., :32], vp=pool.v[..., :32]),
+        lambda: paged_keep(pool.planes[:, ::2], table, lens, cu, lens, lens), lambda: paged_keep(pool.k, table, lens, cu, lens, lens),
+        lambda: paged_keep(pool.planes, table, lens, cu, lens.long(), lens),
+        lambda: paged_keep(pool.planes[..., :1].contiguous()[..., :1, :], table, lens, cu, lens, lens),
+        lambda: rotary(q, k.float(), cos, sin, torch.arange(5, device=dev)), lambda: rotary(q, k[:4], cos, sin, torch.arange(5, device=dev)),
+        lambda: rotary(q, k, cos, sin, torch.arange(4, device=dev)), lambda: rotary(q, k, cos, sin, torch.arange(5, device=dev).float()),
+        lambda: rotary(q, k, cos.repeat(1, 2), sin.repeat(1, 2), torch.arange(5, device=dev)),
+        lambda: rotary(q, k, cos.clone().requires_grad_(), sin, torch.arange(5, device=dev)),
+        lambda: rotary(q.double(), None, cos, sin, torch.arange(5, device=dev)),
+    ]
+    p, t = torch.rand(5, 9, device=dev), torch.zeros(5, dtype=torch.int64, device=dev)
+    bad += [lambda: verify_drafts(p[0], t, cu), lambda: verify_drafts(p.double(), t, cu), lambda: verify_drafts(p, t.int(), cu),
+            lambda: verify_drafts(p, t[:4], cu), lambda: verify_drafts(p, t, cu, parents=t), lambda: verify_drafts(p, t, cu, draft_probs=p),
+            lambda: verify_drafts(p, t, cu, draft_probs=p[:, :8], uniforms=p[:, 0]), lambda: verify_drafts(p, t, cu.long()),
+            lambda: verify_drafts(p, t, cu, uniforms=t), lambda: verify_drafts(p, t, cu, uniforms=p[:4, 0])]
+    for i, f in enumerate(bad):
+        with pytest.raises((TypeError, ValueError, RuntimeError), match="mhc_amd"):
+            f()
+            print("not refused:", i)
+    assert torch.equal(pool.planes.isnan(), before.isnan()) and torch.equal(pool.planes.nan_to_num(), before.nan_to_num())
