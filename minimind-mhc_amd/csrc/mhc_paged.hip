@@ -18,7 +18,7 @@ constexpr int kPagedSeqs = 256;  // up to so many, workgroups are dealt out by t
 // sequence, over part `split` of `splits` of the keys they see.
 struct PagedUnit {
   int seq, start, n, past, len;
-  int first, split, splits, blocks;
+  int first, split, splits, blocks, base;
 };
 struct PagedSeq {
   int start, n, past, len;
@@ -52,10 +52,8 @@ __device__ __forceinline__ double wave_total(double v) {
 // The blocks of one range are neighbours.  Behind the sequences' units come those that clear the
 // rows behind the last one (seq = B).  Workgroup `at` of XCD `xcd` takes the at-th of an eighth of
 // the units: neighbours, which read the same keys, share its L2.
-// `row` >= 0: instead the first range's unit of the block with that row (of Tq), and the distance
-// to the next range's.
 template <int KT>
-__device__ __forceinline__ bool paged_find(const PagedAttnArgs& a, int xcd, int at_xcd, int& w, PagedUnit& u, int row) {
+__device__ __forceinline__ bool paged_find(const PagedAttnArgs& a, int xcd, int at_xcd, int& w, PagedUnit& u) {
   const int lane = __lane_id(), rep = a.heads / a.kv_heads, RB = a.block_rows;
   if (a.B > kPagedSeqs) {  // sequence i has the unit numbers from start(i) rep / RB + i on
     w = at_xcd * 8 + xcd;
@@ -71,7 +69,7 @@ __device__ __forceinline__ bool paged_find(const PagedAttnArgs& a, int xcd, int 
     const bool in = lo < a.B;
     const int first = seq_start(a.cu, lo, a.Tq);
     const PagedSeq q = paged_seq(a, lo, first, in ? a.cu[lo + 1] : a.Tq, in ? a.lengths[lo] : 0);
-    u = PagedUnit{lo, q.start, q.n, q.past, q.len, 0, 0, 1, 1};
+    u = PagedUnit{lo, q.start, q.n, q.past, q.len, 0, 0, 1, 1, 0};
     const int64_t at = (w - ((int64_t)first * rep / RB + lo)) * RB;
     if (at < 0 || at >= (int64_t)q.n * rep) return false;
     u.first = (int)at;
@@ -113,17 +111,15 @@ __device__ __forceinline__ bool paged_find(const PagedAttnArgs& a, int xcd, int 
     }
   }
   const int end = seq_start(a.cu, a.B, a.Tq);
-  if (row < 0) {  // with the units of the rows behind the last sequence
-    const int eighth = (all + (int)(((int64_t)(a.Tq - end) * rep + RB - 1) / RB) + 7) / 8;
-    if (at_xcd >= eighth) return false;
-    w = xcd * eighth + at_xcd;
-  }
+  // with the units of the rows behind the last sequence
+  const int eighth = (all + (int)(((int64_t)(a.Tq - end) * rep + RB - 1) / RB) + 7) / 8;
+  if (at_xcd >= eighth) return false;
+  w = xcd * eighth + at_xcd;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     if (c * 64 >= a.B) break;
     const int first = inc[c] - blocks[c] * splits[c];
-    const bool mine = row >= 0 ? q[c].n > 0 && row >= q[c].start && row < q[c].start + q[c].n : first <= w && w < inc[c];
-    const uint64_t who = __ballot(mine);
+    const uint64_t who = __ballot(first <= w && w < inc[c]);
     if (who) {
       const int l = __ffsll((unsigned long long)who) - 1;
       u.seq = c * 64 + l;
@@ -134,24 +130,23 @@ __device__ __forceinline__ bool paged_find(const PagedAttnArgs& a, int xcd, int 
       u.splits = __builtin_amdgcn_readlane(splits[c], l);
       u.blocks = __builtin_amdgcn_readlane(blocks[c], l);
       const int base = __builtin_amdgcn_readlane(first, l);
-      if (row >= 0) {
-        u.split = 0;
-        u.first = (row - u.start) * rep / RB * RB;
-        w = base + u.first / RB;
-      } else {
-        u.split = min(max((w - base) / u.blocks, 0), u.splits - 1);  // the bounds of both: where cu decreases
-        u.first = max((w - base) % u.blocks, 0) * RB;
-      }
+      u.base = base;
+      u.split = min(max((w - base) / u.blocks, 0), u.splits - 1);  // the bounds of both: where cu decreases
+      u.first = max((w - base) % u.blocks, 0) * RB;
       return true;
     }
   }
-  if (row >= 0) return false;
   // the rows behind the last sequence
   const int64_t at = (int64_t)(w - all) * RB;
-  u = PagedUnit{a.B, end, a.Tq - end, 0, 0, 0, 0, 1, 1};
+  u = PagedUnit{a.B, end, a.Tq - end, 0, 0, 0, 0, 1, 1, 0};
   if (at < 0 || at >= (int64_t)u.n * rep) return false;
   u.first = (int)at;
   return true;
+}
+
+// The units of each sequence, [B]: its first row, its first unit, blocks of rows, ranges.
+__device__ __forceinline__ int4* paged_units(const PagedAttnArgs& a) {
+  return reinterpret_cast<int4*>(a.work + (int64_t)a.units * a.kv_heads * a.block_rows * (a.head_dim + 2));
 }
 
 // A wave's uniform read of the page table, by the scalar unit.
@@ -192,7 +187,7 @@ __global__ __launch_bounds__(64 * RW * KW, (paged_waves<HD, RW, KW, S>)) void pa
   const int kvh = in / 8;
   int w = 0;
   PagedUnit t;
-  if (!paged_find<KT>(a, in % 8, blockIdx.x / (8 * a.kv_heads), w, t, -1) || w >= a.units) return;
+  if (!paged_find<KT>(a, in % 8, blockIdx.x / (8 * a.kv_heads), w, t) || w >= a.units) return;
   for (int* x : {&t.seq, &t.start, &t.n, &t.past, &t.len, &t.first, &t.split, &t.splits, &w}) *x = __builtin_amdgcn_readfirstlane(*x);
   const int rows = t.n * rep;
   const int last_token = (min(t.first + RB, rows) - 1) / rep;
@@ -498,6 +493,9 @@ __global__ __launch_bounds__(64 * RW * KW, (paged_waves<HD, RW, KW, S>)) void pa
 
   // ---- results
   const bool whole = t.splits == 1;
+  // for the join: where the sequence's units are
+  if (a.slots > 0 && t.first == 0 && t.split == 0 && kvh == 0 && tid == 0 && t.seq < a.B)
+    paged_units(a)[t.seq] = make_int4(t.start, t.base, t.blocks, t.splits);
   auto place = [&](int row) {  // of the output
     const int tok = row / rep;
     return ((int64_t)(t.start + tok) * a.heads + kvh * rep + row - tok * rep) * HD;
@@ -575,7 +573,7 @@ __global__ __launch_bounds__(64 * RW * KW, (paged_waves<HD, RW, KW, S>)) void pa
 // Joins the ranges of a row: a lane takes four columns of one of its heads, a wave 64 such; with P > 1 the
 // workgroup's P waves take every P-th range of the same 64, and the sums meet in LDS.  64 rows of 16
 // heads of 128 from 64 ranges: 6 us (P = 1: 25); 1024 rows of 8 heads of 96 from one to three: 11 us (5).
-template <bool F16, int HD, int KT, int P>
+template <bool F16, int HD, int P>
 __global__ __launch_bounds__(P == 16 ? 1024 : 256) void paged_join_kernel(PagedAttnArgs a) {
   __shared__ __align__(16) f32x4_t sums[P][64];
   __shared__ float2 marks[P][64];
@@ -586,15 +584,25 @@ __global__ __launch_bounds__(P == 16 ? 1024 : 256) void paged_join_kernel(PagedA
   const int row = at_wave / chunks;
   if (row >= a.Tq) return;
   const float* ml = a.work + (int64_t)a.units * a.kv_heads * RB * HD;
-  PagedUnit u;
-  int w = 0;
-  if (!paged_find<KT>(a, 0, 0, w, u, row) || u.splits == 1) return;
+  int lo = 0, hi = a.B + 1;  // the last sequence that begins at or before the row
+  while (hi - lo > 1) {
+    const int step = (hi - lo - 1 + 63) / 64;
+    const int64_t at = lo + (int64_t)(lane + 1) * step;
+    const bool below = at < hi && seq_start(a.cu, (int)(at < hi ? at : lo), a.Tq) <= row;
+    lo += __popcll(__ballot(below)) * step;
+    hi = min(hi, lo + step);
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  if (lo >= a.B) return;
+  const int4 u = paged_units(a)[lo];
+  const int blocks = max(u.z, 1);
+  if (u.w == 1) return;
   const int x = (int)(at_wave % chunks) * 64 + lane;
   const bool live = x < a.heads * (HD / 4);
   const int head = live ? x / (HD / 4) : 0, col = live ? x % (HD / 4) * 4 : 0, kvh = head / rep;
-  const int at = (row - u.start) * rep + head % rep;  // a head's row may begin the next block
-  const int first = w + at / RB - u.first / RB;
-  const int splits = min(u.splits, (a.units - first + u.blocks - 1) / u.blocks);  // fewer: bounds that decrease
+  const int at = max(row - u.x, 0) * rep + head % rep, first = u.y + at / RB;
+  // where cu decreases, nothing of this may be true
+  const int splits = first >= 0 && first < a.units ? min(u.w, (a.units - first + blocks - 1) / blocks) : 0;
   float mx = kNoScore, l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
   auto add = [&](const float2& e, const f32x4_t& v) {
@@ -606,7 +614,7 @@ __global__ __launch_bounds__(P == 16 ? 1024 : 256) void paged_join_kernel(PagedA
   };
 #pragma unroll 4
   for (int s = P == 1 ? 0 : wave; s < splits; s += P) {
-    const int64_t part = ((int64_t)(first + s * u.blocks) * a.kv_heads + kvh) * RB + at % RB;
+    const int64_t part = ((int64_t)(first + s * blocks) * a.kv_heads + kvh) * RB + at % RB;
     add(*reinterpret_cast<const float2*>(ml + 2 * part), *reinterpret_cast<const f32x4_t*>(a.work + part * HD + col));
   }
   if constexpr (P > 1) {
@@ -641,11 +649,11 @@ hipError_t run_paged(const PagedAttnArgs& a, hipStream_t s) {
     if (most == 0) return hipGetLastError();
     const int64_t waves = (int64_t)a.Tq * ((a.heads * (HD / 4) + 63) / 64);
     if (waves > 8 * (int64_t)device_cus())
-      paged_join_kernel<F16, HD, KT, 1><<<dim3((unsigned)((waves + 3) / 4)), 256, 0, s>>>(a);
+      paged_join_kernel<F16, HD, 1><<<dim3((unsigned)((waves + 3) / 4)), 256, 0, s>>>(a);
     else if (most < 64 || a.slots < 64 * paged_row_blocks(a))
-      paged_join_kernel<F16, HD, KT, 4><<<dim3((unsigned)waves), 256, 0, s>>>(a);
+      paged_join_kernel<F16, HD, 4><<<dim3((unsigned)waves), 256, 0, s>>>(a);
     else
-      paged_join_kernel<F16, HD, KT, 16><<<dim3((unsigned)waves), 1024, 0, s>>>(a);
+      paged_join_kernel<F16, HD, 16><<<dim3((unsigned)waves), 1024, 0, s>>>(a);
   }
   return hipGetLastError();
 }
@@ -690,7 +698,7 @@ void paged_attn_plan(PagedAttnArgs& a) {
   a.units = units > INT32_MAX ? INT32_MAX : (int)units;
 }
 int64_t paged_attn_workspace(const PagedAttnArgs& a) {
-  return a.slots > 0 ? (int64_t)a.units * a.kv_heads * a.block_rows * (a.head_dim + 2) * 4 : 0;
+  return a.slots > 0 ? (int64_t)a.units * a.kv_heads * a.block_rows * (a.head_dim + 2) * 4 + (int64_t)a.B * 16 : 0;
 }
 int64_t paged_attn_threads(const PagedAttnArgs& a) {
   const int64_t tiles = 256 * paged_blocks(a);
@@ -704,6 +712,7 @@ hipError_t launch_paged_attn(PagedAttnArgs a, hipStream_t s) {
   if (a.block_rows <= 32 && (int64_t)a.width << a.page_shift <= 768 && paged_row_blocks(a) * a.kv_heads <= device_cus()) {
     a.slots = 0;
     a.key_waves = 4;
+    a.units = (int)paged_row_blocks(a) + 2;
   }
   MHC_PACKED_HD(paged_hd, a, s)
 }
