@@ -41,12 +41,6 @@ __device__ __forceinline__ int wave_scan(int v) {  // over the lanes up to this 
   }
   return v;
 }
-__device__ __forceinline__ double wave_total(double v) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
-  return v;
-}
-
 // Unit number w of a kv head.  The keys of all sequences, times their blocks of rows, are cut
 // into about a.slots ranges of the same length; a sequence shorter than one is one unit a block.
 // The blocks of one range are neighbours.  Behind the sequences' units come those that clear the
@@ -78,7 +72,7 @@ __device__ __forceinline__ bool paged_find(const PagedAttnArgs& a, int xcd, int 
   constexpr int C = kPagedSeqs / 64;
   PagedSeq q[C];
   int blocks[C];
-  double work = 0.0;
+  float work = 0.f;  // of the lane's sequences, in tiles; past 2^24 rounded, the same in every workgroup
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int i = c * 64 + lane;
@@ -88,16 +82,17 @@ __device__ __forceinline__ bool paged_find(const PagedAttnArgs& a, int xcd, int 
       const int s0 = a.cu[i], s1 = a.cu[i + 1], past = a.lengths[i];
       q[c] = paged_seq(a, i, s0, s1, past);
       blocks[c] = (int)(((int64_t)q[c].n * rep + RB - 1) / RB);
-      work += (double)blocks[c] * ((q[c].len + KT - 1) / KT);
+      work += (float)blocks[c] * (float)((q[c].len + KT - 1) / KT);
     }
   }
   int per = INT32_MAX;
   if (a.slots > 0) {  // a block's last range is half one on average
-    int all = 0;
+    float all = 0.f;
 #pragma unroll
-    for (int c = 0; c < C; ++c) all += blocks[c];
-    const double want = fmax(a.slots - 0.5 * wave_total(all), 0.5 * a.slots);
-    per = max((int)fmin(wave_total(work) / want, 1e9) + 1, a.least);
+    for (int c = 0; c < C; ++c) all += (float)blocks[c];
+    const float want = fmaxf((float)a.slots - 0.5f * wave_sum(all), 0.5f * (float)a.slots);
+    per = max((int)fminf(wave_sum(work) / want, 1e9f) + 1, a.least);
+    per = __builtin_amdgcn_readfirstlane(per);
   }
   int splits[C], inc[C], all = 0;
 #pragma unroll
