@@ -88,7 +88,7 @@ __device__ __forceinline__ double wave_sum64(double v) {
 // workgroup goes over a vocabulary row only where a draw was rejected (or greedy, at each node)
 // and for the next token: a pass of sums over a wave's contiguous part each, then the part that
 // holds the border again, over all threads.  Bound by latencies in turn and, over a wide row, by one CU's 64-bit arithmetic: 64 chains of 8 at
-// a vocabulary of 6400 in fp32 11.8 us; one row of 50257 in bf16 without drafts 12.9, each rejected draft 6 to 7 more.
+// a vocabulary of 6400 in fp32 11.8 us; one row of 50257 in bf16 without drafts 12.9, the first rejected draft 4.5 more, the second 7.
 template <int DT, int W>
 __global__ __launch_bounds__(64 * W) void verify_kernel(VerifyArgs a) {
   constexpr int PER = ProbRow<DT>::PER, TH = 64 * W;

@@ -5,8 +5,8 @@
 //   (causal: up to its own; a tree: its bits),  O_t = sum_j softmax(S_t)_j v_j
 // 16-bit tensors, fp32 scores, sums and outputs.  The probabilities are a product's operand: rounded to
 // 16 bits, and up to 32 rows a sequence and kv head, where the keys' bytes bound the launch, what the rounding
-// took as a second operand (64 single tokens and trees of 16: +0 to 2%, the outputs' error 2.2e-3 -> 1.7e-3 of their
-// size, bf16's own rounding); with more rows it would take 8 to 20%.  The outputs are rounded once.
+// took as a second operand (64 single tokens and trees of 16: -1 to 4%, the outputs' error 2.2e-3 -> 1.7e-3 of their
+// size, bf16's own rounding); with more rows it would take 3 to 23%.  The outputs are rounded once.
 #include "mhc_packed.hpp"
 
 namespace mhc {
@@ -156,9 +156,9 @@ __device__ __forceinline__ int scalar_int(const int* p) {
 // a page number is one scalar read a group.  No wave leaves a step early: with a way out, for tiles
 // that none of a wave's rows sees, the compiler spilled 56 registers at head_dim 128 (64 tokens over
 // 65001 keys, 16 / 2 heads: 117 us instead of 51).
-// Up to 32 rows the keys' bytes bound it: 64 single tokens over 725 to 2175 keys, 8 / 4 heads of 96, 146 MB, 31 to 33 us, 4.5 TB/s;
-// trees of 16 there 36 to 39 us.  With more rows the matrix cores (35% of the time), the softmax (VALU 39%) and the LDS take turns: that tree of 64 tokens
-// 51 to 53 us, 650 TFLOP/s; 6 chunks of 500 over up to 4100 keys, heads of 64, 40 us, 470 TFLOP/s (VALU 52%).
+// Up to 32 rows the keys' bytes bound it: 64 single tokens over 725 to 2175 keys, 8 / 4 heads of 96, 146 MB, 33 us, 4.4 TB/s;
+// trees of 16 there 39 us.  With more rows the matrix cores (35% of the time), the softmax (VALU 39%) and the LDS take turns: that tree of 64 tokens
+// 51 to 53 us, 650 TFLOP/s; 6 chunks of 500 over up to 4100 keys, heads of 64, 41 us, 460 TFLOP/s (VALU 52%).
 template <int HD, int RW, int KW, int S>
 constexpr int paged_waves =  // of a SIMD, as the tiles' LDS lets in: two at most
     160 * 1024 / (KW * S * 4 * (RW == 1 ? 32 : 64) * HD) * RW * KW >= 8 ? 2 : 1;
@@ -570,7 +570,7 @@ __global__ __launch_bounds__(64 * RW * KW, (paged_waves<HD, RW, KW, S>)) void pa
 
 // Joins the ranges of a row: a lane takes four columns of one of its heads, a wave 64 such; with P > 1 the
 // workgroup's P waves take every P-th range of the same 64, and the sums meet in LDS.  64 rows of 16
-// heads of 128 from 64 ranges: 6 to 8 us (P = 1: 25); 1024 rows of 8 heads of 96 from one to four with P = 1: 5 us
+// heads of 128 from 64 ranges: 6 to 8 us (P = 1: 25); 1024 rows of 8 heads of 96 from a few with P = 1: 5 us
 // (P = 4: 11).
 template <bool F16, int HD, int P>
 __global__ __launch_bounds__(P == 16 ? 1024 : 256) void paged_join_kernel(PagedAttnArgs a) {
