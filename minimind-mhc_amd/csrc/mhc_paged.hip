@@ -158,7 +158,7 @@ __device__ __forceinline__ int scalar_int(const int* p) {
 // 65001 keys, 16 / 2 heads: 117 us instead of 51).
 // Up to 32 rows the keys' bytes bound it: 64 single tokens over 725 to 2175 keys, 8 / 4 heads of 96, 146 MB, 33 us, 4.4 TB/s;
 // trees of 16 there 39 us.  With more rows the matrix cores (35% of the time), the softmax (VALU 39%) and the LDS take turns: that tree of 64 tokens
-// 51 to 53 us, 650 TFLOP/s; 6 chunks of 500 over up to 4100 keys, heads of 64, 41 us, 460 TFLOP/s (VALU 52%).
+// 51 to 53 us, 650 TFLOP/s; 6 chunks of 500 over up to 4100 keys, heads of 64, 41 us, 460 TFLOP/s (VALU 51%).
 template <int HD, int RW, int KW, int S>
 constexpr int paged_waves =  // of a SIMD, as the tiles' LDS lets in: two at most
     160 * 1024 / (KW * S * 4 * (RW == 1 ? 32 : 64) * HD) * RW * KW >= 8 ? 2 : 1;
