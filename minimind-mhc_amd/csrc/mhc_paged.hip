@@ -3,10 +3,12 @@
 // new rows' own keys are stored already, behind the `past` ones before them.
 //   S_tj = scale q_t . k_j  for j < past, and for j - past a row of the same sequence that t sees
 //   (causal: up to its own; a tree: its bits),  O_t = sum_j softmax(S_t)_j v_j
-// 16-bit tensors, fp32 scores, sums and outputs.  The probabilities are a product's operand: rounded to
-// 16 bits, and up to 32 rows a sequence and kv head, where the keys' bytes bound the launch, what the rounding
-// took as a second operand (64 single tokens and trees of 16: -1 to 4%, the outputs' error 2.2e-3 -> 1.7e-3 of their
-// size, bf16's own rounding); with more rows it would take 3 to 23%.  The outputs are rounded once.
+// 16-bit tensors, fp32 scores, sums and outputs.  The probabilities are a product's operand in two parts: rounded to
+// 16 bits, and what the rounding took.  With the first part alone the outputs' error was 1.4 times that of their own
+// rounding.  The second costs nothing up to 32 rows a sequence and kv head, where the keys' bytes bound the launch, and
+// 1 to 24% above (8 trees of 30, heads of 128, 40.1 -> 40.4 us; chunks of 500, heads of 64, 45 -> 55; one tree of 64 over
+// 65001 keys 58 -> 70).  Each product with the second part right behind that with the first: apart, two
+// dozen registers more, and 3 to 5% slower at head_dim 128.  The outputs are rounded once.
 #include "mhc_packed.hpp"
 
 namespace mhc {
@@ -157,8 +159,8 @@ __device__ __forceinline__ int scalar_int(const int* p) {
 // that none of a wave's rows sees, the compiler spilled 56 registers at head_dim 128 (64 tokens over
 // 65001 keys, 16 / 2 heads: 117 us instead of 51).
 // Up to 32 rows the keys' bytes bound it: 64 single tokens over 725 to 2175 keys, 8 / 4 heads of 96, 146 MB, 33 us, 4.4 TB/s;
-// trees of 16 there 39 us.  With more rows the matrix cores (35% of the time), the softmax (VALU 39%) and the LDS take turns: that tree of 64 tokens
-// 51 to 53 us, 650 TFLOP/s; 6 chunks of 500 over up to 4100 keys, heads of 64, 41 us, 460 TFLOP/s (VALU 51%).
+// trees of 16 there 39 us.  With more rows the matrix cores, the softmax and the LDS take turns: that tree of 64 tokens 70 us
+// a call, join included, 6 chunks of 500 over up to 4100 keys, heads of 64, 55.
 template <int HD, int RW, int KW, int S>
 constexpr int paged_waves =  // of a SIMD, as the tiles' LDS lets in: two at most
     160 * 1024 / (KW * S * 4 * (RW == 1 ? 32 : 64) * HD) * RW * KW >= 8 ? 2 : 1;
@@ -170,7 +172,6 @@ __global__ __launch_bounds__(64 * RW * KW, (paged_waves<HD, RW, KW, S>)) void pa
   constexpr int UG = HD / 32;               // 1 KiB units of a group
   constexpr int TILE = KT * HD;             // elements
   constexpr int WAVES = RW * KW, RB = 16 * U * RW;
-  constexpr bool FINE = RW == 1;
   static_assert(RW == 1 || KW == 1, "waves that share a tile take the same steps");
   __shared__ __align__(16) uint16_t lds[KW][S][2][TILE];
   static_assert(KW == 1 || sizeof(lds) >= WAVES * 16 * U * (HD + 2) * 4, "the waves' sums take the tiles' place");
@@ -425,7 +426,7 @@ __global__ __launch_bounds__(64 * RW * KW, (paged_waves<HD, RW, KW, S>)) void pa
           for (int j = 0; j < 4; ++j) o[u][d][j] *= f;
       }
     }
-    U32x4 pf[U][NH], pr[U][NH];  // the probabilities rounded, and (FINE) what the rounding took
+    U32x4 pf[U][NH], pr[U][NH];  // the probabilities rounded, and what the rounding took
     auto softmax = [&](int hh) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -438,7 +439,7 @@ __global__ __launch_bounds__(64 * RW * KW, (paged_waves<HD, RW, KW, S>)) void pa
           for (int x = 0; x < 2; ++x) {
             const uint32_t w = pack2<F16>(p[2 * x], p[2 * x + 1]);
             pf[u][hh].v[2 * q + x] = w;
-            if (FINE) pr[u][hh].v[2 * q + x] = pack2<F16>(p[2 * x] - elem_lo<F16>(w), p[2 * x + 1] - elem_hi<F16>(w));
+            pr[u][hh].v[2 * q + x] = pack2<F16>(p[2 * x] - elem_lo<F16>(w), p[2 * x + 1] - elem_hi<F16>(w));
           }
         }
     };
@@ -446,14 +447,14 @@ __global__ __launch_bounds__(64 * RW * KW, (paged_waves<HD, RW, KW, S>)) void pa
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         l[u] = mfma16<F16>(ones, pf[u][hh], l[u]);
-        if (FINE) l[u] = mfma16<F16>(ones, pr[u][hh], l[u]);
+        l[u] = mfma16<F16>(ones, pr[u][hh], l[u]);
       }
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           o[u][d] = mfma16<F16>(va[hh][d], pf[u][hh], o[u][d]);
-          if (FINE) o[u][d] = mfma16<F16>(va[hh][d], pr[u][hh], o[u][d]);
+          o[u][d] = mfma16<F16>(va[hh][d], pr[u][hh], o[u][d]);
         }
     };
     softmax(0);
@@ -675,10 +676,10 @@ hipError_t paged_hd(const PagedAttnArgs& a, hipStream_t s) {
 //     heads of 96: -, 38.6, 37.6, 36.0 (5: 35.8, 6: 40); trees of 16 nodes there -, 45.8, 45.4, 43.9 (5: 45.2).
 //     Where that would be more than 256 ranges of a sequence, four waves share one instead (one token
 //     over 65001 keys, 16 / 2 heads of 128: 34.5 with 512 ranges, 24.7 with 128 of four waves).
-//   * Up to 64 rows, two waves: 4 trees of 30 nodes over 8000 keys 23.7, 22.4, 23.8, 33.0; one of 32 over 65001
-//     keys 38.1, 33.1, 35.7, 42.5.
-//   * More, four waves: 6 chunks of 500 over 4100 keys, heads of 64: 82, 54, 49, 54; of 96: 97, 63, 70, -;
-//     one tree of 64 nodes over 65001 keys, 16 / 2 heads of 128: 67, 58, 67, 71.
+//   * Up to 64 rows, two waves (from here on the same inputs on every call): 4 trees of 30 nodes over 2667 to 8001 keys
+//     24.7, 22.3, 29.1, 29.3; one of 32 over 65001 keys 45.7, 32.3, 43.4, 43.8.
+//   * More, four waves: 6 chunks of 500 over up to 4100 keys, heads of 64: 73, 55, 50, 56; of 96: 101, 71, 76, 76;
+//     one tree of 64 nodes over 65001 keys, 16 / 2 heads of 128: 80, 67, 81, 81.
 void paged_attn_plan(PagedAttnArgs& a) {
   const int rep = a.heads / a.kv_heads;
   const int64_t B = a.B > 0 ? a.B : 1, rows = (int64_t)a.Tq * rep, each = (rows + B - 1) / B;
