@@ -186,7 +186,7 @@ __global__ __launch_bounds__(64 * RW * KW, (paged_waves<HD, RW, KW, S>)) void pa
   const int kvh = in / 8;
   int w = 0;
   PagedUnit t;
-  if (!paged_find<KT>(a, in % 8, blockIdx.x / (8 * a.kv_heads), w, t) || w >= a.units) return;
+  if (!paged_find<KT>(a, in % 8, blockIdx.x / (8 * a.kv_heads), w, t) || (unsigned)w >= (unsigned)a.units) return;
   for (int* x : {&t.seq, &t.start, &t.n, &t.past, &t.len, &t.first, &t.split, &t.splits, &w}) *x = __builtin_amdgcn_readfirstlane(*x);
   const int rows = t.n * rep;
   const int last_token = (min(t.first + RB, rows) - 1) / rep;
@@ -595,14 +595,15 @@ __global__ __launch_bounds__(P == 16 ? 1024 : 256) void paged_join_kernel(PagedA
   lo = __builtin_amdgcn_readfirstlane(lo);
   if (lo >= a.B) return;
   const int4 u = paged_units(a)[lo];
-  const int blocks = max(u.z, 1);
-  if (u.w == 1) return;
+  // Where cu decreases, the row may be none of the sequence's, and a sequence without rows has no record: what
+  // stands there is anything.  Within these bounds nothing below leaves the workspace.
+  if (u.x < 0 || u.x > row || u.y < 0 || u.y >= a.units || u.z < 1 || u.z > a.units || u.w <= 1) return;
+  const int blocks = u.z;
   const int x = (int)(at_wave % chunks) * 64 + lane;
   const bool live = x < a.heads * (HD / 4);
   const int head = live ? x / (HD / 4) : 0, col = live ? x % (HD / 4) * 4 : 0, kvh = head / rep;
-  const int at = max(row - u.x, 0) * rep + head % rep, first = u.y + at / RB;
-  // where cu decreases, nothing of this may be true
-  const int splits = first >= 0 && first < a.units ? min(u.w, (a.units - first + blocks - 1) / blocks) : 0;
+  const int at = (row - u.x) * rep + head % rep, first = u.y + at / RB;
+  const int splits = first < a.units ? min(u.w, (a.units - first + blocks - 1) / blocks) : 0;
   float mx = kNoScore, l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
   auto add = [&](const float2& e, const f32x4_t& v) {

@@ -1,10 +1,11 @@
 """More of the operators on a cache of pages: how near outputs are to the formula whatever the
-number of rows."""
+number of rows, and bounds that make no sense."""
 from __future__ import annotations
 
 import pytest
 import torch
 
+from model import _hip as H
 from model.paged import paged_attention
 from test_gpu_paged import BF, EPS, F16, exact, ints, make, random_tree, starts
 
@@ -30,3 +31,34 @@ def test_probabilities_lose_nothing_to_16_bits(dev, hd, heads, kv, page, past, n
     bar = EPS[dtype] * out.abs() + 2.0 ** -14 * size + (2.0 ** -25 if dtype == F16 else 0.0)
     worst = ((got - out).abs() - bar).max().item()
     assert worst <= 0.0, worst
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("record", [
+    (-2 ** 30, 2 ** 26, 1, 2), (-2 ** 31, 0, 1, 2 ** 31 - 1), (0, -1000, 1, 5), (2 ** 31 - 1, 3, 2, 2), (0, 2 ** 31 - 1, 2 ** 31 - 1, 9),
+    (0, 5, 0, 3), (0, 5, -7, 3), (0, 5, 2 ** 31 - 1, 2 ** 31 - 1), (0, 0, 1, -1), (0, 0, 1, 2 ** 31 - 1)])
+def test_bounds_that_decrease_read_nothing_outside_the_workspace(dev, record):
+    """Sequence 1 begins behind its end: no workgroup writes its record for the join, which rows 0 to 29 come out
+    at.  Whatever stands there, NaN before and behind the workspace does not reach an output."""
+    heads, kv, hd, page, width, cu = 8, 4, 64, 16, 64, [0, 40, 0, 30]
+    T, B = 45, 3
+    torch.manual_seed(0)
+    q = torch.randn(T, heads, hd, device=dev).to(BF)
+    k, v = (torch.randn(B * width, page, kv, hd, device=dev).to(BF) for _ in range(2))
+    table = torch.arange(B * width, dtype=torch.int32, device=dev).view(B, width)
+    lens, cu = ints([900] * B, dev), ints(cu, dev)
+    lib = H.load()
+    nbytes = lib.mhc_paged_attn_workspace_bytes(B, T, heads, kv, hd)
+    assert nbytes > 0 and nbytes % 16 == 0
+    room = 1 << 20  # floats before and behind
+    buf = torch.full((2 * room + nbytes // 4,), float("nan"), device=dev)
+    ws = buf[room:room + nbytes // 4]
+    ws.zero_()
+    ws.view(torch.int32)[-4 * B:].view(B, 4).copy_(ints([record] * B, dev))
+    out = torch.full_like(q, 7.0)
+    assert lib.mhc_paged_attn_fwd(
+        q.data_ptr(), heads * hd, hd, k.data_ptr(), v.data_ptr(), page * kv * hd, kv * hd, hd, table.data_ptr(), lens.data_ptr(),
+        cu.data_ptr(), None, 0, out.data_ptr(), ws.data_ptr(), nbytes, B, T, heads, kv, hd, width, B * width, page, 1, 0.1,
+        H.stream(dev)) == 0
+    assert bool(torch.isfinite(out).all())
+    assert bool(buf[:room].isnan().all()) and bool(buf[room + nbytes // 4:].isnan().all())
