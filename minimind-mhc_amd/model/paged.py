@@ -224,6 +224,10 @@ def paged_keep(planes: torch.Tensor, page_table: torch.Tensor, lengths: torch.Te
     return new
 
 
+def _capturing(t: torch.Tensor) -> bool:
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 class DraftTree:
     """Drafted tokens of a PackedBatch: each sequence's first row is its last token, the others a tree
     behind it, parents before children.  A model call with drafts=DraftTree(...) over a PagedCache
@@ -278,7 +282,9 @@ class PagedCache:
     itself, as does reserve(), and raises where none are left.  The host counts what the sequences may
     have at most; after keep(), which only the device knows the result of, it counts all of a tree's
     rows, until settle() looks at the lengths and takes back the pages that are not needed.  A call that
-    is captured into a graph hands out none: reserve() what its replays will need before.  Rows that
+    is captured into a graph hands out none: reserve() what its replays will need before.  Replays move
+    the lengths on where the host does not see it: from a cache's first captured call on, reserve() and
+    calls that hand out pages look at the lengths first (a synchronisation).  Rows that
     have no page are dropped, and their sequence's outputs mean nothing from then on."""
 
     def __init__(self, config, sequences: int, capacity: int, page: int = 64, pages: Optional[int] = None,
@@ -298,6 +304,7 @@ class PagedCache:
             self.lengths = torch.zeros(sequences, dtype=torch.int32, device=device)
         self.layers = [(self.planes[2 * i], self.planes[2 * i + 1]) for i in range(config.num_hidden_layers)]
         self.sequences, self.capacity, self.page = sequences, capacity, page
+        self.replays = False  # whether a call was captured, whose replays the host does not count
         self.clear()
 
     def clear(self) -> None:
@@ -321,6 +328,8 @@ class PagedCache:
         rows = [int(rows)] * self.sequences if not hasattr(rows, "__len__") else [int(n) for n in rows]
         if len(rows) != self.sequences:
             raise ValueError(f"mhc_amd: rows of {len(rows)} sequences for a cache of {self.sequences}")
+        if self.replays:
+            self._look()
         need = []
         for i, n in enumerate(rows):
             if n and self.most[i] + n > self.capacity:
@@ -340,9 +349,13 @@ class PagedCache:
         at = torch.tensor([seqs, slots], device=self.page_table.device)
         self.page_table[at[0], at[1]] = torch.tensor(numbers, dtype=torch.int32, device=self.page_table.device)
 
+    def _look(self) -> None:
+        """The host's count from the lengths themselves (a synchronisation)."""
+        self.most = [min(max(n, 0), self.capacity) for n in self.lengths.tolist()]
+
     def settle(self) -> None:
         """Looks at the lengths (a synchronisation) and takes back the pages behind them."""
-        self.most = [min(max(n, 0), self.capacity) for n in self.lengths.tolist()]
+        self._look()
         seqs, slots = [], []
         for i, n in enumerate(self.most):
             keep = -(-n // self.page)
@@ -370,8 +383,10 @@ class PagedCache:
         self._count(batch)
 
     def _count(self, batch: PackedBatch) -> None:
-        """The rows of a call, as far as the host knows them (a captured call has stored none)."""
-        if self.lengths.is_cuda and torch.cuda.is_current_stream_capturing():
+        """The rows of a call, as far as the host knows them (a captured call has stored none yet, and
+        any number once it is replayed)."""
+        if _capturing(self.lengths):
+            self.replays = True
             return
         new = [batch.rows] * self.sequences if batch.lengths is None else batch.lengths
         self.most = [min(a + b, self.capacity) for a, b in zip(self.most, new)]
@@ -407,12 +422,11 @@ class PagedCall:
         if drafts is not None and drafts.batch is not batch:
             raise ValueError("mhc_amd: drafts of another batch")
         self.batch, self.cache, self.drafts = batch, cache, drafts
-        capturing = cache.lengths.is_cuda and torch.cuda.is_current_stream_capturing()
         # positions that the host knows the sequences reach, and a bound on those they may reach
         self.reach, self.most = 0, cache.capacity
         if batch.lengths is not None:
             self.reach = max((n for n in batch.lengths), default=0)
-            if not capturing:
+            if not _capturing(cache.lengths):
                 cache.reserve(batch.lengths)
         self.depths = None if drafts is None else drafts.depths
         deep = batch.positions if self.depths is None else self.depths.long()

@@ -1,0 +1,56 @@
+"""Captured steps over a cache of pages: rounds of reserving and replaying, and eager calls between them, against a
+cache that only eager calls have filled."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from model.packed import PackedBatch
+from model.paged import PagedCache
+from test_gpu_paged_model import _model
+
+
+def same(cache, other):
+    """The sequences' keys and values in both caches, whatever their pages."""
+    assert torch.equal(cache.lengths, other.lengths)
+    for s, n in enumerate(other.lengths.tolist()):
+        key = torch.arange(n, device=cache.lengths.device)
+        a, b = (c.planes.flatten(1, 2)[:, c.rows_of(torch.full_like(key, s), key)] for c in (cache, other))
+        assert torch.equal(a, b), s
+
+
+@pytest.mark.gpu
+def test_rounds_of_reserve_replays_and_eager_calls(dev):
+    m = _model(dev).eval()
+    cache, other = (PagedCache(m.config, 2, 400, 16, pages=50, device=dev) for _ in range(2))
+    g = torch.Generator(device=dev).manual_seed(3)
+    ids = lambda n: torch.randint(0, 500, (1, n), generator=g, device=dev)
+    one, token = PackedBatch.from_lengths([1, 1], device=dev), ids(2)
+    prompt, chunk = PackedBatch.from_lengths([30, 3], device=dev), PackedBatch.from_lengths([0, 20], device=dev)
+    first, more = ids(33), ids(20)
+    with torch.inference_mode():
+        for c in (cache, other):
+            m(first, packed=prompt, past_key_values=c)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):  # warm up on the cache that is not captured
+            m(token, packed=one, past_key_values=other)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        other.lengths.copy_(cache.lengths)
+        other.settle()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = m(token, packed=one, past_key_values=cache)
+        for turn in range(3):
+            cache.reserve(18)
+            for _ in range(18):
+                token.copy_(ids(2))
+                graph.replay()
+                want = m(token, packed=one, past_key_values=other)
+                torch.cuda.synchronize()
+                assert torch.equal(out.logits, want.logits), turn
+            got, want = (m(more, packed=chunk, past_key_values=c) for c in (cache, other))
+            assert torch.equal(got.logits, want.logits), turn
+            same(cache, other)
+        assert cache.lengths.tolist() == [84, 117] and [len(x) for x in cache.owned] == [6, 8]
