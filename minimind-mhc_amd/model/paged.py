@@ -285,7 +285,8 @@ class PagedCache:
     is captured into a graph hands out none: reserve() what its replays will need before.  Replays move
     the lengths on where the host does not see it: from a cache's first captured call on, reserve() and
     calls that hand out pages look at the lengths first (a synchronisation).  Rows that
-    have no page are dropped, and their sequence's outputs mean nothing from then on."""
+    have no page are dropped, and their sequence's outputs mean nothing from then on: wherever the host
+    looks, a length behind the sequence's pages raises (free() it, or set its length back)."""
 
     def __init__(self, config, sequences: int, capacity: int, page: int = 64, pages: Optional[int] = None,
                  dtype=torch.bfloat16, device="cuda"):
@@ -329,7 +330,7 @@ class PagedCache:
         if len(rows) != self.sequences:
             raise ValueError(f"mhc_amd: rows of {len(rows)} sequences for a cache of {self.sequences}")
         if self.replays:
-            self._look()
+            self._look([i for i, n in enumerate(rows) if n])
         need = []
         for i, n in enumerate(rows):
             if n and self.most[i] + n > self.capacity:
@@ -349,13 +350,20 @@ class PagedCache:
         at = torch.tensor([seqs, slots], device=self.page_table.device)
         self.page_table[at[0], at[1]] = torch.tensor(numbers, dtype=torch.int32, device=self.page_table.device)
 
-    def _look(self) -> None:
-        """The host's count from the lengths themselves (a synchronisation)."""
-        self.most = [min(max(n, 0), self.capacity) for n in self.lengths.tolist()]
+    def _look(self, sequences) -> None:
+        """The host's count from the lengths themselves (a synchronisation); raises where one of these
+        sequences has lost rows."""
+        have = self.lengths.tolist()
+        self.most = [min(max(n, 0), self.capacity) for n in have]
+        for i in sequences:
+            if have[i] > len(self.owned[i]) * self.page:
+                raise RuntimeError(f"mhc_amd: sequence {i} has {have[i]} keys and pages for {len(self.owned[i]) * self.page}: "
+                                   "rows were dropped (free() it, or set its length back)")
 
     def settle(self) -> None:
-        """Looks at the lengths (a synchronisation) and takes back the pages behind them."""
-        self._look()
+        """Looks at the lengths (a synchronisation) and takes back the pages behind them.  Raises where a
+        sequence's length is behind its pages (one without any page is not in use)."""
+        self._look([i for i, pages in enumerate(self.owned) if pages])
         seqs, slots = [], []
         for i, n in enumerate(self.most):
             keep = -(-n // self.page)

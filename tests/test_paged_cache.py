@@ -77,3 +77,39 @@ def test_calls_after_replays_hand_out_pages_and_raise_where_none_are_left():
         with pytest.raises(ValueError, match="may not fit"):
             model(torch.zeros(1, 41, dtype=torch.int64), packed=batch([41]), past_key_values=cache)
         assert cache.lengths.tolist() == [160]
+
+
+def test_dropped_rows_are_noticed():
+    """Replays past what was reserved: settling says so, and so does the next call of that sequence."""
+    model = tiny()
+    with torch.no_grad():
+        cache, tokens = begin(model, [30, 10])
+        cache.reserve(2)
+        for _ in range(3):  # the first sequence's 33rd key has no page
+            with replayed():
+                step(model, cache, tokens)
+        assert cache.lengths.tolist() == [33, 13]
+        for call in (cache.settle, lambda: cache.reserve(1), lambda: cache.reserve([1, 0]),
+                     lambda: model(torch.zeros(1, 1, dtype=torch.int64), packed=batch([1, 0]), past_key_values=cache)):
+            with pytest.raises(RuntimeError, match="sequence 0 has 33 keys and pages for 32"):
+                call()
+        assert [len(x) for x in cache.owned] == [2, 1] and cache.lengths.tolist() == [33, 13]
+        model(torch.zeros(1, 1, dtype=torch.int64), packed=batch([0, 1]), past_key_values=cache)  # not that sequence's
+        cache.lengths[0] = 32  # rolled back to what is there
+        cache.settle()
+        tokens[0] = tokens[0][:32]
+        tokens[1] = torch.cat([tokens[1], torch.zeros(1, dtype=torch.int64)])
+        as_without_a_cache(model, step(model, cache, tokens), tokens)
+        cache.reserve(1)
+        for _ in range(20):
+            with replayed():
+                step(model, cache, tokens)
+        with pytest.raises(RuntimeError, match="rows were dropped"):
+            cache.settle()
+        cache.free(0)
+        cache.free(1)
+        cache.settle()
+        with replayed():  # a slot that is not in use: nothing of it is kept, and nothing is amiss
+            step(model, cache, tokens)
+        cache.settle()
+        assert cache.lengths.tolist() == [1, 1] and cache.owned == [[], []]
