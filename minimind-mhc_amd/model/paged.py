@@ -281,12 +281,13 @@ class PagedCache:
     A call's new rows need pages before it: a call with a batch made from_lengths hands them out by
     itself, as does reserve(), and raises where none are left.  The host counts what the sequences may
     have at most; after keep(), which only the device knows the result of, it counts all of a tree's
-    rows, until settle() looks at the lengths and takes back the pages that are not needed.  A call that
-    is captured into a graph hands out none: reserve() what its replays will need before.  Replays move
-    the lengths on where the host does not see it: from a cache's first captured call on, reserve() and
-    calls that hand out pages look at the lengths first (a synchronisation).  Rows that
-    have no page are dropped, and their sequence's outputs mean nothing from then on: wherever the host
-    looks, a length behind the sequence's pages raises (free() it, or set its length back)."""
+    rows, until it looks at the lengths: where its count leaves no room, or in settle(), which takes back
+    the pages that are not needed.  A call that is captured into a graph hands out none: reserve() what its
+    replays will need before.  Replays move the lengths on where the host does not see it: from a cache's
+    first captured call on, reserve() and calls that hand out pages look at the lengths first (a
+    synchronisation).  Rows that have no page are dropped, and their sequence's outputs mean nothing from
+    then on: wherever the host looks, a length behind the sequence's pages raises (free() it, or set its
+    length back)."""
 
     def __init__(self, config, sequences: int, capacity: int, page: int = 64, pages: Optional[int] = None,
                  dtype=torch.bfloat16, device="cuda"):
@@ -311,6 +312,8 @@ class PagedCache:
     def clear(self) -> None:
         """Empties every sequence and takes all pages back."""
         self.most = [0] * self.sequences  # keys that each sequence has at most
+        self.held = [0] * self.sequences  # keys that reserve() was asked for pages for
+        self.drafted = [0] * self.sequences  # rows behind those that keep() may still move
         self.owned = [[] for _ in range(self.sequences)]
         self.free_pages = list(range(self.planes.shape[1]))[::-1]
         self.lengths.zero_()
@@ -320,24 +323,47 @@ class PagedCache:
         """Empties a sequence and takes its pages back."""
         self.free_pages += self.owned[sequence][::-1]
         self.owned[sequence], self.most[sequence] = [], 0
+        self.held[sequence] = self.drafted[sequence] = 0
         self.lengths[sequence] = 0
         self.page_table[sequence] = -1
 
-    def reserve(self, rows) -> None:
-        """Pages for so many more rows of each sequence (a number, or one for each): all of them or, with
-        an error, none."""
+    def _rows(self, rows) -> list:
         rows = [int(rows)] * self.sequences if not hasattr(rows, "__len__") else [int(n) for n in rows]
         if len(rows) != self.sequences:
             raise ValueError(f"mhc_amd: rows of {len(rows)} sequences for a cache of {self.sequences}")
-        if self.replays:
-            self._look([i for i, n in enumerate(rows) if n])
+        return rows
+
+    def reserve(self, rows) -> None:
+        """Pages for so many more rows of each sequence (a number, or one for each): all of them or, with
+        an error, none.  Where the host's count leaves no room for them it looks at the lengths (a
+        synchronisation) and takes back pages behind them, but none that were reserved."""
+        rows = self._rows(rows)
+        self._provide(rows)
+        self.held = [max(h, m + n) if n else h for h, m, n in zip(self.held, self.most, rows)]
+
+    def _need(self, rows):
+        """Pages that so many more rows of each sequence take, or the error where there is no room."""
         need = []
         for i, n in enumerate(rows):
             if n and self.most[i] + n > self.capacity:
-                raise ValueError(f"mhc_amd: {self.most[i]} + {n} keys may not fit a sequence's {self.capacity}")
+                return ValueError(f"mhc_amd: {self.most[i]} + {n} keys may not fit a sequence's {self.capacity}")
             need.append(max(0, -(-(self.most[i] + n) // self.page) - len(self.owned[i])) if n else 0)
         if sum(need) > len(self.free_pages):
-            raise RuntimeError(f"mhc_amd: {sum(need)} pages needed, {len(self.free_pages)} left")
+            return RuntimeError(f"mhc_amd: {sum(need)} pages needed, {len(self.free_pages)} left")
+        return need
+
+    def _provide(self, rows: list) -> None:
+        asked = [i for i, n in enumerate(rows) if n]
+        if self.replays:
+            self._look(asked)
+        need = self._need(rows)
+        if isinstance(need, Exception):
+            if not self.replays:
+                self._look(asked)
+            self._take_back()
+            need = self._need(rows)
+        if isinstance(need, Exception):
+            raise need
         if not any(need):
             return
         seqs, slots, numbers = [], [], []
@@ -361,12 +387,18 @@ class PagedCache:
                                    "rows were dropped (free() it, or set its length back)")
 
     def settle(self) -> None:
-        """Looks at the lengths (a synchronisation) and takes back the pages behind them.  Raises where a
-        sequence's length is behind its pages (one without any page is not in use)."""
+        """Looks at the lengths (a synchronisation) and takes back the pages behind them, reserved or not
+        (but those of drafts that keep() may still move).  Raises where a sequence's length is behind its
+        pages (one without any page is not in use)."""
         self._look([i for i, pages in enumerate(self.owned) if pages])
+        self.held = [0] * self.sequences
+        self._take_back()
+
+    def _take_back(self) -> None:
+        """Takes back the pages that nobody counts on."""
         seqs, slots = [], []
         for i, n in enumerate(self.most):
-            keep = -(-n // self.page)
+            keep = -(-max(n + self.drafted[i], self.held[i]) // self.page)
             slots += range(keep, len(self.owned[i]))
             seqs += [i] * (len(self.owned[i]) - keep)
             self.free_pages += self.owned[i][keep:][::-1]
@@ -397,6 +429,7 @@ class PagedCache:
             self.replays = True
             return
         new = [batch.rows] * self.sequences if batch.lengths is None else batch.lengths
+        self.drafted = [0 if n else d for n, d in zip(new, self.drafted)]
         self.most = [min(a + b, self.capacity) for a, b in zip(self.most, new)]
 
     def rows_of(self, sequence: torch.Tensor, key: torch.Tensor) -> torch.Tensor:
@@ -435,7 +468,7 @@ class PagedCall:
         if batch.lengths is not None:
             self.reach = max((n for n in batch.lengths), default=0)
             if not _capturing(cache.lengths):
-                cache.reserve(batch.lengths)
+                cache._provide(batch.lengths)
         self.depths = None if drafts is None else drafts.depths
         deep = batch.positions if self.depths is None else self.depths.long()
         self.past = cache.lengths[batch.sequence.clamp_max(cache.sequences - 1)]
@@ -451,6 +484,8 @@ class PagedCall:
         if self.drafts is None:
             self.cache.lengths.copy_(self.cache.grown(self.batch))
             self.cache._count(self.batch)
+        elif not _capturing(self.cache.lengths) and self.batch.lengths is not None:
+            self.cache.drafted = [n or d for n, d in zip(self.batch.lengths, self.cache.drafted)]
 
     def attention(self, m, q, k, v, tables, layer: int) -> torch.Tensor:
         """q [1, rows, heads, head_dim], k, v [1, rows, kv heads, head_dim], the projections of the

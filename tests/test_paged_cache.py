@@ -113,3 +113,80 @@ def test_dropped_rows_are_noticed():
             step(model, cache, tokens)
         cache.settle()
         assert cache.lengths.tolist() == [1, 1] and cache.owned == [[], []]
+
+
+def drafts(model, cache, n, seed):
+    """A verify_step of n nodes for each sequence whose drafts are mostly wrong; its kept rows."""
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.randint(0, 50, (1, n * cache.sequences), generator=g)
+    return model.verify_step(ids, batch([n] * cache.sequences), cache).kept
+
+
+@pytest.mark.parametrize("sizes", [dict(capacity=64), dict(capacity=120, pages=6)])
+def test_many_drafts_without_settling(sizes):
+    """What the host counts at most no longer fits; what is there does, for as long as it does."""
+    model = tiny(max_position_embeddings=256)
+    with torch.no_grad():
+        cache, _ = begin(model, [8, 3], **sizes)
+        have, steps = [8, 3], 0
+        while max(have) + 8 <= 64 and steps < 14:
+            kept = drafts(model, cache, 8, steps)
+            have = [a + b for a, b in zip(have, kept.tolist())]
+            assert cache.lengths.tolist() == have
+            steps += 1
+        assert steps == 14 or max(have) + 8 > 64
+        assert sum(len(x) for x in cache.owned) + len(cache.free_pages) == cache.planes.shape[1]
+        cache.settle()
+        assert cache.most == have
+        free = len(cache.free_pages)
+        with pytest.raises(ValueError, match="may not fit"):  # that one is true
+            cache.reserve([cache.capacity - have[0] + 1, 0])
+        if free * 16 < cache.capacity - have[0] - 16:
+            with pytest.raises(RuntimeError, match="pages needed"):
+                cache.reserve([cache.capacity - have[0], 0])
+        assert len(cache.free_pages) == free and cache.most == have
+
+
+def test_lengths_that_the_host_does_not_know_are_looked_at():
+    """A batch whose lengths only the device knows counts all its rows for every sequence."""
+    from model.packed import PackedBatch
+    model = tiny()
+    with torch.no_grad():
+        cache, tokens = begin(model, [4, 4], capacity=48, pages=6)
+        cache.reserve(4)
+        free = PackedBatch(torch.tensor([0, 4, 8], dtype=torch.int32), 8)
+        new = torch.randint(0, 50, (8,))
+        for _ in range(5):  # far more than fits, if every row were each sequence's
+            cache.lengths.fill_(4)
+            model(new[None], packed=free, past_key_values=cache)
+        tokens = [torch.cat([t, n]) for t, n in zip(tokens, new.split(4))]
+        as_without_a_cache(model, step(model, cache, tokens), tokens)
+        more = torch.randint(0, 50, (60,))
+        got = model(more[None], packed=batch([30, 30]), past_key_values=cache).logits[0, [29, 59]]
+        as_without_a_cache(model, got, [torch.cat([t, n]) for t, n in zip(tokens, more.split(30))])
+
+
+def test_what_is_not_taken_back_for_another_sequence():
+    """Pages that were reserved, and those of drafts that are not kept yet."""
+    model = tiny()
+    with torch.no_grad():
+        cache, tokens = begin(model, [5, 5, 5], capacity=64, pages=6)
+        cache.reserve([0, 0, 20])  # sequence 2: a page more
+        b = batch([30, 0, 0])
+        ids = torch.randint(0, 50, (30,))
+        model(ids[None], packed=b, past_key_values=cache, drafts=paged.DraftTree(b))  # sequence 0: two more, the last
+        assert not cache.free_pages
+        with pytest.raises(RuntimeError, match="1 pages needed, 0 left"):
+            model(torch.zeros(1, 20, dtype=torch.int64), packed=batch([0, 20, 0]), past_key_values=cache)
+        cache.settle()  # takes back what was reserved, not the drafts
+        assert [len(x) for x in cache.owned] == [3, 1, 1]
+        more = torch.randint(0, 50, (20,))
+        model(more[None], packed=batch([0, 20, 0]), past_key_values=cache)
+        cache.keep(b, torch.tensor([30, 0, 0], dtype=torch.int32), torch.arange(30, dtype=torch.int32))
+        tokens[0], tokens[1] = torch.cat([tokens[0], ids]), torch.cat([tokens[1], more])
+        assert cache.lengths.tolist() == [35, 25, 5] == cache.most
+        as_without_a_cache(model, step(model, cache, tokens), tokens)
+        cache.clear()
+        cache.reserve([1, 1, 1])
+        cache.settle()
+        assert cache.owned == [[], [], []] and len(cache.free_pages) == 6
