@@ -386,12 +386,18 @@ class PagedCache:
                 raise RuntimeError(f"mhc_amd: sequence {i} has {have[i]} keys and pages for {len(self.owned[i]) * self.page}: "
                                    "rows were dropped (free() it, or set its length back)")
 
-    def settle(self) -> None:
-        """Looks at the lengths (a synchronisation) and takes back the pages behind them, reserved or not
-        (but those of drafts that keep() may still move).  Raises where a sequence's length is behind its
-        pages (one without any page is not in use)."""
+    def settle(self, spare=None) -> None:
+        """Looks at the lengths (a synchronisation) and takes back the pages behind them, but for those of so
+        many spare rows of each sequence (a number, or one for each).  None: what is reserved stays in a cache
+        with captured calls, whose replays count on it, and goes in any other.  Pages of drafts that keep()
+        may still move stay.  Raises where a sequence's length is behind its pages (one without any page is
+        not in use)."""
+        spare = None if spare is None else self._rows(spare)
         self._look([i for i, pages in enumerate(self.owned) if pages])
-        self.held = [0] * self.sequences
+        if spare is not None:
+            self.held = [m + n for m, n in zip(self.most, spare)]
+        elif not self.replays:
+            self.held = [0] * self.sequences
         self._take_back()
 
     def _take_back(self) -> None:

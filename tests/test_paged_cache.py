@@ -190,3 +190,28 @@ def test_what_is_not_taken_back_for_another_sequence():
         cache.reserve([1, 1, 1])
         cache.settle()
         assert cache.owned == [[], [], []] and len(cache.free_pages) == 6
+
+
+def test_settling_between_replays_keeps_what_was_reserved_for_them():
+    model = tiny()
+    with torch.no_grad():
+        cache, tokens = begin(model, [14, 2], capacity=100)
+        cache.reserve(40)
+        for turn in range(40):
+            with replayed():
+                got = step(model, cache, tokens)
+            if turn % 10 == 5:
+                cache.settle()
+        as_without_a_cache(model, got, tokens)
+        assert cache.lengths.tolist() == [54, 42] and [len(x) for x in cache.owned] == [4, 3]
+        cache.reserve([30, 1])
+        assert [len(x) for x in cache.owned] == [6, 3]
+        cache.settle(spare=[10, 0])
+        assert [len(x) for x in cache.owned] == [4, 3] and cache.held == [64, 42]
+        cache.settle(spare=100)  # what there is: it hands out none
+        assert [len(x) for x in cache.owned] == [4, 3]
+        with pytest.raises(ValueError, match="rows of 3"):
+            cache.settle(spare=[1, 2, 3])
+        cache.lengths.copy_(torch.tensor([20, 3]))
+        cache.settle(spare=0)
+        assert [len(x) for x in cache.owned] == [2, 1]
