@@ -490,7 +490,9 @@ class PagedCall:
         if self.drafts is None:
             self.cache.lengths.copy_(self.cache.grown(self.batch))
             self.cache._count(self.batch)
-        elif not _capturing(self.cache.lengths) and self.batch.lengths is not None:
+        elif _capturing(self.cache.lengths):
+            self.cache.replays = True
+        elif self.batch.lengths is not None:
             self.cache.drafted = [n or d for n, d in zip(self.batch.lengths, self.cache.drafted)]
 
     def attention(self, m, q, k, v, tables, layer: int) -> torch.Tensor:

@@ -215,3 +215,21 @@ def test_settling_between_replays_keeps_what_was_reserved_for_them():
         cache.lengths.copy_(torch.tensor([20, 3]))
         cache.settle(spare=0)
         assert [len(x) for x in cache.owned] == [2, 1]
+
+
+def test_captured_drafts_that_are_kept_outside_the_graph():
+    """The forward pass of a tree in a graph, verification and keeping outside: its replays need their pages too."""
+    model = tiny()
+    with torch.no_grad():
+        cache, tokens = begin(model, [14], capacity=100)
+        cache.reserve(20)
+        b, ids = batch([10]), torch.randint(0, 50, (10,))
+        for turn in range(2):
+            with replayed():
+                model(ids[None], packed=b, past_key_values=cache, drafts=paged.DraftTree(b))
+            cache.settle()
+            assert len(cache.owned[0]) == 3
+            cache.keep(b, torch.tensor([10], dtype=torch.int32), torch.arange(10, dtype=torch.int32))
+            tokens[0] = torch.cat([tokens[0], ids])
+        cache.settle()
+        as_without_a_cache(model, step(model, cache, tokens), tokens)
