@@ -468,8 +468,9 @@ class MiniMindModel(nn.Module):
             raise ValueError("packed sequences need a PackedCache or a PagedCache as past_key_values")
         if drafts is not None and not isinstance(cache, PagedCache):
             raise ValueError("drafts need a PagedCache as past_key_values")
-        call = PagedCall(packed, cache, drafts) if isinstance(cache, PagedCache) else PackedCall(packed, cache, slots=True)
         table = self.freqs_cos.shape[0]
+        call = (PagedCall(packed, cache, drafts, table) if isinstance(cache, PagedCache)
+                else PackedCall(packed, cache, slots=True))
         if call.reach > table:
             raise ValueError(f"a packed sequence reaches {call.reach} positions, max_position_embeddings is {table}")
         return call, cache, None

@@ -461,20 +461,22 @@ class PagedCache:
 
 
 class PagedCall:
-    """One model call on a PackedBatch over a PagedCache: where its rows stand."""
+    """One model call on a PackedBatch over a PagedCache: where its rows stand.  A call that is refused
+    has handed out no pages; table: the positions that the model has, if it is to be refused for those."""
 
-    def __init__(self, batch: PackedBatch, cache: PagedCache, drafts: Optional[DraftTree] = None):
+    def __init__(self, batch: PackedBatch, cache: PagedCache, drafts: Optional[DraftTree] = None,
+                 table: Optional[int] = None):
         if len(batch) != cache.sequences:
             raise ValueError(f"mhc_amd: a batch of {len(batch)} sequences on a cache of {cache.sequences}")
         if drafts is not None and drafts.batch is not batch:
             raise ValueError("mhc_amd: drafts of another batch")
         self.batch, self.cache, self.drafts = batch, cache, drafts
         # positions that the host knows the sequences reach, and a bound on those they may reach
-        self.reach, self.most = 0, cache.capacity
-        if batch.lengths is not None:
-            self.reach = max((n for n in batch.lengths), default=0)
-            if not _capturing(cache.lengths):
-                cache._provide(batch.lengths)
+        self.reach, self.most = max(batch.lengths or [0]), cache.capacity
+        if table is not None and self.reach > table:
+            raise ValueError(f"a packed sequence reaches {self.reach} positions, max_position_embeddings is {table}")
+        if batch.lengths is not None and not _capturing(cache.lengths):
+            cache._provide(batch.lengths)
         self.depths = None if drafts is None else drafts.depths
         deep = batch.positions if self.depths is None else self.depths.long()
         self.past = cache.lengths[batch.sequence.clamp_max(cache.sequences - 1)]

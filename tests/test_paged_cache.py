@@ -233,3 +233,13 @@ def test_captured_drafts_that_are_kept_outside_the_graph():
             tokens[0] = torch.cat([tokens[0], ids])
         cache.settle()
         as_without_a_cache(model, step(model, cache, tokens), tokens)
+
+
+def test_a_call_that_reaches_past_the_tables_hands_out_nothing():
+    model = tiny(max_position_embeddings=20)
+    with torch.no_grad():
+        cache, _ = begin(model, [3, 3], capacity=64, pages=6)
+        table = cache.page_table.clone()
+        with pytest.raises(ValueError, match="max_position_embeddings is 20"):
+            model(torch.zeros(1, 42, dtype=torch.int64), packed=batch([2, 40]), past_key_values=cache)
+        assert torch.equal(cache.page_table, table) and len(cache.free_pages) == 4 and cache.most == [3, 3]
