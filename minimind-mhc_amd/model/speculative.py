@@ -30,6 +30,29 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t.clone() if t.data_ptr() % 16 else t
 
 
+def _checked(probs, tokens, cu_seqlens, parents, draft_probs, uniforms, types, dev):
+    """(tokens, parents, uniforms, cu_seqlens) of a call, checked and in order."""
+    if probs.dim() != 2 or probs.shape[1] < 1:
+        raise ValueError(f"mhc_amd: probs must be [rows, V], got {tuple(probs.shape)}")
+    T = probs.shape[0]
+    for name, t in (("probs", probs), ("draft_probs", draft_probs)):
+        if t is not None and t.dtype not in types:
+            raise TypeError(f"mhc_amd: {name} must be fp32, bf16 or fp16, got {t.dtype}")
+    if draft_probs is not None:
+        if draft_probs.shape != probs.shape:
+            raise ValueError(f"mhc_amd: draft_probs {tuple(draft_probs.shape)} and probs {tuple(probs.shape)} differ")
+        if uniforms is None:
+            raise ValueError("mhc_amd: draft_probs need uniforms")
+    tokens = _row_ints("tokens", tokens, T, torch.int64)
+    if parents is not None:
+        parents = _row_ints("parents", parents, T, torch.int32)
+    if uniforms is not None:
+        if not uniforms.is_floating_point() or tuple(uniforms.shape) != (T,):
+            raise ValueError(f"mhc_amd: uniforms must be [{T}] floating point, got {tuple(uniforms.shape)} {uniforms.dtype}")
+        uniforms = uniforms.detach().to(torch.float32).contiguous()
+    return tokens, parents, uniforms, _bounds("cu_seqlens", cu_seqlens, None, dev)
+
+
 def verify_drafts(probs: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.Tensor,
                   parents: Optional[torch.Tensor] = None, draft_probs: Optional[torch.Tensor] = None,
                   uniforms: Optional[torch.Tensor] = None):
@@ -59,25 +82,8 @@ def verify_drafts(probs: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.T
     in the sequence, in order, then -1.  Rows behind the last sequence keep -1.  Not differentiable.
     """
     dev = H.require_device(probs, tokens, parents, draft_probs, uniforms)
-    if probs.dim() != 2 or probs.shape[1] < 1:
-        raise ValueError(f"mhc_amd: probs must be [rows, V], got {tuple(probs.shape)}")
+    tokens, parents, uniforms, cu = _checked(probs, tokens, cu_seqlens, parents, draft_probs, uniforms, _TYPES, dev)
     T, V = probs.shape
-    for name, t in (("probs", probs), ("draft_probs", draft_probs)):
-        if t is not None and t.dtype not in _TYPES:
-            raise TypeError(f"mhc_amd: {name} must be fp32, bf16 or fp16, got {t.dtype}")
-    if draft_probs is not None:
-        if draft_probs.shape != probs.shape:
-            raise ValueError(f"mhc_amd: draft_probs {tuple(draft_probs.shape)} and probs {tuple(probs.shape)} differ")
-        if uniforms is None:
-            raise ValueError("mhc_amd: draft_probs need uniforms")
-    tokens = _row_ints("tokens", tokens, T, torch.int64)
-    if parents is not None:
-        parents = _row_ints("parents", parents, T, torch.int32)
-    if uniforms is not None:
-        if not uniforms.is_floating_point() or tuple(uniforms.shape) != (T,):
-            raise ValueError(f"mhc_amd: uniforms must be [{T}] floating point, got {tuple(uniforms.shape)} {uniforms.dtype}")
-        uniforms = uniforms.detach().to(torch.float32).contiguous()
-    cu = _bounds("cu_seqlens", cu_seqlens, None, dev)
     probs, n = probs.detach(), cu.numel() - 1
     if draft_probs is not None:
         draft_probs = draft_probs.detach()
@@ -97,12 +103,15 @@ def verify_drafts(probs: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.T
 
 
 def plain_verify(probs, tokens, cu_seqlens, parents=None, draft_probs=None, uniforms=None):
-    """verify_drafts on the host, a sequence at a time, for tensors that are on no GPU."""
+    """verify_drafts on the host, a sequence at a time, for tensors that are on no GPU (probabilities of
+    64 bits too)."""
+    tokens, parents, uniforms, cu = _checked(probs, tokens, cu_seqlens, parents, draft_probs, uniforms,
+                                             (*_TYPES, torch.float64), probs.device)
     T, V = probs.shape
-    ends = [0, *(min(max(e, 0), T) for e in cu_seqlens.tolist()[1:])]
+    ends = [0, *(min(max(e, 0), T) for e in cu.tolist()[1:])]
     tokens = tokens.tolist()
     up = parents.tolist() if parents is not None else None
-    u = uniforms.float().double().tolist() if uniforms is not None else None
+    u = uniforms.double().tolist() if uniforms is not None else None
     p_all, q_all = (None if t is None else torch.where((t > 0) & torch.isfinite(t), t, 0).double() for t in (probs, draft_probs))
     path, kept, following = torch.full((T,), -1, dtype=torch.int32), [], []
     for a, b in zip(ends, ends[1:]):
