@@ -123,8 +123,11 @@ def plain_verify(probs, tokens, cu_seqlens, parents=None, draft_probs=None, unif
         path[a] = 0
 
         def enter():
-            raw = probs[a + node].float()
-            best = int(torch.where(raw.isnan(), -float("inf"), raw).argmax()) if u is None and not raw.isnan().all() else -1
+            best = -1
+            if u is None:
+                raw = probs[a + node].double()
+                there = raw[~raw.isnan()]
+                best = int((raw == there.max()).nonzero()[0]) if len(there) else -1
             return best, p_all[a + node].clone(), None if q_all is None else q_all[a + node], 0.0, 1.0
         best, p, q, ratio, norm = enter()
         for j in range(1, b - a):

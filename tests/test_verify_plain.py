@@ -38,3 +38,18 @@ def test_verify_step_refuses_drafts_without_numbers():
     with pytest.raises(ValueError, match="uniforms"):
         model.verify_step(torch.zeros(1, 3, dtype=torch.int64), batch([3]), cache, draft_probs=torch.rand(3, 50))
     assert cache.lengths.tolist() == [0]
+
+
+def test_greedy_rows_of_64_bits_and_without_finite_numbers():
+    """The first of the largest numbers: not of their fp32 roundings, and never a NaN."""
+    nan, inf = float("nan"), float("inf")
+    rows = torch.tensor([[1.0, 1.0 + 2.0 ** -40, 0.5], [nan, -inf, -inf], [nan, nan, nan], [-inf, -inf, nan],
+                         [-3.0, nan, -2.0]], dtype=torch.float64)
+    cu = torch.arange(6, dtype=torch.int32)
+    kept, path, following = plain_verify(rows, torch.zeros(5, dtype=torch.int64), cu)
+    assert following.tolist() == [1, 1, -1, 0, 2] and kept.tolist() == [1] * 5
+    # drafts after each: accepted where they are that token
+    both = rows.repeat_interleave(2, 0)
+    tokens = torch.tensor([0, 1, 0, 1, 0, 0, 0, 0, 0, 2])
+    kept, _, _ = plain_verify(both, tokens, torch.arange(0, 11, 2, dtype=torch.int32))
+    assert kept.tolist() == [2, 2, 1, 2, 2]
