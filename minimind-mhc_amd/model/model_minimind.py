@@ -47,7 +47,7 @@ from .mhc_fused_no_hres import MHCConnection_FusedNoHres
 from .packed import PackedBatch, PackedCache, PackedCall
 from .paged import DraftTree, PagedCache, PagedCall
 from .rotary import plain_rotary, rotary
-from .speculative import plain_verify, verify_drafts
+from .speculative import verify
 
 
 class MiniMindConfig:
@@ -545,8 +545,7 @@ class MiniMindForCausalLM(nn.Module):
         drafts = DraftTree(packed, parents)
         logits = self(input_ids, packed=packed, past_key_values=cache, drafts=drafts).logits[0]
         probs = logits if uniforms is None else torch.softmax(logits.float() / temperature, -1)
-        kept, path, following = (verify_drafts if probs.is_cuda else plain_verify)(
-            probs, input_ids[0], packed.cu_seqlens, parents, draft_probs, uniforms)
+        kept, path, following = verify(probs, input_ids[0], packed.cu_seqlens, parents, draft_probs, uniforms)
         cache.keep(packed, kept, path)
         return SimpleNamespace(kept=kept, path=path, next_tokens=following, logits=logits[None])
 

@@ -163,3 +163,11 @@ def plain_verify(probs, tokens, cu_seqlens, parents=None, draft_probs=None, unif
         kept.append(count)
         following.append(best)
     return torch.tensor(kept, dtype=torch.int32), path, torch.tensor(following, dtype=torch.int64)
+
+
+def verify(probs, tokens, cu_seqlens, parents=None, draft_probs=None, uniforms=None):
+    """verify_drafts; on the host (a synchronisation) where there is no GPU or a type that the kernel does not take."""
+    if probs.is_cuda and all(t is None or t.dtype in _TYPES for t in (probs, draft_probs)):
+        return verify_drafts(probs, tokens, cu_seqlens, parents, draft_probs, uniforms)
+    args = (None if t is None else t.detach().cpu() for t in (probs, tokens, cu_seqlens, parents, draft_probs, uniforms))
+    return tuple(t.to(probs.device) for t in plain_verify(*args))

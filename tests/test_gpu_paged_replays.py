@@ -54,3 +54,28 @@ def test_rounds_of_reserve_replays_and_eager_calls(dev):
             assert torch.equal(got.logits, want.logits), turn
             same(cache, other)
         assert cache.lengths.tolist() == [84, 117] and [len(x) for x in cache.owned] == [6, 8]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", ["greedy", "certain", "draft", "wide draft"])
+def test_verify_step_of_a_64_bit_model(dev, mode):
+    """What the kernel does not take is verified on the host; the results are on the GPU, as ever."""
+    from model.speculative import plain_verify
+    dtype = torch.float32 if mode == "wide draft" else torch.float64
+    m = _model(dev, dtype, use_mhc=0).eval()
+    cache = PagedCache(m.config, 2, 100, 16, dtype=dtype, device=dev)
+    b = PackedBatch.from_lengths([5, 3], device=dev)
+    g = torch.Generator().manual_seed(0)
+    ids = torch.randint(0, 500, (1, 8), generator=g).to(dev)
+    u = None if mode == "greedy" else torch.rand(8, generator=g).to(dev)
+    draft = torch.full((8, 500), 1 / 500, dtype=torch.float64, device=dev) if "draft" in mode else None
+    with torch.inference_mode():
+        m(ids[:, :7], packed=PackedBatch.from_lengths([4, 3], device=dev), past_key_values=cache)
+        res = m.verify_step(ids, b, cache, None, draft, u)
+        host = lambda t: None if t is None else t.cpu()
+        logits = res.logits[0]
+        probs = logits if u is None else torch.softmax(logits.float(), -1)
+        want = plain_verify(host(probs), ids[0].cpu(), b.cu_seqlens.cpu(), None, host(draft), host(u))
+    for got, w in zip((res.kept, res.path, res.next_tokens), want):
+        assert got.device == dev and got.dtype == w.dtype and torch.equal(got.cpu(), w)
+    assert cache.lengths.tolist() == [4 + int(want[0][0]), 3 + int(want[0][1])]
