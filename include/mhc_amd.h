@@ -628,7 +628,7 @@ int mhc_paged_append(const void* q, int64_t q_stride_t, int64_t q_stride_h, cons
                      int64_t stride_p, int64_t stride_t, int64_t stride_h, int64_t T, int B, int heads, int kv_heads, int head_dim, int rotary_dim, int width, int pages,
                      int page, int flags, int dtype, hipStream_t stream);
 
-/* Bytes of workspace mhc_paged_attn_fwd needs (0: none), or -1 for a shape it does not take. */
+/* Bytes of workspace mhc_paged_attn_fwd needs on the current device (0: none), or -1 for a shape it does not take. */
 int64_t mhc_paged_attn_workspace_bytes(int B, int64_t Tq, int heads, int kv_heads, int head_dim);
 
 /* out [Tq, heads, head_dim] (contiguous) = softmax(scale q k^T) v, scale > 0, head_dim 64, 96 or 128.  A

@@ -127,8 +127,8 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace(*sizes) -> int:
-    """Bytes, which the sizes alone decide: asked of the library once for each."""
+def _workspace(device: int, *sizes) -> int:
+    """Bytes, which the sizes and the current device's compute units decide: asked of the library once for each."""
     return max(H.load().mhc_paged_attn_workspace_bytes(*sizes), 0)
 
 
@@ -180,7 +180,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         row, head = heads * hd, hd
     out = torch.empty((T, heads, hd), dtype=q.dtype, device=dev)
     with _ops.launch_device(q):
-        nbytes = _workspace(n, T, heads, kv, hd)
+        nbytes = _workspace(dev.index, n, T, heads, kv, hd)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
         H.check(H.load().mhc_paged_attn_fwd(
             q.data_ptr(), row, head, k_pages.data_ptr(), v_pages.data_ptr(), *strides,

@@ -62,3 +62,14 @@ def test_bounds_that_decrease_read_nothing_outside_the_workspace(dev, record):
         H.stream(dev)) == 0
     assert bool(torch.isfinite(out).all())
     assert bool(buf[:room].isnan().all()) and bool(buf[room + nbytes // 4:].isnan().all())
+
+
+@pytest.mark.gpu
+def test_workspace_sizes_are_kept_for_each_device(dev, monkeypatch):
+    """The split follows the device's compute units: a size that one device was asked for is not another's."""
+    from model import paged
+    seen, ask = [], paged._workspace
+    monkeypatch.setattr(paged, "_workspace", lambda *a: seen.append(a) or ask(*a))
+    pool, q = make(dev, BF, [900], [1], 16, 8, 4, 96)
+    paged_attention(q, pool.k, pool.v, pool.table, ints([900], dev), ints([0, 1], dev))
+    assert seen == [(dev.index, 1, 1, 8, 4, 96)]
