@@ -260,7 +260,7 @@ hipError_t launch_heads(const RotaryArgs& a, bool append, hipStream_t s) {
   const int64_t blocks = (a.T + rows - 1) / rows;
   constexpr int64_t kLine = 1 << 23;  // a dimension of a launch holds less than 2^32 threads
   const dim3 grid((unsigned)(blocks < kLine ? blocks : kLine), (unsigned)((blocks + kLine - 1) / kLine));
-  if constexpr (DT != kF32) {
+  if constexpr (DT != kF32 && HB != 3) {  // three heads: not appended
     if (append) {
       rotary_kernel<DT, V, HB, true><<<grid, 256, 0, s>>>(a);
       return hipGetLastError();
