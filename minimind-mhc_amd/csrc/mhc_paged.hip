@@ -14,6 +14,7 @@
 namespace mhc {
 namespace {
 
+constexpr int kPagedStages = 2;  // tiles of a ring: one in use, one in flight
 constexpr int kPagedSeqs = 256;  // up to so many, workgroups are dealt out by the keys' lengths
 
 // What a workgroup does: rows `first` and on (row = token * rep + head of the group) of a
@@ -161,11 +162,11 @@ __device__ __forceinline__ int scalar_int(const int* p) {
 // Up to 32 rows the keys' bytes bound it: 64 single tokens over 725 to 2175 keys, 8 / 4 heads of 96, 146 MB, 33 us, 4.4 TB/s;
 // trees of 16 there 39 us.  With more rows the matrix cores, the softmax and the LDS take turns: that tree of 64 tokens 70 us
 // a call, join included, 6 chunks of 500 over up to 4100 keys, heads of 64, 55.
-template <int HD, int RW, int KW, int S>
+template <int HD, int RW, int KW>
 constexpr int paged_waves =  // of a SIMD, as the tiles' LDS lets in: two at most
-    160 * 1024 / (KW * S * 4 * (RW == 1 ? 32 : 64) * HD) * RW * KW >= 8 ? 2 : 1;
-template <bool F16, int HD, int RW, int KW, int U, int S>
-__global__ __launch_bounds__(64 * RW * KW, (paged_waves<HD, RW, KW, S>)) void paged_kernel(PagedAttnArgs a) {
+    160 * 1024 / (KW * kPagedStages * 4 * (RW == 1 ? 32 : 64) * HD) * RW * KW >= 8 ? 2 : 1;
+template <bool F16, int HD, int RW, int KW, int U>
+__global__ __launch_bounds__(64 * RW * KW, (paged_waves<HD, RW, KW>)) void paged_kernel(PagedAttnArgs a) {
   constexpr int KT = RW == 1 ? 32 : 64;
   constexpr int NC = HD / 32, ND = HD / 16, NT = KT / 16, NH = KT / 32;
   constexpr int GW = NT / RW;               // groups of 16 keys that a wave loads of a tile
@@ -173,7 +174,7 @@ __global__ __launch_bounds__(64 * RW * KW, (paged_waves<HD, RW, KW, S>)) void pa
   constexpr int TILE = KT * HD;             // elements
   constexpr int WAVES = RW * KW, RB = 16 * U * RW;
   static_assert(RW == 1 || KW == 1, "waves that share a tile take the same steps");
-  __shared__ __align__(16) uint16_t lds[KW][S][2][TILE];
+  __shared__ __align__(16) uint16_t lds[KW][kPagedStages][2][TILE];
   static_assert(KW == 1 || sizeof(lds) >= WAVES * 16 * U * (HD + 2) * 4, "the waves' sums take the tiles' place");
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -267,12 +268,6 @@ __global__ __launch_bounds__(64 * RW * KW, (paged_waves<HD, RW, KW, S>)) void pa
     look(1);
     arrived();
     lost = __any((unsigned)entry >= (unsigned)a.pages);
-#pragma unroll
-    for (int i = 1; i < S - 1; ++i)
-      if (i < steps) {
-        issue(i, lds[kw][i][0], lds[kw][i][1]);
-        look(i + 1);
-      }
     for (int p = p0 + 64; p <= p1; p += 64) lost |= __any((unsigned)table[min(p + lane, p1)] >= (unsigned)a.pages);
   } else {
     arrived();
@@ -299,8 +294,8 @@ __global__ __launch_bounds__(64 * RW * KW, (paged_waves<HD, RW, KW, S>)) void pa
   auto step = [&](int i, const uint16_t* __restrict__ ks, const uint16_t* __restrict__ vs, uint16_t* __restrict__ kd,
                   uint16_t* __restrict__ vd) {
     const int kt = t0 + i * KW + kw, s0 = kt * KT;
-    if (i + S - 1 < steps) issue(i + S - 1, kd, vd);
-    look(i + S);
+    if (i + 1 < steps) issue(i + 1, kd, vd);
+    look(i + 2);
     uint32_t none = 0;  // groups in no page
     if (lost) {
 #pragma unroll
@@ -479,15 +474,11 @@ __global__ __launch_bounds__(64 * RW * KW, (paged_waves<HD, RW, KW, S>)) void pa
       outputs(1);
     }
   };
-  int stage = 0;
   for (int i = 0; i < steps; ++i) {
-    constexpr int LOADS = 2 * GW * UG;
-    if (S > 2 && i + S - 1 <= steps) tile_wait<(S - 2) * LOADS>();
-    else tile_wait<0>();
+    tile_wait<0>();
     if (RW > 1) tile_barrier();  // the tile has landed for every wave, and all are done with the one before
-    const int next = stage == 0 ? S - 1 : stage - 1;
-    step(i, lds[kw][stage][0], lds[kw][stage][1], lds[kw][next][0], lds[kw][next][1]);
-    stage = stage == S - 1 ? 0 : stage + 1;
+    const int stage = i & 1;
+    step(i, lds[kw][stage][0], lds[kw][stage][1], lds[kw][1 - stage][0], lds[kw][1 - stage][1]);
   }
 
   // ---- results
@@ -642,7 +633,7 @@ int64_t paged_blocks(const PagedAttnArgs& a) { return ((int64_t)a.units + 7) / 8
 
 template <bool F16, int HD, int RW, int KW, int U>
 hipError_t run_paged(const PagedAttnArgs& a, hipStream_t s) {
-  paged_kernel<F16, HD, RW, KW, U, 2><<<dim3((unsigned)paged_blocks(a)), 64 * RW * KW, 0, s>>>(a);
+  paged_kernel<F16, HD, RW, KW, U><<<dim3((unsigned)paged_blocks(a)), 64 * RW * KW, 0, s>>>(a);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   if (a.slots > 0) {
     constexpr int KT = RW == 1 ? 32 : 64;
