@@ -311,6 +311,7 @@ class PagedCache:
 
     def clear(self) -> None:
         """Empties every sequence and takes all pages back."""
+        self._outside_a_capture()
         self.most = [0] * self.sequences  # keys that each sequence has at most
         self.held = [0] * self.sequences  # keys that reserve() was asked for pages for
         self.drafted = [0] * self.sequences  # rows behind those that keep() may still move
@@ -321,11 +322,16 @@ class PagedCache:
 
     def free(self, sequence: int) -> None:
         """Empties a sequence and takes its pages back."""
+        self._outside_a_capture()
         self.free_pages += self.owned[sequence][::-1]
         self.owned[sequence], self.most[sequence] = [], 0
         self.held[sequence] = self.drafted[sequence] = 0
         self.lengths[sequence] = 0
         self.page_table[sequence] = -1
+
+    def _outside_a_capture(self) -> None:
+        if _capturing(self.lengths):
+            raise RuntimeError("mhc_amd: pages are handed out and taken back outside of a captured call")
 
     def _rows(self, rows) -> list:
         rows = [int(rows)] * self.sequences if not hasattr(rows, "__len__") else [int(n) for n in rows]
@@ -337,6 +343,7 @@ class PagedCache:
         """Pages for so many more rows of each sequence (a number, or one for each): all of them or, with
         an error, none.  Where the host's count leaves no room for them it looks at the lengths (a
         synchronisation) and takes back pages behind them, but none that were reserved."""
+        self._outside_a_capture()
         rows = self._rows(rows)
         self._provide(rows)
         self.held = [max(h, m + n) if n else h for h, m, n in zip(self.held, self.most, rows)]
@@ -392,6 +399,7 @@ class PagedCache:
         with captured calls, whose replays count on it, and goes in any other.  Pages of drafts that keep()
         may still move stay.  Raises where a sequence's length is behind its pages (one without any page is
         not in use)."""
+        self._outside_a_capture()
         spare = None if spare is None else self._rows(spare)
         self._look([i for i, pages in enumerate(self.owned) if pages])
         if spare is not None:

@@ -243,3 +243,16 @@ def test_a_call_that_reaches_past_the_tables_hands_out_nothing():
         with pytest.raises(ValueError, match="max_position_embeddings is 20"):
             model(torch.zeros(1, 42, dtype=torch.int64), packed=batch([2, 40]), past_key_values=cache)
         assert torch.equal(cache.page_table, table) and len(cache.free_pages) == 4 and cache.most == [3, 3]
+
+
+def test_pages_are_not_handed_out_or_taken_back_while_capturing():
+    """The host's part would happen once and the device's with every replay."""
+    model = tiny()
+    with torch.no_grad():
+        cache, _ = begin(model, [14, 2])
+        state = lambda: (cache.most, cache.held, cache.owned, cache.free_pages, cache.lengths.tolist(), cache.page_table.tolist())
+        before = repr(state())
+        for call in (lambda: cache.reserve(40), cache.settle, lambda: cache.free(0), cache.clear):
+            with replayed(), pytest.raises(RuntimeError, match="captur"):
+                call()
+        assert repr(state()) == before
