@@ -307,18 +307,21 @@ class PagedCache:
         self.layers = [(self.planes[2 * i], self.planes[2 * i + 1]) for i in range(config.num_hidden_layers)]
         self.sequences, self.capacity, self.page = sequences, capacity, page
         self.replays = False  # whether a call was captured, whose replays the host does not count
-        self.clear()
+        self._empty()
 
     def clear(self) -> None:
         """Empties every sequence and takes all pages back."""
         self._outside_a_capture()
+        self._empty()
+        self.lengths.zero_()
+        self.page_table.fill_(-1)
+
+    def _empty(self) -> None:
         self.most = [0] * self.sequences  # keys that each sequence has at most
         self.held = [0] * self.sequences  # keys that reserve() was asked for pages for
         self.drafted = [0] * self.sequences  # rows behind those that keep() may still move
         self.owned = [[] for _ in range(self.sequences)]
         self.free_pages = list(range(self.planes.shape[1]))[::-1]
-        self.lengths.zero_()
-        self.page_table.fill_(-1)
 
     def free(self, sequence: int) -> None:
         """Empties a sequence and takes its pages back."""

@@ -256,3 +256,5 @@ def test_pages_are_not_handed_out_or_taken_back_while_capturing():
             with replayed(), pytest.raises(RuntimeError, match="captur"):
                 call()
         assert repr(state()) == before
+        with replayed():
+            assert pages(model, 2).owned == [[], []]
