@@ -87,8 +87,10 @@ __device__ __forceinline__ double wave_sum64(double v) {
 // p and q at it in the parent's row), every wave walks the tree from LDS, and the whole
 // workgroup goes over a vocabulary row only where a draw was rejected (or greedy, at each node)
 // and for the next token: a pass of sums over a wave's contiguous part each, then the part that
-// holds the border again, over all threads.  Bound by latencies in turn and, over a wide row, by one CU's 64-bit arithmetic: 64 chains of 8 at
-// a vocabulary of 6400 in fp32 11.8 us; one row of 50257 in bf16 without drafts 12.9, the first rejected draft 4.5 more, the second 7.
+// holds the border again, over all threads.  Bound by latencies in turn: 64 chains of 8 at a vocabulary of 6400 in fp32 11.9 us.
+// Over a wide row one CU works alone, its VALU busy for 47% of its cycles; with sixteen waves a lane has 128 registers, and the
+// compiler moves 38 to 43 to scratch memory (four waves: none).  One row of 50257 in bf16 without drafts 12.9 us, the first
+// rejected draft 4.7 more, the second, which should read nothing, 6.9 (fp32: 6.7 and 10.8).  What of that is arithmetic and what scratch was not measured.
 template <int DT, int W>
 __global__ __launch_bounds__(64 * W) void verify_kernel(VerifyArgs a) {
   constexpr int PER = ProbRow<DT>::PER, TH = 64 * W;
@@ -148,8 +150,8 @@ __global__ __launch_bounds__(64 * W) void verify_kernel(VerifyArgs a) {
         if (w[i] > 0.0 && gone(block * PER + i - P.off)) w[i] = 0.0;
     }
   };
-  // The sum of that; also leaves the waves' sums in s_sum.  A row of up to G blocks a lane stays in
-  // registers for the node's next rejections.
+  // The sum of that; also leaves the waves' sums in s_sum.  A row of up to G blocks a lane is
+  // kept for the node's next rejections: in registers with four waves, partly in scratch memory with sixteen.
   constexpr int G = kDraftBlocks;
   U32x4 pw[G], qw[G];
   bool have_p = false, have_q = false;  // of the node
@@ -493,7 +495,7 @@ __global__ __launch_bounds__(256) void keep_kernel(KeepArgs a) {
 
 template <int DT>
 hipError_t launch_verify_dt(const VerifyArgs& a, hipStream_t s) {
-  // four waves hold a row of up to 2048 blocks in registers, sixteen one of 8192
+  // four waves keep a row of up to 2048 blocks (in registers), sixteen one of 8192
   if (a.V > 2048 * ProbRow<DT>::PER - 2 * ProbRow<DT>::PER) verify_kernel<DT, 16><<<dim3((unsigned)a.B), 1024, 0, s>>>(a);
   else verify_kernel<DT, 4><<<dim3((unsigned)a.B), 256, 0, s>>>(a);
   return hipGetLastError();

@@ -15,7 +15,11 @@ namespace mhc {
 namespace {
 
 constexpr int kPagedStages = 2;  // tiles of a ring: one in use, one in flight
-constexpr int kPagedSeqs = 256;  // up to so many, workgroups are dealt out by the keys' lengths
+// Up to so many sequences, workgroups are dealt out by the keys' lengths; of more, each block of rows is one
+// workgroup over all of its keys.  Single tokens, 8 / 4 heads of 96, over 233 to 700 keys: 256 sequences 39.4 us, 257
+// 36.9 (with 1 kv head, which leaves the chip half empty, 20.0 and 23.9).  A long one among short ones is
+// what that costs: 65001 keys beside 100 each, 256 sequences 64 us, 257 1624.
+constexpr int kPagedSeqs = 256;
 
 // What a workgroup does: rows `first` and on (row = token * rep + head of the group) of a
 // sequence, over part `split` of `splits` of the keys they see.
@@ -160,8 +164,9 @@ __device__ __forceinline__ int scalar_int(const int* p) {
 // that none of a wave's rows sees, the compiler spilled 56 registers at head_dim 128 (64 tokens over
 // 65001 keys, 16 / 2 heads: 117 us instead of 51).
 // Up to 32 rows the keys' bytes bound it: 64 single tokens over 725 to 2175 keys, 8 / 4 heads of 96, 146 MB, 33 us, 4.4 TB/s;
-// trees of 16 there 39 us.  With more rows the matrix cores, the softmax and the LDS take turns: that tree of 64 tokens 70 us
-// a call, join included, 6 chunks of 500 over up to 4100 keys, heads of 64, 55.
+// trees of 16 there 37 us.  With more rows no unit is at its limit, products, softmax and LDS reads take turns: that tree of 64
+// tokens 65 us, 530 TFLOP/s (of the busy CUs' cycles MFMA 43%, VALU 49%; CUs busy 80% of the launch); 6 chunks of 500
+// over up to 4100 keys, heads of 64, 50 us, 380 TFLOP/s (38%, 59%; 70%).
 template <int HD, int RW, int KW>
 constexpr int paged_waves =  // of a SIMD, as the tiles' LDS lets in: two at most
     160 * 1024 / (KW * kPagedStages * 4 * (RW == 1 ? 32 : 64) * HD) * RW * KW >= 8 ? 2 : 1;
@@ -561,9 +566,11 @@ __global__ __launch_bounds__(64 * RW * KW, (paged_waves<HD, RW, KW>)) void paged
 }
 
 // Joins the ranges of a row: a lane takes four columns of one of its heads, a wave 64 such; with P > 1 the
-// workgroup's P waves take every P-th range of the same 64, and the sums meet in LDS.  64 rows of 16
-// heads of 128 from 64 ranges: 6 to 8 us (P = 1: 25); 1024 rows of 8 heads of 96 from a few with P = 1: 5 us
-// (P = 4: 11).
+// workgroup's P waves take every P-th range of the same 64, and the sums meet in LDS.  P follows the rows and the
+// ranges that there can be.  Microseconds of a whole attention call with P = 1, 4, 16 (the rule's in brackets): one token
+// over 65001 keys, 16 / 2 heads of 128, 35.0, 23.9, [22.9]; 8 rows over 65001, 8 / 4 heads of 96, 52.9, 31.5, [28.9]; 64 rows
+// over 65001, 16 / 2 of 128, 75.4, [70.6], 78.0; 4 trees of 30 over 8001 26.0, [23.4], 25.8; 4 tokens over 8001 23.7,
+// [18.6], 18.2; 16 over 4001 24.5, [23.6], 23.9; 100 rows over 4001 22.6, [20.5], 23.5; 64 trees of 16 over up to 2175 [36.5], 39.9, 64.0.
 template <bool F16, int HD, int P>
 __global__ __launch_bounds__(P == 16 ? 1024 : 256) void paged_join_kernel(PagedAttnArgs a) {
   __shared__ __align__(16) f32x4_t sums[P][64];
@@ -663,6 +670,9 @@ hipError_t paged_hd(const PagedAttnArgs& a, hipStream_t s) {
 }  // namespace
 
 // How the work is cut; only totals are known here, the sequences' own lengths are read on the device.
+// Rows of a workgroup follow from the mean rows a sequence, which suits sequences alike.  Others pay: 60 single tokens
+// and 4 chunks of 500 in one call over 725 to 2175 keys, 8 / 4 heads of 96, with 16, 32, 64, 128 rows 95, 100, 89, [80] us,
+// in calls of their own 29 and 38; 63 tokens and one chunk 54, [48], 58, 60, apart 30 and 26.
 // Microseconds a call in a captured graph, join included, for 1, 2, 3, 4 workgroups a CU:
 //   * Up to 32 rows a sequence and kv head, a wave each: 64 single tokens over 725 to 2175 keys, 8 / 4
 //     heads of 96: -, 38.6, 37.6, 36.0 (5: 35.8, 6: 40); trees of 16 nodes there -, 45.8, 45.4, 43.9 (5: 45.2).
@@ -672,6 +682,13 @@ hipError_t paged_hd(const PagedAttnArgs& a, hipStream_t s) {
 //     24.7, 22.3, 29.1, 29.3; one of 32 over 65001 keys 45.7, 32.3, 43.4, 43.8.
 //   * More, four waves: 6 chunks of 500 over up to 4100 keys, heads of 64: 73, 55, 50, 56; of 96: 101, 71, 76, 76;
 //     one tree of 64 nodes over 65001 keys, 16 / 2 heads of 128: 80, 67, 81, 81.
+// Keys are not cut with four blocks of rows a place and more.  Cut and whole, sequences of a third to all of the longest's
+// keys, 8 / 4 heads of 96: 96 chunks of 400 over 2000 keys (5.4 blocks a place) 389 and 367 us, 140 (7.9) 531 and 514.  Below
+// four cutting costs about as much where lengths are that much alike (64 chunks, 3.6, 279 and 266; 128 trees of 30 over 700 keys, 1.9, 36.0
+// and 32.3), but it is what keeps a long sequence among short ones from being one workgroup's.
+// A range has 4 tiles at least, or 2 of the larger ones.  With 1, 2, 4, 8: a single token over 900 keys 9.9, 10.0, [11.4],
+// 14.1 us; 8 trees of 5 12.5, 11.3, [12.0], 14.6; 32 tokens over 400 11.0, 11.0, [12.0], 13.9; two trees of 64 over 900 15.0, [16.7], 19.3,
+// 25.6; a chunk of 300 22.3, [18.6], 18.7, 22.0.  (All the same inputs on every call.)
 void paged_attn_plan(PagedAttnArgs& a) {
   const int rep = a.heads / a.kv_heads;
   const int64_t B = a.B > 0 ? a.B : 1, rows = (int64_t)a.Tq * rep, each = (rows + B - 1) / B;
