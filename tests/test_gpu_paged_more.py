@@ -7,7 +7,7 @@ import torch
 
 from model import _hip as H
 from model.paged import paged_attention
-from test_gpu_paged import BF, EPS, F16, exact, ints, make, random_tree, starts
+from test_gpu_paged import BF, EPS, F16, close, exact, ints, make, random_tree, starts
 
 
 @pytest.mark.gpu
@@ -73,3 +73,18 @@ def test_workspace_sizes_are_kept_for_each_device(dev, monkeypatch):
     pool, q = make(dev, BF, [900], [1], 16, 8, 4, 96)
     paged_attention(q, pool.k, pool.v, pool.table, ints([900], dev), ints([0, 1], dev))
     assert seen == [(dev.index, 1, 1, 8, 4, 96)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("past,new", [
+    ([3000] + [i % 40 for i in range(255)], [1] * 256), ([i % 40 for i in range(199)] + [3000] + [5] * 60, [1] * 260),
+    ([700, 90, 0, 1500, 33] * 4, [1, 1, 200, 1, 1] * 4), ([20, 500] * 3 + [900], [1, 2] * 3 + [400]),
+    ([i % 70 for i in range(290)], [1] * 100 + [130] + [1] * 100 + [0] * 60 + [3] * 29)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_sequences_that_are_not_alike(dev, past, new, tree):
+    """One long sequence among many short ones, on both sides of 256; single tokens and chunks in one call."""
+    pool, q = make(dev, BF, past, new, 16, 8, 4, 64)
+    bits, sees = random_tree(new, 5) if tree else (None, None)
+    got = paged_attention(q, pool.k, pool.v, pool.table, ints(past, dev), ints(starts(new), dev),
+                          tree=None if bits is None else bits.to(dev), scale=0.11)
+    close(got, exact(pool, q, past, new, 0.11, sees), BF)
