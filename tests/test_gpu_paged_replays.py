@@ -79,3 +79,47 @@ def test_verify_step_of_a_64_bit_model(dev, mode):
     for got, w in zip((res.kept, res.path, res.next_tokens), want):
         assert got.device == dev and got.dtype == w.dtype and torch.equal(got.cpu(), w)
     assert cache.lengths.tolist() == [4 + int(want[0][0]), 3 + int(want[0][1])]
+
+
+@pytest.mark.gpu
+def test_rounds_of_captured_verify_steps(dev):
+    """Whole steps with drafts in a graph, reserved for and settled between rounds, against eager steps on a cache whose
+    host count is only a bound; both end where the pages do."""
+    m = _model(dev).eval()
+    cache, other = (PagedCache(m.config, 2, 160, 16, pages=14, device=dev) for _ in range(2))
+    g = torch.Generator(device=dev).manual_seed(5)
+    draw = lambda n: torch.randint(0, 500, (1, n), generator=g, device=dev)
+    b, prompt = PackedBatch.from_lengths([4, 4], device=dev), PackedBatch.from_lengths([40, 9], device=dev)
+    ids, u, first = draw(8), torch.rand(8, generator=g, device=dev), draw(49)
+    with torch.inference_mode():
+        for c in (cache, other):
+            m(first, packed=prompt, past_key_values=c)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            m.verify_step(ids, b, other, None, None, u)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        other.lengths.copy_(cache.lengths)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            with pytest.raises(RuntimeError, match="captured"):
+                cache.reserve(4)
+            res = m.verify_step(ids, b, cache, None, None, u)
+        for turn in range(12):
+            cache.reserve(12)  # three steps of four nodes at most
+            for _ in range(3):
+                ids.copy_(draw(8))
+                u.copy_(torch.rand(8, generator=g, device=dev) * (0.005 if turn % 3 else 1.0))
+                graph.replay()
+                want = m.verify_step(ids, b, other, None, None, u)
+                torch.cuda.synchronize()
+                assert torch.equal(res.logits, want.logits) and torch.equal(res.next_tokens, want.next_tokens), turn
+            same(cache, other)
+            if turn % 2:
+                cache.settle(spare=0)
+        longest = max(cache.lengths.tolist())
+        assert longest > 76
+        for c in (cache, other):  # what does not fit is refused, by its true length
+            with pytest.raises(ValueError, match=f"{longest} . {161 - longest} keys may not fit"):
+                c.reserve([161 - longest] * 2 if c.lengths[0] >= c.lengths[1] else [0, 161 - longest])
